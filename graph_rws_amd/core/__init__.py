@@ -20,6 +20,7 @@ from .ops import (  # noqa: F401
     spmm,
     spmm_tc,
     spmm_transpose,
+    top_logits,
 )
 
 
@@ -48,4 +49,5 @@ __all__ = [
     "sample_all_layers",
     "SamplingTimingResult",
     "window_seeds",
+    "top_logits",
 ]

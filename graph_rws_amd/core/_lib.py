@@ -60,6 +60,15 @@ class HacsView(ctypes.Structure):
                 ("use_hacs", ctypes.c_int32), ("locality_enabled", ctypes.c_int32)]
 
 
+class HeadView(ctypes.Structure):
+    """grws_head (include/grws.h)."""
+    _fields_ = [("hidden", _vp), ("weight", _vp), ("bias", _vp), ("rows", _vp), ("labels", _vp),
+                ("teacher_index", _vp), ("teacher_logits", _vp), ("ld_hidden", ctypes.c_int64),
+                ("ld_weight", ctypes.c_int64), ("hidden_rows", ctypes.c_int64), ("n", ctypes.c_int64),
+                ("width", ctypes.c_int64), ("classes", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("k", ctypes.c_int32), ("index_is_i64", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
 # name -> (restype, argtypes)
 _PROTOS = {
     "grws_last_error": (ctypes.c_char_p, []),
@@ -241,6 +250,15 @@ _PROTOS = {
     "grws_cross_entropy_bwd": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
                                               ctypes.c_int64, _vp, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp,
                                               ctypes.c_int32, ctypes.c_int64, _vp]),
+    "grws_head_fwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(HeadView)]),
+    "grws_head_fwd": (ctypes.c_int, [ctypes.POINTER(HeadView), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                     ctypes.c_size_t, _vp]),
+    "grws_head_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(HeadView)]),
+    "grws_head_bwd": (ctypes.c_int, [ctypes.POINTER(HeadView), _vp, _vp, _vp, _vp, _vp, ctypes.c_int32, _vp,
+                                     ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, ctypes.c_size_t, _vp]),
+    "grws_top_logits_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
+    "grws_top_logits": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                       ctypes.c_int32, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "grws_relabel_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
     "grws_relabel": (ctypes.c_int, [_vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int64,
                                     _vp, _vp, ctypes.c_int64, _vp, ctypes.c_size_t, _c_i64p,

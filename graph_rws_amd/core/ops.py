@@ -1819,3 +1819,136 @@ def cross_entropy_bwd(logits: torch.Tensor, rows: Optional[torch.Tensor], labels
            labels.numel(), L.ptr(lse), L.ptr(dl), L.ptr(counts), L.ptr(grad), L.dtype_code(grad.dtype),
            grad.stride(0), L.stream_of(logits.device))
     return grad
+
+
+# ---------------------------------------------------------------------------
+# classifier over many classes (csrc/head.hip) and top logits (csrc/top.hip)
+# ---------------------------------------------------------------------------
+def _unit_columns(t: torch.Tensor) -> torch.Tensor:
+    """t with unit column stride and rows that do not overlap (a copy where
+    it has neither)."""
+    ok = (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+    return t if ok else t.contiguous()
+
+
+def _row_pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class HeadCall:
+    """The checked arguments of one classifier call: hidden [N, D], weight
+    [V, D], bias [V] or None, rows int64 [n] or None, and either labels
+    int64 [n] or a teacher's (index int32/int64 [n, K], logits [n, K],
+    temperature).  Holds the tensors that its view points to."""
+
+    def __init__(self, hidden, weight, bias=None, rows=None, labels=None, teacher_index=None, teacher_logits=None,
+                 temperature: float = 1.0):
+        who = "linear_cross_entropy" if labels is not None else "linear_distill"
+        L.require_device(who, hidden.device, weight, bias, rows, labels, teacher_index, teacher_logits)
+        if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] or weight.numel() == 0:
+            raise ValueError(f"{who}: hidden must be [rows, width] and weight [classes, width] (got "
+                             f"{tuple(hidden.shape)} and {tuple(weight.shape)})")
+        code = L.dtype_code(hidden.dtype)
+        if weight.dtype != hidden.dtype or (bias is not None and bias.dtype != hidden.dtype):
+            raise TypeError(f"{who}: hidden, weight and bias must have one dtype")
+        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError(f"{who}: bias must be [classes]")
+        if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int64):
+            raise ValueError(f"{who}: rows must be int64 [n]")
+        k = 0
+        if labels is not None:
+            if labels.dim() != 1 or labels.dtype != torch.int64:
+                raise ValueError(f"{who}: labels must be int64 [n]")
+            n = labels.shape[0]
+            self.labels, self.index, self.logits = labels.contiguous(), None, None
+        else:
+            if (teacher_index.dim() != 2 or teacher_index.dtype not in (torch.int32, torch.int64)
+                    or teacher_logits.shape != teacher_index.shape or not teacher_logits.is_floating_point()):
+                raise ValueError(f"{who}: teacher_index must be int32 or int64 [n, k] and teacher_logits [n, k]")
+            n, k = teacher_index.shape
+            if not 1 <= k <= 1024:
+                raise ValueError(f"{who}: 1 to 1024 teacher entries a row (got {k})")
+            if not 0.0 < float(temperature) < float("inf"):
+                raise ValueError(f"{who}: the temperature must be positive (got {temperature})")
+            self.labels = None
+            self.index, self.logits = teacher_index.contiguous(), teacher_logits.detach().float().contiguous()
+        if rows is not None and rows.shape[0] != n:
+            raise ValueError(f"{who}: {rows.shape[0]} rows for {n} targets")
+        if rows is None and n > hidden.shape[0]:
+            raise ValueError(f"{who}: {n} targets for {hidden.shape[0]} rows of hidden")
+        self.who, self.n, self.k = who, n, k
+        self.hidden, self.weight = _unit_columns(hidden.detach()), _unit_columns(weight.detach())
+        self.bias = bias.detach().contiguous() if bias is not None else None
+        self.rows = rows.contiguous() if rows is not None else None
+        self.view = L.HeadView(L.ptr(self.hidden), L.ptr(self.weight), L.ptr(self.bias), L.ptr(self.rows),
+                               L.ptr(self.labels), L.ptr(self.index), L.ptr(self.logits), _row_pitch(self.hidden),
+                               _row_pitch(self.weight), hidden.shape[0], n, hidden.shape[1], weight.shape[0], code,
+                               k, int(k > 0 and self.index.dtype == torch.int64), float(temperature))
+
+
+def head_fwd(call: HeadCall):
+    """(loss f32 scalar, row_loss f32 [n], counts int64 [3] = {hits, counted
+    rows, bad input}, saved) of a HeadCall (csrc/head.hip); no host sync."""
+    dev = call.hidden.device
+    n, k = call.n, call.k
+    f = torch.empty(1 + n * (2 + max(k, 1) + k), dtype=torch.float32, device=dev)
+    loss, row_loss, lse = f[0], f[1:1 + n], f[1 + n:1 + 2 * n]
+    logit = f[1 + 2 * n:1 + 2 * n + n * max(k, 1)]
+    prob = f[1 + 2 * n + n * max(k, 1):] if k else None
+    counts = torch.empty(3, dtype=torch.int64, device=dev)
+    ref = ctypes.byref(call.view)
+    wsb = int(L.load().grws_head_fwd_workspace_bytes(ref))
+    ws = torch.empty(max(1, wsb), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        L.call("grws_head_fwd", ref, L.ptr(lse), L.ptr(logit), L.ptr(prob), L.ptr(row_loss), L.ptr(loss),
+               L.ptr(counts), L.ptr(ws), wsb, L.stream_of(dev))
+    return loss, row_loss, counts, (lse, logit, prob)
+
+
+def head_bwd(call: HeadCall, saved, counts: torch.Tensor, dloss: torch.Tensor, need=(True, True, True)):
+    """(d_hidden, d_weight, d_bias), None where not needed, of head_fwd's
+    loss (dloss a scalar) or row_loss (dloss [n])."""
+    dev = call.hidden.device
+    lse, logit, prob = saved
+    dl = dloss.detach().float().contiguous()
+    dh = dw = db = None
+    if need[0]:
+        some = call.rows is not None or call.n < call.hidden.shape[0]
+        dh = (torch.zeros if some else torch.empty)(call.hidden.shape, dtype=call.hidden.dtype, device=dev)
+    if need[1]:
+        dw = torch.empty(call.weight.shape, dtype=call.weight.dtype, device=dev)
+    if need[2] and call.bias is not None:
+        db = torch.empty(call.bias.shape, dtype=call.bias.dtype, device=dev)
+    ref = ctypes.byref(call.view)
+    wsb = int(L.load().grws_head_bwd_workspace_bytes(ref))
+    ws = torch.empty(max(1, wsb), dtype=torch.uint8, device=dev)
+    width = call.hidden.shape[1]
+    with torch.cuda.device(dev):
+        L.call("grws_head_bwd", ref, L.ptr(lse), L.ptr(logit), L.ptr(prob), L.ptr(counts), L.ptr(dl),
+               int(dloss.dim() == 1), L.ptr(dh), width, L.ptr(dw), width, L.ptr(db), L.ptr(ws), wsb,
+               L.stream_of(dev))
+    return dh, dw, db
+
+
+def top_logits(logits: torch.Tensor, k: int):
+    """(values [n, k] in the logits' dtype, classes int32 [n, k]): the k
+    largest logits of each row, largest first; of equal ones the lowest class
+    first, NaN as the largest (csrc/top.hip).  1 <= k <= min(classes, 1024).
+    The lists that linear_distill takes of a teacher; no gradient."""
+    L.require_device("top_logits", logits.device)
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"top_logits: logits must be [rows, classes] (got {tuple(logits.shape)})")
+    if not 1 <= k <= min(logits.shape[1], 1024):
+        raise ValueError(f"top_logits: k must be 1..{min(logits.shape[1], 1024)} (got {k})")
+    code = L.dtype_code(logits.dtype)
+    x = _unit_columns(logits.detach())
+    n, classes = x.shape
+    dev = x.device
+    values = torch.empty((n, k), dtype=x.dtype, device=dev)
+    index = torch.empty((n, k), dtype=torch.int32, device=dev)
+    wsb = int(L.load().grws_top_logits_workspace_bytes(n, classes, k))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    with torch.cuda.device(dev):
+        L.call("grws_top_logits", L.ptr(x), code, _row_pitch(x), n, classes, k, L.ptr(values), L.ptr(index),
+               L.ptr(ws), wsb, L.stream_of(dev))
+    return values, index

@@ -37,6 +37,8 @@ SOURCES = [
     "gemm_tn.hip",
     "repack.hip",
     "fused.hip",
+    "head.hip",
+    "top.hip",
     "probe.hip",
 ]
 

@@ -1,0 +1,1359 @@
+// Classifier over many classes fused with its loss (gfx950): softmax cross
+// entropy and distillation from a teacher's top logits on
+//     z = H W^T + b        H [n x D] rows of hidden, W [V x D] classes,
+// without ever keeping z, and their gradients.
+//
+// Mathematics.  With y = z log2(e) / T and L_i = log2 sum_v 2^y_iv:
+//   cross entropy (T = 1)   loss_i = ln2 (L_i - y_i,label)
+//   distillation            loss_i = T^2 (sum_k q_ik ln q_ik
+//                                         + ln2 (L_i - sum_k q_ik y_i,k)),
+//                           q_i = softmax of the teacher's listed logits / T
+//   gradient                dz_iv = s_i T (2^(y_iv - L_i) - q_iv),
+//                           dH = dz W, dW = dz^T H, db = column sums of dz,
+// where q of cross entropy is 1 at the label.
+//
+// Forward: one product whose epilogue reduces each 16 TP classes of a row to
+// (max, sum of 2^(y - max)) in registers; a second kernel joins them.
+// Backward: pieces of the classes.  For each piece the product is made again
+// and its epilogue writes G = 2^(y - L) in 16 bits to a scratch matrix, a
+// small kernel subtracts the targets, and two products read G: dW's rows of
+// the piece (complete), and dH (added up over the pieces in fp32).
+//
+// G is rounded to the operands' 16-bit type because the matrix cores take no
+// wider one; p - q is formed in fp32 and rounded once.  Its factor s_i T is
+// applied to the fp32 sums instead (f16: G carries 2^15, so that
+// probabilities down to 2^-29 stay normal numbers).
+//
+// F32 operands: x = a + b + c with three bf16 (the top, middle and low 8 of
+// 24 significant bits, truncated, so the split is exact and never
+// overflows), and the product is the sum of the six plane products
+// ac, ca, bb, ba, ab, aa; the three left out are below 2^-23 of |x||y|, a
+// rounding of the fp32 sum.  Six bf16 MFMAs take less time than one f32 MFMA
+// of the same products (2,500 / 6 against 157 TFLOP/s).
+//
+// The product (gemm_core).  Out[q][p] = sum_k P[p,k] Q[q,k]; work-groups own
+// BP x BQ tiles, waves TP x TQ tiles of v_mfma_f32_16x16x32.  Both operands
+// go straight to LDS (16-byte buffer loads with range checks, so ragged
+// edges read zeros), two stages of 64 k.  An operand is either contiguous
+// along k (rows of 128 B a stage, 16-byte chunks XORed with the row so that
+// a b128 read of 16 rows spreads over all banks) or strided along k (rows of
+// BP or BQ columns, 32-byte chunks XORed with the row, read by gfx950's
+// transposing LDS read, two per 32 k).
+#include "grws_internal.h"
+
+namespace grws {
+namespace {
+
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef short short8_t __attribute__((ext_vector_type(8)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 tr_v4bf16_t;
+typedef __attribute__((address_space(3))) tr_v4bf16_t lds_v4bf16_t;
+typedef __attribute__((address_space(3))) short8_t lds_short8_t;
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef __attribute__((address_space(3))) char lds_char_t;
+
+constexpr int kK = 64;               // k per LDS stage
+constexpr int64_t kIgnoreLabel = -100;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kPastEnd = 0x80000000u;  // past every resource: the load returns zeros
+
+// An operand in memory.  Contiguous along k: `rows` rows of `k` elements.
+// Strided along k: `k` rows (the sum's index) of `rows` columns.
+struct Opnd {
+    const char* p;
+    int64_t ld;     // bytes between rows
+    int64_t plane;  // bytes between the planes of a split f32 operand
+    int64_t rows;
+    int64_t k;
+};
+
+struct Gemm {
+    Opnd P, Q;
+    int32_t nseg;    // plane products: 1, or 6 for split f32 operands
+    int32_t ksteps;  // stages of 64 k per plane product
+    int32_t tp, tq;  // tiles along p and q
+    int32_t splits;  // work-groups per tile along k
+};
+
+// The planes of product `seg` (the last six-plane product, and the only one
+// of 16-bit operands, is plane 0 by plane 0); small products come first.
+__device__ __forceinline__ int plane_p(int seg) { return (0x001102 >> (4 * seg)) & 15; }
+__device__ __forceinline__ int plane_q(int seg) { return (0x010120 >> (4 * seg)) & 15; }
+
+template <int DT>
+__device__ __forceinline__ float4_t mma(short8_t a, short8_t b, float4_t c) {
+    if constexpr (DT == GRWS_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b),
+                                                      c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// One operand's tile of B rows (or columns) of a stage: its direct loads and
+// its fragment reads.
+template <bool STRIDED, int B, int NW>
+struct Tile {
+    static constexpr int NL = B / 8 / NW;  // 1 KiB loads per wave and stage
+    static_assert(NL >= 1 && NL * NW * 8 == B, "tile does not split over the waves");
+    const char* base;
+    int64_t ld, plane, left;  // left: strided: k rows; contiguous: k
+    int64_t edge;             // bytes: strided: of the last row; contiguous: up to the last row
+    uint32_t off[NL];
+    int kfirst;  // contiguous: first k of the lane's chunk
+
+    __device__ __forceinline__ void init(const Opnd& o, int64_t t0, int wave, int lane) {
+        ld = o.ld;
+        plane = o.plane;
+        left = o.k;
+        if constexpr (!STRIDED) {
+            base = o.p + t0 * ld;
+            const int64_t rows = o.rows - t0 < B ? o.rows - t0 : B;
+            edge = (rows - 1) * ld;
+            const int chunk = (lane & 7) ^ (lane >> 3);
+            kfirst = chunk * 8;
+#pragma unroll
+            for (int i = 0; i < NL; ++i)
+                off[i] = (uint32_t)(((wave * NL + i) * 8 + (lane >> 3)) * ld) + chunk * 16;
+        } else {
+            base = o.p + t0 * 2;
+            edge = (o.rows - t0) * 2;
+            kfirst = 0;
+            constexpr int CH = B / 8;  // 16-byte chunks per row
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int row = (wave * NL + i) * (64 / CH) + lane / CH;
+                const int key = ((row & 3) | (((row >> 3) & 3) << 2)) & (CH / 2 - 1);
+                off[i] = (uint32_t)(row * ld) + (uint32_t)(((lane % CH) ^ (key << 1)) * 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void load(char* lds, int pl, int64_t k0, int wave) const {
+        const char* b;
+        int64_t rec;
+        if constexpr (!STRIDED) {
+            b = base + pl * plane + k0 * 2;
+            rec = edge + (left - k0) * 2;
+        } else {
+            b = base + pl * plane + k0 * ld;
+            rec = left > k0 ? (left - k0 - 1) * ld + edge : 0;
+            if (rec > 0x7fffffff) rec = 0x7fffffff;
+        }
+        const __amdgpu_buffer_rsrc_t rs =
+            __builtin_amdgcn_make_buffer_rsrc((void*)b, (short)0, (int)rec, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            uint32_t o = off[i];
+            if constexpr (!STRIDED) o = kfirst < left - k0 ? o : kPastEnd;  // past the row's k: not the next row's
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)((lds_char_t*)lds + (wave * NL + i) * 1024), 16,
+                                                     (int)o, 0, 0, 0);
+        }
+    }
+    // 16 rows (columns) first..first+15 and k = 32 half + 8 (lane / 16) + 0..7
+    // as an MFMA operand: lane l holds row l % 16.
+    static __device__ __forceinline__ short8_t frag(const char* lds, int first, int half, int lane) {
+        if constexpr (!STRIDED) {
+            const int r = lane & 15;
+            const char* p = lds + (first + r) * 128 + (((half * 4 + (lane >> 4)) ^ (r & 7)) * 16);
+            return *(const lds_short8_t*)(lds_char_t*)p;
+        } else {
+            const int g = lane >> 4, a = (lane >> 2) & 3;
+            constexpr int CH = B / 8;
+            const int key = (a | (g << 2)) & (CH / 2 - 1);
+            const char* p = lds + (32 * half + 8 * g + a) * (B * 2) + ((first / 16) ^ key) * 32 + (lane & 3) * 8;
+            const short4_t lo = __builtin_bit_cast(short4_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                                                                 (lds_v4bf16_t*)(lds_char_t*)p));
+            const short4_t hi = __builtin_bit_cast(short4_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                                                                 (lds_v4bf16_t*)(lds_char_t*)(p + 4 * B * 2)));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+// Work-group -> tile.  Work-group b runs on XCD b % 8; each XCD takes a
+// contiguous run of tiles, ordered in columns of 8 q tiles, so that the
+// tiles in flight on an XCD share operand rows in its L2.
+__device__ __forceinline__ void tile_of(const Gemm& g, int& tp, int& tq) {
+    const int n = g.tp * g.tq;
+    const int b = blockIdx.x;
+    const int per = n >> 3, rem = n & 7;
+    const int x = b & 7;
+    const int t = x * per + (x < rem ? x : rem) + (b >> 3);
+    const int col = 8 * g.tp;
+    const int c = t / col;
+    const int w = g.tq - 8 * c < 8 ? g.tq - 8 * c : 8;
+    const int r = t - c * col;
+    tq = 8 * c + r % w;
+    tp = r / w;
+}
+
+template <int DT, bool PS, bool QS, int BP, int BQ, int WP, int WQ>
+struct Core {
+    static constexpr int NW = WP * WQ;
+    static constexpr int TP = BP / WP / 16, TQ = BQ / WQ / 16;
+    static constexpr int STAGE = (BP + BQ) * 128;
+    using TileP = Tile<PS, BP, NW>;
+    using TileQ = Tile<QS, BQ, NW>;
+
+    // acc[i][j]: lane l, element e: p = 16 i + 4 (l / 16) + e, q = 16 j + l % 16
+    // of the wave's block, over stages kb..ke of every plane product
+    static __device__ __forceinline__ void run(const Gemm& g, int tp, int tq, int kb, int ke, char* s0, char* s1,
+                                               float4_t (&acc)[TP][TQ]) {
+        const int lane = threadIdx.x & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wp = (wave % WP) * (TP * 16), wq = (wave / WP) * (TQ * 16);
+        TileP P;
+        TileQ Q;
+        P.init(g.P, (int64_t)tp * BP, wave, lane);
+        Q.init(g.Q, (int64_t)tq * BQ, wave, lane);
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int j = 0; j < TQ; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+        const int per = ke - kb;
+        if (per <= 0) return;  // uniform over the work-group
+        const int total = g.nseg * per;
+        int seg = 6 - g.nseg, ks = kb;
+        auto fetch = [&](char* st) {
+            P.load(st, plane_p(seg), (int64_t)ks * kK, wave);
+            Q.load(st + BP * 128, plane_q(seg), (int64_t)ks * kK, wave);
+            if (++ks == ke) {
+                ks = kb;
+                ++seg;
+            }
+        };
+        auto multiply = [&](const char* st) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                short8_t a[TP], b[TQ];
+#pragma unroll
+                for (int i = 0; i < TP; ++i) a[i] = TileP::frag(st, wp + 16 * i, h, lane);
+#pragma unroll
+                for (int j = 0; j < TQ; ++j) b[j] = TileQ::frag(st + BP * 128, wq + 16 * j, h, lane);
+#pragma unroll
+                for (int i = 0; i < TP; ++i)
+#pragma unroll
+                    for (int j = 0; j < TQ; ++j) acc[i][j] = mma<DT>(a[i], b[j], acc[i][j]);
+                // no reads of the next half among these: 256 registers hold
+                // the accumulators and one half's operands
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // this wave's loads into `cur` have landed before the barrier, which
+        // does not wait for loads into LDS; after it every wave's have, and
+        // every wave is done reading `nxt`
+        auto step = [&](char* cur, char* nxt, bool more) {
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) fetch(nxt);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(cur);
+        };
+        fetch(s0);
+        int t = 0;
+        for (; t + 1 < total; t += 2) {
+            step(s0, s1, true);
+            step(s1, s0, t + 2 < total);
+        }
+        if (t < total) step(s0, s1, false);
+    }
+};
+
+#define GRWS_HEAD_LDS(C)                                              \
+    __shared__ __attribute__((aligned(1024))) char s0[C::STAGE];      \
+    __shared__ __attribute__((aligned(1024))) char s1[C::STAGE];
+
+// ---------------------------------------------------------------------------
+// the product's epilogues
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float4_t load_bias4(const void* bias, int64_t v, int64_t left) {
+    float4_t b{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < left) b[e] = to_float(static_cast<const T*>(bias)[v + e]);
+    return b;
+}
+
+__device__ __forceinline__ float4_t bias4(const void* bias, int32_t dt, int64_t v, int64_t left) {
+    if (dt == GRWS_F32) return load_bias4<float>(bias, v, left);
+    if (dt == GRWS_F16) return load_bias4<_Float16>(bias, v, left);
+    return load_bias4<__hip_bfloat16>(bias, v, left);
+}
+
+// acc -> y = c1 (acc + bias); classes past the last one get `past`
+template <int TP, int TQ>
+__device__ __forceinline__ void scale_logits(float4_t (&acc)[TP][TQ], int64_t vfirst, int64_t classes, float c1,
+                                             const void* bias, int32_t bias_dt, int lane, float past) {
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+        const int64_t v = vfirst + 16 * i + 4 * (lane >> 4);
+        float4_t b{0.f, 0.f, 0.f, 0.f};
+        if (bias) b = bias4(bias, bias_dt, v, classes - v);
+#pragma unroll
+        for (int j = 0; j < TQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = (acc[i][j][e] + b[e]) * c1;
+    }
+    if (vfirst + 16 * TP > classes) {
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (vfirst + 16 * i + 4 * (lane >> 4) + e >= classes) {
+#pragma unroll
+                    for (int j = 0; j < TQ; ++j) acc[i][j][e] = past;
+                }
+    }
+}
+
+struct StatsArgs {
+    Gemm g;
+    int64_t v0, classes;  // first class of the piece, all classes
+    int64_t n, np;        // rows, padded rows
+    float c1;
+    const void* bias;
+    int32_t bias_dt;
+    const int64_t* labels;  // NULL: none to look for
+    float2* part;           // [strips][np]: max, sum of 2^(y - max)
+    float* ylabel;          // [n]
+    int32_t* earlier;       // [n]: an earlier class of the label's strip has the label's logit
+};
+
+// Bound by the matrix cores for wide D and by the exponentials (a quarter of
+// the vector rate) for narrow D.  p are classes and q rows, so a lane holds
+// 4 TP classes of TQ rows and the reduction over classes takes two
+// cross-lane steps a row.
+template <int DT, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
+    using C = Core<DT, false, false, BP, BQ, WP, WQ>;
+    constexpr int TP = C::TP, TQ = C::TQ;
+    GRWS_HEAD_LDS(C)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int tp, tq;
+    tile_of(a.g, tp, tq);
+    float4_t acc[TP][TQ];
+    C::run(a.g, tp, tq, 0, a.g.ksteps, s0, s1, acc);
+    const int wp = wave % WP;
+    const int64_t vfirst = a.v0 + (int64_t)tp * BP + wp * (TP * 16);
+    scale_logits<TP, TQ>(acc, vfirst, a.classes, a.c1, a.bias, a.bias_dt, lane, -INFINITY);
+    const int64_t strip = vfirst / (TP * 16);
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
+        m = fmaxf(m, __shfl_xor(m, 16, kWave));
+        m = fmaxf(m, __shfl_xor(m, 32, kWave));
+        const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf: a sum of zeros
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - ref);
+        s += __shfl_xor(s, 16, kWave);
+        s += __shfl_xor(s, 32, kWave);
+        if (lane < 16) a.part[strip * a.np + row] = make_float2(m, s);
+        if (a.labels) {
+            const int64_t lab = row < a.n ? a.labels[row] - vfirst : -1;
+            const bool here = lab >= 0 && lab < TP * 16 && lab + vfirst < a.classes;
+            if (__any(here)) {
+                const int l = here ? (int)lab : 0;
+                float y = 0.f;
+#pragma unroll
+                for (int i = 0; i < TP; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y = (l >> 4) == i && (l & 3) == e ? acc[i][j][e] : y;
+                y = __shfl(y, (((l >> 2) & 3) << 4) | (lane & 15), kWave);
+                int tie = 0;
+#pragma unroll
+                for (int i = 0; i < TP; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        tie |= acc[i][j][e] == y && 16 * i + 4 * (lane >> 4) + e < l;
+                tie |= __shfl_xor(tie, 16, kWave);
+                tie |= __shfl_xor(tie, 32, kWave);
+                if (here && lane < 16) {
+                    a.ylabel[row] = y;
+                    a.earlier[row] = tie;
+                }
+            }
+        }
+    }
+}
+
+struct GradArgs {
+    Gemm g;
+    int64_t v0, classes, n;
+    float c1;
+    const void* bias;
+    int32_t bias_dt;
+    const float* lse;        // [n], +inf for a row that does not count
+    const float* row_scale;  // [n] or NULL
+    float gscale;
+    uint16_t* G;  // [planes][np][ldg]
+    int64_t ldg, plane;
+};
+
+__device__ __forceinline__ uint16_t top16(float x) { return (uint16_t)(__float_as_uint(x) >> 16); }
+__device__ __forceinline__ float from_top16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
+
+// x = a + b + c exactly: three truncated bf16 (an infinity or NaN stays in
+// the first; a NaN keeps a bit in its upper half)
+__device__ __forceinline__ void split3(float x, uint16_t* a, uint16_t* b, uint16_t* c) {
+    *a = top16(x);
+    if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) {
+        if (x != x) *a |= 0x40;
+        *b = *c = 0;
+        return;
+    }
+    const float r = x - from_top16(*a);
+    *b = top16(r);
+    *c = top16(r - from_top16(*b));
+}
+
+template <int DT>
+__device__ __forceinline__ uint16_t round16(float x) {
+    if constexpr (DT == GRWS_F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+    else return __builtin_bit_cast(uint16_t, __float2bfloat16(x));
+}
+
+template <int DT, bool SPLIT>
+__device__ __forceinline__ void store_g(uint16_t* G, int64_t plane, int64_t at, float x) {
+    if constexpr (SPLIT) {
+        split3(x, G + at, G + plane + at, G + 2 * plane + at);
+    } else {
+        G[at] = round16<DT>(x);
+    }
+}
+
+template <int DT, bool SPLIT, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
+    using C = Core<DT, false, false, BP, BQ, WP, WQ>;
+    constexpr int TP = C::TP, TQ = C::TQ;
+    GRWS_HEAD_LDS(C)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int tp, tq;
+    tile_of(a.g, tp, tq);
+    float4_t acc[TP][TQ];
+    C::run(a.g, tp, tq, 0, a.g.ksteps, s0, s1, acc);
+    const int64_t pfirst = (int64_t)tp * BP + (wave % WP) * (TP * 16);
+    scale_logits<TP, TQ>(acc, a.v0 + pfirst, a.classes, a.c1, a.bias, a.bias_dt, lane, -INFINITY);
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
+        const float l = row < a.n ? a.lse[row] : INFINITY;
+        const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
+#pragma unroll
+        for (int i = 0; i < TP; ++i) {
+            const int64_t at = row * a.ldg + pfirst + 16 * i + 4 * (lane >> 4);
+            uint16_t h[SPLIT ? 3 : 1][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = l == INFINITY ? 0.f : __builtin_amdgcn_exp2f(acc[i][j][e] - l) * s;
+                if constexpr (SPLIT) split3(x, &h[0][e], &h[1][e], &h[2][e]);
+                else h[0][e] = round16<DT>(x);
+            }
+#pragma unroll
+            for (int z = 0; z < (SPLIT ? 3 : 1); ++z)
+                *reinterpret_cast<u32x2_t*>(a.G + z * a.plane + at) =
+                    u32x2_t{(uint32_t)h[z][0] | ((uint32_t)h[z][1] << 16),
+                            (uint32_t)h[z][2] | ((uint32_t)h[z][3] << 16)};
+        }
+    }
+}
+
+// dW rows of a piece: p are columns of H, q the piece's classes, k the rows
+struct WeightArgs {
+    Gemm g;
+    const float* alpha;
+    void* out;  // first class of the piece
+    int64_t ldo, classes, width;  // classes of the piece
+    int32_t vec;  // rows of the output take 4-element stores
+};
+
+template <int DT, int OT, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a) {
+    using C = Core<DT, true, true, BP, BQ, WP, WQ>;
+    constexpr int TP = C::TP, TQ = C::TQ;
+    GRWS_HEAD_LDS(C)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int tp, tq;
+    tile_of(a.g, tp, tq);
+    float4_t acc[TP][TQ];
+    C::run(a.g, tp, tq, 0, a.g.ksteps, s0, s1, acc);
+    const float alpha = *a.alpha;
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        const int64_t v = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
+        if (v >= a.classes) continue;
+#pragma unroll
+        for (int i = 0; i < TP; ++i) {
+            const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
+            if (d >= a.width) continue;
+            const int64_t at = v * a.ldo + d;
+            if constexpr (OT == GRWS_F32) {
+                float* o = static_cast<float*>(a.out) + at;
+                if (a.vec && d + 4 <= a.width) {
+                    *reinterpret_cast<float4_t*>(o) = acc[i][j] * alpha;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < a.width) o[e] = acc[i][j][e] * alpha;
+                }
+            } else {
+                uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+                uint16_t h[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = round16<OT>(acc[i][j][e] * alpha);
+                if (a.vec && d + 4 <= a.width) {
+                    *reinterpret_cast<u32x2_t*>(o) =
+                        u32x2_t{(uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16)};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < a.width) o[e] = h[e];
+                }
+            }
+        }
+    }
+}
+
+// dH of a piece: p are columns of W, q the rows, k the piece's classes, cut
+// into `splits` runs; each run adds to its own fp32 sums (piece after piece,
+// so the order is fixed)
+struct HiddenArgs {
+    Gemm g;
+    float* part;  // [splits][np][dp]
+    int64_t np, dp;
+    int32_t first;  // the first piece stores
+};
+
+template <int DT, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a) {
+    using C = Core<DT, true, false, BP, BQ, WP, WQ>;
+    constexpr int TP = C::TP, TQ = C::TQ;
+    GRWS_HEAD_LDS(C)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int tp, tq;
+    tile_of(a.g, tp, tq);
+    const int sp = blockIdx.y;
+    const int kb = (int)((int64_t)a.g.ksteps * sp / a.g.splits), ke = (int)((int64_t)a.g.ksteps * (sp + 1) / a.g.splits);
+    float4_t acc[TP][TQ];
+    C::run(a.g, tp, tq, kb, ke, s0, s1, acc);
+    float* out = a.part + sp * a.np * a.dp;
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < TP; ++i) {
+            const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
+            if (d >= a.dp) continue;
+            float4_t* o = reinterpret_cast<float4_t*>(out + row * a.dp + d);
+            *o = a.first ? acc[i][j] : *o + acc[i][j];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// small kernels
+// ---------------------------------------------------------------------------
+// A row counts when it has a target: a label in range, or a listed teacher
+// entry.  0: does not count, 1: counts, 2: bad input (counts as none).
+struct Targets {
+    const int64_t* labels;
+    const void* tindex;
+    const float* tlogit;
+    const int64_t* rows;
+    int64_t hidden_rows, classes;
+    int32_t k, i64;
+};
+
+__device__ __forceinline__ int64_t teacher_at(const Targets& t, int64_t i, int k) {
+    return t.i64 ? static_cast<const int64_t*>(t.tindex)[i * t.k + k]
+                 : (int64_t) static_cast<const int32_t*>(t.tindex)[i * t.k + k];
+}
+
+// an entry of weight zero (a logit of -inf) is not listed
+__device__ __forceinline__ bool teacher_listed(const Targets& t, int64_t i, int k, int64_t idx) {
+    return idx >= 0 && idx < t.classes && t.tlogit[i * t.k + k] != -INFINITY;
+}
+
+__device__ __forceinline__ int row_state(const Targets& t, int64_t i) {
+    const int64_t row = t.rows ? t.rows[i] : i;
+    if (row < 0 || row >= t.hidden_rows) return 2;
+    if (t.labels) {
+        const int64_t l = t.labels[i];
+        if (l == kIgnoreLabel) return 0;
+        return l >= 0 && l < t.classes ? 1 : 2;
+    }
+    int st = 0;
+    for (int k = 0; k < t.k; ++k) {
+        const int64_t idx = teacher_at(t, i, k);
+        if (idx < -1 || idx >= t.classes) return 2;
+        if (teacher_listed(t, i, k, idx)) st = 1;
+    }
+    return st;
+}
+
+// hidden[rows] in the layout the products read: np rows of dp elements (one
+// plane, or three for f32), zeros past n and the width and in rows that do
+// not count (what such a row holds, NaN too, stays out of every sum).
+// One wave per row.
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(256) void head_pack_hidden_kernel(Targets t, const T* __restrict__ hidden, int64_t ld,
+                                                               int64_t n, int64_t np, int64_t width, int64_t dp,
+                                                               uint16_t* __restrict__ out) {
+    const int lane = threadIdx.x & 63;
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= np) return;
+    const bool live = i < n && row_state(t, i) == 1;
+    const T* x = hidden + (live ? (t.rows ? t.rows[i] : i) * ld : 0);
+    for (int64_t c = lane; c < dp; c += 64) {
+        const bool in = live && c < width;
+        if constexpr (SPLIT) {
+            uint16_t a = 0, b = 0, d = 0;
+            if (in) split3(x[c], &a, &b, &d);
+            out[i * dp + c] = a;
+            out[(np + i) * dp + c] = b;
+            out[(2 * np + i) * dp + c] = d;
+        } else {
+            out[i * dp + c] = in ? __builtin_bit_cast(uint16_t, x[c]) : (uint16_t)0;
+        }
+    }
+}
+
+// weight rows v0.. of the piece likewise (`vp` rows)
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(256) void head_pack_weight_kernel(const T* __restrict__ w, int64_t ld, int64_t rows,
+                                                               int64_t vp, int64_t width, int64_t dp,
+                                                               uint16_t* __restrict__ out) {
+    const int lane = threadIdx.x & 63;
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= rows) return;
+    for (int64_t c = lane; c < dp; c += 64) {
+        if constexpr (SPLIT) {
+            uint16_t a = 0, b = 0, d = 0;
+            if (c < width) split3(w[i * ld + c], &a, &b, &d);
+            out[i * dp + c] = a;
+            out[(vp + i) * dp + c] = b;
+            out[(2 * vp + i) * dp + c] = d;
+        } else {
+            out[i * dp + c] = c < width ? __builtin_bit_cast(uint16_t, w[i * ld + c]) : (uint16_t)0;
+        }
+    }
+}
+
+// The teacher's probabilities and the student's logits at its entries: one
+// wave per row; 16 lanes share an entry's dot product (4 entries at once).
+// Reads n k rows of W; prob and y are 0 where an entry is not listed.
+template <typename T>
+__global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* __restrict__ hidden, int64_t ldh,
+                                                           const T* __restrict__ w, int64_t ldw, const T* bias,
+                                                           int64_t n, int64_t width, float inv_t, float c1,
+                                                           float* __restrict__ prob, float* __restrict__ y) {
+    const int lane = threadIdx.x & 63;
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= n) return;
+    const bool live = row_state(t, i) == 1;  // uniform over the wave
+    float m = -INFINITY;
+    for (int k = lane; k < t.k && live; k += 64)
+        if (teacher_listed(t, i, k, teacher_at(t, i, k))) m = fmaxf(m, t.tlogit[i * t.k + k] * inv_t);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
+    float s = 0.f;
+    for (int k = lane; k < t.k && live; k += 64)
+        if (teacher_listed(t, i, k, teacher_at(t, i, k))) s += expf(t.tlogit[i * t.k + k] * inv_t - m);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, kWave);
+    for (int k = lane; k < t.k; k += 64) {
+        const bool on = live && teacher_listed(t, i, k, teacher_at(t, i, k));
+        prob[i * t.k + k] = on ? expf(t.tlogit[i * t.k + k] * inv_t - m) / s : 0.f;
+    }
+    const T* h = hidden + (live ? (t.rows ? t.rows[i] : i) * ldh : 0);
+    for (int k0 = 0; k0 < t.k; k0 += 4) {
+        const int k = k0 + (lane >> 4);
+        int64_t idx = -1;
+        if (live && k < t.k) {
+            idx = teacher_at(t, i, k);
+            if (!teacher_listed(t, i, k, idx)) idx = -1;
+        }
+        float d = 0.f;
+        if (idx >= 0)
+            for (int64_t c = lane & 15; c < width; c += 16) d += to_float(h[c]) * to_float(w[idx * ldw + c]);
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) d += __shfl_xor(d, x, kWave);
+        if ((lane & 15) == 0 && k < t.k)
+            y[i * t.k + k] = idx >= 0 ? (d + (bias ? to_float(bias[idx]) : 0.f)) * c1 : 0.f;
+    }
+}
+
+// Joins the strips of 64 rows (8 waves take every eighth strip), then the
+// rows' losses; block partials of (loss, hits, counted rows, bad input).
+__global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2* __restrict__ part, int64_t strips,
+                                                        int32_t strip_classes, int64_t n, int64_t np,
+                                                        float temperature, const float* __restrict__ y,
+                                                        const float* __restrict__ prob,
+                                                        const int32_t* __restrict__ earlier, float* __restrict__ lse,
+                                                        float* __restrict__ row_loss, double* __restrict__ part_loss,
+                                                        long long* __restrict__ part_cnt) {
+    __shared__ float sm[8][64], ss[8][64];
+    __shared__ int sa[8][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    float m = -INFINITY, s = 0.f;
+    int first = 0x7fffffff;  // the first strip with the maximum
+    if (i < n) {
+#pragma unroll 4
+        for (int64_t k = wave; k < strips; k += 8) {
+            const float2 v = part[k * np + i];
+            if (v.x > m) {
+                s = s * __builtin_amdgcn_exp2f(m - v.x) + v.y;
+                m = v.x;
+                first = (int)k;
+            } else {
+                s += v.x == -INFINITY ? v.y : v.y * __builtin_amdgcn_exp2f(v.x - m);
+            }
+        }
+    }
+    sm[wave][lane] = m;
+    ss[wave][lane] = s;
+    sa[wave][lane] = first;
+    __syncthreads();
+    if (wave != 0) return;
+    for (int w = 1; w < 8; ++w) {
+        const float om = sm[w][lane], os = ss[w][lane];
+        if (om > m) {
+            s = s * __builtin_amdgcn_exp2f(m - om) + os;
+            m = om;
+            first = sa[w][lane];
+        } else {
+            s += om == -INFINITY ? os : os * __builtin_amdgcn_exp2f(om - m);
+            if (om == m && sa[w][lane] < first) first = sa[w][lane];
+        }
+    }
+    double loss = 0.0;
+    int hit = 0, valid = 0, bad = 0;
+    if (i < n) {
+        const int st = row_state(t, i);
+        const float l = m + log2f(s);
+        float r = 0.f;
+        if (st == 1) {
+            valid = 1;
+            if (t.labels) {
+                const float yl = y[i];
+                r = (l - yl) * kLn2;
+                hit = yl == m && !earlier[i] && first == (int)(t.labels[i] / strip_classes);
+            } else {
+                // an entry of probability zero says nothing of its class
+                // (whose logit may be -inf)
+                float a = 0.f;
+                for (int k = 0; k < t.k; ++k) {
+                    const float q = prob[i * t.k + k];
+                    if (!(q <= 0.f)) a += q * (logf(q) + (l - y[i * t.k + k]) * kLn2);
+                }
+                r = a * temperature * temperature;
+            }
+            loss = (double)r;
+        } else if (st == 2) {
+            bad = 1;
+            r = __int_as_float(0x7fc00000);
+        }
+        lse[i] = st == 1 ? l : INFINITY;
+        row_loss[i] = r;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        loss += __shfl_xor(loss, d, kWave);
+        hit += __shfl_xor(hit, d, kWave);
+        valid += __shfl_xor(valid, d, kWave);
+        bad |= __shfl_xor(bad, d, kWave);
+    }
+    if (lane == 0) {
+        part_loss[blockIdx.x] = loss;
+        part_cnt[3 * blockIdx.x] = hit;
+        part_cnt[3 * blockIdx.x + 1] = valid;
+        part_cnt[3 * blockIdx.x + 2] = bad;
+    }
+}
+
+// loss = sum / counted (NaN when no row counts or an input is bad); one
+// work-group, parts added in a fixed order
+__global__ __launch_bounds__(256) void head_finish_kernel(const double* __restrict__ part_loss,
+                                                          const long long* __restrict__ part_cnt, int64_t nparts,
+                                                          float* __restrict__ loss, int64_t* __restrict__ counts) {
+    __shared__ double sl[256];
+    __shared__ long long sc[256], sv[256], sb[256];
+    double L = 0.0;
+    long long C = 0, V = 0, B = 0;
+    for (int64_t k = threadIdx.x; k < nparts; k += 256) {
+        L += part_loss[k];
+        C += part_cnt[3 * k];
+        V += part_cnt[3 * k + 1];
+        B |= part_cnt[3 * k + 2];
+    }
+    sl[threadIdx.x] = L;
+    sc[threadIdx.x] = C;
+    sv[threadIdx.x] = V;
+    sb[threadIdx.x] = B;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    L = 0.0;
+    C = V = B = 0;
+    for (int t = 0; t < 256; ++t) {
+        L += sl[t];
+        C += sc[t];
+        V += sv[t];
+        B |= sb[t];
+    }
+    loss[0] = (B || V == 0) ? __int_as_float(0x7fc00000) : (float)(L / (double)V);
+    counts[0] = C;
+    counts[1] = V;
+    counts[2] = B;
+}
+
+// The factor of the gradient sums: dloss T / (counted gscale), or for a
+// gradient per row the largest |dloss| in place of dloss / counted, with
+// the rows' shares of it in row_scale (so that G stays within 16 bits' range)
+__global__ void head_alpha_kernel(const float* __restrict__ dloss, const int64_t* __restrict__ counts, int per_row,
+                                  float factor, float* __restrict__ alpha, const uint32_t* __restrict__ most) {
+    if (per_row) alpha[0] = __uint_as_float(*most) * factor;
+    else alpha[0] = counts[1] > 0 ? dloss[0] / (float)counts[1] * factor : 0.f;
+}
+
+__global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict__ dloss,
+                                                        const float* __restrict__ lse, int64_t n,
+                                                        uint32_t* __restrict__ most) {
+    // of non-negative floats the largest is the largest as an integer (a NaN
+    // above all): the order of the atomics does not matter
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    uint32_t m = i < n && lse[i] != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const uint32_t o = __shfl_xor(m, d, kWave);
+        m = o > m ? o : m;
+    }
+    if ((threadIdx.x & 63) == 0 && m) atomicMax(most, m);
+}
+
+__global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __restrict__ dloss, int64_t n,
+                                                             const uint32_t* __restrict__ most,
+                                                             float* __restrict__ scale) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const float m = __uint_as_float(*most);
+    scale[i] = m > 0.f ? dloss[i] / m : 0.f * m;
+}
+
+// G at the targets: the rounded p - q.  A class listed twice by a teacher
+// counts with both probabilities, written by its first entry.
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const float* __restrict__ lse,
+                                                            const float* __restrict__ y,
+                                                            const float* __restrict__ prob,
+                                                            const float* __restrict__ row_scale, float gscale,
+                                                            int64_t n, int64_t v0, int64_t vc, uint16_t* G,
+                                                            int64_t ldg, int64_t plane) {
+    const int K = t.labels ? 1 : t.k;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= n * K) return;
+    const int64_t i = at / K;
+    const int k = (int)(at % K);
+    if (lse[i] == INFINITY) return;
+    const int64_t v = t.labels ? t.labels[i] : teacher_at(t, i, k);
+    if (v < v0 || v >= v0 + vc) return;
+    float q = 1.f;
+    if (!t.labels) {
+        q = prob[at];
+        for (int o = 0; o < K; ++o)
+            if (o != k && teacher_at(t, i, o) == v) {
+                if (o < k) return;
+                q += prob[i * K + o];
+            }
+        // an unlisted entry (a teacher's -inf) has no logit kept
+        if (!teacher_listed(t, i, k, v)) {
+            for (int o = k + 1; o < K; ++o)
+                if (teacher_at(t, i, o) == v && teacher_listed(t, i, o, v)) {
+                    const float s = row_scale ? row_scale[i] * gscale : gscale;
+                    store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[i * K + o] - lse[i]) - q) * s);
+                    return;
+                }
+            return;
+        }
+    }
+    const float s = row_scale ? row_scale[i] * gscale : gscale;
+    store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[at] - lse[i]) - q) * s);
+}
+
+// Column sums of a piece of G over runs of 256 rows: 4 waves of 64 rows,
+// 8 columns a lane.
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __restrict__ G, int64_t ldg,
+                                                             int64_t plane, int64_t np, int64_t vp,
+                                                             float* __restrict__ part) {
+    __shared__ float red[4][512];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
+    const int64_t r0 = (int64_t)blockIdx.y * 256 + wave * 64;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < vp) {
+        for (int64_t r = r0; r < r0 + 64 && r < np; ++r) {
+#pragma unroll
+            for (int z = SPLIT ? 2 : 0; z >= 0; --z) {
+                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(G + z * plane + r * ldg + c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint16_t h = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+                    if constexpr (DT == GRWS_F16) s[e] += (float)__builtin_bit_cast(_Float16, h);
+                    else s[e] += from_top16(h);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[wave][lane * 8 + e] = s[e];
+    __syncthreads();
+    for (int x = threadIdx.x; x < 512; x += 256) {
+        const int64_t col = (int64_t)blockIdx.x * 512 + x;
+        if (col < vp) part[blockIdx.y * vp + col] = (red[0][x] + red[1][x]) + (red[2][x] + red[3][x]);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void head_bias_kernel(const float* __restrict__ part, int64_t nparts, int64_t vp,
+                                                        int64_t vc, const float* __restrict__ alpha,
+                                                        T* __restrict__ out) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= vc) return;
+    float s = 0.f;
+    for (int64_t k = 0; k < nparts; ++k) s += part[k * vp + c];
+    out[c] = from_float<T>(s * *alpha);
+}
+
+// dH rows: the splits' sums in order, times alpha, to the rows they belong to
+template <typename T>
+__global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __restrict__ part, int64_t splits,
+                                                              int64_t np, int64_t dp, int64_t n, int64_t width,
+                                                              const int64_t* __restrict__ rows, int64_t hidden_rows,
+                                                              const float* __restrict__ alpha, T* __restrict__ out,
+                                                              int64_t ldo) {
+    const int64_t i = blockIdx.x;
+    const int64_t row = rows ? rows[i] : i;
+    if (row < 0 || row >= hidden_rows) return;
+    const float a = *alpha;
+    for (int64_t d = threadIdx.x; d < width; d += 256) {
+        float s = 0.f;
+        for (int64_t k = 0; k < splits; ++k) s += part[(k * np + i) * dp + d];
+        out[row * ldo + d] = from_float<T>(s * a);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
+int64_t ceil_div(int64_t x, int64_t a) { return (x + a - 1) / a; }
+
+constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // G of a piece, and a packed piece of W
+
+// Sizes of a call, the same for the workspace query and the launch.
+struct Shape {
+    int64_t n, D, V;
+    int planes, esz;
+    bool split;    // f32 operands in three planes
+    bool pack_w;   // W goes through a packed copy
+    int tile;      // 256 or 128
+    int64_t np, dp, vp;
+    int64_t strips, strip_classes;
+};
+
+bool weight_in_place(const grws_head* h) {
+    return h->dtype != GRWS_F32 && h->ld_weight % 8 == 0 && h->width % 8 == 0 &&
+           reinterpret_cast<uintptr_t>(h->weight) % 16 == 0;
+}
+
+Shape shape_of(const grws_head* h, bool backward) {
+    Shape s{};
+    s.n = h->n;
+    s.D = h->width;
+    s.V = h->classes;
+    s.split = h->dtype == GRWS_F32;
+    s.planes = s.split ? 3 : 1;
+    s.pack_w = !weight_in_place(h);
+    s.tile = s.n > 128 && s.V > 128 && ceil_div(s.n, 256) * ceil_div(s.V, 256) >= 256 ? 256 : 128;
+    s.np = up(s.n, s.tile);
+    s.dp = up(s.D, kK);
+    int64_t vp = up(s.V, s.tile);
+    if (backward) {
+        const int64_t most = kPieceBytes / (2 * s.planes * s.np) / s.tile * s.tile;
+        if (vp > most) vp = most < s.tile ? s.tile : most;
+    }
+    if (s.pack_w) {
+        const int64_t most = kPieceBytes / (2 * s.planes * s.dp) / s.tile * s.tile;
+        if (vp > most) vp = most < s.tile ? s.tile : most;
+    }
+    s.vp = vp;
+    s.strip_classes = s.tile / 2;
+    s.strips = up(s.V, s.tile) / s.strip_classes;
+    return s;
+}
+
+int check_head(const grws_head* h) {
+    GRWS_CHECK_ARG(h != nullptr, "head: null description");
+    if (h->dtype != GRWS_F32 && h->dtype != GRWS_F16 && h->dtype != GRWS_BF16)
+        return set_error(GRWS_E_DTYPE, "head: unsupported dtype %d", h->dtype);
+    GRWS_CHECK_ARG(h->n >= 0 && h->n <= INT32_MAX && h->hidden_rows >= 0, "head: bad row count");
+    GRWS_CHECK_ARG(h->width > 0 && h->width <= 65536, "head: width must be 1..65536");
+    GRWS_CHECK_ARG(h->classes > 0 && h->classes <= INT32_MAX - 1024, "head: bad class count");
+    GRWS_CHECK_ARG(h->ld_hidden >= h->width && h->ld_weight >= h->width && h->ld_hidden <= (1 << 21) &&
+                       h->ld_weight <= (1 << 21),
+                   "head: leading dimensions must be the width at least and 2^21 at most");
+    GRWS_CHECK_ARG(h->k >= 0 && h->k <= 1024, "head: at most 1024 teacher entries a row");
+    GRWS_CHECK_ARG(h->temperature > 0.f && h->temperature < INFINITY, "head: the temperature must be positive");
+    if (h->n > 0) {
+        GRWS_CHECK_ARG(h->hidden && h->weight, "head: null pointer");
+        if (h->k == 0) {
+            GRWS_CHECK_ARG(h->labels != nullptr, "head: null labels");
+            GRWS_CHECK_ARG(h->temperature == 1.f, "head: labels take no temperature");
+        } else {
+            GRWS_CHECK_ARG(h->teacher_index && h->teacher_logits && !h->labels, "head: null teacher lists");
+        }
+    }
+    return GRWS_OK;
+}
+
+Targets targets_of(const grws_head* h) {
+    return Targets{h->labels, h->teacher_index, h->teacher_logits, h->rows, h->hidden_rows, h->classes,
+                   h->k, h->index_is_i64};
+}
+
+struct FwdSpace {
+    uint16_t *hp, *wp;
+    float2* part;
+    int32_t* earlier;
+    double* pl;
+    long long* pc;
+};
+
+template <typename A>
+void fwd_space(A& a, const Shape& s, FwdSpace* f) {
+    auto take = [&](auto*& p, int64_t n) {
+        using T = std::remove_reference_t<decltype(*p)>;
+        if constexpr (std::is_same_v<A, Sizer>) a.template take<T>((size_t)n);
+        else p = a.template take<T>((size_t)n);
+    };
+    take(f->hp, s.planes * s.np * s.dp);
+    if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
+    take(f->part, s.strips * s.np);
+    take(f->earlier, s.n);
+    take(f->pl, ceil_div(s.n, 64));
+    take(f->pc, 3 * ceil_div(s.n, 64));
+}
+
+struct BwdShape {
+    int64_t splits, ldg;
+};
+
+BwdShape bwd_shape(const Shape& s) {
+    BwdShape b{};
+    b.ldg = s.vp;
+    // enough work-groups for dH: its tiles times runs of at least 16 stages
+    const int64_t tiles = ceil_div(s.np, s.tile) * ceil_div(s.dp, s.tile);
+    int64_t sp = ceil_div(512, tiles);
+    const int64_t most = s.vp / kK / 16;
+    if (sp > most) sp = most;
+    b.splits = sp < 1 ? 1 : sp;
+    return b;
+}
+
+struct BwdSpace {
+    uint16_t *hp, *wp, *G;
+    float *part, *bias, *alpha, *scale;
+    uint32_t* most;
+};
+
+template <typename A>
+void bwd_space(A& a, const Shape& s, const BwdShape& b, BwdSpace* f) {
+    auto take = [&](auto*& p, int64_t n) {
+        using T = std::remove_reference_t<decltype(*p)>;
+        if constexpr (std::is_same_v<A, Sizer>) a.template take<T>((size_t)n);
+        else p = a.template take<T>((size_t)n);
+    };
+    take(f->hp, s.planes * s.np * s.dp);
+    if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
+    take(f->G, s.planes * s.np * b.ldg);
+    take(f->part, b.splits * s.np * s.dp);
+    take(f->bias, ceil_div(s.np, 256) * s.vp);
+    take(f->alpha, 1);
+    take(f->scale, s.n);
+    take(f->most, 1);
+}
+
+int pack_hidden(const grws_head* h, const Shape& s, const Targets& t, uint16_t* hp, hipStream_t stream) {
+    const dim3 grid((unsigned)ceil_div(s.np, 4));
+    if (s.split)
+        hipLaunchKernelGGL((head_pack_hidden_kernel<float, true>), grid, dim3(256), 0, stream, t,
+                           static_cast<const float*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, hp);
+    else
+        hipLaunchKernelGGL((head_pack_hidden_kernel<uint16_t, false>), grid, dim3(256), 0, stream, t,
+                           static_cast<const uint16_t*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, hp);
+    GRWS_LAUNCH_CHECK();
+    return GRWS_OK;
+}
+
+// The piece's rows of W as an operand, packed first where they have to be.
+int weight_piece(const grws_head* h, const Shape& s, int64_t v0, int64_t vc, uint16_t* wp, bool strided, Opnd* o,
+                 bool pack, hipStream_t stream) {
+    if (!s.pack_w) {
+        const char* p = static_cast<const char*>(h->weight) + v0 * h->ld_weight * 2;
+        *o = strided ? Opnd{p, h->ld_weight * 2, 0, s.D, vc} : Opnd{p, h->ld_weight * 2, 0, vc, s.D};
+        return GRWS_OK;
+    }
+    if (pack) {
+        const dim3 grid((unsigned)ceil_div(vc, 4));
+        if (s.split)
+            hipLaunchKernelGGL((head_pack_weight_kernel<float, true>), grid, dim3(256), 0, stream,
+                               static_cast<const float*>(h->weight) + v0 * h->ld_weight, h->ld_weight, vc, s.vp, s.D,
+                               s.dp, wp);
+        else
+            hipLaunchKernelGGL((head_pack_weight_kernel<uint16_t, false>), grid, dim3(256), 0, stream,
+                               static_cast<const uint16_t*>(h->weight) + v0 * h->ld_weight, h->ld_weight, vc, s.vp,
+                               s.D, s.dp, wp);
+        GRWS_LAUNCH_CHECK();
+    }
+    const char* p = reinterpret_cast<const char*>(wp);
+    const int64_t plane = s.vp * s.dp * 2;
+    *o = strided ? Opnd{p, s.dp * 2, plane, s.dp, vc} : Opnd{p, s.dp * 2, plane, vc, s.dp};
+    return GRWS_OK;
+}
+
+Opnd hidden_operand(const Shape& s, const uint16_t* hp, bool strided) {
+    const char* p = reinterpret_cast<const char*>(hp);
+    const int64_t plane = s.np * s.dp * 2;
+    return strided ? Opnd{p, s.dp * 2, plane, s.dp, s.np} : Opnd{p, s.dp * 2, plane, s.np, s.dp};
+}
+
+Gemm gemm_of(const Shape& s, const Opnd& P, const Opnd& Q, int64_t np, int64_t nq, int64_t k, int64_t splits) {
+    return Gemm{P, Q, s.split ? 6 : 1, (int32_t)ceil_div(k, kK), (int32_t)ceil_div(np, s.tile),
+                (int32_t)ceil_div(nq, s.tile), (int32_t)splits};
+}
+
+// KERNEL<..., BP, BQ, WP, WQ> at the call's tile
+#define GRWS_HEAD_LAUNCH(NAME, ARGS, ...)                                                                            \
+    do {                                                                                                             \
+        GRWS_CHECK_ARG((int64_t)ARGS.g.tp * ARGS.g.tq < INT32_MAX, "head: more than 2^31 tiles");                    \
+        const dim3 grid_((unsigned)(ARGS.g.tp * ARGS.g.tq), (unsigned)ARGS.g.splits);                                \
+        if (s.tile == 256)                                                                                           \
+            hipLaunchKernelGGL((NAME<__VA_ARGS__, 256, 256, 2, 4>), grid_, dim3(512), 0, stream, ARGS);              \
+        else                                                                                                         \
+            hipLaunchKernelGGL((NAME<__VA_ARGS__, 128, 128, 2, 2>), grid_, dim3(256), 0, stream, ARGS);              \
+        GRWS_LAUNCH_CHECK();                                                                                         \
+    } while (0)
+
+}  // namespace
+}  // namespace grws
+
+using namespace grws;
+
+extern "C" size_t grws_head_fwd_workspace_bytes(const grws_head* h) {
+    if (check_head(h) != GRWS_OK || h->n == 0) return 0;
+    Sizer z;
+    FwdSpace f{};
+    fwd_space(z, shape_of(h, false), &f);
+    return z.used;
+}
+
+extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit, float* target_prob,
+                             float* row_loss, float* loss, int64_t* counts, void* workspace, size_t workspace_bytes,
+                             void* stream_) {
+    clear_error();
+    hipStream_t stream = as_stream(stream_);
+    GRWS_TRY(check_head(h));
+    GRWS_CHECK_ARG(loss && counts, "head: null output");
+    if (h->n == 0) {
+        hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(256), 0, stream, nullptr, nullptr, 0, loss, counts);
+        GRWS_LAUNCH_CHECK();
+        return GRWS_OK;
+    }
+    GRWS_CHECK_ARG(lse && target_logit && row_loss && (h->k == 0 || target_prob), "head: null output");
+    const Shape s = shape_of(h, false);
+    const Targets t = targets_of(h);
+    Carver cv(workspace, workspace_bytes);
+    FwdSpace f{};
+    fwd_space(cv, s, &f);
+    if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
+    const float c1 = kLog2e / h->temperature;
+    GRWS_TRY(pack_hidden(h, s, t, f.hp, stream));
+    for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
+        const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
+        Opnd W;
+        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
+        StatsArgs a{gemm_of(s, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, 1), v0, s.V, s.n, s.np, c1,
+                    h->bias, h->dtype, h->labels, f.part, target_logit, f.earlier};
+        if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(head_stats_kernel, a, GRWS_F16);
+        else GRWS_HEAD_LAUNCH(head_stats_kernel, a, GRWS_BF16);
+    }
+    if (h->k > 0) {
+        const dim3 grid((unsigned)ceil_div(s.n, 4));
+#define GRWS_HEAD_TARGETS(T)                                                                                         \
+    hipLaunchKernelGGL(head_targets_kernel<T>, grid, dim3(256), 0, stream, t, static_cast<const T*>(h->hidden),      \
+                       h->ld_hidden, static_cast<const T*>(h->weight), h->ld_weight, static_cast<const T*>(h->bias), \
+                       s.n, s.D, 1.f / h->temperature, c1, target_prob, target_logit)
+        if (h->dtype == GRWS_F32) GRWS_HEAD_TARGETS(float);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_TARGETS(_Float16);
+        else GRWS_HEAD_TARGETS(__hip_bfloat16);
+#undef GRWS_HEAD_TARGETS
+        GRWS_LAUNCH_CHECK();
+    }
+    const int64_t blocks = ceil_div(s.n, 64);
+    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part, ceil_div(s.V, s.strip_classes),
+                       (int32_t)s.strip_classes, s.n, s.np, h->temperature, target_logit, target_prob, f.earlier, lse,
+                       row_loss, f.pl, f.pc);
+    GRWS_LAUNCH_CHECK();
+    hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(256), 0, stream, f.pl, f.pc, blocks, loss, counts);
+    GRWS_LAUNCH_CHECK();
+    return GRWS_OK;
+}
+
+extern "C" size_t grws_head_bwd_workspace_bytes(const grws_head* h) {
+    if (check_head(h) != GRWS_OK || h->n == 0) return 0;
+    Sizer z;
+    BwdSpace f{};
+    const Shape s = shape_of(h, true);
+    bwd_space(z, s, bwd_shape(s), &f);
+    return z.used;
+}
+
+extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* target_logit,
+                             const float* target_prob, const int64_t* counts, const float* dloss, int32_t per_row,
+                             void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw, void* d_bias,
+                             void* workspace, size_t workspace_bytes, void* stream_) {
+    clear_error();
+    hipStream_t stream = as_stream(stream_);
+    GRWS_TRY(check_head(h));
+    GRWS_CHECK_ARG((!d_hidden || ld_dh >= h->width) && (!d_weight || ld_dw >= h->width),
+                   "head: gradients' leading dimensions must be the width at least");
+    if (h->n == 0) {
+        const size_t e = dtype_size(h->dtype);
+        if (d_weight)
+            for (int64_t v = 0; v < (ld_dw == h->width ? 1 : h->classes); ++v)
+                GRWS_TRY(fill_bytes_zero(static_cast<char*>(d_weight) + v * ld_dw * e,
+                                         (ld_dw == h->width ? h->classes : 1) * h->width * e, stream));
+        if (d_bias) GRWS_TRY(fill_bytes_zero(d_bias, h->classes * e, stream));
+        return GRWS_OK;
+    }
+    GRWS_CHECK_ARG(lse && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
+    if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
+    const Shape s = shape_of(h, true);
+    const BwdShape b = bwd_shape(s);
+    const Targets t = targets_of(h);
+    Carver cv(workspace, workspace_bytes);
+    BwdSpace f{};
+    bwd_space(cv, s, b, &f);
+    if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
+    const float c1 = kLog2e / h->temperature;
+    const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
+    const float* row_scale = nullptr;
+    if (per_row) {
+        GRWS_TRY(fill_i32(reinterpret_cast<int32_t*>(f.most), 1, 0, stream));
+        const dim3 grid((unsigned)ceil_div(s.n, 256));
+        hipLaunchKernelGGL(head_most_kernel, grid, dim3(256), 0, stream, dloss, lse, s.n, f.most);
+        GRWS_LAUNCH_CHECK();
+        hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, s.n, f.most, f.scale);
+        GRWS_LAUNCH_CHECK();
+        row_scale = f.scale;
+    }
+    hipLaunchKernelGGL(head_alpha_kernel, dim3(1), dim3(1), 0, stream, dloss, counts, per_row,
+                       h->temperature / gscale, f.alpha, f.most);
+    GRWS_LAUNCH_CHECK();
+    GRWS_TRY(pack_hidden(h, s, t, f.hp, stream));
+    const int64_t plane = s.np * b.ldg;
+    const size_t esz = dtype_size(h->dtype);
+    for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
+        const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
+        const int64_t vt = up(vc, s.tile);
+        Opnd W;
+        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
+        GradArgs a{gemm_of(s, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, 1), v0, s.V, s.n, c1, h->bias,
+                   h->dtype, lse, row_scale, gscale, f.G, b.ldg, plane};
+        const dim3 sgrid((unsigned)ceil_div(s.n * (h->k ? h->k : 1), 256));
+#define GRWS_HEAD_SUB(DT, SP)                                                                                       \
+    hipLaunchKernelGGL((head_subtract_kernel<DT, SP>), sgrid, dim3(256), 0, stream, t, lse, target_logit,           \
+                       target_prob, row_scale, gscale, s.n, v0, vc, f.G, b.ldg, plane)
+        if (s.split) {
+            GRWS_HEAD_LAUNCH(head_grad_kernel, a, GRWS_BF16, true);
+            GRWS_HEAD_SUB(GRWS_BF16, true);
+        } else if (h->dtype == GRWS_F16) {
+            GRWS_HEAD_LAUNCH(head_grad_kernel, a, GRWS_F16, false);
+            GRWS_HEAD_SUB(GRWS_F16, false);
+        } else {
+            GRWS_HEAD_LAUNCH(head_grad_kernel, a, GRWS_BF16, false);
+            GRWS_HEAD_SUB(GRWS_BF16, false);
+        }
+#undef GRWS_HEAD_SUB
+        GRWS_LAUNCH_CHECK();
+        const char* gp = reinterpret_cast<const char*>(f.G);
+        if (d_bias) {
+            const int64_t nparts = ceil_div(s.np, 256);
+            const dim3 grid((unsigned)ceil_div(vt, 512), (unsigned)nparts);
+            if (s.split)
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, true>), grid, dim3(256), 0, stream, f.G, b.ldg,
+                                   plane, s.np, vt, f.bias);
+            else if (h->dtype == GRWS_F16)
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_F16, false>), grid, dim3(256), 0, stream, f.G, b.ldg,
+                                   plane, s.np, vt, f.bias);
+            else
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, false>), grid, dim3(256), 0, stream, f.G, b.ldg,
+                                   plane, s.np, vt, f.bias);
+            GRWS_LAUNCH_CHECK();
+            const dim3 cg((unsigned)ceil_div(vc, 256));
+            char* db = static_cast<char*>(d_bias) + v0 * esz;
+#define GRWS_HEAD_BIAS(T) \
+    hipLaunchKernelGGL(head_bias_kernel<T>, cg, dim3(256), 0, stream, f.bias, nparts, vt, vc, f.alpha, \
+                       reinterpret_cast<T*>(db))
+            if (h->dtype == GRWS_F32) GRWS_HEAD_BIAS(float);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS(_Float16);
+            else GRWS_HEAD_BIAS(__hip_bfloat16);
+#undef GRWS_HEAD_BIAS
+            GRWS_LAUNCH_CHECK();
+        }
+        if (d_weight) {
+            char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
+            const int32_t vec = reinterpret_cast<uintptr_t>(d_weight) % (4 * esz) == 0 && ld_dw % 4 == 0;
+            const Opnd G{gp, b.ldg * 2, plane * 2, b.ldg, s.np};
+            WeightArgs w{gemm_of(s, hidden_operand(s, f.hp, true), G, s.D, vc, s.np, 1), f.alpha, out, ld_dw, vc,
+                         s.D, vec};
+            if (s.split) GRWS_HEAD_LAUNCH(head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(head_dweight_kernel, w, GRWS_F16, GRWS_F16);
+            else GRWS_HEAD_LAUNCH(head_dweight_kernel, w, GRWS_BF16, GRWS_BF16);
+        }
+        if (d_hidden) {
+            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, false, stream));
+            const Opnd G{gp, b.ldg * 2, plane * 2, s.np, vt};
+            HiddenArgs d{gemm_of(s, W, G, s.dp, s.np, vc, b.splits), f.part, s.np, s.dp, v0 == 0};
+            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(head_dhidden_kernel, d, GRWS_F16);
+            else GRWS_HEAD_LAUNCH(head_dhidden_kernel, d, GRWS_BF16);
+        }
+    }
+    if (d_hidden) {
+#define GRWS_HEAD_DH(T)                                                                                              \
+    hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.part, b.splits, s.np, \
+                       s.dp, s.n, s.D, h->rows, h->hidden_rows, f.alpha, static_cast<T*>(d_hidden), ld_dh)
+        if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
+        else GRWS_HEAD_DH(__hip_bfloat16);
+#undef GRWS_HEAD_DH
+        GRWS_LAUNCH_CHECK();
+    }
+    return GRWS_OK;
+}

@@ -1,0 +1,87 @@
+"""Classifier over many classes fused with its loss (csrc/head.hip).
+
+``linear_cross_entropy`` is ``F.cross_entropy(F.linear(hidden[rows], weight,
+bias), labels)`` and ``linear_distill`` the divergence of the same logits
+from a teacher's top logits (``core.top_logits`` makes the lists).  The
+logits [n, classes] are never kept: the forward reduces them in the
+product's epilogue, the backward makes them again piece by piece of the
+classes.
+
+Under autocast hidden, weight and bias are taken in the autocast dtype, as
+``F.linear`` takes them.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd import Function
+
+from ..core import ops as _ops
+
+_REDUCTIONS = ("mean", "none")
+
+
+class _Head(Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, rows, labels, teacher_index, teacher_logits, temperature, per_row):
+        call = _ops.HeadCall(hidden, weight, bias, rows, labels, teacher_index, teacher_logits, temperature)
+        loss, row_loss, counts, saved = _ops.head_fwd(call)
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(hidden, weight, bias, rows, labels, teacher_index, teacher_logits, counts, *saved)
+            ctx.temperature = temperature
+        ctx.mark_non_differentiable(counts)
+        return (row_loss if per_row else loss), counts
+
+    @staticmethod
+    def backward(ctx, dloss, _dcounts):
+        hidden, weight, bias, rows, labels, index, logits, counts, *saved = ctx.saved_tensors
+        call = _ops.HeadCall(hidden, weight, bias, rows, labels, index, logits, ctx.temperature)
+        grads = _ops.head_bwd(call, saved, counts, dloss, ctx.needs_input_grad[:3])
+        return (*grads, None, None, None, None, None, None)
+
+
+def _apply(hidden, weight, bias, rows, labels, index, logits, temperature, reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {_REDUCTIONS} (got {reduction!r})")
+    if torch.is_autocast_enabled("cuda") and hidden.is_cuda:
+        dt = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(dt), weight.to(dt)
+        bias = bias.to(dt) if bias is not None else None
+    with torch.autocast("cuda", enabled=False):
+        return _Head.apply(hidden, weight, bias, rows, labels, index, logits, float(temperature),
+                           reduction == "none")
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                         bias: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None,
+                         reduction: str = "mean"):
+    """(loss, counts) of softmax cross entropy of hidden[rows] @ weight.T +
+    bias against labels.
+
+    hidden [N, D], weight [V, D], bias [V] (one dtype of f32, f16, bf16),
+    labels int64 [n] (-100: the row does not count), rows int64 [n], distinct
+    (None = the first n rows).  reduction "mean": the f32 mean over counted
+    rows, NaN when none counts or a label or row id is out of range; "none":
+    f32 [n], 0 for rows that do not count.  counts: int64 [3] on the device,
+    {rows whose label is the first largest logit, counted rows, bad input}.
+    """
+    return _apply(hidden, weight, bias, rows, labels, None, None, 1.0, reduction)
+
+
+def linear_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_index: torch.Tensor,
+                   teacher_logits: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   rows: Optional[torch.Tensor] = None, temperature: float = 1.0, reduction: str = "mean"):
+    """(loss, counts) of T^2 KL(softmax(teacher / T) || softmax(z / T)) with
+    z = hidden[rows] @ weight.T + bias and the teacher's softmax over its
+    listed classes.
+
+    teacher_index int32 or int64 [n, k] (-1: no entry), teacher_logits
+    [n, k] (-inf: no entry); a row without entries does not count.  The other
+    arguments and reduction as in linear_cross_entropy.  counts: int64 [2] on
+    the device, {counted rows, bad input}.  No gradient reaches the teacher.
+    """
+    if teacher_index is None or teacher_logits is None:
+        raise ValueError("linear_distill: teacher_index and teacher_logits are required")
+    loss, counts = _apply(hidden, weight, bias, rows, None, teacher_index, teacher_logits, temperature, reduction)
+    return loss, counts[1:]

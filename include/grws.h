@@ -822,6 +822,69 @@ int grws_cross_entropy_bwd(const void* logits, int32_t dtype, int64_t ld, int64_
                            int32_t grad_dtype, int64_t ldg, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Classifier over many classes fused with its loss: z = H W^T + b of n rows */
+/* is never kept.  No counterpart in the reference, whose loss               */
+/* (helper/engine.py:22-41) takes logits in memory.                          */
+/*                                                                           */
+/* H: hidden [hidden_rows x ld_hidden], the rows `rows` (int64 [n], distinct; */
+/* NULL = rows 0..n-1); W: weight [classes x ld_weight]; bias [classes] or   */
+/* NULL; all in `dtype`, unit column stride, leading dimensions in elements  */
+/* (at most 2^21).  Width at most 65,536.  Targets, one of                   */
+/*   k = 0: labels int64 [n], -100 ignored; temperature 1;                   */
+/*   k > 0: a teacher's logits f32 [n x k] of the classes teacher_index      */
+/*     (int32, or int64 with index_is_i64) [n x k], k <= 1024, and a         */
+/*     temperature T.  Index -1 (or a logit of -inf) lists nothing; a class  */
+/*     listed twice counts with both probabilities.                          */
+/* Losses: cross entropy lse_i - z_i,label; distillation T^2 KL(softmax of   */
+/* the listed teacher logits / T || softmax(z_i / T)).                       */
+/*                                                                           */
+/* Forward, no sync: lse f32 [n] (log2 of the sum of 2^(z log2(e) / T), +inf */
+/* for rows that do not count) and target_logit f32 [n * max(k, 1)],         */
+/* target_prob f32 [n x k] (k > 0), which the backward takes; row_loss f32   */
+/* [n] (0 for rows that do not count, NaN for bad input); loss f32 scalar,   */
+/* the mean over counted rows (NaN when none counts or an input is bad: a    */
+/* label, class index or row id out of range); counts int64 [3] = {rows      */
+/* whose label is the first largest logit (k = 0), counted rows, bad input}. */
+/* Backward of dloss (f32 scalar of the mean, or with per_row [n] of         */
+/* row_loss): d_hidden (rows of `rows`; zero the others first), d_weight and */
+/* d_bias in `dtype`; NULL skips one.  A row that does not count reaches no  */
+/* gradient, whatever it holds.  Same inputs, same bits.                     */
+/* ------------------------------------------------------------------------ */
+typedef struct grws_head {
+    const void* hidden;
+    const void* weight;
+    const void* bias;
+    const int64_t* rows;
+    const int64_t* labels;
+    const void* teacher_index;
+    const float* teacher_logits;
+    int64_t ld_hidden, ld_weight, hidden_rows;
+    int64_t n, width, classes;
+    int32_t dtype, k, index_is_i64;
+    float temperature;
+} grws_head;
+
+size_t grws_head_fwd_workspace_bytes(const grws_head* head);
+int grws_head_fwd(const grws_head* head, float* lse, float* target_logit, float* target_prob, float* row_loss,
+                  float* loss, int64_t* counts, void* workspace, size_t workspace_bytes, void* stream);
+size_t grws_head_bwd_workspace_bytes(const grws_head* head);
+int grws_head_bwd(const grws_head* head, const float* lse, const float* target_logit, const float* target_prob,
+                  const int64_t* counts, const float* dloss, int32_t per_row, void* d_hidden, int64_t ld_dh,
+                  void* d_weight, int64_t ld_dw, void* d_bias, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* The k largest logits of each row of logits [rows x ld], largest first,   */
+/* with their classes: values [rows x k] in dtype, index int32 [rows x k].  */
+/* Of equal logits the lowest class comes first; NaN counts as the largest. */
+/* 1 <= k <= min(classes, 1024).  Rows of any alignment.  A teacher's lists */
+/* for grws_head.                                                           */
+/* ------------------------------------------------------------------------ */
+size_t grws_top_logits_workspace_bytes(int64_t rows, int64_t classes, int32_t k);
+int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t classes, int32_t k,
+                    void* values, int32_t* index, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Measurement only: no counterpart in the reference.  The random row-      */
 /* gather ceiling that bounds the SpMM's X reads, for benchmark reports.    */
 /* n_idx row indices (int32, a multiple of 8; values outside [0, rows)      */
