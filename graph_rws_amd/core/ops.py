@@ -1891,7 +1891,7 @@ def head_fwd(call: HeadCall):
     rows, bad input}, saved) of a HeadCall (csrc/head.hip); no host sync."""
     dev = call.hidden.device
     n, k = call.n, call.k
-    f = torch.empty(1 + n * (2 + max(k, 1) + k), dtype=torch.float32, device=dev)
+    f = torch.empty(1 + n * (2 + max(k, 1) + 2 * k), dtype=torch.float32, device=dev)
     loss, row_loss, lse = f[0], f[1:1 + n], f[1 + n:1 + 2 * n]
     logit = f[1 + 2 * n:1 + 2 * n + n * max(k, 1)]
     prob = f[1 + 2 * n + n * max(k, 1):] if k else None

@@ -473,13 +473,17 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
     }
 }
 
-// dW rows of a piece: p are columns of H, q the piece's classes, k the rows
+// dW rows of a piece: p are columns of H, q the piece's classes, k the rows,
+// cut into `splits` runs when the tiles alone leave CUs idle (their fp32 sums
+// are added in order by head_weight_out_kernel)
 struct WeightArgs {
     Gemm g;
     const float* alpha;
     void* out;  // first class of the piece
     int64_t ldo, classes, width;  // classes of the piece
     int32_t vec;  // rows of the output take 4-element stores
+    float* part;  // [splits][vp][dp], with splits > 1
+    int64_t vp, dp;
 };
 
 template <int DT, int OT, int BP, int BQ, int WP, int WQ>
@@ -490,8 +494,23 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int tp, tq;
     tile_of(a.g, tp, tq);
+    const int sp = blockIdx.y;
+    const int kb = (int)((int64_t)a.g.ksteps * sp / a.g.splits), ke = (int)((int64_t)a.g.ksteps * (sp + 1) / a.g.splits);
     float4_t acc[TP][TQ];
-    C::run(a.g, tp, tq, 0, a.g.ksteps, s0, s1, acc);
+    C::run(a.g, tp, tq, kb, ke, s0, s1, acc);
+    if (a.g.splits > 1) {
+        float* out = a.part + sp * a.vp * a.dp;
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) {
+            const int64_t v = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < TP; ++i) {
+                const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
+                if (d < a.dp && v < a.classes) *reinterpret_cast<float4_t*>(out + v * a.dp + d) = acc[i][j];
+            }
+        }
+        return;
+    }
     const float alpha = *a.alpha;
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
@@ -589,7 +608,10 @@ __device__ __forceinline__ bool teacher_listed(const Targets& t, int64_t i, int 
     return idx >= 0 && idx < t.classes && t.tlogit[i * t.k + k] != -INFINITY;
 }
 
-__device__ __forceinline__ int row_state(const Targets& t, int64_t i) {
+// `lanes` lanes of a wave, of which this is `sub`, ask together (all of them
+// with the same i); the answer is the same in each.
+template <int LANES>
+__device__ __forceinline__ int row_state(const Targets& t, int64_t i, int sub) {
     const int64_t row = t.rows ? t.rows[i] : i;
     if (row < 0 || row >= t.hidden_rows) return 2;
     if (t.labels) {
@@ -598,12 +620,46 @@ __device__ __forceinline__ int row_state(const Targets& t, int64_t i) {
         return l >= 0 && l < t.classes ? 1 : 2;
     }
     int st = 0;
-    for (int k = 0; k < t.k; ++k) {
+    for (int k = sub; k < t.k; k += LANES) {
         const int64_t idx = teacher_at(t, i, k);
-        if (idx < -1 || idx >= t.classes) return 2;
-        if (teacher_listed(t, i, k, idx)) st = 1;
+        if (idx < -1 || idx >= t.classes) st |= 2;
+        else if (teacher_listed(t, i, k, idx)) st |= 1;
     }
-    return st;
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) st |= __shfl_xor(st, d, kWave);
+    return st & 2 ? 2 : st;
+}
+
+// Copies a row of `width` elements to dp 16-bit elements (three planes of
+// f32), zeros past the width; a wave, 8 elements a lane.
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void pack_row(const T* __restrict__ x, bool live, int64_t width, int64_t dp, bool vec,
+                                         uint16_t* __restrict__ out, int64_t plane, int lane) {
+    for (int64_t c = lane * 8; c < dp; c += 512) {
+        T v[8] = {};
+        if (live && c < width) {
+            if (vec && c + 8 <= width) {
+                __builtin_memcpy(v, __builtin_assume_aligned(x + c, 16), sizeof(v));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < width) v[e] = x[c + e];
+            }
+        }
+        uint16_t h[3][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (SPLIT) split3(v[e], &h[0][e], &h[1][e], &h[2][e]);
+            else h[0][e] = v[e];
+        }
+#pragma unroll
+        for (int z = 0; z < (SPLIT ? 3 : 1); ++z) {
+            u32x4_t w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (uint32_t)h[z][2 * e] | ((uint32_t)h[z][2 * e + 1] << 16);
+            *reinterpret_cast<u32x4_t*>(out + z * plane + c) = w;
+        }
+    }
 }
 
 // hidden[rows] in the layout the products read: np rows of dp elements (one
@@ -613,59 +669,84 @@ __device__ __forceinline__ int row_state(const Targets& t, int64_t i) {
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void head_pack_hidden_kernel(Targets t, const T* __restrict__ hidden, int64_t ld,
                                                                int64_t n, int64_t np, int64_t width, int64_t dp,
-                                                               uint16_t* __restrict__ out) {
+                                                               int32_t vec, uint16_t* __restrict__ out) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= np) return;
-    const bool live = i < n && row_state(t, i) == 1;
+    const bool live = i < n && row_state<64>(t, i, lane) == 1;
     const T* x = hidden + (live ? (t.rows ? t.rows[i] : i) * ld : 0);
-    for (int64_t c = lane; c < dp; c += 64) {
-        const bool in = live && c < width;
-        if constexpr (SPLIT) {
-            uint16_t a = 0, b = 0, d = 0;
-            if (in) split3(x[c], &a, &b, &d);
-            out[i * dp + c] = a;
-            out[(np + i) * dp + c] = b;
-            out[(2 * np + i) * dp + c] = d;
-        } else {
-            out[i * dp + c] = in ? __builtin_bit_cast(uint16_t, x[c]) : (uint16_t)0;
-        }
-    }
+    pack_row<T, SPLIT>(x, live, width, dp, vec, out + i * dp, np * dp, lane);
 }
 
 // weight rows v0.. of the piece likewise (`vp` rows)
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void head_pack_weight_kernel(const T* __restrict__ w, int64_t ld, int64_t rows,
-                                                               int64_t vp, int64_t width, int64_t dp,
+                                                               int64_t vp, int64_t width, int64_t dp, int32_t vec,
                                                                uint16_t* __restrict__ out) {
-    const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= rows) return;
-    for (int64_t c = lane; c < dp; c += 64) {
-        if constexpr (SPLIT) {
-            uint16_t a = 0, b = 0, d = 0;
-            if (c < width) split3(w[i * ld + c], &a, &b, &d);
-            out[i * dp + c] = a;
-            out[(vp + i) * dp + c] = b;
-            out[(2 * vp + i) * dp + c] = d;
-        } else {
-            out[i * dp + c] = c < width ? __builtin_bit_cast(uint16_t, w[i * ld + c]) : (uint16_t)0;
-        }
-    }
+    pack_row<T, SPLIT>(w + i * ld, true, width, dp, vec, out + i * dp, vp * dp, threadIdx.x & 63);
 }
 
-// The teacher's probabilities and the student's logits at its entries: one
-// wave per row; 16 lanes share an entry's dot product (4 entries at once).
-// Reads n k rows of W; prob and y are 0 where an entry is not listed.
+// 8 elements from c (zeros past the width) as floats
+template <typename T>
+__device__ __forceinline__ void load8(const T* x, int64_t c, int64_t width, bool vec, float (&f)[8]) {
+    T v[8] = {};
+    if (vec && c + 8 <= width) {
+        __builtin_memcpy(v, __builtin_assume_aligned(x + c, 16), sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < width) v[e] = x[c + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = to_float(v[e]);
+}
+
+// The student's logits at the teacher's entries, a wave per 4 entries of a
+// row (16 lanes share a dot product): n k rows of W are read, mostly from the
+// L2.  The row's first wave also makes the teacher's probabilities: prob
+// [n k] (0 where an entry is not listed) and, after it, coef [n k], what the
+// gradient subtracts at the entry's class: the sum over the entries that list
+// the class, at the first of them; -1 at every other entry.
 template <typename T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* __restrict__ hidden, int64_t ldh,
                                                            const T* __restrict__ w, int64_t ldw, const T* bias,
-                                                           int64_t n, int64_t width, float inv_t, float c1,
-                                                           float* __restrict__ prob, float* __restrict__ y) {
+                                                           int64_t n, int64_t width, int32_t vec, float inv_t,
+                                                           float c1, float* __restrict__ prob,
+                                                           float* __restrict__ y) {
     const int lane = threadIdx.x & 63;
-    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= n) return;
-    const bool live = row_state(t, i) == 1;  // uniform over the wave
+    const int groups = (t.k + 3) / 4;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= n * groups) return;
+    const int64_t i = at / groups;
+    const int k0 = (int)(at - i * groups) * 4;
+    const bool live = row_state<64>(t, i, lane) == 1;  // uniform over the wave
+    {
+        const T* h = hidden + (live ? (t.rows ? t.rows[i] : i) * ldh : 0);
+        const int k = k0 + (lane >> 4);
+        int64_t idx = -1;
+        if (live && k < t.k) {
+            idx = teacher_at(t, i, k);
+            if (!teacher_listed(t, i, k, idx)) idx = -1;
+        }
+        const T* x = w + (idx >= 0 ? idx * ldw : 0);
+        float d = 0.f;
+        if (idx >= 0) {
+            for (int64_t c = (lane & 15) * 8; c < width; c += 128) {
+                float a[8], b[8];
+                load8(h, c, width, vec, a);
+                load8(x, c, width, vec, b);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d += a[e] * b[e];
+            }
+        }
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) d += __shfl_xor(d, x, kWave);
+        if ((lane & 15) == 0 && k < t.k)
+            y[i * t.k + k] = idx >= 0 ? (d + (bias ? to_float(bias[idx]) : 0.f)) * c1 : 0.f;
+    }
+    if (k0 != 0) return;
     float m = -INFINITY;
     for (int k = lane; k < t.k && live; k += 64)
         if (teacher_listed(t, i, k, teacher_at(t, i, k))) m = fmaxf(m, t.tlogit[i * t.k + k] * inv_t);
@@ -676,29 +757,49 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
         if (teacher_listed(t, i, k, teacher_at(t, i, k))) s += expf(t.tlogit[i * t.k + k] * inv_t - m);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, kWave);
-    for (int k = lane; k < t.k; k += 64) {
-        const bool on = live && teacher_listed(t, i, k, teacher_at(t, i, k));
-        prob[i * t.k + k] = on ? expf(t.tlogit[i * t.k + k] * inv_t - m) / s : 0.f;
-    }
-    const T* h = hidden + (live ? (t.rows ? t.rows[i] : i) * ldh : 0);
-    for (int k0 = 0; k0 < t.k; k0 += 4) {
-        const int k = k0 + (lane >> 4);
-        int64_t idx = -1;
-        if (live && k < t.k) {
-            idx = teacher_at(t, i, k);
-            if (!teacher_listed(t, i, k, idx)) idx = -1;
+    auto entry = [&](int k, int64_t* idx) {
+        *idx = live && k < t.k ? teacher_at(t, i, k) : -1;
+        if (*idx >= 0 && !teacher_listed(t, i, k, *idx)) *idx = -1;
+        return *idx >= 0 ? expf(t.tlogit[i * t.k + k] * inv_t - m) / s : 0.f;
+    };
+    for (int kb = 0; kb < t.k; kb += 64) {
+        const int k = kb + lane;
+        int64_t idx;
+        const float q = entry(k, &idx);
+        float sum = q;
+        bool first = true;
+        for (int ob = 0; ob < t.k; ob += 64) {
+            int64_t oidx;
+            const float oq = entry(ob + lane, &oidx);
+            const int most = t.k - ob < 64 ? t.k - ob : 64;
+            for (int o = 0; o < most; ++o) {
+                const int other = __shfl((int)oidx, o, kWave);
+                const float p = __shfl(oq, o, kWave);
+                if (ob + o != k && other == (int)idx) {
+                    sum += p;
+                    first = first && ob + o > k;
+                }
+            }
         }
-        float d = 0.f;
-        if (idx >= 0)
-            for (int64_t c = lane & 15; c < width; c += 16) d += to_float(h[c]) * to_float(w[idx * ldw + c]);
-#pragma unroll
-        for (int x = 8; x > 0; x >>= 1) d += __shfl_xor(d, x, kWave);
-        if ((lane & 15) == 0 && k < t.k)
-            y[i * t.k + k] = idx >= 0 ? (d + (bias ? to_float(bias[idx]) : 0.f)) * c1 : 0.f;
+        if (k < t.k) {
+            prob[i * t.k + k] = q;
+            prob[(n + i) * t.k + k] = idx >= 0 && first ? sum : -1.f;
+        }
     }
 }
 
-// Joins the strips of 64 rows (8 waves take every eighth strip), then the
+__device__ __forceinline__ void join(float& m, float& s, int& first, float om, float os, int ofirst) {
+    if (om > m) {
+        s = s * __builtin_amdgcn_exp2f(m - om) + os;
+        m = om;
+        first = ofirst;
+    } else {
+        s += om == -INFINITY ? os : os * __builtin_amdgcn_exp2f(om - m);
+        if (om == m && ofirst < first) first = ofirst;
+    }
+}
+
+// Joins the strips of 16 rows (32 at a time: 4 a wave, 8 waves), then the
 // rows' losses; block partials of (loss, hits, counted rows, bad input).
 __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2* __restrict__ part, int64_t strips,
                                                         int32_t strip_classes, int64_t n, int64_t np,
@@ -706,74 +807,93 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
                                                         const float* __restrict__ prob,
                                                         const int32_t* __restrict__ earlier, float* __restrict__ lse,
                                                         float* __restrict__ row_loss, double* __restrict__ part_loss,
-                                                        long long* __restrict__ part_cnt) {
-    __shared__ float sm[8][64], ss[8][64];
-    __shared__ int sa[8][64];
+                                                        int32_t* __restrict__ part_cnt) {
+    __shared__ float sm[32][16], ss[32][16];
+    __shared__ int sa[32][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    const int slot = wave * 4 + (lane >> 4);
+    const int64_t i = (int64_t)blockIdx.x * 16 + (lane & 15);
     float m = -INFINITY, s = 0.f;
     int first = 0x7fffffff;  // the first strip with the maximum
     if (i < n) {
 #pragma unroll 4
-        for (int64_t k = wave; k < strips; k += 8) {
+        for (int64_t k = slot; k < strips; k += 32) {
             const float2 v = part[k * np + i];
-            if (v.x > m) {
-                s = s * __builtin_amdgcn_exp2f(m - v.x) + v.y;
-                m = v.x;
-                first = (int)k;
-            } else {
-                s += v.x == -INFINITY ? v.y : v.y * __builtin_amdgcn_exp2f(v.x - m);
-            }
+            join(m, s, first, v.x, v.y, (int)k);
         }
     }
-    sm[wave][lane] = m;
-    ss[wave][lane] = s;
-    sa[wave][lane] = first;
+    sm[slot][lane & 15] = m;
+    ss[slot][lane & 15] = s;
+    sa[slot][lane & 15] = first;
     __syncthreads();
     if (wave != 0) return;
-    for (int w = 1; w < 8; ++w) {
-        const float om = sm[w][lane], os = ss[w][lane];
-        if (om > m) {
-            s = s * __builtin_amdgcn_exp2f(m - om) + os;
-            m = om;
-            first = sa[w][lane];
+    // 4 lanes a row join 8 slots each, then each other's
+    const int g = lane >> 4, r = lane & 15;
+    m = sm[8 * g][r];
+    s = ss[8 * g][r];
+    first = sa[8 * g][r];
+    for (int w = 1; w < 8; ++w) join(m, s, first, sm[8 * g + w][r], ss[8 * g + w][r], sa[8 * g + w][r]);
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) {
+        const float om = __shfl_xor(m, d, kWave), os = __shfl_xor(s, d, kWave);
+        const int of = __shfl_xor(first, d, kWave);
+        // both sides join in the same order, so the four lanes agree
+        if (lane & d) {
+            float m2 = om, s2 = os;
+            int f2 = of;
+            join(m2, s2, f2, m, s, first);
+            m = m2, s = s2, first = f2;
         } else {
-            s += om == -INFINITY ? os : os * __builtin_amdgcn_exp2f(om - m);
-            if (om == m && sa[w][lane] < first) first = sa[w][lane];
+            join(m, s, first, om, os, of);
         }
     }
+    // the rows' states: a distillation's lists are looked through by 64 lanes
+    int st = 0;
+    if (t.labels) {
+        if (i < n) st = row_state<1>(t, i, 0);
+    } else {
+        for (int x = 0; x < 16; ++x) {
+            const int64_t row = (int64_t)blockIdx.x * 16 + x;
+            if (row >= n) break;  // uniform
+            const int v = row_state<64>(t, row, lane);
+            if (r == x) st = v;
+        }
+    }
+    const float l = m + log2f(s);
+    float a = 0.f;
+    if (!t.labels && st == 1) {
+        // sum of q ln q + q ln2 (L - y); an entry of probability zero says
+        // nothing of its class (whose logit may be -inf)
+        for (int k = g; k < t.k; k += 4) {
+            const float q = prob[i * t.k + k];
+            if (!(q <= 0.f)) a += q * (logf(q) + (l - y[i * t.k + k]) * kLn2);
+        }
+    }
+    a += __shfl_xor(a, 16, kWave);
+    a += __shfl_xor(a, 32, kWave);
     double loss = 0.0;
     int hit = 0, valid = 0, bad = 0;
-    if (i < n) {
-        const int st = row_state(t, i);
-        const float l = m + log2f(s);
-        float r = 0.f;
+    if (g == 0 && i < n) {
+        float v = 0.f;
         if (st == 1) {
             valid = 1;
             if (t.labels) {
                 const float yl = y[i];
-                r = (l - yl) * kLn2;
+                v = (l - yl) * kLn2;
                 hit = yl == m && !earlier[i] && first == (int)(t.labels[i] / strip_classes);
             } else {
-                // an entry of probability zero says nothing of its class
-                // (whose logit may be -inf)
-                float a = 0.f;
-                for (int k = 0; k < t.k; ++k) {
-                    const float q = prob[i * t.k + k];
-                    if (!(q <= 0.f)) a += q * (logf(q) + (l - y[i * t.k + k]) * kLn2);
-                }
-                r = a * temperature * temperature;
+                v = a * temperature * temperature;
             }
-            loss = (double)r;
+            loss = (double)v;
         } else if (st == 2) {
             bad = 1;
-            r = __int_as_float(0x7fc00000);
+            v = __int_as_float(0x7fc00000);
         }
         lse[i] = st == 1 ? l : INFINITY;
-        row_loss[i] = r;
+        row_loss[i] = v;
     }
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
+    for (int d = 8; d > 0; d >>= 1) {
         loss += __shfl_xor(loss, d, kWave);
         hit += __shfl_xor(hit, d, kWave);
         valid += __shfl_xor(valid, d, kWave);
@@ -790,10 +910,10 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
 // loss = sum / counted (NaN when no row counts or an input is bad); one
 // work-group, parts added in a fixed order
 __global__ __launch_bounds__(256) void head_finish_kernel(const double* __restrict__ part_loss,
-                                                          const long long* __restrict__ part_cnt, int64_t nparts,
+                                                          const int32_t* __restrict__ part_cnt, int64_t nparts,
                                                           float* __restrict__ loss, int64_t* __restrict__ counts) {
-    __shared__ double sl[256];
-    __shared__ long long sc[256], sv[256], sb[256];
+    __shared__ double sl[4];
+    __shared__ long long sc[3][4];
     double L = 0.0;
     long long C = 0, V = 0, B = 0;
     for (int64_t k = threadIdx.x; k < nparts; k += 256) {
@@ -802,20 +922,26 @@ __global__ __launch_bounds__(256) void head_finish_kernel(const double* __restri
         V += part_cnt[3 * k + 1];
         B |= part_cnt[3 * k + 2];
     }
-    sl[threadIdx.x] = L;
-    sc[threadIdx.x] = C;
-    sv[threadIdx.x] = V;
-    sb[threadIdx.x] = B;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        L += __shfl_xor(L, d, kWave);
+        C += __shfl_xor(C, d, kWave);
+        V += __shfl_xor(V, d, kWave);
+        B |= __shfl_xor(B, d, kWave);
+    }
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        sl[wave] = L;
+        sc[0][wave] = C;
+        sc[1][wave] = V;
+        sc[2][wave] = B;
+    }
     __syncthreads();
     if (threadIdx.x != 0) return;
-    L = 0.0;
-    C = V = B = 0;
-    for (int t = 0; t < 256; ++t) {
-        L += sl[t];
-        C += sc[t];
-        V += sv[t];
-        B |= sb[t];
-    }
+    L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    C = sc[0][0] + sc[0][1] + sc[0][2] + sc[0][3];
+    V = sc[1][0] + sc[1][1] + sc[1][2] + sc[1][3];
+    B = sc[2][0] | sc[2][1] | sc[2][2] | sc[2][3];
     loss[0] = (B || V == 0) ? __int_as_float(0x7fc00000) : (float)(L / (double)V);
     counts[0] = C;
     counts[1] = V;
@@ -855,12 +981,11 @@ __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __rest
     scale[i] = m > 0.f ? dloss[i] / m : 0.f * m;
 }
 
-// G at the targets: the rounded p - q.  A class listed twice by a teacher
-// counts with both probabilities, written by its first entry.
+// G at the targets: the rounded p - q, q the entry's coefficient.
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const float* __restrict__ lse,
                                                             const float* __restrict__ y,
-                                                            const float* __restrict__ prob,
+                                                            const float* __restrict__ coef,
                                                             const float* __restrict__ row_scale, float gscale,
                                                             int64_t n, int64_t v0, int64_t vc, uint16_t* G,
                                                             int64_t ldg, int64_t plane) {
@@ -868,46 +993,29 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const flo
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (at >= n * K) return;
     const int64_t i = at / K;
-    const int k = (int)(at % K);
-    if (lse[i] == INFINITY) return;
-    const int64_t v = t.labels ? t.labels[i] : teacher_at(t, i, k);
+    const int64_t v = t.labels ? t.labels[i] : teacher_at(t, i, (int)(at - i * K));
     if (v < v0 || v >= v0 + vc) return;
-    float q = 1.f;
-    if (!t.labels) {
-        q = prob[at];
-        for (int o = 0; o < K; ++o)
-            if (o != k && teacher_at(t, i, o) == v) {
-                if (o < k) return;
-                q += prob[i * K + o];
-            }
-        // an unlisted entry (a teacher's -inf) has no logit kept
-        if (!teacher_listed(t, i, k, v)) {
-            for (int o = k + 1; o < K; ++o)
-                if (teacher_at(t, i, o) == v && teacher_listed(t, i, o, v)) {
-                    const float s = row_scale ? row_scale[i] * gscale : gscale;
-                    store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[i * K + o] - lse[i]) - q) * s);
-                    return;
-                }
-            return;
-        }
-    }
+    const float q = t.labels ? 1.f : coef[at], l = lse[i];
+    if (q < 0.f || l == INFINITY) return;
     const float s = row_scale ? row_scale[i] * gscale : gscale;
-    store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[at] - lse[i]) - q) * s);
+    store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[at] - l) - q) * s);
 }
 
-// Column sums of a piece of G over runs of 256 rows: 4 waves of 64 rows,
+// Column sums of a piece of G over runs of 64 rows: 4 waves of 16 rows,
 // 8 columns a lane.
+constexpr int kBiasRows = 64;
+
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __restrict__ G, int64_t ldg,
-                                                             int64_t plane, int64_t np, int64_t vp,
-                                                             float* __restrict__ part) {
+                                                             int64_t plane, int64_t vp, float* __restrict__ part) {
     __shared__ float red[4][512];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
-    const int64_t r0 = (int64_t)blockIdx.y * 256 + wave * 64;
+    const int64_t r0 = (int64_t)blockIdx.y * kBiasRows + wave * (kBiasRows / 4);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c < vp) {
-        for (int64_t r = r0; r < r0 + 64 && r < np; ++r) {
+#pragma unroll 4
+        for (int64_t r = r0; r < r0 + kBiasRows / 4; ++r) {
 #pragma unroll
             for (int z = SPLIT ? 2 : 0; z >= 0; --z) {
                 const u32x4_t v = *reinterpret_cast<const u32x4_t*>(G + z * plane + r * ldg + c);
@@ -929,33 +1037,62 @@ __global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __r
     }
 }
 
+// 16 waves share 64 columns
 template <typename T>
-__global__ __launch_bounds__(256) void head_bias_kernel(const float* __restrict__ part, int64_t nparts, int64_t vp,
-                                                        int64_t vc, const float* __restrict__ alpha,
-                                                        T* __restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= vc) return;
+__global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict__ part, int64_t nparts, int64_t vp,
+                                                         int64_t vc, const float* __restrict__ alpha,
+                                                         T* __restrict__ out) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     float s = 0.f;
-    for (int64_t k = 0; k < nparts; ++k) s += part[k * vp + c];
+    if (c < vc) {
+#pragma unroll 4
+        for (int64_t k = wave; k < nparts; k += 16) s += part[k * vp + c];
+    }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || c >= vc) return;
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += red[w][lane];
     out[c] = from_float<T>(s * *alpha);
 }
 
-// dH rows: the splits' sums in order, times alpha, to the rows they belong to
+// Adds the splits' sums in order and applies alpha, 4 columns a lane: dW of a
+// piece (rows in place), or dH (to the rows they belong to)
+template <typename T>
+__device__ __forceinline__ void sum_splits(const float* __restrict__ part, int64_t splits, int64_t stride,
+                                           int64_t width, float a, T* __restrict__ out) {
+    for (int64_t d = threadIdx.x * 4; d < width; d += blockDim.x * 4) {
+        float4_t s{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int64_t k = 0; k < splits; ++k) s += *reinterpret_cast<const float4_t*>(part + k * stride + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < width) out[d + e] = from_float<T>(s[e] * a);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void head_weight_out_kernel(const float* __restrict__ part, int64_t splits,
+                                                              int64_t vp, int64_t dp, int64_t width,
+                                                              const float* __restrict__ alpha, T* __restrict__ out,
+                                                              int64_t ldo) {
+    const int64_t v = blockIdx.x;
+    sum_splits(part + v * dp, splits, vp * dp, width, *alpha, out + v * ldo);
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __restrict__ part, int64_t splits,
-                                                              int64_t np, int64_t dp, int64_t n, int64_t width,
+                                                              int64_t np, int64_t dp, int64_t width,
                                                               const int64_t* __restrict__ rows, int64_t hidden_rows,
                                                               const float* __restrict__ alpha, T* __restrict__ out,
                                                               int64_t ldo) {
     const int64_t i = blockIdx.x;
     const int64_t row = rows ? rows[i] : i;
     if (row < 0 || row >= hidden_rows) return;
-    const float a = *alpha;
-    for (int64_t d = threadIdx.x; d < width; d += 256) {
-        float s = 0.f;
-        for (int64_t k = 0; k < splits; ++k) s += part[(k * np + i) * dp + d];
-        out[row * ldo + d] = from_float<T>(s * a);
-    }
+    sum_splits(part + i * dp, splits, np * dp, width, *alpha, out + row * ldo);
 }
 
 // ---------------------------------------------------------------------------
@@ -966,21 +1103,50 @@ int64_t ceil_div(int64_t x, int64_t a) { return (x + a - 1) / a; }
 
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // G of a piece, and a packed piece of W
 
+// A product's tile and the runs that its k is cut into: the least of
+//   rounds of work-groups x (stages of a run + what a work-group costs besides)
+// in stages of a 256-tile (1.6 us).  256-tiles run one to a CU, 128-tiles two,
+// at 0.7 of their rate; a run's fp32 sums cost 16 stages to write and add up.
+struct Plan {
+    int tile;
+    int64_t splits;
+};
+
+Plan plan(int64_t p, int64_t q, int64_t stages, int64_t most_splits) {
+    Plan best{128, 1};
+    double least = 1e300;
+    for (int tile = 256; tile >= 128; tile -= 128) {
+        if (tile == 256 && (p <= 128 || q <= 128)) continue;  // padded to 128 only
+        const int64_t tiles = ceil_div(p, tile) * ceil_div(q, tile);
+        const int64_t slots = tile == 256 ? 256 : 512;
+        const double step = tile == 256 ? 1.0 : 0.71;
+        for (int64_t sp = 1; sp <= most_splits && (sp == 1 || tiles * sp <= 4 * slots); ++sp) {
+            const double t = (double)ceil_div(tiles * sp, slots) *
+                             ((double)ceil_div(stages, sp) * step + 4 + (sp > 1 ? 16 * step : 0));
+            if (t < least) least = t, best = Plan{tile, sp};
+        }
+    }
+    return best;
+}
+
 // Sizes of a call, the same for the workspace query and the launch.
 struct Shape {
     int64_t n, D, V;
-    int planes, esz;
-    bool split;    // f32 operands in three planes
-    bool pack_w;   // W goes through a packed copy
-    int tile;      // 256 or 128
-    int64_t np, dp, vp;
-    int64_t strips, strip_classes;
+    int planes;
+    bool split;       // f32 operands in three planes
+    bool pack_w;      // W goes through a packed copy
+    int64_t np, dp, vp;  // padded rows and width; classes of a piece
+    Plan logits, weight, hidden;
+    int64_t strips, strip_classes;  // the forward's
 };
 
 bool weight_in_place(const grws_head* h) {
     return h->dtype != GRWS_F32 && h->ld_weight % 8 == 0 && h->width % 8 == 0 &&
            reinterpret_cast<uintptr_t>(h->weight) % 16 == 0;
 }
+
+// to whole 128-tiles, or 256-tiles where there is more than one of 128
+int64_t pad(int64_t x) { return x <= 128 ? 128 : up(x, 256); }
 
 Shape shape_of(const grws_head* h, bool backward) {
     Shape s{};
@@ -990,21 +1156,24 @@ Shape shape_of(const grws_head* h, bool backward) {
     s.split = h->dtype == GRWS_F32;
     s.planes = s.split ? 3 : 1;
     s.pack_w = !weight_in_place(h);
-    s.tile = s.n > 128 && s.V > 128 && ceil_div(s.n, 256) * ceil_div(s.V, 256) >= 256 ? 256 : 128;
-    s.np = up(s.n, s.tile);
+    s.np = pad(s.n);
     s.dp = up(s.D, kK);
-    int64_t vp = up(s.V, s.tile);
+    s.vp = pad(s.V);
+    auto bound = [&](int64_t row_elements) {
+        int64_t most = kPieceBytes / (2 * s.planes * row_elements) / 256 * 256;
+        if (most < 256) most = 256;
+        if (s.vp > most) s.vp = most;
+    };
+    if (backward) bound(s.np);
+    if (s.pack_w) bound(s.dp);
+    const int64_t seg = s.split ? 6 : 1;
+    s.logits = plan(s.vp, s.np, seg * s.dp / kK, 1);
+    s.strip_classes = s.logits.tile / 2;
+    s.strips = pad(s.V) / s.strip_classes;
     if (backward) {
-        const int64_t most = kPieceBytes / (2 * s.planes * s.np) / s.tile * s.tile;
-        if (vp > most) vp = most < s.tile ? s.tile : most;
+        s.weight = plan(s.D, s.vp, seg * s.np / kK, ceil_div(s.np / kK, 4));
+        s.hidden = plan(s.dp, s.np, seg * s.vp / kK, ceil_div(s.vp / kK, 4));
     }
-    if (s.pack_w) {
-        const int64_t most = kPieceBytes / (2 * s.planes * s.dp) / s.tile * s.tile;
-        if (vp > most) vp = most < s.tile ? s.tile : most;
-    }
-    s.vp = vp;
-    s.strip_classes = s.tile / 2;
-    s.strips = up(s.V, s.tile) / s.strip_classes;
     return s;
 }
 
@@ -1042,7 +1211,7 @@ struct FwdSpace {
     float2* part;
     int32_t* earlier;
     double* pl;
-    long long* pc;
+    int32_t* pc;
 };
 
 template <typename A>
@@ -1056,34 +1225,18 @@ void fwd_space(A& a, const Shape& s, FwdSpace* f) {
     if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
     take(f->part, s.strips * s.np);
     take(f->earlier, s.n);
-    take(f->pl, ceil_div(s.n, 64));
-    take(f->pc, 3 * ceil_div(s.n, 64));
-}
-
-struct BwdShape {
-    int64_t splits, ldg;
-};
-
-BwdShape bwd_shape(const Shape& s) {
-    BwdShape b{};
-    b.ldg = s.vp;
-    // enough work-groups for dH: its tiles times runs of at least 16 stages
-    const int64_t tiles = ceil_div(s.np, s.tile) * ceil_div(s.dp, s.tile);
-    int64_t sp = ceil_div(512, tiles);
-    const int64_t most = s.vp / kK / 16;
-    if (sp > most) sp = most;
-    b.splits = sp < 1 ? 1 : sp;
-    return b;
+    take(f->pl, ceil_div(s.n, 16));
+    take(f->pc, 3 * ceil_div(s.n, 16));
 }
 
 struct BwdSpace {
     uint16_t *hp, *wp, *G;
-    float *part, *bias, *alpha, *scale;
+    float *dh, *dw, *bias, *alpha, *scale;
     uint32_t* most;
 };
 
 template <typename A>
-void bwd_space(A& a, const Shape& s, const BwdShape& b, BwdSpace* f) {
+void bwd_space(A& a, const Shape& s, BwdSpace* f) {
     auto take = [&](auto*& p, int64_t n) {
         using T = std::remove_reference_t<decltype(*p)>;
         if constexpr (std::is_same_v<A, Sizer>) a.template take<T>((size_t)n);
@@ -1091,22 +1244,29 @@ void bwd_space(A& a, const Shape& s, const BwdShape& b, BwdSpace* f) {
     };
     take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
-    take(f->G, s.planes * s.np * b.ldg);
-    take(f->part, b.splits * s.np * s.dp);
-    take(f->bias, ceil_div(s.np, 256) * s.vp);
+    take(f->G, s.planes * s.np * s.vp);
+    take(f->dh, s.hidden.splits * s.np * s.dp);
+    if (s.weight.splits > 1) take(f->dw, s.weight.splits * s.vp * s.dp);
+    take(f->bias, s.np / kBiasRows * s.vp);
     take(f->alpha, 1);
     take(f->scale, s.n);
     take(f->most, 1);
 }
 
+// whether 8 elements of a row may be read as 16-byte vectors
+bool rows_of_16(const void* p, int64_t ld, int32_t dtype) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (dtype == GRWS_F32 ? 4 : 8) == 0;
+}
+
 int pack_hidden(const grws_head* h, const Shape& s, const Targets& t, uint16_t* hp, hipStream_t stream) {
     const dim3 grid((unsigned)ceil_div(s.np, 4));
+    const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype);
     if (s.split)
         hipLaunchKernelGGL((head_pack_hidden_kernel<float, true>), grid, dim3(256), 0, stream, t,
-                           static_cast<const float*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, hp);
+                           static_cast<const float*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp);
     else
         hipLaunchKernelGGL((head_pack_hidden_kernel<uint16_t, false>), grid, dim3(256), 0, stream, t,
-                           static_cast<const uint16_t*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, hp);
+                           static_cast<const uint16_t*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp);
     GRWS_LAUNCH_CHECK();
     return GRWS_OK;
 }
@@ -1121,14 +1281,15 @@ int weight_piece(const grws_head* h, const Shape& s, int64_t v0, int64_t vc, uin
     }
     if (pack) {
         const dim3 grid((unsigned)ceil_div(vc, 4));
+        const int32_t vec = rows_of_16(h->weight, h->ld_weight, h->dtype);
         if (s.split)
             hipLaunchKernelGGL((head_pack_weight_kernel<float, true>), grid, dim3(256), 0, stream,
                                static_cast<const float*>(h->weight) + v0 * h->ld_weight, h->ld_weight, vc, s.vp, s.D,
-                               s.dp, wp);
+                               s.dp, vec, wp);
         else
             hipLaunchKernelGGL((head_pack_weight_kernel<uint16_t, false>), grid, dim3(256), 0, stream,
                                static_cast<const uint16_t*>(h->weight) + v0 * h->ld_weight, h->ld_weight, vc, s.vp,
-                               s.D, s.dp, wp);
+                               s.D, s.dp, vec, wp);
         GRWS_LAUNCH_CHECK();
     }
     const char* p = reinterpret_cast<const char*>(wp);
@@ -1143,17 +1304,17 @@ Opnd hidden_operand(const Shape& s, const uint16_t* hp, bool strided) {
     return strided ? Opnd{p, s.dp * 2, plane, s.dp, s.np} : Opnd{p, s.dp * 2, plane, s.np, s.dp};
 }
 
-Gemm gemm_of(const Shape& s, const Opnd& P, const Opnd& Q, int64_t np, int64_t nq, int64_t k, int64_t splits) {
-    return Gemm{P, Q, s.split ? 6 : 1, (int32_t)ceil_div(k, kK), (int32_t)ceil_div(np, s.tile),
-                (int32_t)ceil_div(nq, s.tile), (int32_t)splits};
+Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64_t np, int64_t nq, int64_t k) {
+    return Gemm{P, Q, s.split ? 6 : 1, (int32_t)ceil_div(k, kK), (int32_t)ceil_div(np, pl.tile),
+                (int32_t)ceil_div(nq, pl.tile), (int32_t)pl.splits};
 }
 
-// KERNEL<..., BP, BQ, WP, WQ> at the call's tile
-#define GRWS_HEAD_LAUNCH(NAME, ARGS, ...)                                                                            \
+// KERNEL<..., BP, BQ, WP, WQ> at a plan's tile
+#define GRWS_HEAD_LAUNCH(PLAN, NAME, ARGS, ...)                                                                      \
     do {                                                                                                             \
         GRWS_CHECK_ARG((int64_t)ARGS.g.tp * ARGS.g.tq < INT32_MAX, "head: more than 2^31 tiles");                    \
         const dim3 grid_((unsigned)(ARGS.g.tp * ARGS.g.tq), (unsigned)ARGS.g.splits);                                \
-        if (s.tile == 256)                                                                                           \
+        if (PLAN.tile == 256)                                                                                        \
             hipLaunchKernelGGL((NAME<__VA_ARGS__, 256, 256, 2, 4>), grid_, dim3(512), 0, stream, ARGS);              \
         else                                                                                                         \
             hipLaunchKernelGGL((NAME<__VA_ARGS__, 128, 128, 2, 2>), grid_, dim3(256), 0, stream, ARGS);              \
@@ -1198,24 +1359,26 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        StatsArgs a{gemm_of(s, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, 1), v0, s.V, s.n, s.np, c1,
+        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, s.np, c1,
                     h->bias, h->dtype, h->labels, f.part, target_logit, f.earlier};
-        if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(head_stats_kernel, a, GRWS_F16);
-        else GRWS_HEAD_LAUNCH(head_stats_kernel, a, GRWS_BF16);
+        if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
+        else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
     }
     if (h->k > 0) {
-        const dim3 grid((unsigned)ceil_div(s.n, 4));
+        const dim3 grid((unsigned)ceil_div(s.n * ((h->k + 3) / 4), 4));
+        const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype) &&
+                            rows_of_16(h->weight, h->ld_weight, h->dtype);
 #define GRWS_HEAD_TARGETS(T)                                                                                         \
     hipLaunchKernelGGL(head_targets_kernel<T>, grid, dim3(256), 0, stream, t, static_cast<const T*>(h->hidden),      \
                        h->ld_hidden, static_cast<const T*>(h->weight), h->ld_weight, static_cast<const T*>(h->bias), \
-                       s.n, s.D, 1.f / h->temperature, c1, target_prob, target_logit)
+                       s.n, s.D, vec, 1.f / h->temperature, c1, target_prob, target_logit)
         if (h->dtype == GRWS_F32) GRWS_HEAD_TARGETS(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_TARGETS(_Float16);
         else GRWS_HEAD_TARGETS(__hip_bfloat16);
 #undef GRWS_HEAD_TARGETS
         GRWS_LAUNCH_CHECK();
     }
-    const int64_t blocks = ceil_div(s.n, 64);
+    const int64_t blocks = ceil_div(s.n, 16);
     hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part, ceil_div(s.V, s.strip_classes),
                        (int32_t)s.strip_classes, s.n, s.np, h->temperature, target_logit, target_prob, f.earlier, lse,
                        row_loss, f.pl, f.pc);
@@ -1230,7 +1393,7 @@ extern "C" size_t grws_head_bwd_workspace_bytes(const grws_head* h) {
     Sizer z;
     BwdSpace f{};
     const Shape s = shape_of(h, true);
-    bwd_space(z, s, bwd_shape(s), &f);
+    bwd_space(z, s, &f);
     return z.used;
 }
 
@@ -1255,14 +1418,14 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
     GRWS_CHECK_ARG(lse && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
     if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
     const Shape s = shape_of(h, true);
-    const BwdShape b = bwd_shape(s);
     const Targets t = targets_of(h);
     Carver cv(workspace, workspace_bytes);
     BwdSpace f{};
-    bwd_space(cv, s, b, &f);
+    bwd_space(cv, s, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
     const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
+    const float* coef = target_prob ? target_prob + s.n * h->k : nullptr;
     const float* row_scale = nullptr;
     if (per_row) {
         GRWS_TRY(fill_i32(reinterpret_cast<int32_t*>(f.most), 1, 0, stream));
@@ -1277,49 +1440,49 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
                        h->temperature / gscale, f.alpha, f.most);
     GRWS_LAUNCH_CHECK();
     GRWS_TRY(pack_hidden(h, s, t, f.hp, stream));
-    const int64_t plane = s.np * b.ldg;
+    const int64_t plane = s.np * s.vp;
     const size_t esz = dtype_size(h->dtype);
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
-        const int64_t vt = up(vc, s.tile);
+        const int64_t vt = up(vc, s.logits.tile);  // G's columns that are written
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        GradArgs a{gemm_of(s, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, 1), v0, s.V, s.n, c1, h->bias,
-                   h->dtype, lse, row_scale, gscale, f.G, b.ldg, plane};
+        GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, c1, h->bias,
+                   h->dtype, lse, row_scale, gscale, f.G, s.vp, plane};
         const dim3 sgrid((unsigned)ceil_div(s.n * (h->k ? h->k : 1), 256));
 #define GRWS_HEAD_SUB(DT, SP)                                                                                       \
     hipLaunchKernelGGL((head_subtract_kernel<DT, SP>), sgrid, dim3(256), 0, stream, t, lse, target_logit,           \
-                       target_prob, row_scale, gscale, s.n, v0, vc, f.G, b.ldg, plane)
+                       coef, row_scale, gscale, s.n, v0, vc, f.G, s.vp, plane)
         if (s.split) {
-            GRWS_HEAD_LAUNCH(head_grad_kernel, a, GRWS_BF16, true);
+            GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, true);
             GRWS_HEAD_SUB(GRWS_BF16, true);
         } else if (h->dtype == GRWS_F16) {
-            GRWS_HEAD_LAUNCH(head_grad_kernel, a, GRWS_F16, false);
+            GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_F16, false);
             GRWS_HEAD_SUB(GRWS_F16, false);
         } else {
-            GRWS_HEAD_LAUNCH(head_grad_kernel, a, GRWS_BF16, false);
+            GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, false);
             GRWS_HEAD_SUB(GRWS_BF16, false);
         }
 #undef GRWS_HEAD_SUB
         GRWS_LAUNCH_CHECK();
         const char* gp = reinterpret_cast<const char*>(f.G);
         if (d_bias) {
-            const int64_t nparts = ceil_div(s.np, 256);
+            const int64_t nparts = s.np / kBiasRows;
             const dim3 grid((unsigned)ceil_div(vt, 512), (unsigned)nparts);
             if (s.split)
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, true>), grid, dim3(256), 0, stream, f.G, b.ldg,
-                                   plane, s.np, vt, f.bias);
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, true>), grid, dim3(256), 0, stream, f.G, s.vp,
+                                   plane, vt, f.bias);
             else if (h->dtype == GRWS_F16)
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_F16, false>), grid, dim3(256), 0, stream, f.G, b.ldg,
-                                   plane, s.np, vt, f.bias);
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_F16, false>), grid, dim3(256), 0, stream, f.G, s.vp,
+                                   plane, vt, f.bias);
             else
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, false>), grid, dim3(256), 0, stream, f.G, b.ldg,
-                                   plane, s.np, vt, f.bias);
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, false>), grid, dim3(256), 0, stream, f.G, s.vp,
+                                   plane, vt, f.bias);
             GRWS_LAUNCH_CHECK();
-            const dim3 cg((unsigned)ceil_div(vc, 256));
+            const dim3 cg((unsigned)ceil_div(vc, 64));
             char* db = static_cast<char*>(d_bias) + v0 * esz;
 #define GRWS_HEAD_BIAS(T) \
-    hipLaunchKernelGGL(head_bias_kernel<T>, cg, dim3(256), 0, stream, f.bias, nparts, vt, vc, f.alpha, \
+    hipLaunchKernelGGL(head_bias_kernel<T>, cg, dim3(1024), 0, stream, f.bias, nparts, vt, vc, f.alpha, \
                        reinterpret_cast<T*>(db))
             if (h->dtype == GRWS_F32) GRWS_HEAD_BIAS(float);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS(_Float16);
@@ -1330,25 +1493,35 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         if (d_weight) {
             char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
             const int32_t vec = reinterpret_cast<uintptr_t>(d_weight) % (4 * esz) == 0 && ld_dw % 4 == 0;
-            const Opnd G{gp, b.ldg * 2, plane * 2, b.ldg, s.np};
-            WeightArgs w{gemm_of(s, hidden_operand(s, f.hp, true), G, s.D, vc, s.np, 1), f.alpha, out, ld_dw, vc,
-                         s.D, vec};
-            if (s.split) GRWS_HEAD_LAUNCH(head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
-            else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(head_dweight_kernel, w, GRWS_F16, GRWS_F16);
-            else GRWS_HEAD_LAUNCH(head_dweight_kernel, w, GRWS_BF16, GRWS_BF16);
+            const Opnd G{gp, s.vp * 2, plane * 2, s.vp, s.np};
+            WeightArgs w{gemm_of(s, s.weight, hidden_operand(s, f.hp, true), G, s.D, vc, s.np), f.alpha, out, ld_dw,
+                         vc, s.D, vec, f.dw, s.vp, s.dp};
+            if (s.split) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_F16, GRWS_F16);
+            else GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_BF16);
+            if (s.weight.splits > 1) {
+#define GRWS_HEAD_DW(T)                                                                                             \
+    hipLaunchKernelGGL(head_weight_out_kernel<T>, dim3((unsigned)vc), dim3(256), 0, stream, f.dw, s.weight.splits,  \
+                       s.vp, s.dp, s.D, f.alpha, reinterpret_cast<T*>(out), ld_dw)
+                if (h->dtype == GRWS_F32) GRWS_HEAD_DW(float);
+                else if (h->dtype == GRWS_F16) GRWS_HEAD_DW(_Float16);
+                else GRWS_HEAD_DW(__hip_bfloat16);
+#undef GRWS_HEAD_DW
+                GRWS_LAUNCH_CHECK();
+            }
         }
         if (d_hidden) {
             GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, false, stream));
-            const Opnd G{gp, b.ldg * 2, plane * 2, s.np, vt};
-            HiddenArgs d{gemm_of(s, W, G, s.dp, s.np, vc, b.splits), f.part, s.np, s.dp, v0 == 0};
-            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(head_dhidden_kernel, d, GRWS_F16);
-            else GRWS_HEAD_LAUNCH(head_dhidden_kernel, d, GRWS_BF16);
+            const Opnd G{gp, s.vp * 2, plane * 2, s.np, vt};
+            HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc), f.dh, s.np, s.dp, v0 == 0};
+            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16);
+            else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16);
         }
     }
     if (d_hidden) {
 #define GRWS_HEAD_DH(T)                                                                                              \
-    hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.part, b.splits, s.np, \
-                       s.dp, s.n, s.D, h->rows, h->hidden_rows, f.alpha, static_cast<T*>(d_hidden), ld_dh)
+    hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, f.alpha, static_cast<T*>(d_hidden), ld_dh)
         if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
         else GRWS_HEAD_DH(__hip_bfloat16);

@@ -840,8 +840,8 @@ int grws_cross_entropy_bwd(const void* logits, int32_t dtype, int64_t ld, int64_
 /*                                                                           */
 /* Forward, no sync: lse f32 [n] (log2 of the sum of 2^(z log2(e) / T), +inf */
 /* for rows that do not count) and target_logit f32 [n * max(k, 1)],         */
-/* target_prob f32 [n x k] (k > 0), which the backward takes; row_loss f32   */
-/* [n] (0 for rows that do not count, NaN for bad input); loss f32 scalar,   */
+/* target_prob f32 [2 x n x k] (k > 0), which the backward takes; row_loss   */
+/* f32 [n] (0 for rows that do not count, NaN for bad input); loss f32 scalar,   */
 /* the mean over counted rows (NaN when none counts or an input is bad: a    */
 /* label, class index or row id out of range); counts int64 [3] = {rows      */
 /* whose label is the first largest logit (k = 0), counted rows, bad input}. */
