@@ -1,81 +1,143 @@
 // The k largest logits of each row with their classes (gfx950): the teacher's
 // side of distillation from top logits.
 //
-// Every logit becomes a 64-bit key, (order-preserving bits of the value,
-// complement of the class), so keys are distinct, a larger key is a larger
-// logit, and of equal logits the lowest class comes first.  -0 equals +0 and
-// a NaN is larger than everything, as in torch's sort.
+// Every logit becomes a 64-bit key, the order-preserving bits of the value
+// above the complement of the class, so keys are distinct, a larger key is a
+// larger logit, and of equal logits the lowest class comes first.  -0 equals
+// +0 and a NaN is larger than everything, as in torch's sort.
 //
 // A work-group streams a row (or one of several stretches of it, when there
-// are few rows) and keeps in LDS the keys above a running bound; when the
-// buffer might overflow, it finds the k-th largest key bit by bit, drops the
-// rest and raises the bound to it.  The row is read once.
+// are few rows) and keeps in LDS the keys above a running bound; the row is
+// read once.  The first bound is the k-th largest of the threads' maxima over
+// the first 8,192 logits (at least k logits reach it); of random logits about
+// 1% pass it, so a row of 50,021 leaves some 450 keys for k = 64, of which
+// the k largest are found digit by digit (8 bits, an LDS histogram each) and
+// ordered by counting.  When the pool overflows (k > 128, rising rows, ties)
+// the k largest are found in between and the bound is raised to the k-th.
 #include "grws_internal.h"
 
 namespace grws {
 namespace {
 
 constexpr int kT = 256;          // threads of a work-group
+constexpr int kWaves = kT / kWave;
 constexpr int kMaxK = 1024;
-constexpr int kVec = 8;          // logits a thread takes per step
+constexpr int kVec = 8;          // logits of a load (two loads of f32)
+constexpr int kLoads = 4;        // loads a thread has in flight
+constexpr int kMine = kVec * kLoads;
+constexpr int kChunk = kT * kMine;       // logits of a step
 constexpr int kCap = kMaxK + kT * kVec;  // keys in LDS
 constexpr int kPer = kCap / kT;
 
-__device__ __forceinline__ uint32_t order_bits(float x) {
-    if (x != x) return 0xffffffffu;
-    const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+// Order-preserving bits of a logit: 16 for the 16-bit types, 32 for f32.
+template <typename T>
+__device__ __forceinline__ uint32_t order_of(T x) {
+    constexpr uint32_t SIGN = sizeof(T) == 2 ? 0x8000u : 0x80000000u;
+    constexpr uint32_t ALL = SIGN | (SIGN - 1);
+    uint32_t u;
+    if constexpr (sizeof(T) == 2) u = __builtin_bit_cast(uint16_t, x);
+    else u = __builtin_bit_cast(uint32_t, x);
+    const float f = to_float(x);
+    if (f != f) return ALL;
+    if (f == 0.f) u = 0;
+    return u & SIGN ? ~u & ALL : u | SIGN;
 }
 
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t cls) {
-    return ((uint64_t)order_bits(x) << 32) | (uint32_t)~cls;
+// The logit with these order bits (a NaN for the largest).
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t o) {
+    constexpr uint32_t SIGN = sizeof(T) == 2 ? 0x8000u : 0x80000000u;
+    constexpr uint32_t ALL = SIGN | (SIGN - 1);
+    const uint32_t u = o & SIGN ? o & (SIGN - 1) : ~o & ALL;
+    if constexpr (sizeof(T) == 2) return to_float(__builtin_bit_cast(T, (uint16_t)u));
+    else return __uint_as_float(u);
 }
 
 struct Pool {
     uint64_t keys[kCap];
+    int32_t hist[2][256];
+    uint32_t most[kT];  // the threads' maxima
+    uint32_t first;     // the first bound's order bits
     int32_t count;
-    int32_t waves[2][kT / kWave];
 };
 
-// Number of the work-group's threads' keys that are >= bound.
-__device__ __forceinline__ int count_from(const uint64_t (&mine)[kPer], uint64_t bound, Pool& p, int turn) {
-    int c = 0;
+// The need-th largest bin from the top: the digit, the keys in it, and how
+// many of them are needed.  Every wave works it out for itself.
+__device__ __forceinline__ int find_digit(const int32_t* hist, int& need, int& in_bin) {
+    const int lane = threadIdx.x & 63;
+    int c[4], sum = 0;  // lane 0 holds the four largest digits
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) c += __builtin_popcountll(__ballot(mine[i] >= bound));
-    if ((threadIdx.x & 63) == 0) p.waves[turn][threadIdx.x >> 6] = c;
-    __syncthreads();
-    c = 0;
+    for (int j = 0; j < 4; ++j) {
+        c[j] = hist[255 - 4 * lane - j];
+        sum += c[j];
+    }
+    int incl = sum;
 #pragma unroll
-    for (int w = 0; w < kT / kWave; ++w) c += p.waves[turn][w];
-    return c;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d, kWave);
+        if (lane >= d) incl += o;
+    }
+    const int l = __builtin_ctzll(__ballot(incl >= need));
+    int above = __shfl(incl - sum, l, kWave);
+    int digit = 0, in = 0;
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int x = __shfl(c[j], l, kWave);
+        if (!found) {
+            if (above + x >= need) {
+                found = true;
+                digit = 255 - 4 * l - j;
+                in = x;
+            } else {
+                above += x;
+            }
+        }
+    }
+    need -= above;
+    in_bin = in;
+    return digit;
 }
 
-// Keeps the k largest keys of the pool (all, when there are no more) and
-// returns the k-th (0 when there are fewer).  Keys are distinct and not 0.
-__device__ __forceinline__ uint64_t keep_best(Pool& p, int k) {
+// Keeps the k largest keys of the pool, of `bits` bits (all, when there are
+// no more), and returns a bound that exactly they reach (0: all).
+__device__ __forceinline__ uint64_t keep_best(Pool& p, int k, int bits) {
     __syncthreads();
     const int n = p.count;
+    if (n <= k) return 0;  // uniform over the work-group
     uint64_t mine[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int at = i * kT + threadIdx.x;
         mine[i] = at < n ? p.keys[at] : 0;
     }
-    if (n < k) return 0;
+    p.hist[0][threadIdx.x] = 0;
     uint64_t bound = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t trial = bound | (1ull << bit);
-        if (count_from(mine, trial, p, bit & 1) >= k) bound = trial;
+    int need = k, turn = 0;
+    for (int shift = (bits + 7) / 8 * 8 - 8; shift >= 0; shift -= 8, turn ^= 1) {
+        __syncthreads();  // this histogram is clear, the last one read
+        p.hist[turn ^ 1][threadIdx.x] = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            // of the keys with the bound's digits above
+            if (mine[i] != 0 && ((mine[i] ^ bound) >> shift) < 256)
+                atomicAdd(&p.hist[turn][(mine[i] >> shift) & 255], 1);
+        }
+        __syncthreads();
+        int in_bin;
+        const int digit = find_digit(p.hist[turn], need, in_bin);
+        bound |= (uint64_t)digit << shift;
+        if (in_bin == need) break;  // the whole bin is in
     }
-    __syncthreads();  // every thread has its keys and the last counts
     if (threadIdx.x == 0) p.count = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const bool in = mine[i] >= bound && mine[i] != 0;
         const uint64_t b = __ballot(in);
+        if (!b) continue;  // uniform over the wave
         int at = 0;
-        if ((threadIdx.x & 63) == 0 && b) at = atomicAdd(&p.count, __builtin_popcountll(b));
+        if ((threadIdx.x & 63) == 0) at = atomicAdd(&p.count, __builtin_popcountll(b));
         at = __shfl(at, 0, kWave) + __builtin_popcountll(b & lanemask_lt());
         if (in) p.keys[at] = mine[i];
     }
@@ -83,10 +145,14 @@ __device__ __forceinline__ uint64_t keep_best(Pool& p, int k) {
     return bound;
 }
 
-// Offers every thread's kVec keys (0: none) to the pool.
-__device__ __forceinline__ void offer(Pool& p, const uint64_t (&x)[kVec], int k, uint64_t& bound) {
+// Offers every thread's kVec keys (0: none) to the pool, which has room for
+// them or is cut to its best.  `bound`: keys up to it are not wanted.
+__device__ __forceinline__ void offer(Pool& p, const uint64_t (&x)[kVec], int k, int bits, uint64_t& bound) {
     __syncthreads();
-    if (p.count + kT * kVec > kCap) bound = keep_best(p, k);  // uniform: the count is read after the barrier
+    if (p.count + kT * kVec > kCap) {  // uniform: the count is read after the barrier
+        const uint64_t b = keep_best(p, k, bits);
+        if (b > 0 && b - 1 > bound) bound = b - 1;
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
@@ -100,55 +166,156 @@ __device__ __forceinline__ void offer(Pool& p, const uint64_t (&x)[kVec], int k,
     }
 }
 
-// The pool's keys, largest first, by counting the larger ones.
+// The pool's k largest, largest first, by counting the larger ones.
 template <typename T>
-__device__ __forceinline__ void write_best(Pool& p, int k, const T* row, T* values, int32_t* index) {
-    keep_best(p, k);
+__device__ __forceinline__ void write_best(Pool& p, int k, int bits, int class_bits, const T* row, T* values,
+                                           int32_t* index) {
+    keep_best(p, k, bits);
     __syncthreads();
     const int n = p.count < k ? p.count : k;
+    const uint64_t low = (1ull << class_bits) - 1;
     for (int a = threadIdx.x; a < n; a += kT) {
         const uint64_t key = p.keys[a];
         int rank = 0;
         for (int b = 0; b < n; ++b) rank += p.keys[b] > key;
-        const uint32_t cls = ~(uint32_t)key;
+        const uint32_t cls = (uint32_t)(low - (key & low));
         index[rank] = (int32_t)cls;
         values[rank] = row[cls];
     }
 }
 
+// The first bound: order bits that at least k of the threads' maxima reach
+// (their upper 16 bits; the first wave, 4 maxima a lane).
+__device__ __forceinline__ uint32_t first_bound(Pool& p, uint32_t most, int k, int value_bits) {
+    p.most[threadIdx.x] = most;
+    __syncthreads();
+    if (threadIdx.x < kWave) {
+        uint32_t m[kWaves];
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) m[j] = p.most[threadIdx.x + j * kWave];
+        uint32_t bound = 0;
+        for (int bit = value_bits - 1; bit >= value_bits - 16; --bit) {
+            const uint32_t trial = bound | (1u << bit);
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < kWaves; ++j) c += __builtin_popcountll(__ballot(m[j] >= trial));
+            if (c >= k) bound = trial;
+        }
+        if (threadIdx.x == 0) p.first = bound;
+    }
+    __syncthreads();
+    return p.first;
+}
+
 template <typename T, bool FINAL>
-__global__ __launch_bounds__(kT) void top_rows_kernel(const T* __restrict__ logits, int64_t ld, int32_t classes,
-                                                      int32_t k, int32_t stretch, T* __restrict__ values,
-                                                      int32_t* __restrict__ index, uint64_t* __restrict__ best) {
+__global__ __launch_bounds__(kT, 5) void top_rows_kernel(const T* __restrict__ logits, int64_t ld, int32_t classes,
+                                                      int32_t class_bits, int32_t k, int32_t stretch,
+                                                      T* __restrict__ values, int32_t* __restrict__ index,
+                                                      uint64_t* __restrict__ best) {
+    constexpr int VB = sizeof(T) * 8;
+    struct Vec {
+        uint32_t w[kVec * sizeof(T) / 4];
+    };
     __shared__ Pool p;
     const int64_t r = blockIdx.x;
     const T* row = logits + r * ld;
     const int32_t c0 = (int32_t)blockIdx.y * stretch;
     const int32_t c1 = classes - c0 < stretch ? classes : c0 + stretch;
+    const int bits = VB + class_bits;
+    const uint64_t low = (1ull << class_bits) - 1;
     if (threadIdx.x == 0) p.count = 0;
     uint64_t bound = 0;
-    for (int32_t c = c0; c < c1; c += kT * kVec) {
+    float least = -INFINITY;  // the bound's logit: smaller ones are not looked at
+    for (int32_t c = c0; c < c1; c += kChunk) {
+        // load i of a thread: logits c + 2,048 i + 8 thread + 0..7
+        Vec v[kLoads];
         const int32_t at = c + (int32_t)threadIdx.x * kVec;
-        uint64_t x[kVec];
-        if (at + kVec <= c1) {
-            T v[kVec];
-            __builtin_memcpy(v, row + at, sizeof(v));  // rows of any alignment
+        const bool whole = c + kChunk <= c1;  // uniform
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) x[i] = key_of(to_float(v[i]), (uint32_t)(at + i));
-        } else {
+        for (int i = 0; i < kLoads; ++i) {
+            const int32_t f = at + i * kT * kVec;
+            if (whole || f + kVec <= c1) {
+                __builtin_memcpy(&v[i], row + f, sizeof(Vec));  // rows of any alignment
+            } else {
+                T x[kVec];
 #pragma unroll
-            for (int i = 0; i < kVec; ++i)
-                x[i] = at + i < c1 ? key_of(to_float(row[at + i]), (uint32_t)(at + i)) : 0;
+                for (int e = 0; e < kVec; ++e) x[e] = f + e < c1 ? row[f + e] : from_float<T>(0.f);
+                __builtin_memcpy(&v[i], x, sizeof(Vec));
+            }
         }
-        offer(p, x, k, bound);
+        auto get = [&](int i) -> T {
+            const uint32_t w = v[i / kVec].w[(i % kVec) * (int)sizeof(T) / 4];
+            if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)(w >> (16 * (i & 1))));
+            else return __builtin_bit_cast(T, w);
+        };
+        auto cls = [&](int i) { return at + (i / kVec) * kT * kVec + i % kVec; };
+        // a candidate is read again (few are, from the L1 or L2) instead of
+        // holding 32 keys in registers
+        auto key = [&](int i) {
+            const int32_t x = cls(i);
+            return ((uint64_t)order_of<T>(row[x]) << class_bits) | (low - (uint32_t)x);
+        };
+        if (c == c0 && k <= kT / 2 && c1 - c0 >= 4 * kT) {  // uniform
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i)
+                if (cls(i) < c1) {
+                    const uint32_t o = order_of<T>(get(i));
+                    most = o > most ? o : most;
+                }
+            const uint32_t o = first_bound(p, most, k, VB);
+            if (o > 0) {
+                bound = ((uint64_t)o << class_bits) - 1;
+                least = value_of<T>(o);
+            }
+        }
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (!(to_float(get(i)) < least) && (whole || cls(i) < c1)) mask |= 1u << i;
+        // room for the wave's candidates; what does not fit shows in the count
+        __syncthreads();
+        const int before = p.count;
+        __syncthreads();
+        const int mine = __builtin_popcount(mask);
+        int incl = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d, kWave);
+            if ((int)(threadIdx.x & 63) >= d) incl += o;
+        }
+        int base = 0;
+        if ((threadIdx.x & 63) == 63 && incl) base = atomicAdd(&p.count, incl);
+        base = __shfl(base, 63, kWave) + incl - mine;
+        if (base + mine <= kCap) {
+#pragma unroll 1
+            for (uint32_t m = mask; m; m &= m - 1) {
+                const uint64_t x = key(__builtin_ctz(m));
+                // a logit equal to the bound's, of a later class, keeps its place as an empty key
+                p.keys[base++] = x > bound ? x : 0;
+            }
+        }
+        __syncthreads();
+        if (p.count > kCap) {  // uniform: again, 8 a thread at a time
+            __syncthreads();
+            if (threadIdx.x == 0) p.count = before;
+#pragma unroll 1
+            for (int i = 0; i < kLoads; ++i) {
+                uint64_t x[kVec];
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) x[e] = (mask >> (i * kVec + e)) & 1 ? key(i * kVec + e) : 0;
+                offer(p, x, k, bits, bound);
+            }
+            if (bound > 0) least = value_of<T>((uint32_t)((bound + 1) >> class_bits));
+        }
     }
     if constexpr (FINAL) {
-        write_best(p, k, row, values + r * k, index + r * k);
+        write_best(p, k, bits, class_bits, row, values + r * k, index + r * k);
     } else {
-        keep_best(p, k);
+        keep_best(p, k, bits);
         __syncthreads();
         uint64_t* out = best + (r * gridDim.y + blockIdx.y) * k;
-        const int n = p.count;
+        const int n = p.count < k ? p.count : k;
         for (int a = threadIdx.x; a < k; a += kT) out[a] = a < n ? p.keys[a] : 0;
     }
 }
@@ -156,11 +323,13 @@ __global__ __launch_bounds__(kT) void top_rows_kernel(const T* __restrict__ logi
 // Joins the stretches of a row: `count` keys (0: none), the k largest.
 template <typename T>
 __global__ __launch_bounds__(kT) void top_join_kernel(const T* __restrict__ logits, int64_t ld,
-                                                      const uint64_t* __restrict__ best, int64_t count, int32_t k,
-                                                      T* __restrict__ values, int32_t* __restrict__ index) {
+                                                      const uint64_t* __restrict__ best, int64_t count,
+                                                      int32_t class_bits, int32_t k, T* __restrict__ values,
+                                                      int32_t* __restrict__ index) {
     __shared__ Pool p;
     const int64_t r = blockIdx.x;
     if (threadIdx.x == 0) p.count = 0;
+    const int bits = (int)sizeof(T) * 8 + class_bits;
     uint64_t bound = 0;
     for (int64_t c = 0; c < count; c += kT * kVec) {
         uint64_t x[kVec];
@@ -169,9 +338,9 @@ __global__ __launch_bounds__(kT) void top_join_kernel(const T* __restrict__ logi
             const int64_t at = c + i * kT + threadIdx.x;
             x[i] = at < count ? best[r * count + at] : 0;
         }
-        offer(p, x, k, bound);
+        offer(p, x, k, bits, bound);
     }
-    write_best(p, k, logits + r * ld, values + r * k, index + r * k);
+    write_best(p, k, bits, class_bits, logits + r * ld, values + r * k, index + r * k);
 }
 
 // Stretches of a row: one when the rows alone fill the chip (4 work-groups
@@ -217,20 +386,22 @@ extern "C" int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, in
     if (!cv.ok)
         return set_error(GRWS_E_CAPACITY, "top_logits: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const int32_t stretch = (int32_t)((classes + n - 1) / n);
+    int32_t class_bits = 1;
+    while ((1ll << class_bits) < classes) ++class_bits;
     const dim3 grid((unsigned)rows, (unsigned)n);
 #define GRWS_TOP(T)                                                                                                \
     do {                                                                                                           \
         const T* x = static_cast<const T*>(logits);                                                                \
         T* v = static_cast<T*>(values);                                                                            \
         if (n == 1) {                                                                                              \
-            hipLaunchKernelGGL((top_rows_kernel<T, true>), grid, dim3(kT), 0, stream, x, ld, (int32_t)classes, k,  \
-                               stretch, v, index, best);                                                           \
+            hipLaunchKernelGGL((top_rows_kernel<T, true>), grid, dim3(kT), 0, stream, x, ld, (int32_t)classes,     \
+                               class_bits, k, stretch, v, index, best);                                                           \
         } else {                                                                                                   \
-            hipLaunchKernelGGL((top_rows_kernel<T, false>), grid, dim3(kT), 0, stream, x, ld, (int32_t)classes, k, \
-                               stretch, v, index, best);                                                           \
+            hipLaunchKernelGGL((top_rows_kernel<T, false>), grid, dim3(kT), 0, stream, x, ld, (int32_t)classes,    \
+                               class_bits, k, stretch, v, index, best);                                                           \
             GRWS_LAUNCH_CHECK();                                                                                   \
             hipLaunchKernelGGL(top_join_kernel<T>, dim3((unsigned)rows), dim3(kT), 0, stream, x, ld, best,         \
-                               (int64_t)n * k, k, v, index);                                                       \
+                               (int64_t)n * k, class_bits, k, v, index);                                                       \
         }                                                                                                          \
     } while (0)
     if (dtype == GRWS_F32) GRWS_TOP(float);
