@@ -7,6 +7,7 @@ allocated here with torch's caching allocator; the library allocates nothing.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import weakref
 import os
@@ -1885,31 +1886,45 @@ class HeadCall:
                                _row_pitch(self.weight), hidden.shape[0], n, hidden.shape[1], weight.shape[0], code,
                                k, int(k > 0 and self.index.dtype == torch.int64), float(temperature))
 
+    def saved_pointers(self, saved: torch.Tensor):
+        """Addresses of lse, the targets' logits and the teacher's
+        probabilities in the buffer that head_fwd saves."""
+        p, n = saved.data_ptr(), self.n
+        return p, p + 4 * n, p + 4 * n * (1 + self.k) if self.k else None
 
-def head_fwd(call: HeadCall):
-    """(loss f32 scalar, row_loss f32 [n], counts int64 [3] = {hits, counted
-    rows, bad input}, saved) of a HeadCall (csrc/head.hip); no host sync."""
+
+def _on_device(dev: torch.device):
+    """A context in which dev is the current device (none needed when it is)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def head_fwd(call: HeadCall, per_row: bool):
+    """(loss, counts int64 [3] = {hits, counted rows, bad input}, saved) of a
+    HeadCall (csrc/head.hip): the f32 mean, or per_row f32 [n].  saved: what
+    head_bwd takes.  No host sync."""
     dev = call.hidden.device
     n, k = call.n, call.k
-    f = torch.empty(1 + n * (2 + max(k, 1) + 2 * k), dtype=torch.float32, device=dev)
-    loss, row_loss, lse = f[0], f[1:1 + n], f[1 + n:1 + 2 * n]
-    logit = f[1 + 2 * n:1 + 2 * n + n * max(k, 1)]
-    prob = f[1 + 2 * n + n * max(k, 1):] if k else None
+    out = torch.empty((n,) if per_row else (), dtype=torch.float32, device=dev)
     counts = torch.empty(3, dtype=torch.int64, device=dev)
+    # lse [n], the targets' logits [n * max(k, 1)], the teacher's probabilities [2 * n * k]
+    saved = torch.empty(n * (1 + max(k, 1) + 2 * k), dtype=torch.float32, device=dev)
+    lse, logit, prob = call.saved_pointers(saved)
     ref = ctypes.byref(call.view)
-    wsb = int(L.load().grws_head_fwd_workspace_bytes(ref))
-    ws = torch.empty(max(1, wsb), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        L.call("grws_head_fwd", ref, L.ptr(lse), L.ptr(logit), L.ptr(prob), L.ptr(row_loss), L.ptr(loss),
-               L.ptr(counts), L.ptr(ws), wsb, L.stream_of(dev))
-    return loss, row_loss, counts, (lse, logit, prob)
+    lib = L.load()
+    wsb = lib.grws_head_fwd_workspace_bytes(ref)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        L.call("grws_head_fwd", ref, lse, logit, prob, out.data_ptr() if per_row else None,
+               None if per_row else out.data_ptr(), counts.data_ptr(), ws.data_ptr(), wsb, L.stream_of(dev))
+    return out, counts, saved
 
 
-def head_bwd(call: HeadCall, saved, counts: torch.Tensor, dloss: torch.Tensor, need=(True, True, True)):
+def head_bwd(call: HeadCall, saved: torch.Tensor, counts: torch.Tensor, dloss: torch.Tensor,
+             need=(True, True, True)):
     """(d_hidden, d_weight, d_bias), None where not needed, of head_fwd's
-    loss (dloss a scalar) or row_loss (dloss [n])."""
+    loss (dloss a scalar, or [n] per row)."""
     dev = call.hidden.device
-    lse, logit, prob = saved
+    lse, logit, prob = call.saved_pointers(saved)
     dl = dloss.detach().float().contiguous()
     dh = dw = db = None
     if need[0]:
@@ -1920,13 +1935,13 @@ def head_bwd(call: HeadCall, saved, counts: torch.Tensor, dloss: torch.Tensor, n
     if need[2] and call.bias is not None:
         db = torch.empty(call.bias.shape, dtype=call.bias.dtype, device=dev)
     ref = ctypes.byref(call.view)
-    wsb = int(L.load().grws_head_bwd_workspace_bytes(ref))
-    ws = torch.empty(max(1, wsb), dtype=torch.uint8, device=dev)
+    lib = L.load()
+    wsb = lib.grws_head_bwd_workspace_bytes(ref)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     width = call.hidden.shape[1]
-    with torch.cuda.device(dev):
-        L.call("grws_head_bwd", ref, L.ptr(lse), L.ptr(logit), L.ptr(prob), L.ptr(counts), L.ptr(dl),
-               int(dloss.dim() == 1), L.ptr(dh), width, L.ptr(dw), width, L.ptr(db), L.ptr(ws), wsb,
-               L.stream_of(dev))
+    with _on_device(dev):
+        L.call("grws_head_bwd", ref, lse, logit, prob, counts.data_ptr(), dl.data_ptr(), int(dloss.dim() == 1),
+               L.ptr(dh), width, L.ptr(dw), width, L.ptr(db), ws.data_ptr(), wsb, L.stream_of(dev))
     return dh, dw, db
 
 
@@ -1948,7 +1963,7 @@ def top_logits(logits: torch.Tensor, k: int):
     index = torch.empty((n, k), dtype=torch.int32, device=dev)
     wsb = int(L.load().grws_top_logits_workspace_bytes(n, classes, k))
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         L.call("grws_top_logits", L.ptr(x), code, _row_pitch(x), n, classes, k, L.ptr(values), L.ptr(index),
                L.ptr(ws), wsb, L.stream_of(dev))
     return values, index

@@ -399,6 +399,7 @@ struct GradArgs {
     const void* bias;
     int32_t bias_dt;
     const float* lse;        // [n], +inf for a row that does not count
+    const int64_t* labels;   // NULL: the targets are subtracted by head_subtract_kernel
     const float* row_scale;  // [n] or NULL
     float gscale;
     uint16_t* G;  // [planes][np][ldg]
@@ -455,12 +456,28 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
         const float l = row < a.n ? a.lse[row] : INFINITY;
         const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
 #pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                acc[i][j][e] = l == INFINITY ? 0.f : __builtin_amdgcn_exp2f(acc[i][j][e] - l);
+        if (a.labels) {
+            const int64_t lab = l != INFINITY ? a.labels[row] - a.v0 - pfirst : -1;
+            const bool here = lab >= 0 && lab < TP * 16;
+            if (__any(here)) {
+                const int at = here ? (int)lab - 4 * (lane >> 4) : -1;
+#pragma unroll
+                for (int i = 0; i < TP; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= at == 16 * i + e ? 1.f : 0.f;
+            }
+        }
+#pragma unroll
         for (int i = 0; i < TP; ++i) {
             const int64_t at = row * a.ldg + pfirst + 16 * i + 4 * (lane >> 4);
             uint16_t h[SPLIT ? 3 : 1][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = l == INFINITY ? 0.f : __builtin_amdgcn_exp2f(acc[i][j][e] - l) * s;
+                const float x = acc[i][j][e] * s;
                 if constexpr (SPLIT) split3(x, &h[0][e], &h[1][e], &h[2][e]);
                 else h[0][e] = round16<DT>(x);
             }
@@ -469,6 +486,34 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
                 *reinterpret_cast<u32x2_t*>(a.G + z * a.plane + at) =
                     u32x2_t{(uint32_t)h[z][0] | ((uint32_t)h[z][1] << 16),
                             (uint32_t)h[z][2] | ((uint32_t)h[z][3] << 16)};
+        }
+    }
+}
+
+// four consecutive elements of a row with `left` of them to go
+template <int OT>
+__device__ __forceinline__ void store4(void* out, int64_t at, float4_t v, int64_t left, int32_t vec) {
+    if constexpr (OT == GRWS_F32) {
+        float* o = static_cast<float*>(out) + at;
+        if (vec && left >= 4) {
+            *reinterpret_cast<float4_t*>(o) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < left) o[e] = v[e];
+        }
+    } else {
+        uint16_t* o = static_cast<uint16_t*>(out) + at;
+        uint16_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = round16<OT>(v[e]);
+        if (vec && left >= 4) {
+            *reinterpret_cast<u32x2_t*>(o) =
+                u32x2_t{(uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16)};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < left) o[e] = h[e];
         }
     }
 }
@@ -520,30 +565,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
         for (int i = 0; i < TP; ++i) {
             const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
             if (d >= a.width) continue;
-            const int64_t at = v * a.ldo + d;
-            if constexpr (OT == GRWS_F32) {
-                float* o = static_cast<float*>(a.out) + at;
-                if (a.vec && d + 4 <= a.width) {
-                    *reinterpret_cast<float4_t*>(o) = acc[i][j] * alpha;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < a.width) o[e] = acc[i][j][e] * alpha;
-                }
-            } else {
-                uint16_t* o = static_cast<uint16_t*>(a.out) + at;
-                uint16_t h[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) h[e] = round16<OT>(acc[i][j][e] * alpha);
-                if (a.vec && d + 4 <= a.width) {
-                    *reinterpret_cast<u32x2_t*>(o) =
-                        u32x2_t{(uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16)};
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < a.width) o[e] = h[e];
-                }
-            }
+            store4<OT>(a.out, v * a.ldo + d, acc[i][j] * alpha, a.width - d, a.vec);
         }
     }
 }
@@ -556,9 +578,16 @@ struct HiddenArgs {
     float* part;  // [splits][np][dp]
     int64_t np, dp;
     int32_t first;  // the first piece stores
+    // the last piece of a single run writes dH itself
+    int32_t last;
+    int32_t vec;  // rows of the output take 4-element stores
+    const float* alpha;
+    void* out;
+    int64_t ldo, n, width, hidden_rows;
+    const int64_t* rows;
 };
 
-template <int DT, int BP, int BQ, int WP, int WQ>
+template <int DT, int OT, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a) {
     using C = Core<DT, true, false, BP, BQ, WP, WQ>;
     constexpr int TP = C::TP, TQ = C::TQ;
@@ -571,15 +600,23 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
     float4_t acc[TP][TQ];
     C::run(a.g, tp, tq, kb, ke, s0, s1, acc);
     float* out = a.part + sp * a.np * a.dp;
+    const float alpha = a.last ? *a.alpha : 0.f;
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
+        int64_t to = -1;
+        if (a.last && row < a.n) {
+            to = a.rows ? a.rows[row] : row;
+            if (to >= a.hidden_rows) to = -1;
+        }
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
             const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
             if (d >= a.dp) continue;
             float4_t* o = reinterpret_cast<float4_t*>(out + row * a.dp + d);
-            *o = a.first ? acc[i][j] : *o + acc[i][j];
+            const float4_t v = a.first ? acc[i][j] : *o + acc[i][j];
+            if (!a.last) *o = v;
+            else if (to >= 0 && d < a.width) store4<OT>(a.out, to * a.ldo + d, v * alpha, a.width - d, a.vec);
         }
     }
 }
@@ -630,6 +667,17 @@ __device__ __forceinline__ int row_state(const Targets& t, int64_t i, int sub) {
     return st & 2 ? 2 : st;
 }
 
+// The factor of the gradient sums: dloss T / (counted gscale), or for a
+// gradient per row the largest |dloss| in place of dloss / counted, with
+// the rows' shares of it in row_scale (so that G stays within 16 bits' range)
+struct Alpha {
+    float* out;  // NULL: none
+    const float* dloss;
+    const int64_t* counts;
+    const uint32_t* most;  // NULL: of the mean
+    float factor;
+};
+
 // Copies a row of `width` elements to dp 16-bit elements (three planes of
 // f32), zeros past the width; a wave, 8 elements a lane.
 template <typename T, bool SPLIT>
@@ -665,14 +713,22 @@ __device__ __forceinline__ void pack_row(const T* __restrict__ x, bool live, int
 // hidden[rows] in the layout the products read: np rows of dp elements (one
 // plane, or three for f32), zeros past n and the width and in rows that do
 // not count (what such a row holds, NaN too, stays out of every sum).
-// One wave per row.
+// One wave per row; the first also makes alpha (see Alpha) or clears `done`.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void head_pack_hidden_kernel(Targets t, const T* __restrict__ hidden, int64_t ld,
                                                                int64_t n, int64_t np, int64_t width, int64_t dp,
-                                                               int32_t vec, uint16_t* __restrict__ out) {
+                                                               int32_t vec, uint16_t* __restrict__ out, Alpha al,
+                                                               int32_t* __restrict__ done) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= np) return;
+    if (i == 0 && lane == 0) {
+        if (done) *done = 0;
+        if (al.out) {
+            if (al.most) *al.out = __uint_as_float(*al.most) * al.factor;
+            else *al.out = al.counts[1] > 0 ? al.dloss[0] / (float)al.counts[1] * al.factor : 0.f;
+        }
+    }
     const bool live = i < n && row_state<64>(t, i, lane) == 1;
     const T* x = hidden + (live ? (t.rows ? t.rows[i] : i) * ld : 0);
     pack_row<T, SPLIT>(x, live, width, dp, vec, out + i * dp, np * dp, lane);
@@ -714,14 +770,15 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
                                                            const T* __restrict__ w, int64_t ldw, const T* bias,
                                                            int64_t n, int64_t width, int32_t vec, float inv_t,
                                                            float c1, float* __restrict__ prob,
-                                                           float* __restrict__ y) {
+                                                           float* __restrict__ y, int32_t* __restrict__ state) {
     const int lane = threadIdx.x & 63;
     const int groups = (t.k + 3) / 4;
     const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (at >= n * groups) return;
     const int64_t i = at / groups;
     const int k0 = (int)(at - i * groups) * 4;
-    const bool live = row_state<64>(t, i, lane) == 1;  // uniform over the wave
+    const int st = row_state<64>(t, i, lane);
+    const bool live = st == 1;  // uniform over the wave
     {
         const T* h = hidden + (live ? (t.rows ? t.rows[i] : i) * ldh : 0);
         const int k = k0 + (lane >> 4);
@@ -747,6 +804,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
             y[i * t.k + k] = idx >= 0 ? (d + (bias ? to_float(bias[idx]) : 0.f)) * c1 : 0.f;
     }
     if (k0 != 0) return;
+    if (lane == 0) state[i] = st;
     float m = -INFINITY;
     for (int k = lane; k < t.k && live; k += 64)
         if (teacher_listed(t, i, k, teacher_at(t, i, k))) m = fmaxf(m, t.tlogit[i * t.k + k] * inv_t);
@@ -799,15 +857,42 @@ __device__ __forceinline__ void join(float& m, float& s, int& first, float om, f
     }
 }
 
+// loss = sum / counted (NaN when no row counts or an input is bad), by one
+// wave; parts are added in a fixed order
+__device__ __forceinline__ void finish_loss(const volatile double* part_loss, const volatile int32_t* part_cnt,
+                                            int64_t nparts, int lane, float* loss, int64_t* counts) {
+    double L = 0.0;
+    long long C = 0, V = 0, B = 0;
+    for (int64_t k = lane; k < nparts; k += 64) {
+        L += part_loss[k];
+        C += part_cnt[3 * k];
+        V += part_cnt[3 * k + 1];
+        B |= part_cnt[3 * k + 2];
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        L += __shfl_xor(L, d, kWave);
+        C += __shfl_xor(C, d, kWave);
+        V += __shfl_xor(V, d, kWave);
+        B |= __shfl_xor(B, d, kWave);
+    }
+    if (lane != 0) return;
+    if (loss) loss[0] = (B || V == 0) ? __int_as_float(0x7fc00000) : (float)(L / (double)V);
+    counts[0] = C;
+    counts[1] = V;
+    counts[2] = B;
+}
+
 // Joins the strips of 16 rows (32 at a time: 4 a wave, 8 waves), then the
-// rows' losses; block partials of (loss, hits, counted rows, bad input).
+// rows' losses, and their mean and counts (loss_out and row_loss may be NULL).
 __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2* __restrict__ part, int64_t strips,
                                                         int32_t strip_classes, int64_t n, int64_t np,
                                                         float temperature, const float* __restrict__ y,
                                                         const float* __restrict__ prob,
-                                                        const int32_t* __restrict__ earlier, float* __restrict__ lse,
-                                                        float* __restrict__ row_loss, double* __restrict__ part_loss,
-                                                        int32_t* __restrict__ part_cnt) {
+                                                        const int32_t* __restrict__ flags, float* __restrict__ lse,
+                                                        float* __restrict__ row_loss, double* part_loss,
+                                                        int32_t* part_cnt, int32_t* done,
+                                                        float* __restrict__ loss_out, int64_t* __restrict__ counts) {
     __shared__ float sm[32][16], ss[32][16];
     __shared__ int sa[32][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -847,18 +932,8 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             join(m, s, first, om, os, of);
         }
     }
-    // the rows' states: a distillation's lists are looked through by 64 lanes
     int st = 0;
-    if (t.labels) {
-        if (i < n) st = row_state<1>(t, i, 0);
-    } else {
-        for (int x = 0; x < 16; ++x) {
-            const int64_t row = (int64_t)blockIdx.x * 16 + x;
-            if (row >= n) break;  // uniform
-            const int v = row_state<64>(t, row, lane);
-            if (r == x) st = v;
-        }
-    }
+    if (i < n) st = t.labels ? row_state<1>(t, i, 0) : flags[i];
     const float l = m + log2f(s);
     float a = 0.f;
     if (!t.labels && st == 1) {
@@ -880,7 +955,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             if (t.labels) {
                 const float yl = y[i];
                 v = (l - yl) * kLn2;
-                hit = yl == m && !earlier[i] && first == (int)(t.labels[i] / strip_classes);
+                hit = yl == m && !flags[i] && first == (int)(t.labels[i] / strip_classes);
             } else {
                 v = a * temperature * temperature;
             }
@@ -890,7 +965,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             v = __int_as_float(0x7fc00000);
         }
         lse[i] = st == 1 ? l : INFINITY;
-        row_loss[i] = v;
+        if (row_loss) row_loss[i] = v;
     }
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) {
@@ -899,62 +974,29 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
         valid += __shfl_xor(valid, d, kWave);
         bad |= __shfl_xor(bad, d, kWave);
     }
+    // the last work-group to arrive adds the parts, in their order
+    int last = 0;
     if (lane == 0) {
         part_loss[blockIdx.x] = loss;
         part_cnt[3 * blockIdx.x] = hit;
         part_cnt[3 * blockIdx.x + 1] = valid;
         part_cnt[3 * blockIdx.x + 2] = bad;
     }
+    if (!done) return;
+    if (lane == 0) {
+        __threadfence();
+        last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+    }
+    if (!__shfl(last, 0, kWave)) return;
+    __threadfence();
+    finish_loss(part_loss, part_cnt, gridDim.x, lane, loss_out, counts);
 }
 
-// loss = sum / counted (NaN when no row counts or an input is bad); one
-// work-group, parts added in a fixed order
-__global__ __launch_bounds__(256) void head_finish_kernel(const double* __restrict__ part_loss,
-                                                          const int32_t* __restrict__ part_cnt, int64_t nparts,
-                                                          float* __restrict__ loss, int64_t* __restrict__ counts) {
-    __shared__ double sl[4];
-    __shared__ long long sc[3][4];
-    double L = 0.0;
-    long long C = 0, V = 0, B = 0;
-    for (int64_t k = threadIdx.x; k < nparts; k += 256) {
-        L += part_loss[k];
-        C += part_cnt[3 * k];
-        V += part_cnt[3 * k + 1];
-        B |= part_cnt[3 * k + 2];
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        L += __shfl_xor(L, d, kWave);
-        C += __shfl_xor(C, d, kWave);
-        V += __shfl_xor(V, d, kWave);
-        B |= __shfl_xor(B, d, kWave);
-    }
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-        sl[wave] = L;
-        sc[0][wave] = C;
-        sc[1][wave] = V;
-        sc[2][wave] = B;
-    }
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    C = sc[0][0] + sc[0][1] + sc[0][2] + sc[0][3];
-    V = sc[1][0] + sc[1][1] + sc[1][2] + sc[1][3];
-    B = sc[2][0] | sc[2][1] | sc[2][2] | sc[2][3];
-    loss[0] = (B || V == 0) ? __int_as_float(0x7fc00000) : (float)(L / (double)V);
-    counts[0] = C;
-    counts[1] = V;
-    counts[2] = B;
-}
-
-// The factor of the gradient sums: dloss T / (counted gscale), or for a
-// gradient per row the largest |dloss| in place of dloss / counted, with
-// the rows' shares of it in row_scale (so that G stays within 16 bits' range)
-__global__ void head_alpha_kernel(const float* __restrict__ dloss, const int64_t* __restrict__ counts, int per_row,
-                                  float factor, float* __restrict__ alpha, const uint32_t* __restrict__ most) {
-    if (per_row) alpha[0] = __uint_as_float(*most) * factor;
-    else alpha[0] = counts[1] > 0 ? dloss[0] / (float)counts[1] * factor : 0.f;
+// the same in a launch of its own (also of no rows at all)
+__global__ __launch_bounds__(64) void head_finish_kernel(const double* part_loss, const int32_t* part_cnt,
+                                                         int64_t nparts, float* __restrict__ loss,
+                                                         int64_t* __restrict__ counts) {
+    finish_loss(part_loss, part_cnt, nparts, threadIdx.x, loss, counts);
 }
 
 __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict__ dloss,
@@ -981,7 +1023,8 @@ __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __rest
     scale[i] = m > 0.f ? dloss[i] / m : 0.f * m;
 }
 
-// G at the targets: the rounded p - q, q the entry's coefficient.
+// G at a teacher's entries: the rounded p - q, q the entry's coefficient.
+// (A label's place is known to the product's epilogue: one for a row.)
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const float* __restrict__ lse,
                                                             const float* __restrict__ y,
@@ -989,13 +1032,12 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const flo
                                                             const float* __restrict__ row_scale, float gscale,
                                                             int64_t n, int64_t v0, int64_t vc, uint16_t* G,
                                                             int64_t ldg, int64_t plane) {
-    const int K = t.labels ? 1 : t.k;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= n * K) return;
-    const int64_t i = at / K;
-    const int64_t v = t.labels ? t.labels[i] : teacher_at(t, i, (int)(at - i * K));
+    if (at >= n * t.k) return;
+    const int64_t i = at / t.k;
+    const int64_t v = teacher_at(t, i, (int)(at - i * t.k));
     if (v < v0 || v >= v0 + vc) return;
-    const float q = t.labels ? 1.f : coef[at], l = lse[i];
+    const float q = coef[at], l = lse[i];
     if (q < 0.f || l == INFINITY) return;
     const float s = row_scale ? row_scale[i] * gscale : gscale;
     store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[at] - l) - q) * s);
@@ -1101,6 +1143,10 @@ __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __res
 int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 int64_t ceil_div(int64_t x, int64_t a) { return (x + a - 1) / a; }
 
+// work-groups of head_join_kernel up to which the last of them finishes the
+// loss (each writes its L2's lines back for it: 1,024 of them take 29 us more
+// against a launch of 5)
+constexpr int64_t kJoinBlocks = 64;
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // G of a piece, and a packed piece of W
 
 // A product's tile and the runs that its k is cut into: the least of
@@ -1209,9 +1255,9 @@ Targets targets_of(const grws_head* h) {
 struct FwdSpace {
     uint16_t *hp, *wp;
     float2* part;
-    int32_t* earlier;
+    int32_t* flags;  // labels: StatsArgs::earlier; a teacher's lists: the rows' states
     double* pl;
-    int32_t* pc;
+    int32_t *pc, *done;
 };
 
 template <typename A>
@@ -1224,9 +1270,10 @@ void fwd_space(A& a, const Shape& s, FwdSpace* f) {
     take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
     take(f->part, s.strips * s.np);
-    take(f->earlier, s.n);
+    take(f->flags, s.n);
     take(f->pl, ceil_div(s.n, 16));
     take(f->pc, 3 * ceil_div(s.n, 16));
+    take(f->done, 1);
 }
 
 struct BwdSpace {
@@ -1245,7 +1292,7 @@ void bwd_space(A& a, const Shape& s, BwdSpace* f) {
     take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
     take(f->G, s.planes * s.np * s.vp);
-    take(f->dh, s.hidden.splits * s.np * s.dp);
+    if (s.hidden.splits > 1 || s.vp < s.V) take(f->dh, s.hidden.splits * s.np * s.dp);
     if (s.weight.splits > 1) take(f->dw, s.weight.splits * s.vp * s.dp);
     take(f->bias, s.np / kBiasRows * s.vp);
     take(f->alpha, 1);
@@ -1258,15 +1305,18 @@ bool rows_of_16(const void* p, int64_t ld, int32_t dtype) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (dtype == GRWS_F32 ? 4 : 8) == 0;
 }
 
-int pack_hidden(const grws_head* h, const Shape& s, const Targets& t, uint16_t* hp, hipStream_t stream) {
+int pack_hidden(const grws_head* h, const Shape& s, const Targets& t, uint16_t* hp, const Alpha& alpha,
+                int32_t* done, hipStream_t stream) {
     const dim3 grid((unsigned)ceil_div(s.np, 4));
     const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype);
     if (s.split)
         hipLaunchKernelGGL((head_pack_hidden_kernel<float, true>), grid, dim3(256), 0, stream, t,
-                           static_cast<const float*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp);
+                           static_cast<const float*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp, alpha,
+                           done);
     else
         hipLaunchKernelGGL((head_pack_hidden_kernel<uint16_t, false>), grid, dim3(256), 0, stream, t,
-                           static_cast<const uint16_t*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp);
+                           static_cast<const uint16_t*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp, alpha,
+                           done);
     GRWS_LAUNCH_CHECK();
     return GRWS_OK;
 }
@@ -1340,13 +1390,14 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
     clear_error();
     hipStream_t stream = as_stream(stream_);
     GRWS_TRY(check_head(h));
-    GRWS_CHECK_ARG(loss && counts, "head: null output");
+    GRWS_CHECK_ARG(counts && (loss || row_loss || h->n == 0), "head: null output");
     if (h->n == 0) {
-        hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(256), 0, stream, nullptr, nullptr, 0, loss, counts);
+        hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(64), 0, stream, nullptr, nullptr, (int64_t)0, loss,
+                           counts);
         GRWS_LAUNCH_CHECK();
         return GRWS_OK;
     }
-    GRWS_CHECK_ARG(lse && target_logit && row_loss && (h->k == 0 || target_prob), "head: null output");
+    GRWS_CHECK_ARG(lse && target_logit && (h->k == 0 || target_prob), "head: null output");
     const Shape s = shape_of(h, false);
     const Targets t = targets_of(h);
     Carver cv(workspace, workspace_bytes);
@@ -1354,13 +1405,13 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
     fwd_space(cv, s, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
-    GRWS_TRY(pack_hidden(h, s, t, f.hp, stream));
+    GRWS_TRY(pack_hidden(h, s, t, f.hp, Alpha{}, f.done, stream));
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
         StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, s.np, c1,
-                    h->bias, h->dtype, h->labels, f.part, target_logit, f.earlier};
+                    h->bias, h->dtype, h->labels, f.part, target_logit, f.flags};
         if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
         else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
     }
@@ -1371,7 +1422,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
 #define GRWS_HEAD_TARGETS(T)                                                                                         \
     hipLaunchKernelGGL(head_targets_kernel<T>, grid, dim3(256), 0, stream, t, static_cast<const T*>(h->hidden),      \
                        h->ld_hidden, static_cast<const T*>(h->weight), h->ld_weight, static_cast<const T*>(h->bias), \
-                       s.n, s.D, vec, 1.f / h->temperature, c1, target_prob, target_logit)
+                       s.n, s.D, vec, 1.f / h->temperature, c1, target_prob, target_logit, f.flags)
         if (h->dtype == GRWS_F32) GRWS_HEAD_TARGETS(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_TARGETS(_Float16);
         else GRWS_HEAD_TARGETS(__hip_bfloat16);
@@ -1380,11 +1431,13 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
     }
     const int64_t blocks = ceil_div(s.n, 16);
     hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part, ceil_div(s.V, s.strip_classes),
-                       (int32_t)s.strip_classes, s.n, s.np, h->temperature, target_logit, target_prob, f.earlier, lse,
-                       row_loss, f.pl, f.pc);
+                       (int32_t)s.strip_classes, s.n, s.np, h->temperature, target_logit, target_prob, f.flags, lse,
+                       row_loss, f.pl, f.pc, blocks <= kJoinBlocks ? f.done : nullptr, loss, counts);
     GRWS_LAUNCH_CHECK();
-    hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(256), 0, stream, f.pl, f.pc, blocks, loss, counts);
-    GRWS_LAUNCH_CHECK();
+    if (blocks > kJoinBlocks) {
+        hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(64), 0, stream, f.pl, f.pc, blocks, loss, counts);
+        GRWS_LAUNCH_CHECK();
+    }
     return GRWS_OK;
 }
 
@@ -1436,10 +1489,8 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         GRWS_LAUNCH_CHECK();
         row_scale = f.scale;
     }
-    hipLaunchKernelGGL(head_alpha_kernel, dim3(1), dim3(1), 0, stream, dloss, counts, per_row,
-                       h->temperature / gscale, f.alpha, f.most);
-    GRWS_LAUNCH_CHECK();
-    GRWS_TRY(pack_hidden(h, s, t, f.hp, stream));
+    const Alpha alpha{f.alpha, dloss, counts, per_row ? f.most : nullptr, h->temperature / gscale};
+    GRWS_TRY(pack_hidden(h, s, t, f.hp, alpha, nullptr, stream));
     const int64_t plane = s.np * s.vp;
     const size_t esz = dtype_size(h->dtype);
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
@@ -1448,23 +1499,21 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
         GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, c1, h->bias,
-                   h->dtype, lse, row_scale, gscale, f.G, s.vp, plane};
-        const dim3 sgrid((unsigned)ceil_div(s.n * (h->k ? h->k : 1), 256));
-#define GRWS_HEAD_SUB(DT, SP)                                                                                       \
-    hipLaunchKernelGGL((head_subtract_kernel<DT, SP>), sgrid, dim3(256), 0, stream, t, lse, target_logit,           \
-                       coef, row_scale, gscale, s.n, v0, vc, f.G, s.vp, plane)
-        if (s.split) {
-            GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, true);
-            GRWS_HEAD_SUB(GRWS_BF16, true);
-        } else if (h->dtype == GRWS_F16) {
-            GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_F16, false);
-            GRWS_HEAD_SUB(GRWS_F16, false);
-        } else {
-            GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, false);
-            GRWS_HEAD_SUB(GRWS_BF16, false);
-        }
+                   h->dtype, lse, h->labels, row_scale, gscale, f.G, s.vp, plane};
+        if (s.split) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, true);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_F16, false);
+        else GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, false);
+        if (h->k > 0) {
+            const dim3 grid((unsigned)ceil_div(s.n * h->k, 256));
+#define GRWS_HEAD_SUB(DT, SP)                                                                                 \
+    hipLaunchKernelGGL((head_subtract_kernel<DT, SP>), grid, dim3(256), 0, stream, t, lse, target_logit, coef, \
+                       row_scale, gscale, s.n, v0, vc, f.G, s.vp, plane)
+            if (s.split) GRWS_HEAD_SUB(GRWS_BF16, true);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_SUB(GRWS_F16, false);
+            else GRWS_HEAD_SUB(GRWS_BF16, false);
 #undef GRWS_HEAD_SUB
-        GRWS_LAUNCH_CHECK();
+            GRWS_LAUNCH_CHECK();
+        }
         const char* gp = reinterpret_cast<const char*>(f.G);
         if (d_bias) {
             const int64_t nparts = s.np / kBiasRows;
@@ -1513,12 +1562,16 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         if (d_hidden) {
             GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, false, stream));
             const Opnd G{gp, s.vp * 2, plane * 2, s.np, vt};
-            HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc), f.dh, s.np, s.dp, v0 == 0};
-            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16);
-            else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16);
+            const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
+            HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc), f.dh, s.np, s.dp, v0 == 0,
+                         s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
+                         h->hidden_rows, h->rows};
+            if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
+            else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
         }
     }
-    if (d_hidden) {
+    if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
                        s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, f.alpha, static_cast<T*>(d_hidden), ld_dh)

@@ -26,16 +26,16 @@ class _Head(Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, rows, labels, teacher_index, teacher_logits, temperature, per_row):
         call = _ops.HeadCall(hidden, weight, bias, rows, labels, teacher_index, teacher_logits, temperature)
-        loss, row_loss, counts, saved = _ops.head_fwd(call)
+        loss, counts, saved = _ops.head_fwd(call, per_row)
         if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(hidden, weight, bias, rows, labels, teacher_index, teacher_logits, counts, *saved)
+            ctx.save_for_backward(hidden, weight, bias, rows, labels, teacher_index, teacher_logits, counts, saved)
             ctx.temperature = temperature
         ctx.mark_non_differentiable(counts)
-        return (row_loss if per_row else loss), counts
+        return loss, counts
 
     @staticmethod
     def backward(ctx, dloss, _dcounts):
-        hidden, weight, bias, rows, labels, index, logits, counts, *saved = ctx.saved_tensors
+        hidden, weight, bias, rows, labels, index, logits, counts, saved = ctx.saved_tensors
         call = _ops.HeadCall(hidden, weight, bias, rows, labels, index, logits, ctx.temperature)
         grads = _ops.head_bwd(call, saved, counts, dloss, ctx.needs_input_grad[:3])
         return (*grads, None, None, None, None, None, None)
@@ -44,13 +44,11 @@ class _Head(Function):
 def _apply(hidden, weight, bias, rows, labels, index, logits, temperature, reduction):
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS} (got {reduction!r})")
-    if torch.is_autocast_enabled("cuda") and hidden.is_cuda:
+    if hidden.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dt), weight.to(dt)
         bias = bias.to(dt) if bias is not None else None
-    with torch.autocast("cuda", enabled=False):
-        return _Head.apply(hidden, weight, bias, rows, labels, index, logits, float(temperature),
-                           reduction == "none")
+    return _Head.apply(hidden, weight, bias, rows, labels, index, logits, float(temperature), reduction == "none")
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,

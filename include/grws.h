@@ -843,7 +843,8 @@ int grws_cross_entropy_bwd(const void* logits, int32_t dtype, int64_t ld, int64_
 /* target_prob f32 [2 x n x k] (k > 0), which the backward takes; row_loss   */
 /* f32 [n] (0 for rows that do not count, NaN for bad input); loss f32 scalar,   */
 /* the mean over counted rows (NaN when none counts or an input is bad: a    */
-/* label, class index or row id out of range); counts int64 [3] = {rows      */
+/* label, class index or row id out of range; loss or row_loss may be NULL,  */
+/* not both); counts int64 [3] = {rows                                       */
 /* whose label is the first largest logit (k = 0), counted rows, bad input}. */
 /* Backward of dloss (f32 scalar of the mean, or with per_row [n] of         */
 /* row_loss): d_hidden (rows of `rows`; zero the others first), d_weight and */

@@ -450,6 +450,18 @@ def test_autocast(cuda_device):
         assert a.dtype == torch.float32 and torch.equal(a, r.float())
 
 
+def test_loss_may_change_in_place(cuda_device):
+    """Dividing the loss in place (gradient accumulation) leaves what the
+    backward needs alone."""
+    h, w, _, labels = _inputs(cuda_device, 30, 16, 60, torch.float32, 12)
+    h.requires_grad_(True)
+    loss, _ = linear_cross_entropy(h, w, labels)
+    want = torch.autograd.grad(loss, [h])[0]
+    loss, _ = linear_cross_entropy(h, w, labels)
+    loss /= 4
+    assert float((torch.autograd.grad(loss, [h])[0] - want / 4).abs().max()) <= 1e-7
+
+
 def test_skips_what_needs_no_gradient(cuda_device):
     h, w, b, labels = _inputs(cuda_device, 90, 48, 200, torch.bfloat16, 12, bias=True)
     every = [x.requires_grad_(True) for x in (h, w, b)]
