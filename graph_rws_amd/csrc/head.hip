@@ -57,7 +57,7 @@ typedef __attribute__((address_space(3))) short8_t lds_short8_t;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef __attribute__((address_space(3))) char lds_char_t;
 
-constexpr int kK = 64;               // k per LDS stage
+constexpr int kK = 64;               // k of a stage; the operands' k is padded to whole stages
 constexpr int64_t kIgnoreLabel = -100;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -76,7 +76,7 @@ struct Opnd {
 struct Gemm {
     Opnd P, Q;
     int32_t nseg;    // plane products: 1, or 6 for split f32 operands
-    int32_t ksteps;  // stages of 64 k per plane product
+    int32_t ksteps;  // stages per plane product
     int32_t tp, tq;  // tiles along p and q
     int32_t splits;  // work-groups per tile along k
 };
@@ -97,16 +97,33 @@ __device__ __forceinline__ float4_t mma(short8_t a, short8_t b, float4_t c) {
 }
 
 // One operand's tile of B rows (or columns) of a stage: its direct loads and
-// its fragment reads.
-template <bool STRIDED, int B, int NW>
+// its fragment reads.  PAIRED (P contiguous along k only): fragments 2 i and
+// 2 i + 1 share 32 rows so that a lane's outputs of both are 8 consecutive
+// ones: row r of fragment f is row 8 (r / 4) + 4 (f % 2) + r % 4.
+template <bool STRIDED, int B, int NW, bool PAIRED = false>
 struct Tile {
-    static constexpr int NL = B / 8 / NW;  // 1 KiB loads per wave and stage
-    static_assert(NL >= 1 && NL * NW * 8 == B, "tile does not split over the waves");
+    static constexpr int BYTES = B * kK * 2;
+    static constexpr int NL = BYTES / 1024 / NW;  // 1 KiB loads per wave and stage
+    static_assert(NL == 4 && NL * NW * 1024 == BYTES, "four loads a wave");
+    static constexpr int CH = STRIDED ? B / 8 : kK / 8;  // 16-byte chunks per row
+    static constexpr int ROWS = 64 / CH;                 // rows of a load
     const char* base;
     int64_t ld, plane, left;  // left: strided: k rows; contiguous: k
     int64_t edge;             // bytes: strided: of the last row; contiguous: up to the last row
-    uint32_t off[NL];
-    int kfirst;  // contiguous: first k of the lane's chunk
+    uint32_t off[2];          // of the loads' two patterns
+    int kfirst[2];            // contiguous: first k of the lane's chunk
+    const char* cur;          // of the next load
+    int64_t rec, some;        // bytes and k from there on
+
+    // what a row's chunks (strided: pairs of them) are XORed with, so that
+    // the rows that one LDS read takes lie in different banks
+    static __device__ __forceinline__ int key(int row) {
+        if constexpr (STRIDED) return ((row & 3) | (((row >> 3) & 3) << 2)) & (CH / 2 - 1);
+        else return PAIRED ? (row & 3) | ((row >> 1) & 4) : row & 7;
+    }
+    // loads 0..3 have the keys of loads 0 1 0 1 (ROWS < 4 or 8) or 0 0 2 2
+    static constexpr int pattern(int i) { return STRIDED && ROWS == 4 ? i >> 1 : i & 1; }
+    static constexpr int first_of(int pat) { return STRIDED && ROWS == 4 ? 2 * pat : pat; }
 
     __device__ __forceinline__ void init(const Opnd& o, int64_t t0, int wave, int lane) {
         ld = o.ld;
@@ -116,57 +133,61 @@ struct Tile {
             base = o.p + t0 * ld;
             const int64_t rows = o.rows - t0 < B ? o.rows - t0 : B;
             edge = (rows - 1) * ld;
-            const int chunk = (lane & 7) ^ (lane >> 3);
-            kfirst = chunk * 8;
-#pragma unroll
-            for (int i = 0; i < NL; ++i)
-                off[i] = (uint32_t)(((wave * NL + i) * 8 + (lane >> 3)) * ld) + chunk * 16;
         } else {
             base = o.p + t0 * 2;
             edge = (o.rows - t0) * 2;
-            kfirst = 0;
-            constexpr int CH = B / 8;  // 16-byte chunks per row
+        }
 #pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int row = (wave * NL + i) * (64 / CH) + lane / CH;
-                const int key = ((row & 3) | (((row >> 3) & 3) << 2)) & (CH / 2 - 1);
-                off[i] = (uint32_t)(row * ld) + (uint32_t)(((lane % CH) ^ (key << 1)) * 16);
-            }
+        for (int v = 0; v < 2; ++v) {
+            const int row = (wave * NL + first_of(v)) * ROWS + lane / CH;
+            const int chunk = (lane % CH) ^ (STRIDED ? key(row) << 1 : key(row));
+            off[v] = (uint32_t)(row * ld) + (uint32_t)(chunk * 16);
+            kfirst[v] = chunk * 8;
         }
     }
-    __device__ __forceinline__ void load(char* lds, int pl, int64_t k0, int wave) const {
-        const char* b;
-        int64_t rec;
+    // the next load() reads plane `pl` from k0 on
+    __device__ __forceinline__ void start(int pl, int64_t k0) {
         if constexpr (!STRIDED) {
-            b = base + pl * plane + k0 * 2;
+            cur = base + pl * plane + k0 * 2;
             rec = edge + (left - k0) * 2;
         } else {
-            b = base + pl * plane + k0 * ld;
-            rec = left > k0 ? (left - k0 - 1) * ld + edge : 0;
-            if (rec > 0x7fffffff) rec = 0x7fffffff;
+            cur = base + pl * plane + k0 * ld;
+            rec = (left - k0 - 1) * ld + edge;
         }
+        some = left - k0;
+    }
+    __device__ __forceinline__ void load(char* lds, int wave) {
+        int records = rec > 0x7fffffff ? 0x7fffffff : (int)rec;
+        if constexpr (STRIDED) records = rec < 0 ? 0 : records;
         const __amdgpu_buffer_rsrc_t rs =
-            __builtin_amdgcn_make_buffer_rsrc((void*)b, (short)0, (int)rec, 0x00020000);
+            __builtin_amdgcn_make_buffer_rsrc((void*)cur, (short)0, records, 0x00020000);
+#pragma unroll
+        for (int v = 0; v < 2; ++v) asm volatile("" : "+v"(off[v]));  // the four sums are made here, not kept
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            uint32_t o = off[i];
-            if constexpr (!STRIDED) o = kfirst < left - k0 ? o : kPastEnd;  // past the row's k: not the next row's
+            const int v = pattern(i);
+            uint32_t o = off[v] + (uint32_t)((i - first_of(v)) * ROWS * ld);
+            if constexpr (!STRIDED) o = kfirst[v] < some ? o : kPastEnd;  // past the row's k: not the next row's
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)((lds_char_t*)lds + (wave * NL + i) * 1024), 16,
                                                      (int)o, 0, 0, 0);
         }
+        const int64_t step = STRIDED ? kK * ld : kK * 2;
+        cur += step;
+        rec -= step;
+        some -= kK;
     }
-    // 16 rows (columns) first..first+15 and k = 32 half + 8 (lane / 16) + 0..7
-    // as an MFMA operand: lane l holds row l % 16.
-    static __device__ __forceinline__ short8_t frag(const char* lds, int first, int half, int lane) {
+    // rows (columns) of fragment f from `first` and k = 32 half + 8 (lane / 16)
+    // + 0..7 as an MFMA operand: lane l holds row l % 16.
+    static __device__ __forceinline__ short8_t frag(const char* lds, int first, int f, int half, int lane) {
         if constexpr (!STRIDED) {
             const int r = lane & 15;
-            const char* p = lds + (first + r) * 128 + (((half * 4 + (lane >> 4)) ^ (r & 7)) * 16);
+            const int in = PAIRED ? 32 * (f >> 1) + 8 * (r >> 2) + 4 * (f & 1) + (r & 3) : 16 * f + r;
+            const char* p = lds + (first + in) * (kK * 2) + (((half * 4 + (lane >> 4)) ^ key(in)) * 16);
             return *(const lds_short8_t*)(lds_char_t*)p;
         } else {
             const int g = lane >> 4, a = (lane >> 2) & 3;
-            constexpr int CH = B / 8;
-            const int key = (a | (g << 2)) & (CH / 2 - 1);
-            const char* p = lds + (32 * half + 8 * g + a) * (B * 2) + ((first / 16) ^ key) * 32 + (lane & 3) * 8;
+            const char* p = lds + (32 * half + 8 * g + a) * (B * 2) + ((first / 16 + f) ^ key(8 * g + a)) * 32 +
+                            (lane & 3) * 8;
             const short4_t lo = __builtin_bit_cast(short4_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
                                                                  (lds_v4bf16_t*)(lds_char_t*)p));
             const short4_t hi = __builtin_bit_cast(short4_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
@@ -197,14 +218,25 @@ template <int DT, bool PS, bool QS, int BP, int BQ, int WP, int WQ>
 struct Core {
     static constexpr int NW = WP * WQ;
     static constexpr int TP = BP / WP / 16, TQ = BQ / WQ / 16;
-    static constexpr int STAGE = (BP + BQ) * 128;
-    using TileP = Tile<PS, BP, NW>;
+    static constexpr bool PAIRED = !PS;
+    using TileP = Tile<PS, BP, NW, PAIRED>;
     using TileQ = Tile<QS, BQ, NW>;
+    // p of element e of accumulator i, of the wave's block
+    static __device__ __forceinline__ int p_of(int i, int lane) {
+        return PAIRED ? 32 * (i >> 1) + 8 * (lane >> 4) + 4 * (i & 1) : 16 * i + 4 * (lane >> 4);
+    }
 
-    // acc[i][j]: lane l, element e: p = 16 i + 4 (l / 16) + e, q = 16 j + l % 16
-    // of the wave's block, over stages kb..ke of every plane product
-    static __device__ __forceinline__ void run(const Gemm& g, int tp, int tq, int kb, int ke, char* s0, char* s1,
-                                               float4_t (&acc)[TP][TQ]) {
+    static __device__ __forceinline__ void zero(float4_t (&acc)[TP][TQ]) {
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int j = 0; j < TQ; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // Adds to acc[i][j] (lane l, element e: p = p_of(i, l) + e, q = 16 j +
+    // l % 16 of the wave's block) stages kb..ke of every plane product.
+    static __device__ __forceinline__ void run(const Gemm& g, int tp, int tq, int kb, int ke, char* p0, char* q0,
+                                               char* p1, char* q1, float4_t (&acc)[TP][TQ]) {
         const int lane = threadIdx.x & 63;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wp = (wave % WP) * (TP * 16), wq = (wave / WP) * (TQ * 16);
@@ -212,30 +244,48 @@ struct Core {
         TileQ Q;
         P.init(g.P, (int64_t)tp * BP, wave, lane);
         Q.init(g.Q, (int64_t)tq * BQ, wave, lane);
-#pragma unroll
-        for (int i = 0; i < TP; ++i)
-#pragma unroll
-            for (int j = 0; j < TQ; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
         const int per = ke - kb;
         if (per <= 0) return;  // uniform over the work-group
         const int total = g.nseg * per;
         int seg = 6 - g.nseg, ks = kb;
-        auto fetch = [&](char* st) {
-            P.load(st, plane_p(seg), (int64_t)ks * kK, wave);
-            Q.load(st + BP * 128, plane_q(seg), (int64_t)ks * kK, wave);
+        P.start(plane_p(seg), (int64_t)kb * kK);
+        Q.start(plane_q(seg), (int64_t)kb * kK);
+        int left = total;  // stages to fetch
+        auto fetch = [&](char* sp, char* sq) {
+            if (left-- <= 0) return;  // uniform
+            P.load(sp, wave);
+            Q.load(sq, wave);
             if (++ks == ke) {
                 ks = kb;
                 ++seg;
+                P.start(plane_p(seg), (int64_t)kb * kK);
+                Q.start(plane_q(seg), (int64_t)kb * kK);
             }
         };
-        auto multiply = [&](const char* st) {
+        // This wave's loads into this stage have landed before the barrier, which
+        // does not wait for loads into LDS; after it every wave's have, and
+        // every wave is done reading the other stage.  The buffers are named
+        // arrays, one an operand and stage: the compiler otherwise waits for
+        // the loads into the next stage before it reads this one (dW at 8,192
+        // x 131,072 x 4,096 took 1.12 ms a piece instead of 0.90).  The next
+        // stage's loads go out behind the first reads, whose latency covers
+        // their address arithmetic.
+        auto step = [&](char* cp, char* cq, char* np, char* nq) {
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kK / 32; ++h) {
                 short8_t a[TP], b[TQ];
 #pragma unroll
-                for (int i = 0; i < TP; ++i) a[i] = TileP::frag(st, wp + 16 * i, h, lane);
+                for (int j = 0; j < TQ; ++j) b[j] = TileQ::frag(cq, wq, j, h, lane);
 #pragma unroll
-                for (int j = 0; j < TQ; ++j) b[j] = TileQ::frag(st + BP * 128, wq + 16 * j, h, lane);
+                for (int i = 0; i < TP; ++i) a[i] = TileP::frag(cp, wp, i, h, lane);
+                if (h == 0) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(np, nq);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
                 for (int i = 0; i < TP; ++i)
 #pragma unroll
@@ -245,30 +295,21 @@ struct Core {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // this wave's loads into `cur` have landed before the barrier, which
-        // does not wait for loads into LDS; after it every wave's have, and
-        // every wave is done reading `nxt`
-        auto step = [&](char* cur, char* nxt, bool more) {
-            __builtin_amdgcn_s_waitcnt(0);
-            __syncthreads();
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) fetch(nxt);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(cur);
-        };
-        fetch(s0);
+        fetch(p0, q0);
         int t = 0;
         for (; t + 1 < total; t += 2) {
-            step(s0, s1, true);
-            step(s1, s0, t + 2 < total);
+            step(p0, q0, p1, q1);
+            step(p1, q1, p0, q0);
         }
-        if (t < total) step(s0, s1, false);
+        if (t < total) step(p0, q0, p1, q1);
     }
 };
 
-#define GRWS_HEAD_LDS(C)                                              \
-    __shared__ __attribute__((aligned(1024))) char s0[C::STAGE];      \
-    __shared__ __attribute__((aligned(1024))) char s1[C::STAGE];
+#define GRWS_HEAD_LDS(C)                                               \
+    __shared__ __attribute__((aligned(1024))) char p0[C::TileP::BYTES]; \
+    __shared__ __attribute__((aligned(1024))) char q0[C::TileQ::BYTES]; \
+    __shared__ __attribute__((aligned(1024))) char p1[C::TileP::BYTES]; \
+    __shared__ __attribute__((aligned(1024))) char q1[C::TileQ::BYTES];
 
 // ---------------------------------------------------------------------------
 // the product's epilogues
@@ -288,29 +329,21 @@ __device__ __forceinline__ float4_t bias4(const void* bias, int32_t dt, int64_t 
     return load_bias4<__hip_bfloat16>(bias, v, left);
 }
 
-// acc -> y = c1 (acc + bias); classes past the last one get `past`
-template <int TP, int TQ>
-__device__ __forceinline__ void scale_logits(float4_t (&acc)[TP][TQ], int64_t vfirst, int64_t classes, float c1,
-                                             const void* bias, int32_t bias_dt, int lane, float past) {
+// The sums of a wave's classes begin with their bias, or -inf past the last
+// class (whose weights read as zeros).
+template <typename C, int TP, int TQ>
+__device__ __forceinline__ void begin_logits(float4_t (&acc)[TP][TQ], int64_t vfirst, int64_t classes,
+                                             const void* bias, int32_t bias_dt, int lane) {
 #pragma unroll
     for (int i = 0; i < TP; ++i) {
-        const int64_t v = vfirst + 16 * i + 4 * (lane >> 4);
+        const int64_t v = vfirst + C::p_of(i, lane);
         float4_t b{0.f, 0.f, 0.f, 0.f};
         if (bias) b = bias4(bias, bias_dt, v, classes - v);
 #pragma unroll
-        for (int j = 0; j < TQ; ++j)
+        for (int e = 0; e < 4; ++e)
+            if (v + e >= classes) b[e] = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = (acc[i][j][e] + b[e]) * c1;
-    }
-    if (vfirst + 16 * TP > classes) {
-#pragma unroll
-        for (int i = 0; i < TP; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (vfirst + 16 * i + 4 * (lane >> 4) + e >= classes) {
-#pragma unroll
-                    for (int j = 0; j < TQ; ++j) acc[i][j][e] = past;
-                }
+        for (int j = 0; j < TQ; ++j) acc[i][j] = b;
     }
 }
 
@@ -340,10 +373,9 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
     int tp, tq;
     tile_of(a.g, tp, tq);
     float4_t acc[TP][TQ];
-    C::run(a.g, tp, tq, 0, a.g.ksteps, s0, s1, acc);
-    const int wp = wave % WP;
-    const int64_t vfirst = a.v0 + (int64_t)tp * BP + wp * (TP * 16);
-    scale_logits<TP, TQ>(acc, vfirst, a.classes, a.c1, a.bias, a.bias_dt, lane, -INFINITY);
+    const int64_t vfirst = a.v0 + (int64_t)tp * BP + (wave % WP) * (TP * 16);
+    begin_logits<C>(acc, vfirst, a.classes, a.bias, a.bias_dt, lane);
+    C::run(a.g, tp, tq, 0, a.g.ksteps, p0, q0, p1, q1, acc);
     const int64_t strip = vfirst / (TP * 16);
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
@@ -355,12 +387,13 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
             for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
         m = fmaxf(m, __shfl_xor(m, 16, kWave));
         m = fmaxf(m, __shfl_xor(m, 32, kWave));
+        m *= a.c1;
         const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf: a sum of zeros
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - ref);
+            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -ref));
         s += __shfl_xor(s, 16, kWave);
         s += __shfl_xor(s, 32, kWave);
         if (lane < 16) a.part[strip * a.np + row] = make_float2(m, s);
@@ -373,22 +406,24 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
 #pragma unroll
                 for (int i = 0; i < TP; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y = (l >> 4) == i && (l & 3) == e ? acc[i][j][e] : y;
-                y = __shfl(y, (((l >> 2) & 3) << 4) | (lane & 15), kWave);
+                    for (int e = 0; e < 4; ++e) y = C::p_of(i, lane) + e == l ? acc[i][j][e] : y;
+                y = __shfl(y, (((l >> 3) & 3) << 4) | (lane & 15), kWave);  // its lane: p_of's
+
                 int tie = 0;
 #pragma unroll
                 for (int i = 0; i < TP; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        tie |= acc[i][j][e] == y && 16 * i + 4 * (lane >> 4) + e < l;
+                        tie |= acc[i][j][e] == y && C::p_of(i, lane) + e < l;
                 tie |= __shfl_xor(tie, 16, kWave);
                 tie |= __shfl_xor(tie, 32, kWave);
                 if (here && lane < 16) {
-                    a.ylabel[row] = y;
+                    a.ylabel[row] = y * a.c1;
                     a.earlier[row] = tie;
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);  // one q at a time: the registers are full
     }
 }
 
@@ -447,46 +482,51 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
     int tp, tq;
     tile_of(a.g, tp, tq);
     float4_t acc[TP][TQ];
-    C::run(a.g, tp, tq, 0, a.g.ksteps, s0, s1, acc);
     const int64_t pfirst = (int64_t)tp * BP + (wave % WP) * (TP * 16);
-    scale_logits<TP, TQ>(acc, a.v0 + pfirst, a.classes, a.c1, a.bias, a.bias_dt, lane, -INFINITY);
+    begin_logits<C>(acc, a.v0 + pfirst, a.classes, a.bias, a.bias_dt, lane);
+    C::run(a.g, tp, tq, 0, a.g.ksteps, p0, q0, p1, q1, acc);
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
+        // of a row that does not count, whose lse is +inf, all are 2^-inf
+        // (its hidden row is zeros, so a logit is its bias)
         const float l = row < a.n ? a.lse[row] : INFINITY;
         const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                acc[i][j][e] = l == INFINITY ? 0.f : __builtin_amdgcn_exp2f(acc[i][j][e] - l);
+                acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -l));
         if (a.labels) {
             const int64_t lab = l != INFINITY ? a.labels[row] - a.v0 - pfirst : -1;
             const bool here = lab >= 0 && lab < TP * 16;
             if (__any(here)) {
-                const int at = here ? (int)lab - 4 * (lane >> 4) : -1;
+                const int at = here ? (int)lab : -1;
 #pragma unroll
                 for (int i = 0; i < TP; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= at == 16 * i + e ? 1.f : 0.f;
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= at == C::p_of(i, lane) + e ? 1.f : 0.f;
             }
         }
 #pragma unroll
-        for (int i = 0; i < TP; ++i) {
-            const int64_t at = row * a.ldg + pfirst + 16 * i + 4 * (lane >> 4);
-            uint16_t h[SPLIT ? 3 : 1][4];
+        for (int i = 0; i < TP; i += 2) {  // 8 consecutive classes of accumulators i and i + 1
+            const int64_t at = row * a.ldg + pfirst + C::p_of(i, lane);
+            uint16_t h[SPLIT ? 3 : 1][8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = acc[i][j][e] * s;
+            for (int e = 0; e < 8; ++e) {
+                const float x = acc[i + (e >> 2)][j][e & 3] * s;
                 if constexpr (SPLIT) split3(x, &h[0][e], &h[1][e], &h[2][e]);
                 else h[0][e] = round16<DT>(x);
             }
 #pragma unroll
-            for (int z = 0; z < (SPLIT ? 3 : 1); ++z)
-                *reinterpret_cast<u32x2_t*>(a.G + z * a.plane + at) =
-                    u32x2_t{(uint32_t)h[z][0] | ((uint32_t)h[z][1] << 16),
-                            (uint32_t)h[z][2] | ((uint32_t)h[z][3] << 16)};
+            for (int z = 0; z < (SPLIT ? 3 : 1); ++z) {
+                u32x4_t w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)h[z][2 * e] | ((uint32_t)h[z][2 * e + 1] << 16);
+                *reinterpret_cast<u32x4_t*>(a.G + z * a.plane + at) = w;
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);  // one q at a time: the registers are full
     }
 }
 
@@ -542,7 +582,8 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
     const int sp = blockIdx.y;
     const int kb = (int)((int64_t)a.g.ksteps * sp / a.g.splits), ke = (int)((int64_t)a.g.ksteps * (sp + 1) / a.g.splits);
     float4_t acc[TP][TQ];
-    C::run(a.g, tp, tq, kb, ke, s0, s1, acc);
+    C::zero(acc);
+    C::run(a.g, tp, tq, kb, ke, p0, q0, p1, q1, acc);
     if (a.g.splits > 1) {
         float* out = a.part + sp * a.vp * a.dp;
 #pragma unroll
@@ -550,7 +591,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
             const int64_t v = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
 #pragma unroll
             for (int i = 0; i < TP; ++i) {
-                const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
+                const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + C::p_of(i, lane);
                 if (d < a.dp && v < a.classes) *reinterpret_cast<float4_t*>(out + v * a.dp + d) = acc[i][j];
             }
         }
@@ -563,7 +604,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
         if (v >= a.classes) continue;
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
-            const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
+            const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + C::p_of(i, lane);
             if (d >= a.width) continue;
             store4<OT>(a.out, v * a.ldo + d, acc[i][j] * alpha, a.width - d, a.vec);
         }
@@ -598,7 +639,8 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
     const int sp = blockIdx.y;
     const int kb = (int)((int64_t)a.g.ksteps * sp / a.g.splits), ke = (int)((int64_t)a.g.ksteps * (sp + 1) / a.g.splits);
     float4_t acc[TP][TQ];
-    C::run(a.g, tp, tq, kb, ke, s0, s1, acc);
+    C::zero(acc);
+    C::run(a.g, tp, tq, kb, ke, p0, q0, p1, q1, acc);
     float* out = a.part + sp * a.np * a.dp;
     const float alpha = a.last ? *a.alpha : 0.f;
 #pragma unroll
@@ -611,7 +653,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
         }
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
-            const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + 16 * i + 4 * (lane >> 4);
+            const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + C::p_of(i, lane);
             if (d >= a.dp) continue;
             float4_t* o = reinterpret_cast<float4_t*>(out + row * a.dp + d);
             const float4_t v = a.first ? acc[i][j] : *o + acc[i][j];
@@ -1156,20 +1198,20 @@ constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // G of a piece, and a pack
 struct Plan {
     int tile;
     int64_t splits;
+    double cost;
 };
 
-Plan plan(int64_t p, int64_t q, int64_t stages, int64_t most_splits) {
-    Plan best{128, 1};
-    double least = 1e300;
+Plan plan(int64_t p, int64_t q, int64_t stages, int64_t most_splits, double besides) {
+    Plan best{128, 1, 1e300};
     for (int tile = 256; tile >= 128; tile -= 128) {
         if (tile == 256 && (p <= 128 || q <= 128)) continue;  // padded to 128 only
         const int64_t tiles = ceil_div(p, tile) * ceil_div(q, tile);
         const int64_t slots = tile == 256 ? 256 : 512;
-        const double step = tile == 256 ? 1.0 : 0.71;
+        const double step = tile == 256 ? 1.0 : 0.71, fixed = tile == 256 ? besides : 0.5 * besides;
         for (int64_t sp = 1; sp <= most_splits && (sp == 1 || tiles * sp <= 4 * slots); ++sp) {
             const double t = (double)ceil_div(tiles * sp, slots) *
-                             ((double)ceil_div(stages, sp) * step + 4 + (sp > 1 ? 16 * step : 0));
-            if (t < least) least = t, best = Plan{tile, sp};
+                             ((double)ceil_div(stages, sp) * step + fixed + (sp > 1 ? 16 * step : 0));
+            if (t < best.cost) best = Plan{tile, sp, t};
         }
     }
     return best;
@@ -1182,6 +1224,7 @@ struct Shape {
     bool split;       // f32 operands in three planes
     bool pack_w;      // W goes through a packed copy
     int64_t np, dp, vp;  // padded rows and width; classes of a piece
+    int64_t ldg;         // pitch of G: rows start 256 bytes apart mod 4 KiB
     Plan logits, weight, hidden;
     int64_t strips, strip_classes;  // the forward's
 };
@@ -1213,13 +1256,31 @@ Shape shape_of(const grws_head* h, bool backward) {
     if (backward) bound(s.np);
     if (s.pack_w) bound(s.dp);
     const int64_t seg = s.split ? 6 : 1;
-    s.logits = plan(s.vp, s.np, seg * s.dp / kK, 1);
+    // the pieces: as few and as equal as the bound allows, or up to three
+    // more where the tiles then fill the rounds better
+    const int64_t fewest = ceil_div(s.V, s.vp), whole = s.vp;
+    double least = 1e300;
+    for (int64_t pieces = fewest; pieces < fewest + (fewest > 1 ? 4 : 1); ++pieces) {
+        int64_t vp = fewest > 1 ? up(ceil_div(s.V, pieces), 256) : whole;
+        if (vp > whole) vp = whole;
+        const Plan l = plan(vp, s.np, seg * s.dp / kK, 1, 6);
+        Plan w{}, d{};
+        if (backward) {
+            w = plan(s.D, vp, seg * s.np / kK, ceil_div(s.np / kK, 4), 4);
+            d = plan(s.dp, s.np, seg * vp / kK, ceil_div(vp / kK, 4), 4);
+        }
+        const double t = (double)ceil_div(s.V, vp) * (l.cost + w.cost + d.cost + 6);
+        if (t < least) {
+            least = t;
+            s.vp = vp;
+            s.logits = l;
+            s.weight = w;
+            s.hidden = d;
+        }
+    }
     s.strip_classes = s.logits.tile / 2;
     s.strips = pad(s.V) / s.strip_classes;
-    if (backward) {
-        s.weight = plan(s.D, s.vp, seg * s.np / kK, ceil_div(s.np / kK, 4));
-        s.hidden = plan(s.dp, s.np, seg * s.vp / kK, ceil_div(s.vp / kK, 4));
-    }
+    s.ldg = s.vp + 128;
     return s;
 }
 
@@ -1291,7 +1352,7 @@ void bwd_space(A& a, const Shape& s, BwdSpace* f) {
     };
     take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
-    take(f->G, s.planes * s.np * s.vp);
+    take(f->G, s.planes * s.np * s.ldg);
     if (s.hidden.splits > 1 || s.vp < s.V) take(f->dh, s.hidden.splits * s.np * s.dp);
     if (s.weight.splits > 1) take(f->dw, s.weight.splits * s.vp * s.dp);
     take(f->bias, s.np / kBiasRows * s.vp);
@@ -1359,7 +1420,7 @@ Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64
                 (int32_t)ceil_div(nq, pl.tile), (int32_t)pl.splits};
 }
 
-// KERNEL<..., BP, BQ, WP, WQ> at a plan's tile
+// KERNEL<..., BP, BQ, WP, WQ> at a plan's configuration
 #define GRWS_HEAD_LAUNCH(PLAN, NAME, ARGS, ...)                                                                      \
     do {                                                                                                             \
         GRWS_CHECK_ARG((int64_t)ARGS.g.tp * ARGS.g.tq < INT32_MAX, "head: more than 2^31 tiles");                    \
@@ -1491,7 +1552,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
     }
     const Alpha alpha{f.alpha, dloss, counts, per_row ? f.most : nullptr, h->temperature / gscale};
     GRWS_TRY(pack_hidden(h, s, t, f.hp, alpha, nullptr, stream));
-    const int64_t plane = s.np * s.vp;
+    const int64_t plane = s.np * s.ldg;
     const size_t esz = dtype_size(h->dtype);
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
@@ -1499,7 +1560,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
         GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, c1, h->bias,
-                   h->dtype, lse, h->labels, row_scale, gscale, f.G, s.vp, plane};
+                   h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane};
         if (s.split) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, true);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_F16, false);
         else GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, false);
@@ -1507,7 +1568,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             const dim3 grid((unsigned)ceil_div(s.n * h->k, 256));
 #define GRWS_HEAD_SUB(DT, SP)                                                                                 \
     hipLaunchKernelGGL((head_subtract_kernel<DT, SP>), grid, dim3(256), 0, stream, t, lse, target_logit, coef, \
-                       row_scale, gscale, s.n, v0, vc, f.G, s.vp, plane)
+                       row_scale, gscale, s.n, v0, vc, f.G, s.ldg, plane)
             if (s.split) GRWS_HEAD_SUB(GRWS_BF16, true);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_SUB(GRWS_F16, false);
             else GRWS_HEAD_SUB(GRWS_BF16, false);
@@ -1519,13 +1580,13 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             const int64_t nparts = s.np / kBiasRows;
             const dim3 grid((unsigned)ceil_div(vt, 512), (unsigned)nparts);
             if (s.split)
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, true>), grid, dim3(256), 0, stream, f.G, s.vp,
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, true>), grid, dim3(256), 0, stream, f.G, s.ldg,
                                    plane, vt, f.bias);
             else if (h->dtype == GRWS_F16)
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_F16, false>), grid, dim3(256), 0, stream, f.G, s.vp,
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_F16, false>), grid, dim3(256), 0, stream, f.G, s.ldg,
                                    plane, vt, f.bias);
             else
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, false>), grid, dim3(256), 0, stream, f.G, s.vp,
+                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, false>), grid, dim3(256), 0, stream, f.G, s.ldg,
                                    plane, vt, f.bias);
             GRWS_LAUNCH_CHECK();
             const dim3 cg((unsigned)ceil_div(vc, 64));
@@ -1542,7 +1603,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         if (d_weight) {
             char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
             const int32_t vec = reinterpret_cast<uintptr_t>(d_weight) % (4 * esz) == 0 && ld_dw % 4 == 0;
-            const Opnd G{gp, s.vp * 2, plane * 2, s.vp, s.np};
+            const Opnd G{gp, s.ldg * 2, plane * 2, s.ldg, s.np};
             WeightArgs w{gemm_of(s, s.weight, hidden_operand(s, f.hp, true), G, s.D, vc, s.np), f.alpha, out, ld_dw,
                          vc, s.D, vec, f.dw, s.vp, s.dp};
             if (s.split) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
@@ -1561,7 +1622,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         }
         if (d_hidden) {
             GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, false, stream));
-            const Opnd G{gp, s.vp * 2, plane * 2, s.np, vt};
+            const Opnd G{gp, s.ldg * 2, plane * 2, s.np, vt};
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
             HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc), f.dh, s.np, s.dp, v0 == 0,
                          s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
