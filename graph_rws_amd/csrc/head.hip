@@ -315,7 +315,7 @@ struct Core {
 // the product's epilogues
 // ---------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ float4_t load_bias4(const void* bias, int64_t v, int64_t left) {
+__device__ __forceinline__ float4_t load_bias4(const void* bias, int64_t v, int left) {
     float4_t b{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -323,7 +323,7 @@ __device__ __forceinline__ float4_t load_bias4(const void* bias, int64_t v, int6
     return b;
 }
 
-__device__ __forceinline__ float4_t bias4(const void* bias, int32_t dt, int64_t v, int64_t left) {
+__device__ __forceinline__ float4_t bias4(const void* bias, int32_t dt, int64_t v, int left) {
     if (dt == GRWS_F32) return load_bias4<float>(bias, v, left);
     if (dt == GRWS_F16) return load_bias4<_Float16>(bias, v, left);
     return load_bias4<__hip_bfloat16>(bias, v, left);
@@ -334,14 +334,17 @@ __device__ __forceinline__ float4_t bias4(const void* bias, int32_t dt, int64_t 
 template <typename C, int TP, int TQ>
 __device__ __forceinline__ void begin_logits(float4_t (&acc)[TP][TQ], int64_t vfirst, int64_t classes,
                                              const void* bias, int32_t bias_dt, int lane) {
+    C::zero(acc);
+    if (!bias && vfirst + 16 * TP <= classes) return;  // uniform
+    const int left = (int)(classes - vfirst < 16 * TP ? classes - vfirst : 16 * TP);
 #pragma unroll
     for (int i = 0; i < TP; ++i) {
-        const int64_t v = vfirst + C::p_of(i, lane);
+        const int p = C::p_of(i, lane);
         float4_t b{0.f, 0.f, 0.f, 0.f};
-        if (bias) b = bias4(bias, bias_dt, v, classes - v);
+        if (bias) b = bias4(bias, bias_dt, vfirst + p, left - p);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (v + e >= classes) b[e] = -INFINITY;
+            if (p + e >= left) b[e] = -INFINITY;
 #pragma unroll
         for (int j = 0; j < TQ; ++j) acc[i][j] = b;
     }
@@ -408,7 +411,6 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y = C::p_of(i, lane) + e == l ? acc[i][j][e] : y;
                 y = __shfl(y, (((l >> 3) & 3) << 4) | (lane & 15), kWave);  // its lane: p_of's
-
                 int tie = 0;
 #pragma unroll
                 for (int i = 0; i < TP; ++i)
@@ -925,8 +927,10 @@ __device__ __forceinline__ void finish_loss(const volatile double* part_loss, co
     counts[2] = B;
 }
 
-// Joins the strips of 16 rows (32 at a time: 4 a wave, 8 waves), then the
-// rows' losses, and their mean and counts (loss_out and row_loss may be NULL).
+// Joins the strips of R rows (512 / R at a time), then the rows' losses, and
+// their mean and counts (loss_out and row_loss may be NULL).  R = 4 spreads
+// few rows over more work-groups: 333 rows of 512 strips 15 -> 8 us.
+template <int R>
 __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2* __restrict__ part, int64_t strips,
                                                         int32_t strip_classes, int64_t n, int64_t np,
                                                         float temperature, const float* __restrict__ y,
@@ -935,45 +939,48 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
                                                         float* __restrict__ row_loss, double* part_loss,
                                                         int32_t* part_cnt, int32_t* done,
                                                         float* __restrict__ loss_out, int64_t* __restrict__ counts) {
-    __shared__ float sm[32][16], ss[32][16];
-    __shared__ int sa[32][16];
+    __shared__ float sm[8][R], ss[8][R];
+    __shared__ int sa[8][R];
+    constexpr int G = 64 / R;  // lanes of a wave that share a row
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int slot = wave * 4 + (lane >> 4);
-    const int64_t i = (int64_t)blockIdx.x * 16 + (lane & 15);
+    const int r = lane % R, g = lane / R;
+    const int64_t i = (int64_t)blockIdx.x * R + r;
     float m = -INFINITY, s = 0.f;
     int first = 0x7fffffff;  // the first strip with the maximum
+    auto join_lanes = [&]() {
+#pragma unroll
+        for (int d = R; d < 64; d <<= 1) {
+            const float om = __shfl_xor(m, d, kWave), os = __shfl_xor(s, d, kWave);
+            const int of = __shfl_xor(first, d, kWave);
+            // both sides join in the same order, so a row's lanes agree
+            if (lane & d) {
+                float m2 = om, s2 = os;
+                int f2 = of;
+                join(m2, s2, f2, m, s, first);
+                m = m2, s = s2, first = f2;
+            } else {
+                join(m, s, first, om, os, of);
+            }
+        }
+    };
     if (i < n) {
 #pragma unroll 4
-        for (int64_t k = slot; k < strips; k += 32) {
+        for (int64_t k = wave * G + g; k < strips; k += 8 * G) {
             const float2 v = part[k * np + i];
             join(m, s, first, v.x, v.y, (int)k);
         }
     }
-    sm[slot][lane & 15] = m;
-    ss[slot][lane & 15] = s;
-    sa[slot][lane & 15] = first;
+    join_lanes();
+    if (g == 0) {
+        sm[wave][r] = m;
+        ss[wave][r] = s;
+        sa[wave][r] = first;
+    }
     __syncthreads();
     if (wave != 0) return;
-    // 4 lanes a row join 8 slots each, then each other's
-    const int g = lane >> 4, r = lane & 15;
-    m = sm[8 * g][r];
-    s = ss[8 * g][r];
-    first = sa[8 * g][r];
-    for (int w = 1; w < 8; ++w) join(m, s, first, sm[8 * g + w][r], ss[8 * g + w][r], sa[8 * g + w][r]);
-#pragma unroll
-    for (int d = 16; d < 64; d <<= 1) {
-        const float om = __shfl_xor(m, d, kWave), os = __shfl_xor(s, d, kWave);
-        const int of = __shfl_xor(first, d, kWave);
-        // both sides join in the same order, so the four lanes agree
-        if (lane & d) {
-            float m2 = om, s2 = os;
-            int f2 = of;
-            join(m2, s2, f2, m, s, first);
-            m = m2, s = s2, first = f2;
-        } else {
-            join(m, s, first, om, os, of);
-        }
-    }
+    m = -INFINITY, s = 0.f, first = 0x7fffffff;
+    for (int w = g; w < 8; w += G) join(m, s, first, sm[w][r], ss[w][r], sa[w][r]);
+    join_lanes();
     int st = 0;
     if (i < n) st = t.labels ? row_state<1>(t, i, 0) : flags[i];
     const float l = m + log2f(s);
@@ -981,13 +988,13 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
     if (!t.labels && st == 1) {
         // sum of q ln q + q ln2 (L - y); an entry of probability zero says
         // nothing of its class (whose logit may be -inf)
-        for (int k = g; k < t.k; k += 4) {
+        for (int k = g; k < t.k; k += G) {
             const float q = prob[i * t.k + k];
             if (!(q <= 0.f)) a += q * (logf(q) + (l - y[i * t.k + k]) * kLn2);
         }
     }
-    a += __shfl_xor(a, 16, kWave);
-    a += __shfl_xor(a, 32, kWave);
+#pragma unroll
+    for (int d = R; d < 64; d <<= 1) a += __shfl_xor(a, d, kWave);
     double loss = 0.0;
     int hit = 0, valid = 0, bad = 0;
     if (g == 0 && i < n) {
@@ -1010,7 +1017,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
         if (row_loss) row_loss[i] = v;
     }
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) {
+    for (int d = R / 2; d > 0; d >>= 1) {
         loss += __shfl_xor(loss, d, kWave);
         hit += __shfl_xor(hit, d, kWave);
         valid += __shfl_xor(valid, d, kWave);
@@ -1332,8 +1339,8 @@ void fwd_space(A& a, const Shape& s, FwdSpace* f) {
     if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
     take(f->part, s.strips * s.np);
     take(f->flags, s.n);
-    take(f->pl, ceil_div(s.n, 16));
-    take(f->pc, 3 * ceil_div(s.n, 16));
+    take(f->pl, ceil_div(s.n, 4));
+    take(f->pc, 3 * ceil_div(s.n, 4));
     take(f->done, 1);
 }
 
@@ -1420,7 +1427,7 @@ Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64
                 (int32_t)ceil_div(nq, pl.tile), (int32_t)pl.splits};
 }
 
-// KERNEL<..., BP, BQ, WP, WQ> at a plan's configuration
+// NAME<..., BP, BQ, WP, WQ> at a plan's tile
 #define GRWS_HEAD_LAUNCH(PLAN, NAME, ARGS, ...)                                                                      \
     do {                                                                                                             \
         GRWS_CHECK_ARG((int64_t)ARGS.g.tp * ARGS.g.tq < INT32_MAX, "head: more than 2^31 tiles");                    \
@@ -1490,10 +1497,15 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
 #undef GRWS_HEAD_TARGETS
         GRWS_LAUNCH_CHECK();
     }
-    const int64_t blocks = ceil_div(s.n, 16);
-    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part, ceil_div(s.V, s.strip_classes),
-                       (int32_t)s.strip_classes, s.n, s.np, h->temperature, target_logit, target_prob, f.flags, lse,
-                       row_loss, f.pl, f.pc, blocks <= kJoinBlocks ? f.done : nullptr, loss, counts);
+    const int64_t rows = s.n <= 1024 ? 4 : 16, blocks = ceil_div(s.n, rows);
+#define GRWS_HEAD_JOIN(R)                                                                                            \
+    hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part,                 \
+                       ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature,          \
+                       target_logit, target_prob, f.flags, lse, row_loss, f.pl, f.pc,                                \
+                       blocks <= kJoinBlocks ? f.done : nullptr, loss, counts)
+    if (rows == 4) GRWS_HEAD_JOIN(4);
+    else GRWS_HEAD_JOIN(16);
+#undef GRWS_HEAD_JOIN
     GRWS_LAUNCH_CHECK();
     if (blocks > kJoinBlocks) {
         hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(64), 0, stream, f.pl, f.pc, blocks, loss, counts);
