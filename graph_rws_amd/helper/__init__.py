@@ -9,7 +9,9 @@ from .timer import (  # noqa: F401
 from .engine import (  # noqa: F401
     compute_loss_and_metrics,
     evaluate,
+    evaluate_head,
     train_epoch_full,
+    train_epoch_head,
     train_epoch_node_sampling,
 )
 from .graphed import GraphedBlockStep, GraphedFullStep, bucket_rows  # noqa: F401

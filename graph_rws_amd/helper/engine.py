@@ -65,6 +65,49 @@ def train_epoch_full(model, graphs_for_model, features: torch.Tensor, labels: to
     return loss.item(), acc
 
 
+def train_epoch_head(model, head, graphs_for_model, features: torch.Tensor, labels: torch.Tensor,
+                     train_idx: torch.Tensor, optimizer: torch.optim.Optimizer, device, teacher=None,
+                     teacher_weight: float = 0.5, temperature: float = 2.0, sync: bool = True):
+    """One full-graph training step of a model with a LinearHead over many
+    classes on its output rows, whose logits are never kept: cross entropy of
+    the rows train_idx (distinct) against labels, and with teacher = (values,
+    classes) [len(train_idx), k], the lists of a teacher's head (head.top),
+    (1 - teacher_weight) of it plus teacher_weight of the distillation loss.
+    optimizer holds the parameters of both.  Returns (loss, acc) as
+    train_epoch_full does."""
+    model.train()
+    head.train()
+    if features.device != device:
+        features = features.to(device)
+    optimizer.zero_grad()
+    hidden = model(graphs_for_model, features)
+    loss, counts = head.loss(hidden, labels[train_idx], rows=train_idx)
+    n = train_idx.numel()
+    if teacher is not None:
+        values, classes = teacher
+        kd, _ = head.distill(hidden, classes, values, rows=train_idx, temperature=temperature)
+        loss = (1.0 - teacher_weight) * loss + teacher_weight * kd
+    acc = counts[0] / n if n > 0 else 0.0
+    loss.backward()
+    torch.nn.utils.clip_grad_norm_(list(model.parameters()) + list(head.parameters()), max_norm=1.0)
+    optimizer.step()
+    if not sync:
+        return loss.detach(), acc
+    return loss.item(), acc
+
+
+@torch.no_grad()
+def evaluate_head(model, head, bcsr_full, features: torch.Tensor, labels: torch.Tensor, eval_idx: torch.Tensor):
+    """(mean loss, accuracy) of a full-graph inference with a LinearHead on
+    the rows eval_idx (distinct)."""
+    model.eval()
+    head.eval()
+    hidden = model.inference(bcsr_full, features)
+    loss, counts = head.loss(hidden, labels[eval_idx], rows=eval_idx)
+    n = eval_idx.numel()
+    return loss.item(), (counts[0] / n).item() if n > 0 else 0.0
+
+
 @torch.no_grad()
 def evaluate(model, bcsr_full, features: torch.Tensor, labels: torch.Tensor,
              eval_idx: torch.Tensor, device):

@@ -7,6 +7,9 @@ logits [n, classes] are never kept: the forward reduces them in the
 product's epilogue, the backward makes them again piece by piece of the
 classes.
 
+``LinearHead`` holds a classifier's weight and bias and makes these calls;
+``helper.train_epoch_head`` trains one on top of a graph model.
+
 Under autocast hidden, weight and bias are taken in the autocast dtype, as
 ``F.linear`` takes them.
 """
@@ -83,3 +86,41 @@ def linear_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_index: to
         raise ValueError("linear_distill: teacher_index and teacher_logits are required")
     loss, counts = _apply(hidden, weight, bias, rows, None, teacher_index, teacher_logits, temperature, reduction)
     return loss, counts[1:]
+
+
+class LinearHead(torch.nn.Module):
+    """Classifier over many classes on top of a model's hidden rows: weight
+    [classes, width] and bias, as torch.nn.Linear has them."""
+
+    def __init__(self, width: int, classes: int, bias: bool = True):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.empty(classes, width))
+        self.bias = torch.nn.Parameter(torch.empty(classes)) if bias else None
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        torch.nn.init.normal_(self.weight, std=self.weight.shape[1] ** -0.5)
+        if self.bias is not None:
+            torch.nn.init.zeros_(self.bias)
+
+    def forward(self, hidden: torch.Tensor) -> torch.Tensor:
+        """The logits themselves, [rows, classes]."""
+        return torch.nn.functional.linear(hidden, self.weight, self.bias)
+
+    def loss(self, hidden, labels, rows=None, reduction: str = "mean"):
+        """linear_cross_entropy of this classifier."""
+        return linear_cross_entropy(hidden, self.weight, labels, self.bias, rows, reduction)
+
+    def distill(self, hidden, teacher_index, teacher_logits, rows=None, temperature: float = 1.0,
+                reduction: str = "mean"):
+        """linear_distill of this classifier (the student)."""
+        return linear_distill(hidden, self.weight, teacher_index, teacher_logits, self.bias, rows, temperature,
+                              reduction)
+
+    @torch.no_grad()
+    def top(self, hidden, k: int, rows_at_once: int = 8192):
+        """(values, classes int32) [rows, k]: this classifier's top logits (the
+        teacher's lists), `rows_at_once` rows of logits in memory at a time."""
+        parts = [_ops.top_logits(self(hidden[i:i + rows_at_once]), k)
+                 for i in range(0, max(1, hidden.shape[0]), rows_at_once)]
+        return torch.cat([v for v, _ in parts]), torch.cat([c for _, c in parts])
