@@ -441,6 +441,8 @@ struct GradArgs {
     float gscale;
     uint16_t* G;  // [planes][np][ldg]
     int64_t ldg, plane;
+    float* bias_part;  // [np / kBiasRows][vt]: column sums, or NULL
+    int64_t vt;
 };
 
 __device__ __forceinline__ uint16_t top16(float x) { return (uint16_t)(__float_as_uint(x) >> 16); }
@@ -474,6 +476,15 @@ __device__ __forceinline__ void store_g(uint16_t* G, int64_t plane, int64_t at, 
         G[at] = round16<DT>(x);
     }
 }
+
+// x of the lane N further in its row of 16
+template <int N>
+__device__ __forceinline__ float rotate(float x) {
+    return __builtin_bit_cast(float,
+                              __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, true));
+}
+
+constexpr int kBiasRows = 64;  // rows of a part of the bias gradient's sums
 
 template <int DT, bool SPLIT, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
@@ -511,12 +522,14 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
             }
         }
 #pragma unroll
+        for (int i = 0; i < TP; ++i) acc[i][j] *= s;
+#pragma unroll
         for (int i = 0; i < TP; i += 2) {  // 8 consecutive classes of accumulators i and i + 1
             const int64_t at = row * a.ldg + pfirst + C::p_of(i, lane);
             uint16_t h[SPLIT ? 3 : 1][8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = acc[i + (e >> 2)][j][e & 3] * s;
+                const float x = acc[i + (e >> 2)][j][e & 3];
                 if constexpr (SPLIT) split3(x, &h[0][e], &h[1][e], &h[2][e]);
                 else h[0][e] = round16<DT>(x);
             }
@@ -529,6 +542,26 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
             }
         }
         __builtin_amdgcn_sched_barrier(0);  // one q at a time: the registers are full
+    }
+    if (a.bias_part) {
+        // the wave's 64 rows: TQ of a lane, then the 16 lanes that share the
+        // classes (rotations within a row of 16 lanes)
+        static_assert(TQ * 16 == kBiasRows, "rows of a part");
+        const int64_t at = ((int64_t)tq * WQ + wave / WP) * a.vt + pfirst;
+#pragma unroll
+        for (int i = 0; i < TP; ++i) {
+            float4_t x = acc[i][0];
+#pragma unroll
+            for (int j = 1; j < TQ; ++j) x += acc[i][j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] += rotate<8>(x[e]);
+                x[e] += rotate<4>(x[e]);
+                x[e] += rotate<2>(x[e]);
+                x[e] += rotate<1>(x[e]);
+            }
+            if ((lane & 15) == 0) *reinterpret_cast<float4_t*>(a.bias_part + at + C::p_of(i, lane)) = x;
+        }
     }
 }
 
@@ -903,10 +936,11 @@ __device__ __forceinline__ void join(float& m, float& s, int& first, float om, f
 
 // loss = sum / counted (NaN when no row counts or an input is bad), by one
 // wave; parts are added in a fixed order
-__device__ __forceinline__ void finish_loss(const volatile double* part_loss, const volatile int32_t* part_cnt,
+__device__ __forceinline__ void finish_loss(const double* part_loss, const int32_t* part_cnt,
                                             int64_t nparts, int lane, float* loss, int64_t* counts) {
     double L = 0.0;
     long long C = 0, V = 0, B = 0;
+#pragma unroll 8
     for (int64_t k = lane; k < nparts; k += 64) {
         L += part_loss[k];
         C += part_cnt[3 * k];
@@ -1092,17 +1126,17 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const flo
     store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[at] - l) - q) * s);
 }
 
-// Column sums of a piece of G over runs of 64 rows: 4 waves of 16 rows,
-// 8 columns a lane.
-constexpr int kBiasRows = 64;
+// Column sums of a piece of G over runs of kBiasRows rows, 4 waves of 16 rows,
+// 8 columns a lane: after head_subtract_kernel (with labels the gradient
+// product's epilogue has made them).
 
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __restrict__ G, int64_t ldg,
                                                              int64_t plane, int64_t vp, float* __restrict__ part) {
     __shared__ float red[4][512];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
-    const int64_t r0 = (int64_t)blockIdx.y * kBiasRows + wave * (kBiasRows / 4);
+    const int64_t c = (int64_t)blockIdx.y * 512 + lane * 8;
+    const int64_t r0 = (int64_t)blockIdx.x * kBiasRows + wave * (kBiasRows / 4);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c < vp) {
 #pragma unroll 4
@@ -1123,8 +1157,8 @@ __global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __r
     for (int e = 0; e < 8; ++e) red[wave][lane * 8 + e] = s[e];
     __syncthreads();
     for (int x = threadIdx.x; x < 512; x += 256) {
-        const int64_t col = (int64_t)blockIdx.x * 512 + x;
-        if (col < vp) part[blockIdx.y * vp + col] = (red[0][x] + red[1][x]) + (red[2][x] + red[3][x]);
+        const int64_t col = (int64_t)blockIdx.y * 512 + x;
+        if (col < vp) part[blockIdx.x * vp + col] = (red[0][x] + red[1][x]) + (red[2][x] + red[3][x]);
     }
 }
 
@@ -1195,8 +1229,12 @@ int64_t ceil_div(int64_t x, int64_t a) { return (x + a - 1) / a; }
 // work-groups of head_join_kernel up to which the last of them finishes the
 // loss (each writes its L2's lines back for it: 1,024 of them take 29 us more
 // against a launch of 5)
-constexpr int64_t kJoinBlocks = 64;
-constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // G of a piece, and a packed piece of W
+constexpr int64_t kJoinBlocks = 128;
+// G of a piece: 16,384 rows x 100,003 classes at width 256 take 5.0 ms with
+// 256 MiB, 4.70 with 512 and 4.54 with 1 GiB (fewer, fuller launches); at
+// 8,192 x 131,072 x 4,096 it makes 1%.
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;
+constexpr int64_t kPackBytes = (int64_t)256 << 20;  // a packed piece of W
 
 // A product's tile and the runs that its k is cut into: the least of
 //   rounds of work-groups x (stages of a run + what a work-group costs besides)
@@ -1255,13 +1293,13 @@ Shape shape_of(const grws_head* h, bool backward) {
     s.np = pad(s.n);
     s.dp = up(s.D, kK);
     s.vp = pad(s.V);
-    auto bound = [&](int64_t row_elements) {
-        int64_t most = kPieceBytes / (2 * s.planes * row_elements) / 256 * 256;
+    auto bound = [&](int64_t bytes, int64_t row_elements) {
+        int64_t most = bytes / (2 * s.planes * row_elements) / 256 * 256;
         if (most < 256) most = 256;
         if (s.vp > most) s.vp = most;
     };
-    if (backward) bound(s.np);
-    if (s.pack_w) bound(s.dp);
+    if (backward) bound(kPieceBytes, s.np);
+    if (s.pack_w) bound(kPackBytes, s.dp);
     const int64_t seg = s.split ? 6 : 1;
     // the pieces: as few and as equal as the bound allows, or up to three
     // more where the tiles then fill the rounds better
@@ -1497,7 +1535,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
 #undef GRWS_HEAD_TARGETS
         GRWS_LAUNCH_CHECK();
     }
-    const int64_t rows = s.n <= 1024 ? 4 : 16, blocks = ceil_div(s.n, rows);
+    const int64_t rows = s.n <= 512 ? 4 : 16, blocks = ceil_div(s.n, rows);
 #define GRWS_HEAD_JOIN(R)                                                                                            \
     hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part,                 \
                        ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature,          \
@@ -1572,7 +1610,8 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
         GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, c1, h->bias,
-                   h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane};
+                   h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane,
+                   d_bias && h->k == 0 ? f.bias : nullptr, vt};
         if (s.split) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, true);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_F16, false);
         else GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, false);
@@ -1590,17 +1629,16 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         const char* gp = reinterpret_cast<const char*>(f.G);
         if (d_bias) {
             const int64_t nparts = s.np / kBiasRows;
-            const dim3 grid((unsigned)ceil_div(vt, 512), (unsigned)nparts);
-            if (s.split)
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, true>), grid, dim3(256), 0, stream, f.G, s.ldg,
-                                   plane, vt, f.bias);
-            else if (h->dtype == GRWS_F16)
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_F16, false>), grid, dim3(256), 0, stream, f.G, s.ldg,
-                                   plane, vt, f.bias);
-            else
-                hipLaunchKernelGGL((head_bias_part_kernel<GRWS_BF16, false>), grid, dim3(256), 0, stream, f.G, s.ldg,
-                                   plane, vt, f.bias);
-            GRWS_LAUNCH_CHECK();
+            if (h->k > 0) {  // with labels head_grad_kernel has made the parts
+                const dim3 grid((unsigned)nparts, (unsigned)ceil_div(vt, 512));
+#define GRWS_HEAD_BIAS_PART(DT, SP)                                                                               \
+    hipLaunchKernelGGL((head_bias_part_kernel<DT, SP>), grid, dim3(256), 0, stream, f.G, s.ldg, plane, vt, f.bias)
+                if (s.split) GRWS_HEAD_BIAS_PART(GRWS_BF16, true);
+                else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS_PART(GRWS_F16, false);
+                else GRWS_HEAD_BIAS_PART(GRWS_BF16, false);
+#undef GRWS_HEAD_BIAS_PART
+                GRWS_LAUNCH_CHECK();
+            }
             const dim3 cg((unsigned)ceil_div(vc, 64));
             char* db = static_cast<char*>(d_bias) + v0 * esz;
 #define GRWS_HEAD_BIAS(T) \

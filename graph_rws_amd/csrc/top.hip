@@ -337,6 +337,48 @@ __global__ __launch_bounds__(kT, MAXK <= kSmallK ? 8 : 5) void top_rows_kernel(c
     }
 }
 
+// Short rows and small k: a wave holds a row in its registers and takes the
+// largest key k times (a local maximum, six exchanges, and the owner drops
+// it).  Bound by those exchanges, 0.15 us each; a work-group a row spends
+// 9 us in its 20 barriers on 1,024 rows of 172 classes.
+constexpr int kWaveClasses = 1024;
+constexpr int kWaveK = 16;
+
+template <typename T, int PER>
+__global__ __launch_bounds__(kT) void top_wave_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows,
+                                                      int32_t classes, int32_t class_bits, int32_t k,
+                                                      T* __restrict__ values, int32_t* __restrict__ index) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    if (r >= rows) return;  // uniform over the wave
+    const T* row = logits + r * ld;
+    const uint64_t low = (1ull << class_bits) - 1;
+    uint64_t key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = i * 64 + lane;
+        key[i] = c < classes ? ((uint64_t)order_of<T>(row[c]) << class_bits) | (low - (uint32_t)c) : 0;
+    }
+    for (int a = 0; a < k; ++a) {
+        uint64_t m = key[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) m = key[i] > m ? key[i] : m;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            const uint64_t o = __shfl_xor((unsigned long long)m, d, kWave);
+            m = o > m ? o : m;
+        }
+        const int c = (int)(low - (m & low));
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (key[i] == m) {  // one lane's: keys are distinct
+                key[i] = 0;
+                index[r * k + a] = c;
+                values[r * k + a] = row[c];
+            }
+    }
+}
+
 // Joins the stretches of a row: `count` keys (0: none), the k largest.
 template <typename T, int MAXK>
 __global__ __launch_bounds__(kT) void top_join_kernel(const T* __restrict__ logits, int64_t ld,
@@ -398,14 +440,32 @@ extern "C" int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, in
     GRWS_CHECK_ARG(k >= 1 && k <= kMaxK && k <= classes, "top_logits: k must be 1..min(classes, 1024)");
     if (rows == 0) return GRWS_OK;
     GRWS_CHECK_ARG(logits && values && index, "top_logits: null pointer");
+    int32_t class_bits = 1;
+    while ((1ll << class_bits) < classes) ++class_bits;
+    if (classes <= kWaveClasses && k <= kWaveK) {
+        const dim3 blocks((unsigned)((rows + kWaves - 1) / kWaves));
+#define GRWS_TOP_WAVE(T, PER)                                                                                    \
+    hipLaunchKernelGGL((top_wave_kernel<T, PER>), blocks, dim3(kT), 0, stream, static_cast<const T*>(logits), ld, \
+                       rows, (int32_t)classes, class_bits, k, static_cast<T*>(values), index)
+#define GRWS_TOP_ROWS(T)                             \
+    do {                                             \
+        if (classes <= 256) GRWS_TOP_WAVE(T, 4);     \
+        else GRWS_TOP_WAVE(T, 16);                   \
+    } while (0)
+        if (dtype == GRWS_F32) GRWS_TOP_ROWS(float);
+        else if (dtype == GRWS_F16) GRWS_TOP_ROWS(_Float16);
+        else GRWS_TOP_ROWS(__hip_bfloat16);
+#undef GRWS_TOP_ROWS
+#undef GRWS_TOP_WAVE
+        GRWS_LAUNCH_CHECK();
+        return GRWS_OK;
+    }
     const int32_t n = stretches(rows, classes, k);
     Carver cv(workspace, workspace_bytes);
     uint64_t* best = n > 1 ? cv.take<uint64_t>((size_t)rows * n * k) : nullptr;
     if (!cv.ok)
         return set_error(GRWS_E_CAPACITY, "top_logits: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const int32_t stretch = (int32_t)((classes + n - 1) / n);
-    int32_t class_bits = 1;
-    while ((1ll << class_bits) < classes) ++class_bits;
     const dim3 grid((unsigned)rows, (unsigned)n);
 #define GRWS_TOP_K(T, MAXK)                                                                                        \
     do {                                                                                                           \
