@@ -1836,55 +1836,64 @@ def _row_pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-class HeadCall:
-    """The checked arguments of one classifier call: hidden [N, D], weight
-    [V, D], bias [V] or None, rows int64 [n] or None, and either labels
+def check_head(hidden, weight, bias=None, rows=None, labels=None, teacher_index=None, teacher_logits=None,
+               temperature: float = 1.0) -> None:
+    """Raises unless the arguments are a classifier call's: hidden [N, D],
+    weight [V, D], bias [V] or None, rows int64 [n] or None, and either labels
     int64 [n] or a teacher's (index int32/int64 [n, K], logits [n, K],
-    temperature).  Holds the tensors that its view points to."""
+    temperature), all on one GPU."""
+    who = "linear_cross_entropy" if labels is not None else "linear_distill"
+    L.require_device(who, hidden.device, weight, bias, rows, labels, teacher_index, teacher_logits)
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] or weight.numel() == 0:
+        raise ValueError(f"{who}: hidden must be [rows, width] and weight [classes, width] (got "
+                         f"{tuple(hidden.shape)} and {tuple(weight.shape)})")
+    L.dtype_code(hidden.dtype)
+    if weight.dtype != hidden.dtype or (bias is not None and bias.dtype != hidden.dtype):
+        raise TypeError(f"{who}: hidden, weight and bias must have one dtype")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"{who}: bias must be [classes]")
+    if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int64):
+        raise ValueError(f"{who}: rows must be int64 [n]")
+    if labels is not None:
+        if labels.dim() != 1 or labels.dtype != torch.int64:
+            raise ValueError(f"{who}: labels must be int64 [n]")
+        n = labels.shape[0]
+    else:
+        if (teacher_index.dim() != 2 or teacher_index.dtype not in (torch.int32, torch.int64)
+                or teacher_logits.shape != teacher_index.shape or not teacher_logits.is_floating_point()):
+            raise ValueError(f"{who}: teacher_index must be int32 or int64 [n, k] and teacher_logits [n, k]")
+        n, k = teacher_index.shape
+        if not 1 <= k <= 1024:
+            raise ValueError(f"{who}: 1 to 1024 teacher entries a row (got {k})")
+        if not 0.0 < float(temperature) < float("inf"):
+            raise ValueError(f"{who}: the temperature must be positive (got {temperature})")
+    if rows is not None and rows.shape[0] != n:
+        raise ValueError(f"{who}: {rows.shape[0]} rows for {n} targets")
+    if rows is None and n > hidden.shape[0]:
+        raise ValueError(f"{who}: {n} targets for {hidden.shape[0]} rows of hidden")
+
+
+class HeadCall:
+    """The library's view of one classifier call (arguments as check_head
+    takes them), with the tensors that it points to."""
 
     def __init__(self, hidden, weight, bias=None, rows=None, labels=None, teacher_index=None, teacher_logits=None,
                  temperature: float = 1.0):
-        who = "linear_cross_entropy" if labels is not None else "linear_distill"
-        L.require_device(who, hidden.device, weight, bias, rows, labels, teacher_index, teacher_logits)
-        if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] or weight.numel() == 0:
-            raise ValueError(f"{who}: hidden must be [rows, width] and weight [classes, width] (got "
-                             f"{tuple(hidden.shape)} and {tuple(weight.shape)})")
-        code = L.dtype_code(hidden.dtype)
-        if weight.dtype != hidden.dtype or (bias is not None and bias.dtype != hidden.dtype):
-            raise TypeError(f"{who}: hidden, weight and bias must have one dtype")
-        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
-            raise ValueError(f"{who}: bias must be [classes]")
-        if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int64):
-            raise ValueError(f"{who}: rows must be int64 [n]")
-        k = 0
-        if labels is not None:
-            if labels.dim() != 1 or labels.dtype != torch.int64:
-                raise ValueError(f"{who}: labels must be int64 [n]")
-            n = labels.shape[0]
-            self.labels, self.index, self.logits = labels.contiguous(), None, None
-        else:
-            if (teacher_index.dim() != 2 or teacher_index.dtype not in (torch.int32, torch.int64)
-                    or teacher_logits.shape != teacher_index.shape or not teacher_logits.is_floating_point()):
-                raise ValueError(f"{who}: teacher_index must be int32 or int64 [n, k] and teacher_logits [n, k]")
-            n, k = teacher_index.shape
-            if not 1 <= k <= 1024:
-                raise ValueError(f"{who}: 1 to 1024 teacher entries a row (got {k})")
-            if not 0.0 < float(temperature) < float("inf"):
-                raise ValueError(f"{who}: the temperature must be positive (got {temperature})")
-            self.labels = None
-            self.index, self.logits = teacher_index.contiguous(), teacher_logits.detach().float().contiguous()
-        if rows is not None and rows.shape[0] != n:
-            raise ValueError(f"{who}: {rows.shape[0]} rows for {n} targets")
-        if rows is None and n > hidden.shape[0]:
-            raise ValueError(f"{who}: {n} targets for {hidden.shape[0]} rows of hidden")
-        self.who, self.n, self.k = who, n, k
-        self.hidden, self.weight = _unit_columns(hidden.detach()), _unit_columns(weight.detach())
-        self.bias = bias.detach().contiguous() if bias is not None else None
+        self.hidden, self.weight = _unit_columns(hidden), _unit_columns(weight)
+        self.bias = bias.contiguous() if bias is not None else None
         self.rows = rows.contiguous() if rows is not None else None
-        self.view = L.HeadView(L.ptr(self.hidden), L.ptr(self.weight), L.ptr(self.bias), L.ptr(self.rows),
+        if labels is not None:
+            self.labels, self.index, self.logits = labels.contiguous(), None, None
+            self.n, self.k, i64 = labels.shape[0], 0, 0
+        else:
+            self.labels = None
+            self.index, self.logits = teacher_index.contiguous(), teacher_logits.float().contiguous()
+            self.n, self.k = teacher_index.shape
+            i64 = int(teacher_index.dtype == torch.int64)
+        self.view = L.HeadView(self.hidden.data_ptr(), self.weight.data_ptr(), L.ptr(self.bias), L.ptr(self.rows),
                                L.ptr(self.labels), L.ptr(self.index), L.ptr(self.logits), _row_pitch(self.hidden),
-                               _row_pitch(self.weight), hidden.shape[0], n, hidden.shape[1], weight.shape[0], code,
-                               k, int(k > 0 and self.index.dtype == torch.int64), float(temperature))
+                               _row_pitch(self.weight), hidden.shape[0], self.n, hidden.shape[1], weight.shape[0],
+                               L.dtype_code(hidden.dtype), self.k, i64, float(temperature))
 
     def saved_pointers(self, saved: torch.Tensor):
         """Addresses of lse, the targets' logits and the teacher's
@@ -1925,7 +1934,7 @@ def head_bwd(call: HeadCall, saved: torch.Tensor, counts: torch.Tensor, dloss: t
     loss (dloss a scalar, or [n] per row)."""
     dev = call.hidden.device
     lse, logit, prob = call.saved_pointers(saved)
-    dl = dloss.detach().float().contiguous()
+    dl = dloss.float().contiguous()
     dh = dw = db = None
     if need[0]:
         some = call.rows is not None or call.n < call.hidden.shape[0]

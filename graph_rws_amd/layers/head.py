@@ -51,6 +51,7 @@ def _apply(hidden, weight, bias, rows, labels, index, logits, temperature, reduc
         dt = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dt), weight.to(dt)
         bias = bias.to(dt) if bias is not None else None
+    _ops.check_head(hidden, weight, bias, rows, labels, index, logits, temperature)
     return _Head.apply(hidden, weight, bias, rows, labels, index, logits, float(temperature), reduction == "none")
 
 
