@@ -22,7 +22,11 @@
 // G is rounded to the operands' 16-bit type because the matrix cores take no
 // wider one; p - q is formed in fp32 and rounded once.  Its factor s_i T is
 // applied to the fp32 sums instead (f16: G carries 2^15, so that
-// probabilities down to 2^-29 stay normal numbers).
+// probabilities down to 2^-29 stay normal numbers).  Up to kFewClasses classes
+// G keeps a second plane, what the rounding left over: there a handful of its
+// entries make most of a sum and the rounding shows (0.0027 of a bf16 gradient
+// against 0.0017 for rounding the gradient alone), and the second product is
+// short.
 //
 // F32 operands: x = a + b + c with three bf16 (the top, middle and low 8 of
 // 24 significant bits, truncated, so the split is exact and never
@@ -75,14 +79,15 @@ struct Opnd {
 
 struct Gemm {
     Opnd P, Q;
-    int32_t nseg;    // plane products: 1, or 6 for split f32 operands
+    int32_t nseg;    // plane products: 1, 6 for split f32 operands, or 2 (Q, which is G, in two planes)
     int32_t ksteps;  // stages per plane product
     int32_t tp, tq;  // tiles along p and q
     int32_t splits;  // work-groups per tile along k
 };
 
-// The planes of product `seg` (the last six-plane product, and the only one
-// of 16-bit operands, is plane 0 by plane 0); small products come first.
+// The planes of product `seg`: the last nseg of these six, small products
+// first (plane 0 by plane 0 is the only one of 16-bit operands, plane 0 by Q's
+// plane 1 the one before).
 __device__ __forceinline__ int plane_p(int seg) { return (0x001102 >> (4 * seg)) & 15; }
 __device__ __forceinline__ int plane_q(int seg) { return (0x010120 >> (4 * seg)) & 15; }
 
@@ -468,12 +473,20 @@ __device__ __forceinline__ uint16_t round16(float x) {
     else return __builtin_bit_cast(uint16_t, __float2bfloat16(x));
 }
 
-template <int DT, bool SPLIT>
-__device__ __forceinline__ void store_g(uint16_t* G, int64_t plane, int64_t at, float x) {
-    if constexpr (SPLIT) {
-        split3(x, G + at, G + plane + at, G + 2 * plane + at);
+template <int DT>
+__device__ __forceinline__ float from16(uint16_t h) {
+    if constexpr (DT == GRWS_F16) return (float)__builtin_bit_cast(_Float16, h);
+    else return from_top16(h);
+}
+
+// an entry of G in its planes
+template <int DT, int PLANES>
+__device__ __forceinline__ void planes_of(float x, uint16_t (&h)[PLANES]) {
+    if constexpr (PLANES == 3) {
+        split3(x, &h[0], &h[1], &h[2]);
     } else {
-        G[at] = round16<DT>(x);
+        h[0] = round16<DT>(x);
+        if constexpr (PLANES == 2) h[1] = round16<DT>(x - from16<DT>(h[0]));
     }
 }
 
@@ -486,7 +499,7 @@ __device__ __forceinline__ float rotate(float x) {
 
 constexpr int kBiasRows = 64;  // rows of a part of the bias gradient's sums
 
-template <int DT, bool SPLIT, int BP, int BQ, int WP, int WQ>
+template <int DT, int PLANES, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
     using C = Core<DT, false, false, BP, BQ, WP, WQ>;
     constexpr int TP = C::TP, TQ = C::TQ;
@@ -526,18 +539,14 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
 #pragma unroll
         for (int i = 0; i < TP; i += 2) {  // 8 consecutive classes of accumulators i and i + 1
             const int64_t at = row * a.ldg + pfirst + C::p_of(i, lane);
-            uint16_t h[SPLIT ? 3 : 1][8];
+            uint16_t h[8][PLANES];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = acc[i + (e >> 2)][j][e & 3];
-                if constexpr (SPLIT) split3(x, &h[0][e], &h[1][e], &h[2][e]);
-                else h[0][e] = round16<DT>(x);
-            }
+            for (int e = 0; e < 8; ++e) planes_of<DT, PLANES>(acc[i + (e >> 2)][j][e & 3], h[e]);
 #pragma unroll
-            for (int z = 0; z < (SPLIT ? 3 : 1); ++z) {
+            for (int z = 0; z < PLANES; ++z) {
                 u32x4_t w;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)h[z][2 * e] | ((uint32_t)h[z][2 * e + 1] << 16);
+                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)h[2 * e][z] | ((uint32_t)h[2 * e + 1][z] << 16);
                 *reinterpret_cast<u32x4_t*>(a.G + z * a.plane + at) = w;
             }
         }
@@ -1108,7 +1117,7 @@ __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __rest
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.
 // (A label's place is known to the product's epilogue: one for a row.)
-template <int DT, bool SPLIT>
+template <int DT, int PLANES>
 __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const float* __restrict__ lse,
                                                             const float* __restrict__ y,
                                                             const float* __restrict__ coef,
@@ -1123,14 +1132,17 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const flo
     const float q = coef[at], l = lse[i];
     if (q < 0.f || l == INFINITY) return;
     const float s = row_scale ? row_scale[i] * gscale : gscale;
-    store_g<DT, SPLIT>(G, plane, i * ldg + (v - v0), (exp2f(y[at] - l) - q) * s);
+    uint16_t h[PLANES];
+    planes_of<DT, PLANES>((exp2f(y[at] - l) - q) * s, h);
+#pragma unroll
+    for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
 }
 
 // Column sums of a piece of G over runs of kBiasRows rows, 4 waves of 16 rows,
 // 8 columns a lane: after head_subtract_kernel (with labels the gradient
 // product's epilogue has made them).
 
-template <int DT, bool SPLIT>
+template <int DT, int PLANES>
 __global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __restrict__ G, int64_t ldg,
                                                              int64_t plane, int64_t vp, float* __restrict__ part) {
     __shared__ float red[4][512];
@@ -1142,13 +1154,12 @@ __global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __r
 #pragma unroll 4
         for (int64_t r = r0; r < r0 + kBiasRows / 4; ++r) {
 #pragma unroll
-            for (int z = SPLIT ? 2 : 0; z >= 0; --z) {
+            for (int z = PLANES - 1; z >= 0; --z) {
                 const u32x4_t v = *reinterpret_cast<const u32x4_t*>(G + z * plane + r * ldg + c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint16_t h = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-                    if constexpr (DT == GRWS_F16) s[e] += (float)__builtin_bit_cast(_Float16, h);
-                    else s[e] += from_top16(h);
+                    s[e] += from16<DT>(h);
                 }
             }
         }
@@ -1234,6 +1245,7 @@ constexpr int64_t kJoinBlocks = 128;
 // 256 MiB, 4.70 with 512 and 4.54 with 1 GiB (fewer, fuller launches); at
 // 8,192 x 131,072 x 4,096 it makes 1%.
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
+constexpr int64_t kFewClasses = 1024;  // up to here G has a second plane
 constexpr int64_t kPackBytes = (int64_t)256 << 20;  // a packed piece of W
 
 // A product's tile and the runs that its k is cut into: the least of
@@ -1265,7 +1277,7 @@ Plan plan(int64_t p, int64_t q, int64_t stages, int64_t most_splits, double besi
 // Sizes of a call, the same for the workspace query and the launch.
 struct Shape {
     int64_t n, D, V;
-    int planes;
+    int planes, gplanes;  // of the operands, of G
     bool split;       // f32 operands in three planes
     bool pack_w;      // W goes through a packed copy
     int64_t np, dp, vp;  // padded rows and width; classes of a piece
@@ -1289,18 +1301,19 @@ Shape shape_of(const grws_head* h, bool backward) {
     s.V = h->classes;
     s.split = h->dtype == GRWS_F32;
     s.planes = s.split ? 3 : 1;
+    s.gplanes = s.split ? 3 : s.V <= kFewClasses ? 2 : 1;
     s.pack_w = !weight_in_place(h);
     s.np = pad(s.n);
     s.dp = up(s.D, kK);
     s.vp = pad(s.V);
-    auto bound = [&](int64_t bytes, int64_t row_elements) {
-        int64_t most = bytes / (2 * s.planes * row_elements) / 256 * 256;
+    auto bound = [&](int64_t bytes, int64_t column_bytes) {
+        int64_t most = bytes / column_bytes / 256 * 256;
         if (most < 256) most = 256;
         if (s.vp > most) s.vp = most;
     };
-    if (backward) bound(kPieceBytes, s.np);
-    if (s.pack_w) bound(kPackBytes, s.dp);
-    const int64_t seg = s.split ? 6 : 1;
+    if (backward) bound(kPieceBytes, 2 * s.gplanes * s.np);
+    if (s.pack_w) bound(kPackBytes, 2 * s.planes * s.dp);
+    const int64_t seg = s.split ? 6 : 1, gseg = s.split ? 6 : s.gplanes;
     // the pieces: as few and as equal as the bound allows, or up to three
     // more where the tiles then fill the rounds better
     const int64_t fewest = ceil_div(s.V, s.vp), whole = s.vp;
@@ -1311,8 +1324,8 @@ Shape shape_of(const grws_head* h, bool backward) {
         const Plan l = plan(vp, s.np, seg * s.dp / kK, 1, 6);
         Plan w{}, d{};
         if (backward) {
-            w = plan(s.D, vp, seg * s.np / kK, ceil_div(s.np / kK, 4), 4);
-            d = plan(s.dp, s.np, seg * vp / kK, ceil_div(vp / kK, 4), 4);
+            w = plan(s.D, vp, gseg * s.np / kK, ceil_div(s.np / kK, 4), 4);
+            d = plan(s.dp, s.np, gseg * vp / kK, ceil_div(vp / kK, 4), 4);
         }
         const double t = (double)ceil_div(s.V, vp) * (l.cost + w.cost + d.cost + 6);
         if (t < least) {
@@ -1397,7 +1410,7 @@ void bwd_space(A& a, const Shape& s, BwdSpace* f) {
     };
     take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
-    take(f->G, s.planes * s.np * s.ldg);
+    take(f->G, s.gplanes * s.np * s.ldg);
     if (s.hidden.splits > 1 || s.vp < s.V) take(f->dh, s.hidden.splits * s.np * s.dp);
     if (s.weight.splits > 1) take(f->dw, s.weight.splits * s.vp * s.dp);
     take(f->bias, s.np / kBiasRows * s.vp);
@@ -1460,8 +1473,9 @@ Opnd hidden_operand(const Shape& s, const uint16_t* hp, bool strided) {
     return strided ? Opnd{p, s.dp * 2, plane, s.dp, s.np} : Opnd{p, s.dp * 2, plane, s.np, s.dp};
 }
 
-Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64_t np, int64_t nq, int64_t k) {
-    return Gemm{P, Q, s.split ? 6 : 1, (int32_t)ceil_div(k, kK), (int32_t)ceil_div(np, pl.tile),
+Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64_t np, int64_t nq, int64_t k,
+             int planes) {
+    return Gemm{P, Q, planes == 3 ? 6 : planes, (int32_t)ceil_div(k, kK), (int32_t)ceil_div(np, pl.tile),
                 (int32_t)ceil_div(nq, pl.tile), (int32_t)pl.splits};
 }
 
@@ -1516,7 +1530,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, s.np, c1,
+        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, s.np, c1,
                     h->bias, h->dtype, h->labels, f.part, target_logit, f.flags};
         if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
         else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
@@ -1609,20 +1623,26 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         const int64_t vt = up(vc, s.logits.tile);  // G's columns that are written
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp), v0, s.V, s.n, c1, h->bias,
+        GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, c1, h->bias,
                    h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane,
                    d_bias && h->k == 0 ? f.bias : nullptr, vt};
-        if (s.split) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, true);
-        else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_F16, false);
-        else GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, GRWS_BF16, false);
+#define GRWS_HEAD_PLANES(X)                                  \
+    do {                                                     \
+        if (s.split) X(GRWS_BF16, 3);                        \
+        else if (h->dtype == GRWS_F16 && s.gplanes == 1) X(GRWS_F16, 1); \
+        else if (h->dtype == GRWS_F16) X(GRWS_F16, 2);       \
+        else if (s.gplanes == 1) X(GRWS_BF16, 1);            \
+        else X(GRWS_BF16, 2);                                \
+    } while (0)
+#define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
+        GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
+#undef GRWS_HEAD_GRAD
         if (h->k > 0) {
             const dim3 grid((unsigned)ceil_div(s.n * h->k, 256));
-#define GRWS_HEAD_SUB(DT, SP)                                                                                 \
-    hipLaunchKernelGGL((head_subtract_kernel<DT, SP>), grid, dim3(256), 0, stream, t, lse, target_logit, coef, \
+#define GRWS_HEAD_SUB(DT, PL)                                                                                 \
+    hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, lse, target_logit, coef, \
                        row_scale, gscale, s.n, v0, vc, f.G, s.ldg, plane)
-            if (s.split) GRWS_HEAD_SUB(GRWS_BF16, true);
-            else if (h->dtype == GRWS_F16) GRWS_HEAD_SUB(GRWS_F16, false);
-            else GRWS_HEAD_SUB(GRWS_BF16, false);
+            GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
 #undef GRWS_HEAD_SUB
             GRWS_LAUNCH_CHECK();
         }
@@ -1631,11 +1651,9 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             const int64_t nparts = s.np / kBiasRows;
             if (h->k > 0) {  // with labels head_grad_kernel has made the parts
                 const dim3 grid((unsigned)nparts, (unsigned)ceil_div(vt, 512));
-#define GRWS_HEAD_BIAS_PART(DT, SP)                                                                               \
-    hipLaunchKernelGGL((head_bias_part_kernel<DT, SP>), grid, dim3(256), 0, stream, f.G, s.ldg, plane, vt, f.bias)
-                if (s.split) GRWS_HEAD_BIAS_PART(GRWS_BF16, true);
-                else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS_PART(GRWS_F16, false);
-                else GRWS_HEAD_BIAS_PART(GRWS_BF16, false);
+#define GRWS_HEAD_BIAS_PART(DT, PL)                                                                               \
+    hipLaunchKernelGGL((head_bias_part_kernel<DT, PL>), grid, dim3(256), 0, stream, f.G, s.ldg, plane, vt, f.bias)
+                GRWS_HEAD_PLANES(GRWS_HEAD_BIAS_PART);
 #undef GRWS_HEAD_BIAS_PART
                 GRWS_LAUNCH_CHECK();
             }
@@ -1654,7 +1672,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
             const int32_t vec = reinterpret_cast<uintptr_t>(d_weight) % (4 * esz) == 0 && ld_dw % 4 == 0;
             const Opnd G{gp, s.ldg * 2, plane * 2, s.ldg, s.np};
-            WeightArgs w{gemm_of(s, s.weight, hidden_operand(s, f.hp, true), G, s.D, vc, s.np), f.alpha, out, ld_dw,
+            WeightArgs w{gemm_of(s, s.weight, hidden_operand(s, f.hp, true), G, s.D, vc, s.np, s.gplanes), f.alpha, out, ld_dw,
                          vc, s.D, vec, f.dw, s.vp, s.dp};
             if (s.split) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_F16, GRWS_F16);
@@ -1674,7 +1692,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, false, stream));
             const Opnd G{gp, s.ldg * 2, plane * 2, s.np, vt};
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
-            HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc), f.dh, s.np, s.dp, v0 == 0,
+            HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc, s.gplanes), f.dh, s.np, s.dp, v0 == 0,
                          s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
                          h->hidden_rows, h->rows};
             if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
@@ -1682,6 +1700,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
         }
     }
+#undef GRWS_HEAD_PLANES
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
