@@ -942,6 +942,209 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
     }
 }
 
+// Logits of few rows (up to 64, 16 NQ): W is read once, as it lies, straight
+// into the MFMA's operands; nothing of it is packed or staged.  A wave owns 32
+// classes; f32 operands go to the f32 MFMA.  Forward: the strips' statistics
+// (strips of 32 classes); backward (GRAD): G.  Bound by W's stream.
+struct FewArgs {
+    Targets t;
+    const void *hidden, *weight, *bias;
+    int64_t ldh, ldw, n, np, width, v0, vend, classes;  // classes v0..vend of a piece
+    float c1;
+    // forward
+    const int32_t* states;  // of a teacher's lists
+    float2* part;
+    float* ylabel;
+    int32_t* earlier;
+    int32_t* done;
+    // backward
+    const float *lse, *row_scale;
+    float gscale;
+    uint16_t* G;
+    int64_t ldg, plane;
+    float* bias_part;
+    int64_t vt;
+};
+
+template <typename T, int NQ, int PLANES, bool VEC>
+__global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
+    constexpr bool GRAD = PLANES > 0;
+    constexpr int DT = std::is_same_v<T, _Float16> ? GRWS_F16 : GRWS_BF16;
+    constexpr int E = 16 / sizeof(T);  // elements of a 16-byte load
+    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    if (!GRAD && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
+    const int64_t vfirst = a.v0 + ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
+    const T* w[2];
+    const T* h[NQ];
+    bool live[NQ];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t v = vfirst + 16 * i + r;
+        w[i] = static_cast<const T*>(a.weight) + (v < a.classes ? v : 0) * a.ldw;
+    }
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        const int64_t row = 16 * j + r;
+        if constexpr (GRAD) live[j] = row < a.n && a.lse[row] != INFINITY;
+        else live[j] = row < a.n && (a.t.labels ? row_state<1>(a.t, row, 0) : a.states[row]) == 1;
+        h[j] = static_cast<const T*>(a.hidden) + (live[j] ? (a.t.rows ? a.t.rows[row] : row) * a.ldh : 0);
+    }
+    float4_t acc[2][NQ];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+    struct Frag {
+        T x[E];
+    };
+    auto read = [&](const T* p, int64_t c, bool whole) {
+        Frag f;
+        if (VEC && whole) {
+            __builtin_memcpy(&f, __builtin_assume_aligned(p + c, 16), 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) f.x[e] = whole || c + e < a.width ? p[c + e] : from_float<T>(0.f);
+        }
+        return f;
+    };
+    constexpr int STEP = 4 * E;                       // k of a step: the four lane groups
+    constexpr int U = NQ == 1 ? 4 : NQ == 2 ? 3 : 2;  // steps whose loads are in flight
+    auto multiply = [&](int64_t c, int steps, bool whole) {
+        Frag x[U][2], y[U][NQ];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= steps) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[u][i] = read(w[i], c + u * STEP, whole);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                y[u][j] = read(h[j], c + u * STEP, whole);
+                if (!live[j]) y[u][j] = Frag{};  // what such a row holds stays out
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= steps) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) {
+                    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[u][i].x[e], y[u][j].x[e], acc[i][j], 0,
+                                                                             0, 0);
+                    } else {
+                        acc[i][j] = mma<DT>(__builtin_bit_cast(short8_t, x[u][i]),
+                                            __builtin_bit_cast(short8_t, y[u][j]), acc[i][j]);
+                    }
+                }
+        }
+    };
+    int64_t c = g * E;
+    for (; c - g * E + U * STEP <= a.width; c += U * STEP) multiply(c, U, true);
+    for (; c - g * E + STEP <= a.width; c += STEP) multiply(c, 1, true);
+    if (c - g * E < a.width) multiply(c, 1, false);
+    // class vfirst + 16 i + 4 g + e
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t v = vfirst + 16 * i + 4 * g + e;
+            const bool in = v < a.vend;
+            const float b = a.bias && in ? to_float(static_cast<const T*>(a.bias)[v]) : 0.f;
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) acc[i][j][e] = in ? acc[i][j][e] + b : -INFINITY;
+        }
+    float4_t sums[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        const int64_t row = 16 * j + r;
+        const int64_t lab = live[j] && a.t.labels ? a.t.labels[row] - vfirst : -1;
+        const bool here = lab >= 0 && lab < 32;
+        const int l = here ? (int)lab : -1;
+        if constexpr (!GRAD) {
+            float m = -INFINITY, y = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    m = fmaxf(m, acc[i][j][e]);
+                    y = 16 * i + 4 * g + e == l ? acc[i][j][e] : y;
+                }
+            m = fmaxf(m, __shfl_xor(m, 16, kWave));
+            m = fmaxf(m, __shfl_xor(m, 32, kWave)) * a.c1;
+            y = __shfl(y, (((l >> 2) & 3) << 4) | r, kWave);
+            const float ref = m == -INFINITY ? 0.f : m;
+            float s = 0.f;
+            int tie = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -ref));
+                    tie |= acc[i][j][e] == y && 16 * i + 4 * g + e < l;
+                }
+            s += __shfl_xor(s, 16, kWave);
+            s += __shfl_xor(s, 32, kWave);
+            tie |= __shfl_xor(tie, 16, kWave);
+            tie |= __shfl_xor(tie, 32, kWave);
+            if (g == 0) {
+                a.part[vfirst / 32 * a.np + row] = make_float2(m, s);
+                if (here) {
+                    a.ylabel[row] = y * a.c1;
+                    a.earlier[row] = tie;
+                }
+            }
+        } else {
+            const float lse = live[j] ? a.lse[row] : INFINITY;
+            const float sc = a.row_scale && live[j] ? a.row_scale[row] * a.gscale : a.gscale;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint16_t x[4][PLANES > 0 ? PLANES : 1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -lse));
+                    p = (16 * i + 4 * g + e == l ? p - 1.f : p) * sc;
+                    sums[i][e] += p;
+                    planes_of<DT, PLANES>(p, x[e]);
+                }
+#pragma unroll
+                for (int z = 0; z < PLANES; ++z)
+                    *reinterpret_cast<u32x2_t*>(a.G + z * a.plane + row * a.ldg + (vfirst - a.v0) + 16 * i + 4 * g) =
+                        u32x2_t{(uint32_t)x[0][z] | ((uint32_t)x[1][z] << 16),
+                                (uint32_t)x[2][z] | ((uint32_t)x[3][z] << 16)};
+            }
+        }
+    }
+    if constexpr (GRAD) {
+        // the padding rows, which dW's product reads
+        for (int64_t row = 16 * NQ + r; row < a.np; row += 16)
+#pragma unroll
+            for (int z = 0; z < PLANES; ++z)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    *reinterpret_cast<u32x2_t*>(a.G + z * a.plane + row * a.ldg + (vfirst - a.v0) + 16 * i + 4 * g) =
+                        u32x2_t{0u, 0u};
+        if (a.bias_part) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sums[i][e] += rotate<8>(sums[i][e]);
+                    sums[i][e] += rotate<4>(sums[i][e]);
+                    sums[i][e] += rotate<2>(sums[i][e]);
+                    sums[i][e] += rotate<1>(sums[i][e]);
+                }
+                for (int64_t b = 0; b < a.np / kBiasRows; ++b)
+                    if (r == 0)
+                        *reinterpret_cast<float4_t*>(a.bias_part + b * a.vt + (vfirst - a.v0) + 16 * i + 4 * g) =
+                            b == 0 ? sums[i] : float4_t{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void join(float& m, float& s, int& first, float om, float os, int ofirst) {
     if (om > m) {
         s = s * __builtin_amdgcn_exp2f(m - om) + os;
@@ -1256,6 +1459,8 @@ constexpr int64_t kJoinBlocks = 128;
 // 8,192 x 131,072 x 4,096 it makes 1%.
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 constexpr int64_t kFewClasses = 1024;  // up to here G has a second plane
+// Rows up to which head_few_kernel makes the logits: FEWNOTE
+constexpr int64_t kFewRows = 16, kFewPacked = 64;
 constexpr int64_t kPackBytes = (int64_t)256 << 20;  // a packed piece of W
 
 // A product's tile and the runs that its k is cut into: the least of
@@ -1290,6 +1495,7 @@ struct Shape {
     int planes, gplanes;  // of the operands, of G
     bool split;       // f32 operands in three planes
     bool pack_w;      // W goes through a packed copy
+    bool few;         // few rows: head_few_kernel makes the logits
     int64_t np, dp, vp;  // padded rows and width; classes of a piece
     int64_t ldg;         // pitch of G: rows start 256 bytes apart mod 4 KiB
     Plan logits, weight, hidden;
@@ -1313,6 +1519,7 @@ Shape shape_of(const grws_head* h, bool backward) {
     s.planes = s.split ? 3 : 1;
     s.gplanes = s.split ? 3 : s.V <= kFewClasses ? 2 : 1;
     s.pack_w = !weight_in_place(h);
+    s.few = s.n <= (s.pack_w ? kFewPacked : kFewRows);
     s.np = pad(s.n);
     s.dp = up(s.D, kK);
     s.vp = pad(s.V);
@@ -1346,7 +1553,7 @@ Shape shape_of(const grws_head* h, bool backward) {
             s.hidden = d;
         }
     }
-    s.strip_classes = s.logits.tile / 2;
+    s.strip_classes = s.few ? 32 : s.logits.tile / 2;
     s.strips = pad(s.V) / s.strip_classes;
     s.ldg = s.vp + 128;
     return s;
@@ -1396,12 +1603,12 @@ void fwd_space(A& a, const Shape& s, FwdSpace* f) {
         if constexpr (std::is_same_v<A, Sizer>) a.template take<T>((size_t)n);
         else p = a.template take<T>((size_t)n);
     };
-    take(f->hp, s.planes * s.np * s.dp);
-    if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
+    if (!s.few) take(f->hp, s.planes * s.np * s.dp);
+    if (s.pack_w && !s.few) take(f->wp, s.planes * s.vp * s.dp);
     take(f->part, s.strips * s.np);
     take(f->flags, s.n);
-    take(f->pl, ceil_div(s.n, 4));
-    take(f->pc, 3 * ceil_div(s.n, 4));
+    take(f->pl, s.n <= 8 ? 8 : ceil_div(s.n, 4));
+    take(f->pc, s.n <= 8 ? 24 : 3 * ceil_div(s.n, 4));
     take(f->done, 1);
 }
 
@@ -1489,6 +1696,23 @@ Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64
                 (int32_t)ceil_div(nq, pl.tile), (int32_t)pl.splits};
 }
 
+template <typename T, int PLANES>
+int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
+    const bool vec = rows_of_16(h->weight, h->ld_weight, h->dtype) && rows_of_16(h->hidden, h->ld_hidden, h->dtype);
+    const dim3 grid((unsigned)ceil_div(a.vt, 128));
+#define GRWS_HEAD_FEW(NQ)                                                                                         \
+    do {                                                                                                          \
+        if (vec) hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, true>), grid, dim3(256), 0, stream, a);        \
+        else hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, false>), grid, dim3(256), 0, stream, a);           \
+    } while (0)
+    if (a.n <= 16) GRWS_HEAD_FEW(1);
+    else if (a.n <= 32) GRWS_HEAD_FEW(2);
+    else GRWS_HEAD_FEW(4);
+#undef GRWS_HEAD_FEW
+    GRWS_LAUNCH_CHECK();
+    return GRWS_OK;
+}
+
 // NAME<..., BP, BQ, WP, WQ> at a plan's tile
 #define GRWS_HEAD_LAUNCH(PLAN, NAME, ARGS, ...)                                                                      \
     do {                                                                                                             \
@@ -1535,16 +1759,6 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
     fwd_space(cv, s, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
-    GRWS_TRY(pack_hidden(h, s, t, f.hp, Alpha{}, f.done, stream));
-    for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
-        const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
-        Opnd W;
-        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, s.np, c1,
-                    h->bias, h->dtype, h->labels, f.part, target_logit, f.flags};
-        if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
-        else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
-    }
     if (h->k > 0) {
         const dim3 grid((unsigned)ceil_div(s.n * ((h->k + 3) / 4), 4));
         const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype) &&
@@ -1559,13 +1773,33 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
 #undef GRWS_HEAD_TARGETS
         GRWS_LAUNCH_CHECK();
     }
-    const int64_t rows = s.n <= 512 ? 4 : 16, blocks = ceil_div(s.n, rows);
+    if (s.few) {
+        FewArgs a{t, h->hidden, h->weight, h->bias, h->ld_hidden, h->ld_weight, s.n, s.np, s.D, 0, s.V, s.V, c1,
+                  f.flags, f.part, target_logit, f.flags, f.done};
+        a.vt = pad(s.V);
+        if (h->dtype == GRWS_F32) GRWS_TRY((launch_few<float, 0>(h, a, stream)));
+        else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 0>(h, a, stream)));
+        else GRWS_TRY((launch_few<__hip_bfloat16, 0>(h, a, stream)));
+    } else {
+        GRWS_TRY(pack_hidden(h, s, t, f.hp, Alpha{}, f.done, stream));
+    }
+    for (int64_t v0 = 0; v0 < s.V && !s.few; v0 += s.vp) {
+        const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
+        Opnd W;
+        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
+        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, s.np, c1,
+                    h->bias, h->dtype, h->labels, f.part, target_logit, f.flags};
+        if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
+        else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
+    }
+    const int64_t rows = s.n <= 8 ? 1 : s.n <= 512 ? 4 : 16, blocks = ceil_div(s.n, rows);
 #define GRWS_HEAD_JOIN(R)                                                                                            \
     hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part,                 \
                        ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature,          \
                        target_logit, target_prob, f.flags, lse, row_loss, f.pl, f.pc,                                \
                        blocks <= kJoinBlocks ? f.done : nullptr, loss, counts)
-    if (rows == 4) GRWS_HEAD_JOIN(4);
+    if (rows == 1) GRWS_HEAD_JOIN(1);
+    else if (rows == 4) GRWS_HEAD_JOIN(4);
     else GRWS_HEAD_JOIN(16);
 #undef GRWS_HEAD_JOIN
     GRWS_LAUNCH_CHECK();
@@ -1630,12 +1864,8 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
     const size_t esz = dtype_size(h->dtype);
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
-        const int64_t vt = up(vc, s.logits.tile);  // G's columns that are written
+        const int64_t vt = up(vc, s.few ? 128 : s.logits.tile);  // G's columns that are written
         Opnd W;
-        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, c1, h->bias,
-                   h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane,
-                   d_bias && h->k == 0 ? f.bias : nullptr, vt};
 #define GRWS_HEAD_PLANES(X)                                  \
     do {                                                     \
         if (s.split) X(GRWS_BF16, 3);                        \
@@ -1644,9 +1874,28 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         else if (s.gplanes == 1) X(GRWS_BF16, 1);            \
         else X(GRWS_BF16, 2);                                \
     } while (0)
+        if (s.few) {
+            FewArgs a{};
+            a.t = t;
+            a.hidden = h->hidden, a.weight = h->weight, a.bias = h->bias;
+            a.ldh = h->ld_hidden, a.ldw = h->ld_weight, a.n = s.n, a.np = s.np, a.width = s.D;
+            a.v0 = v0, a.vend = v0 + vc, a.classes = s.V, a.c1 = c1;
+            a.lse = lse, a.row_scale = row_scale, a.gscale = gscale, a.G = f.G, a.ldg = s.ldg, a.plane = plane;
+            a.bias_part = d_bias && h->k == 0 ? f.bias : nullptr, a.vt = vt;
+            if (s.split) GRWS_TRY((launch_few<float, 3>(h, a, stream)));
+            else if (h->dtype == GRWS_F16 && s.gplanes == 1) GRWS_TRY((launch_few<_Float16, 1>(h, a, stream)));
+            else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 2>(h, a, stream)));
+            else if (s.gplanes == 1) GRWS_TRY((launch_few<__hip_bfloat16, 1>(h, a, stream)));
+            else GRWS_TRY((launch_few<__hip_bfloat16, 2>(h, a, stream)));
+        } else {
+            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
+            GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, c1, h->bias,
+                       h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane,
+                       d_bias && h->k == 0 ? f.bias : nullptr, vt};
 #define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
-        GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
+            GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
 #undef GRWS_HEAD_GRAD
+        }
         if (h->k > 0) {
             const dim3 grid((unsigned)ceil_div(s.n * h->k, 256));
 #define GRWS_HEAD_SUB(DT, PL)                                                                                 \
@@ -1699,7 +1948,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             }
         }
         if (d_hidden) {
-            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, false, stream));
+            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, s.few, stream));
             const Opnd G{gp, s.ldg * 2, plane * 2, s.np, vt};
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
             HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc, s.gplanes), f.dh, s.np, s.dp, v0 == 0,
