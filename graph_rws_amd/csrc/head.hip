@@ -942,7 +942,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
     }
 }
 
-// Logits of few rows (up to 64, 16 NQ): W is read once, as it lies, straight
+// Logits of few rows (16 NQ a work-group, 64 at most): W is read once, as it lies, straight
 // into the MFMA's operands; nothing of it is packed or staged.  A wave owns 32
 // classes; f32 operands go to the f32 MFMA.  Forward: the strips' statistics
 // (strips of 32 classes); backward (GRAD): G.  Bound by W's stream.
@@ -972,7 +972,8 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     constexpr int DT = std::is_same_v<T, _Float16> ? GRWS_F16 : GRWS_BF16;
     constexpr int E = 16 / sizeof(T);  // elements of a 16-byte load
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    if (!GRAD && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
+    const int64_t first = (int64_t)blockIdx.y * (16 * NQ);  // row
+    if (!GRAD && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.done = 0;
     const int64_t vfirst = a.v0 + ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
     const T* w[2];
     const T* h[NQ];
@@ -984,7 +985,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-        const int64_t row = 16 * j + r;
+        const int64_t row = first + 16 * j + r;
         if constexpr (GRAD) live[j] = row < a.n && a.lse[row] != INFINITY;
         else live[j] = row < a.n && (a.t.labels ? row_state<1>(a.t, row, 0) : a.states[row]) == 1;
         h[j] = static_cast<const T*>(a.hidden) + (live[j] ? (a.t.rows ? a.t.rows[row] : row) * a.ldh : 0);
@@ -1059,7 +1060,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     float4_t sums[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-        const int64_t row = 16 * j + r;
+        const int64_t row = first + 16 * j + r;
         const int64_t lab = live[j] && a.t.labels ? a.t.labels[row] - vfirst : -1;
         const bool here = lab >= 0 && lab < 32;
         const int l = here ? (int)lab : -1;
@@ -1118,8 +1119,9 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
         }
     }
     if constexpr (GRAD) {
-        // the padding rows, which dW's product reads
-        for (int64_t row = 16 * NQ + r; row < a.np; row += 16)
+        // the padding rows, which dW's product reads: the last rows' work-group
+        const bool last = blockIdx.y + 1 == gridDim.y;
+        for (int64_t row = first + 16 * NQ + r; last && row < a.np; row += 16)
 #pragma unroll
             for (int z = 0; z < PLANES; ++z)
 #pragma unroll
@@ -1136,10 +1138,11 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                     sums[i][e] += rotate<2>(sums[i][e]);
                     sums[i][e] += rotate<1>(sums[i][e]);
                 }
-                for (int64_t b = 0; b < a.np / kBiasRows; ++b)
+                // 16 NQ rows are a part, or (up to 64 rows) the only one with rows
+                for (int64_t b = blockIdx.y; b < (last ? a.np / kBiasRows : blockIdx.y + 1); ++b)
                     if (r == 0)
                         *reinterpret_cast<float4_t*>(a.bias_part + b * a.vt + (vfirst - a.v0) + 16 * i + 4 * g) =
-                            b == 0 ? sums[i] : float4_t{0.f, 0.f, 0.f, 0.f};
+                            b == blockIdx.y ? sums[i] : float4_t{0.f, 0.f, 0.f, 0.f};
             }
         }
     }
@@ -1459,8 +1462,12 @@ constexpr int64_t kJoinBlocks = 128;
 // 8,192 x 131,072 x 4,096 it makes 1%.
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 constexpr int64_t kFewClasses = 1024;  // up to here G has a second plane
-// Rows up to which head_few_kernel makes the logits: FEWNOTE
-constexpr int64_t kFewRows = 16, kFewPacked = 64;
+// Rows up to which head_few_kernel makes the logits.  32,000 x 2,048, against
+// the products on packed W: f32 1 row 79 against 485 us, 64 rows 121 against
+// 487 (two readings of W for 128 rows); 16-bit rows that are not 16-byte
+// aligned 57 against 116 at 1 row and 127 against 119 at 64; aligned ones,
+// which need no packing, 34 against 49 at 1 row, 38 against 52 at 16.
+constexpr int64_t kFewRows = 16, kFewPacked = 32, kFewF32 = 128;
 constexpr int64_t kPackBytes = (int64_t)256 << 20;  // a packed piece of W
 
 // A product's tile and the runs that its k is cut into: the least of
@@ -1519,7 +1526,7 @@ Shape shape_of(const grws_head* h, bool backward) {
     s.planes = s.split ? 3 : 1;
     s.gplanes = s.split ? 3 : s.V <= kFewClasses ? 2 : 1;
     s.pack_w = !weight_in_place(h);
-    s.few = s.n <= (s.pack_w ? kFewPacked : kFewRows);
+    s.few = s.n <= (s.split ? kFewF32 : s.pack_w ? kFewPacked : kFewRows);
     s.np = pad(s.n);
     s.dp = up(s.D, kK);
     s.vp = pad(s.V);
@@ -1699,7 +1706,7 @@ Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64
 template <typename T, int PLANES>
 int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
     const bool vec = rows_of_16(h->weight, h->ld_weight, h->dtype) && rows_of_16(h->hidden, h->ld_hidden, h->dtype);
-    const dim3 grid((unsigned)ceil_div(a.vt, 128));
+    const dim3 grid((unsigned)ceil_div(a.vt, 128), (unsigned)ceil_div(a.n, 64));
 #define GRWS_HEAD_FEW(NQ)                                                                                         \
     do {                                                                                                          \
         if (vec) hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, true>), grid, dim3(256), 0, stream, a);        \

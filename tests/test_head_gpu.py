@@ -230,6 +230,35 @@ def test_hits_match_argmax(cuda_device, dt):
     assert int(counts[0]) == _hits(z, labels, clear)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [1, 7, 16, 17, 32, 33, 64, 65, 100, 128])
+@pytest.mark.parametrize("width", [24, 131, 512])
+def test_few_rows(cuda_device, dt, n, width):
+    """Row counts around the small kernel's tiles, aligned widths and not,
+    with and without every row counting, labels and lists."""
+    print(f"case few {dt} {n}x{width}", flush=True)
+    classes = 1533
+    h, w, b, labels = _inputs(cuda_device, n, width, classes, dt, n + width, nodes=n + 3, bias=True)
+    rows = torch.randperm(n + 3, device=cuda_device)[:n]
+    labels[1::6] = -100
+    params = [x.requires_grad_(True) for x in (h, w, b)]
+    loss, counts = linear_cross_entropy(h, w, labels, bias=b, rows=rows, reduction="none")
+    factors = torch.rand(n, device=cuda_device) + 0.5
+    grads = torch.autograd.grad(loss, params, factors)
+    ref = _Ref(h.detach(), w.detach(), b.detach(), rows, *_onehot(labels, classes))
+    assert counts.tolist()[1:] == [ref.count, 0]
+    ref.check_loss(None, loss)
+    ref.check_grads(*grads, factors.double())
+    values, index = ops.top_logits(torch.randn(n, classes, device=cuda_device) * 3, 6)
+    index[1::6] = -1
+    loss, counts = linear_distill(h, w, index, values, bias=b, rows=rows, temperature=2.0)
+    grads = torch.autograd.grad(loss, params)
+    ref = _Ref(h.detach(), w.detach(), b.detach(), rows, *_teacher(index, values, classes, 2.0), 2.0)
+    assert counts.tolist() == [ref.count, 0]
+    ref.check_loss(loss)
+    ref.check_grads(*grads, 1.0 / ref.count)
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 def test_pieces(cuda_device, dt):
     """More rows than one piece of the gradient's scratch takes at all the
