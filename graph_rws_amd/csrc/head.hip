@@ -15,9 +15,10 @@
 // Forward: one product whose epilogue reduces each 16 TP classes of a row to
 // (max, sum of 2^(y - max)) in registers; a second kernel joins them.
 // Backward: pieces of the classes.  For each piece the product is made again
-// and its epilogue writes G = 2^(y - L) in 16 bits to a scratch matrix, a
-// small kernel subtracts the targets, and two products read G: dW's rows of
-// the piece (complete), and dH (added up over the pieces in fp32).
+// and its epilogue writes G = 2^(y - L) in 16 bits to a scratch matrix (less
+// one at the label; a small kernel subtracts a teacher's entries), and two
+// products read G: dW's rows of the piece (complete), and dH (added up over
+// the pieces in fp32).  Few rows have a kernel of their own for the logits.
 //
 // G is rounded to the operands' 16-bit type because the matrix cores take no
 // wider one; p - q is formed in fp32 and rounded once.  Its factor s_i T is
@@ -1794,7 +1795,8 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
         Opnd W;
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, s.np, c1,
+        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes),
+                    v0, s.V, s.n, s.np, c1,
                     h->bias, h->dtype, h->labels, f.part, target_logit, f.flags};
         if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
         else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
@@ -1896,7 +1898,8 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             else GRWS_TRY((launch_few<__hip_bfloat16, 2>(h, a, stream)));
         } else {
             GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-            GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes), v0, s.V, s.n, c1, h->bias,
+            GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes),
+                       v0, s.V, s.n, c1, h->bias,
                        h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane,
                        d_bias && h->k == 0 ? f.bias : nullptr, vt};
 #define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
@@ -1938,7 +1941,8 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
             const int32_t vec = reinterpret_cast<uintptr_t>(d_weight) % (4 * esz) == 0 && ld_dw % 4 == 0;
             const Opnd G{gp, s.ldg * 2, plane * 2, s.ldg, s.np};
-            WeightArgs w{gemm_of(s, s.weight, hidden_operand(s, f.hp, true), G, s.D, vc, s.np, s.gplanes), f.alpha, out, ld_dw,
+            WeightArgs w{gemm_of(s, s.weight, hidden_operand(s, f.hp, true), G, s.D, vc, s.np, s.gplanes),
+                         f.alpha, out, ld_dw,
                          vc, s.D, vec, f.dw, s.vp, s.dp};
             if (s.split) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_F16, GRWS_F16);

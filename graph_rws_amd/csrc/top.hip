@@ -225,8 +225,8 @@ __device__ __forceinline__ uint32_t first_bound(Pool<MAXK>& p, uint32_t most, in
 }
 
 template <typename T, bool FINAL, int MAXK>
-__global__ __launch_bounds__(kT, MAXK <= kSmallK ? 8 : 5) void top_rows_kernel(const T* __restrict__ logits, int64_t ld, int32_t classes,
-                                                      int32_t class_bits, int32_t k, int32_t stretch,
+__global__ __launch_bounds__(kT, MAXK <= kSmallK ? 8 : 5) void top_rows_kernel(
+    const T* __restrict__ logits, int64_t ld, int32_t classes, int32_t class_bits, int32_t k, int32_t stretch,
                                                       T* __restrict__ values, int32_t* __restrict__ index,
                                                       uint64_t* __restrict__ best) {
     constexpr int VB = sizeof(T) * 8, CAP = Sizes<MAXK>::CAP, OFFER = Sizes<MAXK>::OFFER;
