@@ -1149,6 +1149,98 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     }
 }
 
+// dH of few f32 rows: W is read once, as it lies, on the f32 MFMA; a wave owns
+// 64 columns of 16 NQ rows over a run of classes, 16 at a time: lane (g, r)
+// reads columns 4 r .. + 3 of classes 4 g .. + 3 (256 bytes a class), which are
+// the operands of four tiles with columns 4 r + c.  1 row x 32,000 x 2,048 with
+// gradients: 702 -> 468 us against dH from packed planes of W, 64 rows 791 ->
+// 669, 128 rows 895 -> 859.
+struct FewHiddenArgs {
+    const float* weight;  // first class of the piece
+    int64_t ldw, width, dp, n, np, vc;
+    const uint16_t* G;
+    int64_t ldg, plane;
+    float* part;  // [splits][np][dp]
+    int32_t splits, first;
+};
+
+template <int NQ, bool VEC>
+__global__ __launch_bounds__(256) void head_few_dhidden_kernel(FewHiddenArgs a) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const int64_t sp = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (sp >= a.splits) return;  // uniform over the wave
+    const int64_t d0 = (int64_t)blockIdx.x * 64, first = (int64_t)blockIdx.z * (16 * NQ);
+    const int64_t blocks = (a.vc + 15) / 16, kb = blocks * sp / a.splits, ke = blocks * (sp + 1) / a.splits;
+    const int64_t d = d0 + 4 * r;
+    const bool whole = VEC && d + 4 <= a.width;
+    float4_t acc[4][NQ];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) acc[c][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 2;  // blocks whose loads are in flight
+    auto multiply = [&](int64_t b, int some) {
+        float4_t w[U][4], x[U][NQ];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= some) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t v = (b + u) * 16 + 4 * g + k;
+                w[u][k] = float4_t{0.f, 0.f, 0.f, 0.f};
+                if (v < a.vc) {
+                    const float* p = a.weight + v * a.ldw + d;
+                    if (whole) {
+                        w[u][k] = *reinterpret_cast<const float4_t*>(p);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (d + c < a.width) w[u][k][c] = p[c];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                const uint16_t* q = a.G + (first + 16 * j + r) * a.ldg + (b + u) * 16 + 4 * g;
+                uint16_t h[3][4];
+#pragma unroll
+                for (int z = 0; z < 3; ++z) __builtin_memcpy(h[z], __builtin_assume_aligned(q + z * a.plane, 8), 8);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    x[u][j][k] = from_top16(h[0][k]) + (from_top16(h[1][k]) + from_top16(h[2][k]));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= some) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < NQ; ++j)
+                        acc[c][j] =
+                            __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][k][c], x[u][j][k], acc[c][j], 0, 0, 0);
+        }
+    };
+    int64_t b = kb;
+    for (; b + U <= ke; b += U) multiply(b, U);
+    for (; b < ke; ++b) multiply(b, 1);
+    // acc[c][j][e]: column 4 (4 g + e) + c, row 16 j + r
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        const int64_t row = first + 16 * j + r;
+        if (row >= a.n) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float4_t* o =
+                reinterpret_cast<float4_t*>(a.part + (sp * a.np + row) * a.dp + d0 + 16 * g + 4 * e);
+            const float4_t x{acc[0][j][e], acc[1][j][e], acc[2][j][e], acc[3][j][e]};
+            *o = a.first ? x : *o + x;
+        }
+    }
+}
+
 __device__ __forceinline__ void join(float& m, float& s, int& first, float om, float os, int ofirst) {
     if (om > m) {
         s = s * __builtin_amdgcn_exp2f(m - om) + os;
@@ -1561,6 +1653,13 @@ Shape shape_of(const grws_head* h, bool backward) {
             s.hidden = d;
         }
     }
+    if (backward && s.few && s.split) {
+        // dH by head_few_dhidden_kernel: 2,048 waves, of at least 8 blocks of 16 classes
+        int64_t sp = ceil_div(2048, s.dp / 64 * ceil_div(s.n, 64));
+        const int64_t most = s.vp / 128;
+        if (sp > most) sp = most;
+        s.hidden.splits = sp < 2 ? 2 : sp;  // two at least: the runs are added up apart
+    }
     s.strip_classes = s.few ? 32 : s.logits.tile / 2;
     s.strips = pad(s.V) / s.strip_classes;
     s.ldg = s.vp + 128;
@@ -1634,7 +1733,7 @@ void bwd_space(A& a, const Shape& s, BwdSpace* f) {
         else p = a.template take<T>((size_t)n);
     };
     take(f->hp, s.planes * s.np * s.dp);
-    if (s.pack_w) take(f->wp, s.planes * s.vp * s.dp);
+    if (s.pack_w && !(s.few && s.split)) take(f->wp, s.planes * s.vp * s.dp);
     take(f->G, s.gplanes * s.np * s.ldg);
     if (s.hidden.splits > 1 || s.vp < s.V) take(f->dh, s.hidden.splits * s.np * s.dp);
     if (s.weight.splits > 1) take(f->dw, s.weight.splits * s.vp * s.dp);
@@ -1958,7 +2057,23 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
                 GRWS_LAUNCH_CHECK();
             }
         }
-        if (d_hidden) {
+        if (d_hidden && s.few && s.split) {
+            const FewHiddenArgs d{static_cast<const float*>(h->weight) + v0 * h->ld_weight, h->ld_weight, s.D, s.dp, s.n,
+                                  s.np, vc, f.G, s.ldg, plane, f.dh, (int32_t)s.hidden.splits, v0 == 0};
+            const bool vec = rows_of_16(h->weight, h->ld_weight, h->dtype);
+            const dim3 grid((unsigned)(s.dp / 64), (unsigned)ceil_div(s.hidden.splits, 4),
+                            (unsigned)ceil_div(s.n, 64));
+#define GRWS_HEAD_FEW_DH(NQ)                                                                                     \
+    do {                                                                                                         \
+        if (vec) hipLaunchKernelGGL((head_few_dhidden_kernel<NQ, true>), grid, dim3(256), 0, stream, d);          \
+        else hipLaunchKernelGGL((head_few_dhidden_kernel<NQ, false>), grid, dim3(256), 0, stream, d);             \
+    } while (0)
+            if (s.n <= 16) GRWS_HEAD_FEW_DH(1);
+            else if (s.n <= 32) GRWS_HEAD_FEW_DH(2);
+            else GRWS_HEAD_FEW_DH(4);
+#undef GRWS_HEAD_FEW_DH
+            GRWS_LAUNCH_CHECK();
+        } else if (d_hidden) {
             GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, s.few, stream));
             const Opnd G{gp, s.ldg * 2, plane * 2, s.np, vt};
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
