@@ -1415,13 +1415,16 @@ __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict_
     if ((threadIdx.x & 63) == 0 && m) atomicMax(most, m);
 }
 
-__global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __restrict__ dloss, int64_t n,
+// 0 for a row that does not count, whatever dloss holds there: its G is zeros
+// times this
+__global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __restrict__ dloss,
+                                                             const float* __restrict__ lse, int64_t n,
                                                              const uint32_t* __restrict__ most,
                                                              float* __restrict__ scale) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const float m = __uint_as_float(*most);
-    scale[i] = m > 0.f ? dloss[i] / m : 0.f * m;
+    scale[i] = lse[i] == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : 0.f * m;
 }
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.
@@ -1962,7 +1965,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         const dim3 grid((unsigned)ceil_div(s.n, 256));
         hipLaunchKernelGGL(head_most_kernel, grid, dim3(256), 0, stream, dloss, lse, s.n, f.most);
         GRWS_LAUNCH_CHECK();
-        hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, s.n, f.most, f.scale);
+        hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, lse, s.n, f.most, f.scale);
         GRWS_LAUNCH_CHECK();
         row_scale = f.scale;
     }

@@ -1,0 +1,61 @@
+"""Edges of the fused classifier losses (csrc/head.hip): upstream gradients,
+exact comparisons, extreme logits, layouts.
+
+Where two calls have to agree they agree bit for bit; other tolerances are
+stated at the test."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from graph_rws_amd.core import ops
+from graph_rws_amd.layers import linear_cross_entropy, linear_distill
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _inputs(dev, n, width, classes, dt, seed, nodes=None):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    h = torch.randn(nodes or n, width, generator=g, device=dev).to(dt)
+    w = (torch.randn(classes, width, generator=g, device=dev) * 2 / math.sqrt(width)).to(dt)
+    b = torch.randn(classes, generator=g, device=dev).to(dt)
+    labels = torch.randint(0, classes, (n,), generator=g, device=dev)
+    lists = torch.stack([torch.randperm(classes, generator=g, device=dev)[:5] for _ in range(n)]).int()
+    teacher = torch.randn(n, 5, generator=g, device=dev)
+    return h, w, b, labels, lists, teacher
+
+
+def _row_grads(kind, h, w, b, target, factors):
+    """Row losses and the gradients of their sum weighted by factors."""
+    params = [x.detach().requires_grad_(True) for x in (h, w, b)]
+    if kind == "labels":
+        loss, _ = linear_cross_entropy(params[0], params[1], target, bias=params[2], reduction="none")
+    else:
+        loss, _ = linear_distill(params[0], params[1], *target, bias=params[2], temperature=2.0, reduction="none")
+    return [loss.detach(), *torch.autograd.grad(loss, params, factors)]
+
+
+# 9 rows: the kernels of few rows; 200: the products
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+@pytest.mark.parametrize("kind", ["labels", "lists"])
+def test_factors_of_rows_that_do_not_count(cuda_device, dt, n, kind):
+    """Whatever the upstream gradient holds at a row that does not count, the
+    gradients are those of a zero there."""
+    print(f"case dead factors {dt} {n} {kind}", flush=True)
+    h, w, b, labels, lists, teacher = _inputs(cuda_device, n, 40, 300, dt, 5)
+    labels[::4] = -100
+    lists[::4] = -1
+    target = labels if kind == "labels" else (lists, teacher)
+    factors = torch.randn(n, device=cuda_device)
+    factors[::4] = 0
+    want = _row_grads(kind, h, w, b, target, factors)
+    assert all(bool(torch.isfinite(x).all()) for x in want)
+    for bad in (math.nan, math.inf, -math.inf, 3e38):
+        factors[::4] = bad
+        for x, y in zip(want, _row_grads(kind, h, w, b, target, factors)):
+            assert torch.equal(x, y), bad
