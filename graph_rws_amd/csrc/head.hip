@@ -764,7 +764,7 @@ __device__ __forceinline__ int row_state(const Targets& t, int64_t i, int sub) {
 }
 
 // The factor of the gradient sums: dloss T / (counted gscale), or for a
-// gradient per row the largest |dloss| in place of dloss / counted, with
+// gradient per row the largest finite |dloss| in place of dloss / counted, with
 // the rows' shares of it in row_scale (so that G stays within 16 bits' range)
 struct Alpha {
     float* out;  // NULL: none
@@ -1403,10 +1403,12 @@ __global__ __launch_bounds__(64) void head_finish_kernel(const double* part_loss
 __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict__ dloss,
                                                         const float* __restrict__ lse, int64_t n,
                                                         uint32_t* __restrict__ most) {
-    // of non-negative floats the largest is the largest as an integer (a NaN
-    // above all): the order of the atomics does not matter
+    // of non-negative floats the largest is the largest as an integer: the
+    // order of the atomics does not matter.  Infinities and NaN are left out:
+    // they are their rows' own shares, not a factor of every row
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     uint32_t m = i < n && lse[i] != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
+    if (m >= 0x7f800000u) m = 0u;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
         const uint32_t o = __shfl_xor(m, d, kWave);
@@ -1416,7 +1418,7 @@ __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict_
 }
 
 // 0 for a row that does not count, whatever dloss holds there: its G is zeros
-// times this
+// times this.  (Without a factor other than 0, infinity and NaN: 0 or NaN.)
 __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __restrict__ dloss,
                                                              const float* __restrict__ lse, int64_t n,
                                                              const uint32_t* __restrict__ most,
@@ -1424,7 +1426,7 @@ __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __rest
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const float m = __uint_as_float(*most);
-    scale[i] = lse[i] == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : 0.f * m;
+    scale[i] = lse[i] == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : dloss[i] * 0.f;
 }
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.

@@ -59,3 +59,23 @@ def test_factors_of_rows_that_do_not_count(cuda_device, dt, n, kind):
         factors[::4] = bad
         for x, y in zip(want, _row_grads(kind, h, w, b, target, factors)):
             assert torch.equal(x, y), bad
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+@pytest.mark.parametrize("kind", ["labels", "lists"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_bad_factor_stays_in_its_row(cuda_device, dt, n, kind, bad):
+    """An upstream gradient that is not finite spoils its own row of the
+    hidden gradient and no other."""
+    print(f"case bad factor {dt} {n} {kind} {bad}", flush=True)
+    h, w, b, labels, lists, teacher = _inputs(cuda_device, n, 40, 300, dt, 6)
+    target = labels if kind == "labels" else (lists, teacher)
+    factors = torch.randn(n, device=cuda_device)
+    factors[3] = 0
+    want = _row_grads(kind, h, w, b, target, factors)[1]
+    factors[3] = bad
+    got = _row_grads(kind, h, w, b, target, factors)[1]
+    assert not bool(torch.isfinite(got[3]).any())
+    got[3] = want[3]
+    assert torch.equal(got, want)
