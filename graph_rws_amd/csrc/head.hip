@@ -680,6 +680,7 @@ struct HiddenArgs {
     void* out;
     int64_t ldo, n, width, hidden_rows;
     const int64_t* rows;
+    const float* lse;  // +inf: the row gets zeros, whatever alpha and W hold
 };
 
 template <int DT, int OT, int BP, int BQ, int WP, int WQ>
@@ -701,9 +702,11 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
     for (int j = 0; j < TQ; ++j) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
         int64_t to = -1;
+        bool counts = false;
         if (a.last && row < a.n) {
             to = a.rows ? a.rows[row] : row;
             if (to >= a.hidden_rows) to = -1;
+            counts = a.lse[row] != INFINITY;
         }
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
@@ -712,7 +715,9 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
             float4_t* o = reinterpret_cast<float4_t*>(out + row * a.dp + d);
             const float4_t v = a.first ? acc[i][j] : *o + acc[i][j];
             if (!a.last) *o = v;
-            else if (to >= 0 && d < a.width) store4<OT>(a.out, to * a.ldo + d, v * alpha, a.width - d, a.vec);
+            else if (to >= 0 && d < a.width)
+                store4<OT>(a.out, to * a.ldo + d, counts ? v * alpha : float4_t{0.f, 0.f, 0.f, 0.f}, a.width - d,
+                           a.vec);
         }
     }
 }
@@ -1537,12 +1542,15 @@ template <typename T>
 __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __restrict__ part, int64_t splits,
                                                               int64_t np, int64_t dp, int64_t width,
                                                               const int64_t* __restrict__ rows, int64_t hidden_rows,
+                                                              const float* __restrict__ lse,
                                                               const float* __restrict__ alpha, T* __restrict__ out,
                                                               int64_t ldo) {
     const int64_t i = blockIdx.x;
     const int64_t row = rows ? rows[i] : i;
     if (row < 0 || row >= hidden_rows) return;
-    sum_splits(part + i * dp, splits, np * dp, width, *alpha, out + row * ldo);
+    // a row that does not count gets zeros: the sum of no runs
+    const bool counts = lse[i] != INFINITY;
+    sum_splits(part + i * dp, counts ? splits : 0, np * dp, width, counts ? *alpha : 0.f, out + row * ldo);
 }
 
 // ---------------------------------------------------------------------------
@@ -2084,7 +2092,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
             HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc, s.gplanes), f.dh, s.np, s.dp, v0 == 0,
                          s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
-                         h->hidden_rows, h->rows};
+                         h->hidden_rows, h->rows, lse};
             if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
             else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
@@ -2094,7 +2102,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
-                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, f.alpha, static_cast<T*>(d_hidden), ld_dh)
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, lse, f.alpha, static_cast<T*>(d_hidden), ld_dh)
         if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
         else GRWS_HEAD_DH(__hip_bfloat16);

@@ -79,3 +79,18 @@ def test_a_bad_factor_stays_in_its_row(cuda_device, dt, n, kind, bad):
     assert not bool(torch.isfinite(got[3]).any())
     got[3] = want[3]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200, 5000])
+@pytest.mark.parametrize("per_row", [False, True])
+def test_rows_that_do_not_count_get_zero(cuda_device, dt, n, per_row):
+    """An infinite upstream gradient (an overflowed loss scale) leaves zeros
+    in the hidden rows without a target, as F.cross_entropy does."""
+    h, w, b, labels, _, _ = _inputs(cuda_device, n, 40, 300, dt, 7)
+    labels[::4] = -100
+    h.requires_grad_(True)
+    loss, _ = linear_cross_entropy(h, w, labels, bias=b, reduction="none" if per_row else "mean")
+    up = torch.full_like(loss, math.inf)
+    dh = torch.autograd.grad(loss, [h], up)[0]
+    assert not bool(dh[::4].any()), dh[::4]
