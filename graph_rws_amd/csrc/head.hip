@@ -356,6 +356,18 @@ __device__ __forceinline__ void begin_logits(float4_t (&acc)[TP][TQ], int64_t vf
     }
 }
 
+// A strip's exponentials are taken against ref, the rounded m c1: this makes
+// their sum one against m c1 itself.  (The maxima stay logits: two of them can
+// be one float when multiplied by c1, and a hit is a matter of which is larger.)
+__device__ __forceinline__ float past_rounding(float m, float c1, float ref) {
+    return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-fmaf(m, c1, -ref));
+}
+// A maximum (a mask of the type's lowest value) whose m c1 is past f32: what
+// is not equal to it is nothing beside it.
+__device__ __forceinline__ bool too_far(float m, float ref) {
+    return fabsf(ref) == INFINITY && fabsf(m) != INFINITY;
+}
+
 struct StatsArgs {
     Gemm g;
     int64_t v0, classes;  // first class of the piece, all classes
@@ -364,8 +376,8 @@ struct StatsArgs {
     const void* bias;
     int32_t bias_dt;
     const int64_t* labels;  // NULL: none to look for
-    float2* part;           // [strips][np]: max, sum of 2^(y - max)
-    float* ylabel;          // [n]
+    float2* part;           // [strips][np]: largest logit m, sum of 2^((z - m) c1)
+    float* ylabel;          // [n]: the label's logit
     int32_t* earlier;       // [n]: an earlier class of the label's strip has the label's logit
 };
 
@@ -399,8 +411,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
             for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
         m = fmaxf(m, __shfl_xor(m, 16, kWave));
         m = fmaxf(m, __shfl_xor(m, 32, kWave));
-        m *= a.c1;
-        const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf: a sum of zeros
+        const float ref = m == -INFINITY ? 0.f : m * a.c1;  // nothing but -inf: a sum of zeros
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < TP; ++i)
@@ -408,6 +419,17 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
             for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -ref));
         s += __shfl_xor(s, 16, kWave);
         s += __shfl_xor(s, 32, kWave);
+        s *= past_rounding(m, a.c1, ref);
+        if (__any(too_far(m, ref))) {
+            float same = 0.f;
+#pragma unroll
+            for (int i = 0; i < TP; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) same += acc[i][j][e] == m ? 1.f : 0.f;
+            same += __shfl_xor(same, 16, kWave);
+            same += __shfl_xor(same, 32, kWave);
+            s = too_far(m, ref) ? same : s;
+        }
         if (lane < 16) a.part[strip * a.np + row] = make_float2(m, s);
         if (a.labels) {
             const int64_t lab = row < a.n ? a.labels[row] - vfirst : -1;
@@ -429,7 +451,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
                 tie |= __shfl_xor(tie, 16, kWave);
                 tie |= __shfl_xor(tie, 32, kWave);
                 if (here && lane < 16) {
-                    a.ylabel[row] = y * a.c1;
+                    a.ylabel[row] = y;
                     a.earlier[row] = tie;
                 }
             }
@@ -871,7 +893,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* __restrict__ hidden, int64_t ldh,
                                                            const T* __restrict__ w, int64_t ldw, const T* bias,
                                                            int64_t n, int64_t width, int32_t vec, float inv_t,
-                                                           float c1, float* __restrict__ prob,
+                                                           float* __restrict__ prob,
                                                            float* __restrict__ y, int32_t* __restrict__ state) {
     const int lane = threadIdx.x & 63;
     const int groups = (t.k + 3) / 4;
@@ -903,7 +925,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
 #pragma unroll
         for (int x = 8; x > 0; x >>= 1) d += __shfl_xor(d, x, kWave);
         if ((lane & 15) == 0 && k < t.k)
-            y[i * t.k + k] = idx >= 0 ? (d + (bias ? to_float(bias[idx]) : 0.f)) * c1 : 0.f;
+            y[i * t.k + k] = idx >= 0 ? d + (bias ? to_float(bias[idx]) : 0.f) : 0.f;
     }
     if (k0 != 0) return;
     if (lane == 0) state[i] = st;
@@ -1080,16 +1102,18 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                     y = 16 * i + 4 * g + e == l ? acc[i][j][e] : y;
                 }
             m = fmaxf(m, __shfl_xor(m, 16, kWave));
-            m = fmaxf(m, __shfl_xor(m, 32, kWave)) * a.c1;
+            m = fmaxf(m, __shfl_xor(m, 32, kWave));
             y = __shfl(y, (((l >> 2) & 3) << 4) | r, kWave);
-            const float ref = m == -INFINITY ? 0.f : m;
+            const float ref = m == -INFINITY ? 0.f : m * a.c1;
+            const bool far = too_far(m, ref);
             float s = 0.f;
             int tie = 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -ref));
+                    const float z = acc[i][j][e];
+                    s += far ? (z == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(fmaf(z, a.c1, -ref));
                     tie |= acc[i][j][e] == y && 16 * i + 4 * g + e < l;
                 }
             s += __shfl_xor(s, 16, kWave);
@@ -1097,9 +1121,9 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
             tie |= __shfl_xor(tie, 16, kWave);
             tie |= __shfl_xor(tie, 32, kWave);
             if (g == 0) {
-                a.part[vfirst / 32 * a.np + row] = make_float2(m, s);
+                a.part[vfirst / 32 * a.np + row] = make_float2(m, far ? s : s * past_rounding(m, a.c1, ref));
                 if (here) {
-                    a.ylabel[row] = y * a.c1;
+                    a.ylabel[row] = y;
                     a.earlier[row] = tie;
                 }
             }
@@ -1246,13 +1270,13 @@ __global__ __launch_bounds__(256) void head_few_dhidden_kernel(FewHiddenArgs a) 
     }
 }
 
-__device__ __forceinline__ void join(float& m, float& s, int& first, float om, float os, int ofirst) {
+__device__ __forceinline__ void join(float c1, float& m, float& s, int& first, float om, float os, int ofirst) {
     if (om > m) {
-        s = s * __builtin_amdgcn_exp2f(m - om) + os;
+        s = s * __builtin_amdgcn_exp2f((m - om) * c1) + os;
         m = om;
         first = ofirst;
     } else {
-        s += om == -INFINITY ? os : os * __builtin_amdgcn_exp2f(om - m);
+        s += om == -INFINITY ? os : os * __builtin_amdgcn_exp2f((om - m) * c1);
         if (om == m && ofirst < first) first = ofirst;
     }
 }
@@ -1290,7 +1314,7 @@ __device__ __forceinline__ void finish_loss(const double* part_loss, const int32
 template <int R>
 __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2* __restrict__ part, int64_t strips,
                                                         int32_t strip_classes, int64_t n, int64_t np,
-                                                        float temperature, const float* __restrict__ y,
+                                                        float temperature, float c1, const float* __restrict__ y,
                                                         const float* __restrict__ prob,
                                                         const int32_t* __restrict__ flags, float* __restrict__ lse,
                                                         float* __restrict__ row_loss, double* part_loss,
@@ -1313,10 +1337,10 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             if (lane & d) {
                 float m2 = om, s2 = os;
                 int f2 = of;
-                join(m2, s2, f2, m, s, first);
+                join(c1, m2, s2, f2, m, s, first);
                 m = m2, s = s2, first = f2;
             } else {
-                join(m, s, first, om, os, of);
+                join(c1, m, s, first, om, os, of);
             }
         }
     };
@@ -1324,7 +1348,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
 #pragma unroll 4
         for (int64_t k = wave * G + g; k < strips; k += 8 * G) {
             const float2 v = part[k * np + i];
-            join(m, s, first, v.x, v.y, (int)k);
+            join(c1, m, s, first, v.x, v.y, (int)k);
         }
     }
     join_lanes();
@@ -1336,18 +1360,18 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
     __syncthreads();
     if (wave != 0) return;
     m = -INFINITY, s = 0.f, first = 0x7fffffff;
-    for (int w = g; w < 8; w += G) join(m, s, first, sm[w][r], ss[w][r], sa[w][r]);
+    for (int w = g; w < 8; w += G) join(c1, m, s, first, sm[w][r], ss[w][r], sa[w][r]);
     join_lanes();
     int st = 0;
     if (i < n) st = t.labels ? row_state<1>(t, i, 0) : flags[i];
-    const float l = m + log2f(s);
+    const float l = fmaf(m, c1, log2f(s));
     float a = 0.f;
     if (!t.labels && st == 1) {
         // sum of q ln q + q ln2 (L - y); an entry of probability zero says
         // nothing of its class (whose logit may be -inf)
         for (int k = g; k < t.k; k += G) {
             const float q = prob[i * t.k + k];
-            if (!(q <= 0.f)) a += q * (logf(q) + (l - y[i * t.k + k]) * kLn2);
+            if (!(q <= 0.f)) a += q * (logf(q) + (l - y[i * t.k + k] * c1) * kLn2);
         }
     }
 #pragma unroll
@@ -1360,7 +1384,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             valid = 1;
             if (t.labels) {
                 const float yl = y[i];
-                v = (l - yl) * kLn2;
+                v = (l - yl * c1) * kLn2;
                 hit = yl == m && !flags[i] && first == (int)(t.labels[i] / strip_classes);
             } else {
                 v = a * temperature * temperature;
@@ -1441,7 +1465,7 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const flo
                                                             const float* __restrict__ y,
                                                             const float* __restrict__ coef,
                                                             const float* __restrict__ row_scale, float gscale,
-                                                            int64_t n, int64_t v0, int64_t vc, uint16_t* G,
+                                                            float c1, int64_t n, int64_t v0, int64_t vc, uint16_t* G,
                                                             int64_t ldg, int64_t plane) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (at >= n * t.k) return;
@@ -1452,7 +1476,7 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const flo
     if (q < 0.f || l == INFINITY) return;
     const float s = row_scale ? row_scale[i] * gscale : gscale;
     uint16_t h[PLANES];
-    planes_of<DT, PLANES>((exp2f(y[at] - l) - q) * s, h);
+    planes_of<DT, PLANES>((exp2f(fmaf(y[at], c1, -l)) - q) * s, h);
 #pragma unroll
     for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
 }
@@ -1886,7 +1910,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
 #define GRWS_HEAD_TARGETS(T)                                                                                         \
     hipLaunchKernelGGL(head_targets_kernel<T>, grid, dim3(256), 0, stream, t, static_cast<const T*>(h->hidden),      \
                        h->ld_hidden, static_cast<const T*>(h->weight), h->ld_weight, static_cast<const T*>(h->bias), \
-                       s.n, s.D, vec, 1.f / h->temperature, c1, target_prob, target_logit, f.flags)
+                       s.n, s.D, vec, 1.f / h->temperature, target_prob, target_logit, f.flags)
         if (h->dtype == GRWS_F32) GRWS_HEAD_TARGETS(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_TARGETS(_Float16);
         else GRWS_HEAD_TARGETS(__hip_bfloat16);
@@ -1916,7 +1940,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
     const int64_t rows = s.n <= 8 ? 1 : s.n <= 512 ? 4 : 16, blocks = ceil_div(s.n, rows);
 #define GRWS_HEAD_JOIN(R)                                                                                            \
     hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part,                 \
-                       ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature,          \
+                       ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature, c1,      \
                        target_logit, target_prob, f.flags, lse, row_loss, f.pl, f.pc,                                \
                        blocks <= kJoinBlocks ? f.done : nullptr, loss, counts)
     if (rows == 1) GRWS_HEAD_JOIN(1);
@@ -2022,7 +2046,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             const dim3 grid((unsigned)ceil_div(s.n * h->k, 256));
 #define GRWS_HEAD_SUB(DT, PL)                                                                                 \
     hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, lse, target_logit, coef, \
-                       row_scale, gscale, s.n, v0, vc, f.G, s.ldg, plane)
+                       row_scale, gscale, c1, s.n, v0, vc, f.G, s.ldg, plane)
             GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
 #undef GRWS_HEAD_SUB
             GRWS_LAUNCH_CHECK();

@@ -94,3 +94,47 @@ def test_rows_that_do_not_count_get_zero(cuda_device, dt, n, per_row):
     up = torch.full_like(loss, math.inf)
     dh = torch.autograd.grad(loss, [h], up)[0]
     assert not bool(dh[::4].any()), dh[::4]
+
+
+# logits 1.5 + j 2^-23 of these j and j + 1 are one float when both are
+# multiplied by log2 e and rounded
+def _merged():
+    x = (1.5 + np.arange(200) * 2.0 ** -23).astype(np.float32)
+    y = x * np.float32(1.4426950408889634)
+    j = int(np.nonzero(y[1:] == y[:-1])[0][0])
+    assert x[j] != x[j + 1]
+    return j
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+@pytest.mark.parametrize("other", [1, 31, 40, 127, 200, 600])
+def test_hits_of_neighbouring_floats(cuda_device, dt, n, other):
+    """A logit one ulp above the label's is larger, wherever it lies; the
+    logits 1.5 + j 2^-23 are exact in every operand type."""
+    j = _merged()
+    h = torch.tensor([[1.0, 2.0 ** -11]], device=cuda_device).expand(n, 2).contiguous().to(dt)
+    w = torch.zeros(700, 2, device=cuda_device)
+    w[0, 0] = w[other, 0] = 1.5
+    w[0, 1], w[other, 1] = j * 2.0 ** -12, (j + 1) * 2.0 ** -12
+    assert torch.equal(w, w.to(dt).float())
+    labels = torch.zeros(n, dtype=torch.int64, device=cuda_device)
+    labels[1::3] = other
+    labels[2::3] = 5
+    _, counts = linear_cross_entropy(h, w.to(dt), labels)
+    assert counts.tolist() == [len(range(1, n, 3)), n, 0]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+def test_a_strip_of_lowest_logits(cuda_device, dt, n):
+    """Classes masked with the type's lowest value, a whole run of them, are
+    nothing beside the others."""
+    h, w, b, labels, _, _ = _inputs(cuda_device, n, 40, 600, dt, 3)
+    b[130:520] = torch.finfo(dt).min
+    labels = labels % 100
+    loss, counts = linear_cross_entropy(h, w, labels, bias=b, reduction="none")
+    z = h.double() @ w.double().t() + b.double()
+    ref = torch.nn.functional.cross_entropy(z, labels, reduction="none")
+    assert float((loss - ref).abs().max()) <= 1e-4
+    assert int(counts[0]) == int((z.argmax(1) == labels).sum())
