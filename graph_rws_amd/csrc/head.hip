@@ -356,16 +356,17 @@ __device__ __forceinline__ void begin_logits(float4_t (&acc)[TP][TQ], int64_t vf
     }
 }
 
-// A strip's exponentials are taken against ref, the rounded m c1: this makes
-// their sum one against m c1 itself.  (The maxima stay logits: two of them can
-// be one float when multiplied by c1, and a hit is a matter of which is larger.)
-__device__ __forceinline__ float past_rounding(float m, float c1, float ref) {
-    return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-fmaf(m, c1, -ref));
-}
-// A maximum (a mask of the type's lowest value) whose m c1 is past f32: what
-// is not equal to it is nothing beside it.
+// The maxima stay logits: two of them can be one float when multiplied by c1,
+// and a hit is a matter of which is larger.  The exponentials of a strip are
+// taken against the rounded m c1; one that overflows (m a mask of the type's
+// lowest value) leaves nothing of the logits that are not equal to m.
 __device__ __forceinline__ bool too_far(float m, float ref) {
     return fabsf(ref) == INFINITY && fabsf(m) != INFINITY;
+}
+// what makes a strip's sum one against m c1 itself
+__device__ __forceinline__ float past_rounding(float m, float c1) {
+    const float ref = m * c1;
+    return fabsf(ref) == INFINITY ? 1.f : __builtin_amdgcn_exp2f(-fmaf(m, c1, -ref));
 }
 
 struct StatsArgs {
@@ -376,7 +377,7 @@ struct StatsArgs {
     const void* bias;
     int32_t bias_dt;
     const int64_t* labels;  // NULL: none to look for
-    float2* part;           // [strips][np]: largest logit m, sum of 2^((z - m) c1)
+    float2* part;           // [strips][np]: largest logit m, sum of 2^(z c1 - the rounded m c1)
     float* ylabel;          // [n]: the label's logit
     int32_t* earlier;       // [n]: an earlier class of the label's strip has the label's logit
 };
@@ -419,7 +420,6 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
             for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -ref));
         s += __shfl_xor(s, 16, kWave);
         s += __shfl_xor(s, 32, kWave);
-        s *= past_rounding(m, a.c1, ref);
         if (__any(too_far(m, ref))) {
             float same = 0.f;
 #pragma unroll
@@ -1121,7 +1121,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
             tie |= __shfl_xor(tie, 16, kWave);
             tie |= __shfl_xor(tie, 32, kWave);
             if (g == 0) {
-                a.part[vfirst / 32 * a.np + row] = make_float2(m, far ? s : s * past_rounding(m, a.c1, ref));
+                a.part[vfirst / 32 * a.np + row] = make_float2(m, s);
                 if (here) {
                     a.ylabel[row] = y;
                     a.earlier[row] = tie;
@@ -1348,7 +1348,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
 #pragma unroll 4
         for (int64_t k = wave * G + g; k < strips; k += 8 * G) {
             const float2 v = part[k * np + i];
-            join(c1, m, s, first, v.x, v.y, (int)k);
+            join(c1, m, s, first, v.x, v.y * past_rounding(v.x, c1), (int)k);
         }
     }
     join_lanes();
