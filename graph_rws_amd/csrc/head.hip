@@ -1364,14 +1364,17 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
     join_lanes();
     int st = 0;
     if (i < n) st = t.labels ? row_state<1>(t, i, 0) : flags[i];
-    const float l = fmaf(m, c1, log2f(s));
+    // The saved log-sum is one number; the losses take the largest logit and
+    // the logarithm apart, whose rounding is then that of the loss and not of
+    // the logits (a confident row's loss is far below them).
+    const float l = fmaf(m, c1, log2f(s)), lns = log2f(s) * kLn2;
     float a = 0.f;
     if (!t.labels && st == 1) {
-        // sum of q ln q + q ln2 (L - y); an entry of probability zero says
-        // nothing of its class (whose logit may be -inf)
+        // sum of q (ln q + (m - z) / T + ln s); an entry of probability zero
+        // says nothing of its class (whose logit may be -inf)
         for (int k = g; k < t.k; k += G) {
             const float q = prob[i * t.k + k];
-            if (!(q <= 0.f)) a += q * (logf(q) + (l - y[i * t.k + k] * c1) * kLn2);
+            if (!(q <= 0.f)) a += q * (logf(q) + ((m - y[i * t.k + k]) / temperature + lns));
         }
     }
 #pragma unroll
@@ -1384,7 +1387,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             valid = 1;
             if (t.labels) {
                 const float yl = y[i];
-                v = (l - yl * c1) * kLn2;
+                v = m - yl + lns;
                 hit = yl == m && !flags[i] && first == (int)(t.labels[i] / strip_classes);
             } else {
                 v = a * temperature * temperature;

@@ -138,3 +138,24 @@ def test_a_strip_of_lowest_logits(cuda_device, dt, n):
     ref = torch.nn.functional.cross_entropy(z, labels, reduction="none")
     assert float((loss - ref).abs().max()) <= 1e-4
     assert int(counts[0]) == int((z.argmax(1) == labels).sum())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+def test_loss_of_confident_rows(cuda_device, dt, n):
+    """The loss of a row whose label stands 8 above the rest is
+    log(1 + (V - 1) e^-8) to 4e-6 of itself (exp2 and log2 at 2^-21 and their
+    sums), whatever the size of the logits; those are exact."""
+    classes = 400
+    w = torch.zeros(classes, 2, device=cuda_device)
+    w[:, 0], w[:, 1] = 1.0, 0.0
+    w[7, 1] = 8.0
+    for base in (0.0, 30.0, -100.0, 200.0):
+        h = torch.tensor([[base, 1.0]], device=cuda_device).expand(n, 2).contiguous()
+        labels = torch.full((n,), 7, dtype=torch.int64, device=cuda_device)
+        want = math.log1p((classes - 1) * math.exp(-8.0))
+        loss, _ = linear_cross_entropy(h.to(dt), w.to(dt), labels)
+        assert abs(float(loss) - want) <= 4e-6 * want, (base, float(loss), want)
+        index = torch.tensor([[7]], dtype=torch.int32, device=cuda_device).expand(n, 1)
+        kd, _ = linear_distill(h.to(dt), w.to(dt), index, torch.zeros(n, 1, device=cuda_device))
+        assert abs(float(kd) - want) <= 4e-6 * want, (base, float(kd), want)
