@@ -460,13 +460,26 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
     }
 }
 
+// What the forward leaves of a row for the gradients: p = 2^(z c1 - the
+// rounded m c1) * factor.  (Of one log-sum, m c1 + log2 s rounded, nothing
+// would be left of s beside a large m.)
+struct RowStats {
+    const float* top;     // [n]: the largest logit m; +inf: the row does not count
+    const float* factor;  // [n]: one over the sum of the exponentials
+};
+
+// 2^(z c1 - ref), ref the rounded m c1
+__device__ __forceinline__ float above(float z, float c1, float m, float ref, bool far) {
+    return far ? (z == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(fmaf(z, c1, -ref));
+}
+
 struct GradArgs {
     Gemm g;
     int64_t v0, classes, n;
     float c1;
     const void* bias;
     int32_t bias_dt;
-    const float* lse;        // [n], +inf for a row that does not count
+    RowStats stats;
     const int64_t* labels;   // NULL: the targets are subtracted by head_subtract_kernel
     const float* row_scale;  // [n] or NULL
     float gscale;
@@ -543,28 +556,35 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
-        // of a row that does not count, whose lse is +inf, all are 2^-inf
-        // (its hidden row is zeros, so a logit is its bias)
-        const float l = row < a.n ? a.lse[row] : INFINITY;
+        // of a row that does not count, whose largest logit is given as +inf,
+        // all are 2^-inf (its hidden row is zeros, so a logit is its bias)
+        const float m = row < a.n ? a.stats.top[row] : INFINITY, ref = m * a.c1;
         const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
+        const float f = m != INFINITY ? a.stats.factor[row] * s : 0.f;
+        if (__any(too_far(m, ref))) {
 #pragma unroll
-        for (int i = 0; i < TP; ++i)
+            for (int i = 0; i < TP; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -l));
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = above(acc[i][j][e], a.c1, m, ref, too_far(m, ref));
+        } else {
+#pragma unroll
+            for (int i = 0; i < TP; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = above(acc[i][j][e], a.c1, m, ref, false);
+        }
+#pragma unroll
+        for (int i = 0; i < TP; ++i) acc[i][j] *= f;
         if (a.labels) {
-            const int64_t lab = l != INFINITY ? a.labels[row] - a.v0 - pfirst : -1;
+            const int64_t lab = m != INFINITY ? a.labels[row] - a.v0 - pfirst : -1;
             const bool here = lab >= 0 && lab < TP * 16;
             if (__any(here)) {
                 const int at = here ? (int)lab : -1;
 #pragma unroll
                 for (int i = 0; i < TP; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= at == C::p_of(i, lane) + e ? 1.f : 0.f;
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= at == C::p_of(i, lane) + e ? s : 0.f;
             }
         }
-#pragma unroll
-        for (int i = 0; i < TP; ++i) acc[i][j] *= s;
 #pragma unroll
         for (int i = 0; i < TP; i += 2) {  // 8 consecutive classes of accumulators i and i + 1
             const int64_t at = row * a.ldg + pfirst + C::p_of(i, lane);
@@ -702,7 +722,7 @@ struct HiddenArgs {
     void* out;
     int64_t ldo, n, width, hidden_rows;
     const int64_t* rows;
-    const float* lse;  // +inf: the row gets zeros, whatever alpha and W hold
+    const float* top;  // +inf: the row gets zeros, whatever alpha and W hold
 };
 
 template <int DT, int OT, int BP, int BQ, int WP, int WQ>
@@ -728,7 +748,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
         if (a.last && row < a.n) {
             to = a.rows ? a.rows[row] : row;
             if (to >= a.hidden_rows) to = -1;
-            counts = a.lse[row] != INFINITY;
+            counts = a.top[row] != INFINITY;
         }
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
@@ -986,7 +1006,8 @@ struct FewArgs {
     int32_t* earlier;
     int32_t* done;
     // backward
-    const float *lse, *row_scale;
+    RowStats stats;
+    const float* row_scale;
     float gscale;
     uint16_t* G;
     int64_t ldg, plane;
@@ -1014,7 +1035,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
         const int64_t row = first + 16 * j + r;
-        if constexpr (GRAD) live[j] = row < a.n && a.lse[row] != INFINITY;
+        if constexpr (GRAD) live[j] = row < a.n && a.stats.top[row] != INFINITY;
         else live[j] = row < a.n && (a.t.labels ? row_state<1>(a.t, row, 0) : a.states[row]) == 1;
         h[j] = static_cast<const T*>(a.hidden) + (live[j] ? (a.t.rows ? a.t.rows[row] : row) * a.ldh : 0);
     }
@@ -1128,15 +1149,16 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                 }
             }
         } else {
-            const float lse = live[j] ? a.lse[row] : INFINITY;
+            const float m = live[j] ? a.stats.top[row] : INFINITY, ref = m * a.c1;
             const float sc = a.row_scale && live[j] ? a.row_scale[row] * a.gscale : a.gscale;
+            const float f = live[j] ? a.stats.factor[row] * sc : 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 uint16_t x[4][PLANES > 0 ? PLANES : 1];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -lse));
-                    p = (16 * i + 4 * g + e == l ? p - 1.f : p) * sc;
+                    float p = above(acc[i][j][e], a.c1, m, ref, too_far(m, ref)) * f;
+                    p = 16 * i + 4 * g + e == l ? p - sc : p;
                     sums[i][e] += p;
                     planes_of<DT, PLANES>(p, x[e]);
                 }
@@ -1316,8 +1338,8 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
                                                         int32_t strip_classes, int64_t n, int64_t np,
                                                         float temperature, float c1, const float* __restrict__ y,
                                                         const float* __restrict__ prob,
-                                                        const int32_t* __restrict__ flags, float* __restrict__ lse,
-                                                        float* __restrict__ row_loss, double* part_loss,
+                                                        const int32_t* __restrict__ flags, float* __restrict__ top,
+                                                        float* __restrict__ factor, float* __restrict__ row_loss, double* part_loss,
                                                         int32_t* part_cnt, int32_t* done,
                                                         float* __restrict__ loss_out, int64_t* __restrict__ counts) {
     __shared__ float sm[8][R], ss[8][R];
@@ -1364,10 +1386,9 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
     join_lanes();
     int st = 0;
     if (i < n) st = t.labels ? row_state<1>(t, i, 0) : flags[i];
-    // The saved log-sum is one number; the losses take the largest logit and
-    // the logarithm apart, whose rounding is then that of the loss and not of
-    // the logits (a confident row's loss is far below them).
-    const float l = fmaf(m, c1, log2f(s)), lns = log2f(s) * kLn2;
+    // the largest logit and the logarithm are not added before the target's
+    // logit is taken off: a confident row's loss is far below its logits
+    const float lns = log2f(s) * kLn2;
     float a = 0.f;
     if (!t.labels && st == 1) {
         // sum of q (ln q + (m - z) / T + ln s); an entry of probability zero
@@ -1397,7 +1418,9 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             bad = 1;
             v = __int_as_float(0x7fc00000);
         }
-        lse[i] = st == 1 ? l : INFINITY;
+        // a live row with a logit of +inf has nothing but NaN
+        top[i] = st != 1 ? INFINITY : m == INFINITY ? __int_as_float(0x7fc00000) : m;
+        factor[i] = past_rounding(m, c1) / s;
         if (row_loss) row_loss[i] = v;
     }
 #pragma unroll
@@ -1433,13 +1456,13 @@ __global__ __launch_bounds__(64) void head_finish_kernel(const double* part_loss
 }
 
 __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict__ dloss,
-                                                        const float* __restrict__ lse, int64_t n,
+                                                        const float* __restrict__ top, int64_t n,
                                                         uint32_t* __restrict__ most) {
     // of non-negative floats the largest is the largest as an integer: the
     // order of the atomics does not matter.  Infinities and NaN are left out:
     // they are their rows' own shares, not a factor of every row
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    uint32_t m = i < n && lse[i] != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
+    uint32_t m = i < n && top[i] != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
     if (m >= 0x7f800000u) m = 0u;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -1452,19 +1475,19 @@ __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict_
 // 0 for a row that does not count, whatever dloss holds there: its G is zeros
 // times this.  (Without a factor other than 0, infinity and NaN: 0 or NaN.)
 __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __restrict__ dloss,
-                                                             const float* __restrict__ lse, int64_t n,
+                                                             const float* __restrict__ top, int64_t n,
                                                              const uint32_t* __restrict__ most,
                                                              float* __restrict__ scale) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const float m = __uint_as_float(*most);
-    scale[i] = lse[i] == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : dloss[i] * 0.f;
+    scale[i] = top[i] == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : dloss[i] * 0.f;
 }
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.
 // (A label's place is known to the product's epilogue: one for a row.)
 template <int DT, int PLANES>
-__global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const float* __restrict__ lse,
+__global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats stats,
                                                             const float* __restrict__ y,
                                                             const float* __restrict__ coef,
                                                             const float* __restrict__ row_scale, float gscale,
@@ -1475,11 +1498,11 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, const flo
     const int64_t i = at / t.k;
     const int64_t v = teacher_at(t, i, (int)(at - i * t.k));
     if (v < v0 || v >= v0 + vc) return;
-    const float q = coef[at], l = lse[i];
-    if (q < 0.f || l == INFINITY) return;
+    const float q = coef[at], m = stats.top[i], ref = m * c1;
+    if (q < 0.f || m == INFINITY) return;
     const float s = row_scale ? row_scale[i] * gscale : gscale;
     uint16_t h[PLANES];
-    planes_of<DT, PLANES>((exp2f(fmaf(y[at], c1, -l)) - q) * s, h);
+    planes_of<DT, PLANES>((above(y[at], c1, m, ref, too_far(m, ref)) * stats.factor[i] - q) * s, h);
 #pragma unroll
     for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
 }
@@ -1569,14 +1592,14 @@ template <typename T>
 __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __restrict__ part, int64_t splits,
                                                               int64_t np, int64_t dp, int64_t width,
                                                               const int64_t* __restrict__ rows, int64_t hidden_rows,
-                                                              const float* __restrict__ lse,
+                                                              const float* __restrict__ top,
                                                               const float* __restrict__ alpha, T* __restrict__ out,
                                                               int64_t ldo) {
     const int64_t i = blockIdx.x;
     const int64_t row = rows ? rows[i] : i;
     if (row < 0 || row >= hidden_rows) return;
     // a row that does not count gets zeros: the sum of no runs
-    const bool counts = lse[i] != INFINITY;
+    const bool counts = top[i] != INFINITY;
     sum_splits(part + i * dp, counts ? splits : 0, np * dp, width, counts ? *alpha : 0.f, out + row * ldo);
 }
 
@@ -1885,7 +1908,7 @@ extern "C" size_t grws_head_fwd_workspace_bytes(const grws_head* h) {
     return z.used;
 }
 
-extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit, float* target_prob,
+extern "C" int grws_head_fwd(const grws_head* h, float* row_stats, float* target_logit, float* target_prob,
                              float* row_loss, float* loss, int64_t* counts, void* workspace, size_t workspace_bytes,
                              void* stream_) {
     clear_error();
@@ -1898,7 +1921,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
         GRWS_LAUNCH_CHECK();
         return GRWS_OK;
     }
-    GRWS_CHECK_ARG(lse && target_logit && (h->k == 0 || target_prob), "head: null output");
+    GRWS_CHECK_ARG(row_stats && target_logit && (h->k == 0 || target_prob), "head: null output");
     const Shape s = shape_of(h, false);
     const Targets t = targets_of(h);
     Carver cv(workspace, workspace_bytes);
@@ -1944,7 +1967,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
 #define GRWS_HEAD_JOIN(R)                                                                                            \
     hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part,                 \
                        ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature, c1,      \
-                       target_logit, target_prob, f.flags, lse, row_loss, f.pl, f.pc,                                \
+                       target_logit, target_prob, f.flags, row_stats, row_stats + s.n, row_loss, f.pl, f.pc,         \
                        blocks <= kJoinBlocks ? f.done : nullptr, loss, counts)
     if (rows == 1) GRWS_HEAD_JOIN(1);
     else if (rows == 4) GRWS_HEAD_JOIN(4);
@@ -1967,7 +1990,7 @@ extern "C" size_t grws_head_bwd_workspace_bytes(const grws_head* h) {
     return z.used;
 }
 
-extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* target_logit,
+extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const float* target_logit,
                              const float* target_prob, const int64_t* counts, const float* dloss, int32_t per_row,
                              void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw, void* d_bias,
                              void* workspace, size_t workspace_bytes, void* stream_) {
@@ -1985,7 +2008,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         if (d_bias) GRWS_TRY(fill_bytes_zero(d_bias, h->classes * e, stream));
         return GRWS_OK;
     }
-    GRWS_CHECK_ARG(lse && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
+    GRWS_CHECK_ARG(row_stats && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
     if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
     const Shape s = shape_of(h, true);
     const Targets t = targets_of(h);
@@ -1996,13 +2019,14 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
     const float c1 = kLog2e / h->temperature;
     const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
     const float* coef = target_prob ? target_prob + s.n * h->k : nullptr;
+    const RowStats stats{row_stats, row_stats + s.n};
     const float* row_scale = nullptr;
     if (per_row) {
         GRWS_TRY(fill_i32(reinterpret_cast<int32_t*>(f.most), 1, 0, stream));
         const dim3 grid((unsigned)ceil_div(s.n, 256));
-        hipLaunchKernelGGL(head_most_kernel, grid, dim3(256), 0, stream, dloss, lse, s.n, f.most);
+        hipLaunchKernelGGL(head_most_kernel, grid, dim3(256), 0, stream, dloss, stats.top, s.n, f.most);
         GRWS_LAUNCH_CHECK();
-        hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, lse, s.n, f.most, f.scale);
+        hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, stats.top, s.n, f.most, f.scale);
         GRWS_LAUNCH_CHECK();
         row_scale = f.scale;
     }
@@ -2028,7 +2052,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             a.hidden = h->hidden, a.weight = h->weight, a.bias = h->bias;
             a.ldh = h->ld_hidden, a.ldw = h->ld_weight, a.n = s.n, a.np = s.np, a.width = s.D;
             a.v0 = v0, a.vend = v0 + vc, a.classes = s.V, a.c1 = c1;
-            a.lse = lse, a.row_scale = row_scale, a.gscale = gscale, a.G = f.G, a.ldg = s.ldg, a.plane = plane;
+            a.stats = stats, a.row_scale = row_scale, a.gscale = gscale, a.G = f.G, a.ldg = s.ldg, a.plane = plane;
             a.bias_part = d_bias && h->k == 0 ? f.bias : nullptr, a.vt = vt;
             if (s.split) GRWS_TRY((launch_few<float, 3>(h, a, stream)));
             else if (h->dtype == GRWS_F16 && s.gplanes == 1) GRWS_TRY((launch_few<_Float16, 1>(h, a, stream)));
@@ -2039,7 +2063,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
             GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes),
                        v0, s.V, s.n, c1, h->bias,
-                       h->dtype, lse, h->labels, row_scale, gscale, f.G, s.ldg, plane,
+                       h->dtype, stats, h->labels, row_scale, gscale, f.G, s.ldg, plane,
                        d_bias && h->k == 0 ? f.bias : nullptr, vt};
 #define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
             GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
@@ -2048,7 +2072,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         if (h->k > 0) {
             const dim3 grid((unsigned)ceil_div(s.n * h->k, 256));
 #define GRWS_HEAD_SUB(DT, PL)                                                                                 \
-    hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, lse, target_logit, coef, \
+    hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, stats, target_logit, coef, \
                        row_scale, gscale, c1, s.n, v0, vc, f.G, s.ldg, plane)
             GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
 #undef GRWS_HEAD_SUB
@@ -2119,7 +2143,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
             HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc, s.gplanes), f.dh, s.np, s.dp, v0 == 0,
                          s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
-                         h->hidden_rows, h->rows, lse};
+                         h->hidden_rows, h->rows, stats.top};
             if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
             else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
@@ -2129,7 +2153,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
-                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, lse, f.alpha, static_cast<T*>(d_hidden), ld_dh)
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats.top, f.alpha, static_cast<T*>(d_hidden), ld_dh)
         if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
         else GRWS_HEAD_DH(__hip_bfloat16);

@@ -159,3 +159,27 @@ def test_loss_of_confident_rows(cuda_device, dt, n):
         index = torch.tensor([[7]], dtype=torch.int32, device=cuda_device).expand(n, 1)
         kd, _ = linear_distill(h.to(dt), w.to(dt), index, torch.zeros(n, 1, device=cuda_device))
         assert abs(float(kd) - want) <= 4e-6 * want, (base, float(kd), want)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+def test_lowest_logits(cuda_device, dt, n):
+    """Logits of the type's lowest value: rows with nothing else are uniform,
+    and a label there costs what it does in F.cross_entropy."""
+    classes, low = 500, torch.finfo(dt).min
+    h = torch.zeros(n, 8, device=cuda_device, dtype=dt).requires_grad_(True)
+    w = torch.ones(classes, 8, device=cuda_device, dtype=dt).requires_grad_(True)
+    b = torch.full((classes,), low, device=cuda_device, dtype=dt).requires_grad_(True)
+    labels = torch.arange(n, device=cuda_device) % classes
+    loss, _ = linear_cross_entropy(h, w, labels, bias=b, reduction="none")
+    assert float((loss - math.log(classes)).abs().max()) <= 1e-5
+    db = torch.autograd.grad(loss.sum(), [b])[0].double()
+    want = n / classes - torch.bincount(labels, minlength=classes).double()
+    assert float((db - want).abs().max()) <= 0.01
+    b = b.detach().clone()
+    b[250:] = 0
+    loss, counts = linear_cross_entropy(h, w, labels, bias=b, reduction="none")
+    ref = torch.nn.functional.cross_entropy(h.detach().float() @ w.detach().float().t() + b.float(), labels,
+                                            reduction="none")
+    assert float((loss / ref - 1).abs().max()) <= 1e-6
+    assert counts.tolist() == [0, n, 0]
