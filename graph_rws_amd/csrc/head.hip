@@ -357,11 +357,13 @@ __device__ __forceinline__ void begin_logits(float4_t (&acc)[TP][TQ], int64_t vf
 }
 
 // The maxima stay logits: two of them can be one float when multiplied by c1,
-// and a hit is a matter of which is larger.  The exponentials of a strip are
-// taken against the rounded m c1; one that overflows (m a mask of the type's
-// lowest value) leaves nothing of the logits that are not equal to m.
-__device__ __forceinline__ bool too_far(float m, float ref) {
-    return fabsf(ref) == INFINITY && fabsf(m) != INFINITY;
+// and a hit is a matter of which is larger.  The exponentials of a row are
+// 2^(z c - ref), ref the rounded m c, of a largest logit m.  c is c1, but a
+// half where m c1 overflows (m a mask of the type's lowest value): floats of
+// that size lie so far apart that any c leaves zero of a z other than m, and
+// with a power of two m c is exact and leaves one of m.
+__device__ __forceinline__ float base2(float m, float c1) {
+    return fabsf(m * c1) == INFINITY && fabsf(m) != INFINITY ? 0.5f : c1;
 }
 // what makes a strip's sum one against m c1 itself
 __device__ __forceinline__ float past_rounding(float m, float c1) {
@@ -412,24 +414,14 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
             for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
         m = fmaxf(m, __shfl_xor(m, 16, kWave));
         m = fmaxf(m, __shfl_xor(m, 32, kWave));
-        const float ref = m == -INFINITY ? 0.f : m * a.c1;  // nothing but -inf: a sum of zeros
+        const float c1 = base2(m, a.c1), ref = m == -INFINITY ? 0.f : m * c1;  // nothing but -inf: a sum of zeros
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c1, -ref));
+            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref));
         s += __shfl_xor(s, 16, kWave);
         s += __shfl_xor(s, 32, kWave);
-        if (__any(too_far(m, ref))) {
-            float same = 0.f;
-#pragma unroll
-            for (int i = 0; i < TP; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) same += acc[i][j][e] == m ? 1.f : 0.f;
-            same += __shfl_xor(same, 16, kWave);
-            same += __shfl_xor(same, 32, kWave);
-            s = too_far(m, ref) ? same : s;
-        }
         if (lane < 16) a.part[strip * a.np + row] = make_float2(m, s);
         if (a.labels) {
             const int64_t lab = row < a.n ? a.labels[row] - vfirst : -1;
@@ -460,18 +452,11 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
     }
 }
 
-// What the forward leaves of a row for the gradients: p = 2^(z c1 - the
-// rounded m c1) * factor.  (Of one log-sum, m c1 + log2 s rounded, nothing
-// would be left of s beside a large m.)
-struct RowStats {
-    const float* top;     // [n]: the largest logit m; +inf: the row does not count
-    const float* factor;  // [n]: one over the sum of the exponentials
-};
-
-// 2^(z c1 - ref), ref the rounded m c1
-__device__ __forceinline__ float above(float z, float c1, float m, float ref, bool far) {
-    return far ? (z == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(fmaf(z, c1, -ref));
-}
+// What the forward leaves of a row for the gradients: the largest logit m
+// (+inf: the row does not count) and one over the sum of the exponentials, so
+// p = 2^(z c - ref) times that.  (Of one log-sum, m c1 + log2 s rounded,
+// nothing would be left of s beside a large m.)
+typedef const float2* RowStats;
 
 struct GradArgs {
     Gemm g;
@@ -558,20 +543,14 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
         // of a row that does not count, whose largest logit is given as +inf,
         // all are 2^-inf (its hidden row is zeros, so a logit is its bias)
-        const float m = row < a.n ? a.stats.top[row] : INFINITY, ref = m * a.c1;
+        const float2 st = row < a.n ? a.stats[row] : make_float2(INFINITY, 0.f);
+        const float m = st.x, c1 = base2(m, a.c1), ref = m * c1;
         const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
-        const float f = m != INFINITY ? a.stats.factor[row] * s : 0.f;
-        if (__any(too_far(m, ref))) {
+        const float f = st.y * s;
 #pragma unroll
-            for (int i = 0; i < TP; ++i)
+        for (int i = 0; i < TP; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = above(acc[i][j][e], a.c1, m, ref, too_far(m, ref));
-        } else {
-#pragma unroll
-            for (int i = 0; i < TP; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = above(acc[i][j][e], a.c1, m, ref, false);
-        }
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref));
 #pragma unroll
         for (int i = 0; i < TP; ++i) acc[i][j] *= f;
         if (a.labels) {
@@ -722,7 +701,7 @@ struct HiddenArgs {
     void* out;
     int64_t ldo, n, width, hidden_rows;
     const int64_t* rows;
-    const float* top;  // +inf: the row gets zeros, whatever alpha and W hold
+    RowStats stats;  // a row that does not count gets zeros, whatever alpha and W hold
 };
 
 template <int DT, int OT, int BP, int BQ, int WP, int WQ>
@@ -748,7 +727,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
         if (a.last && row < a.n) {
             to = a.rows ? a.rows[row] : row;
             if (to >= a.hidden_rows) to = -1;
-            counts = a.top[row] != INFINITY;
+            counts = a.stats[row].x != INFINITY;
         }
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
@@ -1035,7 +1014,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
         const int64_t row = first + 16 * j + r;
-        if constexpr (GRAD) live[j] = row < a.n && a.stats.top[row] != INFINITY;
+        if constexpr (GRAD) live[j] = row < a.n && a.stats[row].x != INFINITY;
         else live[j] = row < a.n && (a.t.labels ? row_state<1>(a.t, row, 0) : a.states[row]) == 1;
         h[j] = static_cast<const T*>(a.hidden) + (live[j] ? (a.t.rows ? a.t.rows[row] : row) * a.ldh : 0);
     }
@@ -1125,16 +1104,14 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
             m = fmaxf(m, __shfl_xor(m, 16, kWave));
             m = fmaxf(m, __shfl_xor(m, 32, kWave));
             y = __shfl(y, (((l >> 2) & 3) << 4) | r, kWave);
-            const float ref = m == -INFINITY ? 0.f : m * a.c1;
-            const bool far = too_far(m, ref);
+            const float c1 = base2(m, a.c1), ref = m == -INFINITY ? 0.f : m * c1;
             float s = 0.f;
             int tie = 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z = acc[i][j][e];
-                    s += far ? (z == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(fmaf(z, a.c1, -ref));
+                    s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref));
                     tie |= acc[i][j][e] == y && 16 * i + 4 * g + e < l;
                 }
             s += __shfl_xor(s, 16, kWave);
@@ -1149,15 +1126,16 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                 }
             }
         } else {
-            const float m = live[j] ? a.stats.top[row] : INFINITY, ref = m * a.c1;
+            const float2 st = live[j] ? a.stats[row] : make_float2(INFINITY, 0.f);
+            const float m = st.x, c1 = base2(m, a.c1), ref = m * c1;
             const float sc = a.row_scale && live[j] ? a.row_scale[row] * a.gscale : a.gscale;
-            const float f = live[j] ? a.stats.factor[row] * sc : 0.f;
+            const float f = st.y * sc;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 uint16_t x[4][PLANES > 0 ? PLANES : 1];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float p = above(acc[i][j][e], a.c1, m, ref, too_far(m, ref)) * f;
+                    float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref)) * f;
                     p = 16 * i + 4 * g + e == l ? p - sc : p;
                     sums[i][e] += p;
                     planes_of<DT, PLANES>(p, x[e]);
@@ -1338,8 +1316,8 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
                                                         int32_t strip_classes, int64_t n, int64_t np,
                                                         float temperature, float c1, const float* __restrict__ y,
                                                         const float* __restrict__ prob,
-                                                        const int32_t* __restrict__ flags, float* __restrict__ top,
-                                                        float* __restrict__ factor, float* __restrict__ row_loss, double* part_loss,
+                                                        const int32_t* __restrict__ flags, float2* __restrict__ stats,
+                                                        float* __restrict__ row_loss, double* part_loss,
                                                         int32_t* part_cnt, int32_t* done,
                                                         float* __restrict__ loss_out, int64_t* __restrict__ counts) {
     __shared__ float sm[8][R], ss[8][R];
@@ -1419,8 +1397,8 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             v = __int_as_float(0x7fc00000);
         }
         // a live row with a logit of +inf has nothing but NaN
-        top[i] = st != 1 ? INFINITY : m == INFINITY ? __int_as_float(0x7fc00000) : m;
-        factor[i] = past_rounding(m, c1) / s;
+        stats[i] = make_float2(st != 1 ? INFINITY : m == INFINITY ? __int_as_float(0x7fc00000) : m,
+                               st != 1 ? 0.f : past_rounding(m, c1) / s);
         if (row_loss) row_loss[i] = v;
     }
 #pragma unroll
@@ -1456,13 +1434,13 @@ __global__ __launch_bounds__(64) void head_finish_kernel(const double* part_loss
 }
 
 __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict__ dloss,
-                                                        const float* __restrict__ top, int64_t n,
+                                                        RowStats stats, int64_t n,
                                                         uint32_t* __restrict__ most) {
     // of non-negative floats the largest is the largest as an integer: the
     // order of the atomics does not matter.  Infinities and NaN are left out:
     // they are their rows' own shares, not a factor of every row
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    uint32_t m = i < n && top[i] != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
+    uint32_t m = i < n && stats[i].x != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
     if (m >= 0x7f800000u) m = 0u;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -1475,13 +1453,13 @@ __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict_
 // 0 for a row that does not count, whatever dloss holds there: its G is zeros
 // times this.  (Without a factor other than 0, infinity and NaN: 0 or NaN.)
 __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __restrict__ dloss,
-                                                             const float* __restrict__ top, int64_t n,
+                                                             RowStats stats, int64_t n,
                                                              const uint32_t* __restrict__ most,
                                                              float* __restrict__ scale) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const float m = __uint_as_float(*most);
-    scale[i] = top[i] == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : dloss[i] * 0.f;
+    scale[i] = stats[i].x == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : dloss[i] * 0.f;
 }
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.
@@ -1498,11 +1476,11 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats 
     const int64_t i = at / t.k;
     const int64_t v = teacher_at(t, i, (int)(at - i * t.k));
     if (v < v0 || v >= v0 + vc) return;
-    const float q = coef[at], m = stats.top[i], ref = m * c1;
+    const float q = coef[at], m = stats[i].x, c = base2(m, c1);
     if (q < 0.f || m == INFINITY) return;
     const float s = row_scale ? row_scale[i] * gscale : gscale;
     uint16_t h[PLANES];
-    planes_of<DT, PLANES>((above(y[at], c1, m, ref, too_far(m, ref)) * stats.factor[i] - q) * s, h);
+    planes_of<DT, PLANES>((exp2f(fmaf(y[at], c, -(m * c))) * stats[i].y - q) * s, h);
 #pragma unroll
     for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
 }
@@ -1592,14 +1570,14 @@ template <typename T>
 __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __restrict__ part, int64_t splits,
                                                               int64_t np, int64_t dp, int64_t width,
                                                               const int64_t* __restrict__ rows, int64_t hidden_rows,
-                                                              const float* __restrict__ top,
+                                                              RowStats stats,
                                                               const float* __restrict__ alpha, T* __restrict__ out,
                                                               int64_t ldo) {
     const int64_t i = blockIdx.x;
     const int64_t row = rows ? rows[i] : i;
     if (row < 0 || row >= hidden_rows) return;
     // a row that does not count gets zeros: the sum of no runs
-    const bool counts = top[i] != INFINITY;
+    const bool counts = stats[i].x != INFINITY;
     sum_splits(part + i * dp, counts ? splits : 0, np * dp, width, counts ? *alpha : 0.f, out + row * ldo);
 }
 
@@ -1967,7 +1945,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* row_stats, float* target
 #define GRWS_HEAD_JOIN(R)                                                                                            \
     hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part,                 \
                        ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature, c1,      \
-                       target_logit, target_prob, f.flags, row_stats, row_stats + s.n, row_loss, f.pl, f.pc,         \
+                       target_logit, target_prob, f.flags, reinterpret_cast<float2*>(row_stats), row_loss, f.pl, f.pc, \
                        blocks <= kJoinBlocks ? f.done : nullptr, loss, counts)
     if (rows == 1) GRWS_HEAD_JOIN(1);
     else if (rows == 4) GRWS_HEAD_JOIN(4);
@@ -2019,14 +1997,14 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
     const float c1 = kLog2e / h->temperature;
     const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
     const float* coef = target_prob ? target_prob + s.n * h->k : nullptr;
-    const RowStats stats{row_stats, row_stats + s.n};
+    const RowStats stats = reinterpret_cast<RowStats>(row_stats);
     const float* row_scale = nullptr;
     if (per_row) {
         GRWS_TRY(fill_i32(reinterpret_cast<int32_t*>(f.most), 1, 0, stream));
         const dim3 grid((unsigned)ceil_div(s.n, 256));
-        hipLaunchKernelGGL(head_most_kernel, grid, dim3(256), 0, stream, dloss, stats.top, s.n, f.most);
+        hipLaunchKernelGGL(head_most_kernel, grid, dim3(256), 0, stream, dloss, stats, s.n, f.most);
         GRWS_LAUNCH_CHECK();
-        hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, stats.top, s.n, f.most, f.scale);
+        hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, stats, s.n, f.most, f.scale);
         GRWS_LAUNCH_CHECK();
         row_scale = f.scale;
     }
@@ -2143,7 +2121,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
             HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc, s.gplanes), f.dh, s.np, s.dp, v0 == 0,
                          s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
-                         h->hidden_rows, h->rows, stats.top};
+                         h->hidden_rows, h->rows, stats};
             if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
             else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
@@ -2153,7 +2131,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
-                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats.top, f.alpha, static_cast<T*>(d_hidden), ld_dh)
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, f.alpha, static_cast<T*>(d_hidden), ld_dh)
         if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
         else GRWS_HEAD_DH(__hip_bfloat16);

@@ -838,8 +838,8 @@ int grws_cross_entropy_bwd(const void* logits, int32_t dtype, int64_t ld, int64_
 /* Losses: cross entropy lse_i - z_i,label; distillation T^2 KL(softmax of   */
 /* the listed teacher logits / T || softmax(z_i / T)).                       */
 /*                                                                           */
-/* Forward, no sync: row_stats f32 [2 x n] (the rows' largest logits, +inf   */
-/* for rows that do not count, then the reciprocals of their sums of         */
+/* Forward, no sync: row_stats f32 [n x 2], 8-byte aligned (a row's largest  */
+/* logit, +inf when it does not count, and the reciprocal of its sum of      */
 /* exponentials) and target_logit f32 [n * max(k, 1)], target_prob f32       */
 /* [2 x n x k] (k > 0), which the backward takes; row_loss                   */
 /* f32 [n] (0 for rows that do not count, NaN for bad input); loss f32 scalar,   */
