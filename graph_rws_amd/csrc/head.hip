@@ -477,13 +477,21 @@ struct GradArgs {
 __device__ __forceinline__ uint16_t top16(float x) { return (uint16_t)(__float_as_uint(x) >> 16); }
 __device__ __forceinline__ float from_top16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
 
-// x = a + b + c exactly: three truncated bf16 (an infinity or NaN stays in
-// the first; a NaN keeps a bit in its upper half)
+// x = a + b + c exactly: three truncated bf16.  A NaN goes into a (with a bit
+// in its upper half).  An infinity goes into c, which meets only the other
+// operand's a in the six plane products, so that its products have the sign
+// they should (in a it would meet zero planes: NaN); a is then one of its
+// sign, for the other operand's infinities to meet.
 __device__ __forceinline__ void split3(float x, uint16_t* a, uint16_t* b, uint16_t* c) {
     *a = top16(x);
     if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) {
-        if (x != x) *a |= 0x40;
         *b = *c = 0;
+        if (x != x) {
+            *a |= 0x40;
+        } else {
+            *c = *a;
+            *a = (*a & 0x8000) | 0x3f80;
+        }
         return;
     }
     const float r = x - from_top16(*a);

@@ -183,3 +183,28 @@ def test_lowest_logits(cuda_device, dt, n):
                                             reduction="none")
     assert float((loss / ref - 1).abs().max()) <= 1e-6
     assert counts.tolist() == [0, n, 0]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+def test_infinite_operands(cuda_device, dt, n):
+    """An infinity in an operand gives the logits that it gives elsewhere:
+    +-inf where it meets a number, NaN where it meets a zero."""
+    classes, width = 300, 24
+    h, w, b, labels, _, _ = _inputs(cuda_device, n, width, classes, dt, 8)
+    h = h.abs() + 0.25
+    w[5, 3] = -math.inf  # a masked class
+    labels[:] = labels % 100 + 50
+    labels[1] = 5
+    loss, counts = linear_cross_entropy(h, w, labels, bias=b, reduction="none")
+    z = (h.double() @ w.double().t()) + b.double()
+    ref = torch.nn.functional.cross_entropy(z, labels, reduction="none")
+    assert bool(torch.isinf(ref[1])) and torch.equal(torch.isinf(loss), torch.isinf(ref))
+    live = torch.isfinite(ref)
+    assert float((loss[live].double() - ref[live]).abs().max()) <= 1e-4
+    h[2, 3] = 0.0  # 0 x inf
+    h[3, 0] = math.inf
+    loss, _ = linear_cross_entropy(h, w, labels, bias=b, reduction="none")
+    assert bool(torch.isnan(loss[2])) and bool(torch.isnan(loss[3]))
+    keep = [0, 4, 5, 6, 7, 8]
+    assert float((loss[keep].double() - ref[keep]).abs().max()) <= 1e-4
