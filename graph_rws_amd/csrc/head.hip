@@ -453,9 +453,10 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
 }
 
 // What the forward leaves of a row for the gradients: the largest logit m
-// (+inf: the row does not count) and one over the sum of the exponentials, so
-// p = 2^(z c - ref) times that.  (Of one log-sum, m c1 + log2 s rounded,
-// nothing would be left of s beside a large m.)
+// and one over the sum of the exponentials, so p = 2^(z c - ref) times that.
+// (Of one log-sum, m c1 + log2 s rounded, nothing would be left of s beside a
+// large m.)  A row that does not count has m = +inf and a factor of zero, or
+// NaN where its zeros met a weight that is not finite.
 typedef const float2* RowStats;
 
 struct GradArgs {
@@ -554,7 +555,14 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
         const float2 st = row < a.n ? a.stats[row] : make_float2(INFINITY, 0.f);
         const float m = st.x, c1 = base2(m, a.c1), ref = m * c1;
         const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
-        const float f = st.y * s;
+        const bool stray = row >= a.n || (m == INFINITY && st.y != 0.f);
+        const float f = stray ? 0.f : st.y * s;
+        if (__any(stray)) {
+#pragma unroll
+            for (int i = 0; i < TP; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = stray ? -INFINITY : acc[i][j][e];
+        }
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
@@ -1143,7 +1151,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                 uint16_t x[4][PLANES > 0 ? PLANES : 1];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref)) * f;
+                    float p = live[j] ? __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref)) * f : 0.f;
                     p = 16 * i + 4 * g + e == l ? p - sc : p;
                     sums[i][e] += p;
                     planes_of<DT, PLANES>(p, x[e]);
@@ -1406,7 +1414,7 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
         }
         // a live row with a logit of +inf has nothing but NaN
         stats[i] = make_float2(st != 1 ? INFINITY : m == INFINITY ? __int_as_float(0x7fc00000) : m,
-                               st != 1 ? 0.f : past_rounding(m, c1) / s);
+                               st == 1 ? past_rounding(m, c1) / s : s == s ? 0.f : s);
         if (row_loss) row_loss[i] = v;
     }
 #pragma unroll

@@ -208,3 +208,23 @@ def test_infinite_operands(cuda_device, dt, n):
     assert bool(torch.isnan(loss[2])) and bool(torch.isnan(loss[3]))
     keep = [0, 4, 5, 6, 7, 8]
     assert float((loss[keep].double() - ref[keep]).abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+@pytest.mark.parametrize("kind", ["labels", "lists"])
+def test_infinite_weight_and_rows_that_do_not_count(cuda_device, dt, n, kind):
+    """A class masked by a weight of -inf has a probability of zero in the
+    rows that count and no gradient from the others (whose zeros times an
+    infinity are none of it)."""
+    h, w, b, labels, lists, teacher = _inputs(cuda_device, n, 24, 300, dt, 8)
+    h = h.abs() + 0.25
+    w[5, 3] = -math.inf
+    labels[:] = labels % 100 + 50
+    lists[:] = lists % 100 + 50
+    labels[::4] = -100
+    lists[::4] = -1
+    target = labels if kind == "labels" else (lists, teacher)
+    _, _, dw, db = _row_grads(kind, h, w, b, target, torch.ones(n, device=cuda_device))
+    assert bool(torch.isfinite(dw).all()) and bool(torch.isfinite(db).all())
+    assert not bool(dw[5].any()) and float(db[5]) == 0
