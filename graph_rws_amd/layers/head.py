@@ -25,6 +25,20 @@ from ..core import ops as _ops
 _REDUCTIONS = ("mean", "none")
 
 
+class _FirstOnly(Function):
+    """The gradients, tied to the parameters they belong to (the first of the
+    arguments): differentiating them again is an error and not a zero."""
+
+    @staticmethod
+    def forward(ctx, params, *grads):
+        ctx.set_materialize_grads(False)
+        return tuple(g.view_as(g) if g is not None else None for g in grads[params:])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("linear_cross_entropy / linear_distill have no second derivative")
+
+
 class _Head(Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, rows, labels, teacher_index, teacher_logits, temperature, per_row):
@@ -41,6 +55,8 @@ class _Head(Function):
         hidden, weight, bias, rows, labels, index, logits, counts, saved = ctx.saved_tensors
         call = _ops.HeadCall(hidden, weight, bias, rows, labels, index, logits, ctx.temperature)
         grads = _ops.head_bwd(call, saved, counts, dloss, ctx.needs_input_grad[:3])
+        if torch.is_grad_enabled():  # create_graph=True
+            grads = _FirstOnly.apply(4, hidden, weight, bias, dloss, *grads)
         return (*grads, None, None, None, None, None, None)
 
 

@@ -228,3 +228,19 @@ def test_infinite_weight_and_rows_that_do_not_count(cuda_device, dt, n, kind):
     _, _, dw, db = _row_grads(kind, h, w, b, target, torch.ones(n, device=cuda_device))
     assert bool(torch.isfinite(dw).all()) and bool(torch.isfinite(db).all())
     assert not bool(dw[5].any()) and float(db[5]) == 0
+
+
+@pytest.mark.parametrize("kind", ["labels", "lists"])
+def test_no_second_derivative(cuda_device, kind):
+    """A second derivative is refused, not left out."""
+    h, w, b, labels, lists, teacher = _inputs(cuda_device, 30, 16, 60, torch.float32, 9)
+    h.requires_grad_(True)
+    w.requires_grad_(kind == "labels")
+    if kind == "labels":
+        loss, _ = linear_cross_entropy(h, w, labels, bias=b)
+    else:
+        loss, _ = linear_distill(h, w, lists, teacher, bias=None)
+    g = torch.autograd.grad(loss, [h], create_graph=True)[0]
+    assert g.requires_grad
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad((g ** 2).sum() + (h ** 2).sum(), [h])
