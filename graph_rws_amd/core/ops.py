@@ -1825,11 +1825,15 @@ def cross_entropy_bwd(logits: torch.Tensor, rows: Optional[torch.Tensor], labels
 # ---------------------------------------------------------------------------
 # classifier over many classes (csrc/head.hip) and top logits (csrc/top.hip)
 # ---------------------------------------------------------------------------
-def _unit_columns(t: torch.Tensor) -> torch.Tensor:
-    """t with unit column stride and rows that do not overlap (a copy where
-    it has neither)."""
-    ok = (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+def _unit_columns(t: torch.Tensor, most: int = 1 << 62) -> torch.Tensor:
+    """t with unit column stride and rows that do not overlap, `most`
+    elements apart or less (a copy where it is otherwise)."""
+    ok = ((t.shape[1] <= 1 or t.stride(1) == 1)
+          and (t.shape[0] <= 1 or t.shape[1] <= t.stride(0) <= most))
     return t if ok else t.contiguous()
+
+
+_HEAD_PITCH = 1 << 21  # of grws_head: row offsets within a tile take 32 bits
 
 
 def _row_pitch(t: torch.Tensor) -> int:
@@ -1879,7 +1883,7 @@ class HeadCall:
 
     def __init__(self, hidden, weight, bias=None, rows=None, labels=None, teacher_index=None, teacher_logits=None,
                  temperature: float = 1.0):
-        self.hidden, self.weight = _unit_columns(hidden), _unit_columns(weight)
+        self.hidden, self.weight = _unit_columns(hidden, _HEAD_PITCH), _unit_columns(weight, _HEAD_PITCH)
         self.bias = bias.contiguous() if bias is not None else None
         self.rows = rows.contiguous() if rows is not None else None
         if labels is not None:

@@ -244,3 +244,19 @@ def test_no_second_derivative(cuda_device, kind):
     assert g.requires_grad
     with pytest.raises(RuntimeError, match="second"):
         torch.autograd.grad((g ** 2).sum() + (h ** 2).sum(), [h])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_rows_far_apart(cuda_device, dt):
+    """Rows more than 2^21 elements apart."""
+    pitch = (1 << 21) + 24
+    wide = torch.randn(6 * pitch, device=cuda_device).to(dt)
+    h, w = wide.as_strided((6, 32), (pitch, 1)), wide.as_strided((5, 32), (pitch, 1), 64)
+    labels = torch.arange(6, device=cuda_device) % 5
+    out = []
+    for x, y in ((h, w), (h.contiguous(), w.contiguous())):
+        x, y = x.detach().requires_grad_(True), y.detach().requires_grad_(True)
+        loss, _ = linear_cross_entropy(x, y, labels)
+        out.append((loss.detach(), *torch.autograd.grad(loss, [x, y])))
+    for x, y in zip(*out):
+        assert torch.equal(x, y)
