@@ -705,6 +705,16 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
 // into `splits` runs; each run adds to its own fp32 sums (piece after piece,
 // so the order is fixed).  8,192 x 4,096 over 65,536 classes: 3.28 ms (1,343
 // TFLOP/s).
+
+// Whether `rows` lists the row more than once: owner, which holds a listing's
+// number for every listed row, has kAgain there.  Each listing has a gradient
+// of its own and only one of them could be kept: the row gets NaN, which is
+// seen, and not one of them, which is not.
+constexpr int32_t kAgain = -1;
+__device__ __forceinline__ bool listed_again(const int32_t* owner, int64_t row) {
+    return owner && owner[row] == kAgain;
+}
+
 struct HiddenArgs {
     Gemm g;
     float* part;  // [splits][np][dp]
@@ -718,6 +728,7 @@ struct HiddenArgs {
     int64_t ldo, n, width, hidden_rows;
     const int64_t* rows;
     RowStats stats;  // a row that does not count gets zeros, whatever alpha and W hold
+    const int32_t* owner;  // NULL, or see listed_again
 };
 
 template <int DT, int OT, int BP, int BQ, int WP, int WQ>
@@ -745,6 +756,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
             if (to >= a.hidden_rows) to = -1;
             counts = a.stats[row].x != INFINITY;
         }
+        const bool again = to >= 0 && listed_again(a.owner, to);
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
             const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + C::p_of(i, lane);
@@ -753,8 +765,9 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
             const float4_t v = a.first ? acc[i][j] : *o + acc[i][j];
             if (!a.last) *o = v;
             else if (to >= 0 && d < a.width)
-                store4<OT>(a.out, to * a.ldo + d, counts ? v * alpha : float4_t{0.f, 0.f, 0.f, 0.f}, a.width - d,
-                           a.vec);
+                store4<OT>(a.out, to * a.ldo + d,
+                           again ? v * __int_as_float(0x7fc00000) : counts ? v * alpha : float4_t{0.f, 0.f, 0.f, 0.f},
+                           a.width - d, a.vec);
         }
     }
 }
@@ -853,14 +866,17 @@ __device__ __forceinline__ void pack_row(const T* __restrict__ x, bool live, int
 // plane, or three for f32), zeros past n and the width and in rows that do
 // not count (what such a row holds, NaN too, stays out of every sum).
 // One wave per row; the first also makes alpha (see Alpha) or clears `done`.
+// owner (or NULL): owner[rows[i]] = i, of a row listed again any of its i.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void head_pack_hidden_kernel(Targets t, const T* __restrict__ hidden, int64_t ld,
                                                                int64_t n, int64_t np, int64_t width, int64_t dp,
                                                                int32_t vec, uint16_t* __restrict__ out, Alpha al,
-                                                               int32_t* __restrict__ done) {
+                                                               int32_t* __restrict__ done, int32_t* owner) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= np) return;
+    if (owner && lane == 0 && i < n && t.rows[i] >= 0 && t.rows[i] < t.hidden_rows)
+        __hip_atomic_store(owner + t.rows[i], (int32_t)i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (i == 0 && lane == 0) {
         if (done) *done = 0;
         if (al.out) {
@@ -1442,7 +1458,17 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
     finish_loss(part_loss, part_cnt, gridDim.x, lane, loss_out, counts);
 }
 
-// the same in a launch of its own (also of no rows at all)
+// Of a row that is listed again, all but one listing find another's number.
+__global__ __launch_bounds__(256) void head_repeated_kernel(const int64_t* __restrict__ rows, int64_t n,
+                                                            int64_t hidden_rows, int32_t* owner) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i < n ? rows[i] : -1;
+    if (row < 0 || row >= hidden_rows) return;
+    if (__hip_atomic_load(owner + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (int32_t)i)
+        __hip_atomic_store(owner + row, kAgain, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// finish_loss in a launch of its own (also of no rows at all)
 __global__ __launch_bounds__(64) void head_finish_kernel(const double* part_loss, const int32_t* part_cnt,
                                                          int64_t nparts, float* __restrict__ loss,
                                                          int64_t* __restrict__ counts) {
@@ -1586,7 +1612,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __restrict__ part, int64_t splits,
                                                               int64_t np, int64_t dp, int64_t width,
                                                               const int64_t* __restrict__ rows, int64_t hidden_rows,
-                                                              RowStats stats,
+                                                              RowStats stats, const int32_t* __restrict__ owner,
                                                               const float* __restrict__ alpha, T* __restrict__ out,
                                                               int64_t ldo) {
     const int64_t i = blockIdx.x;
@@ -1594,7 +1620,8 @@ __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __res
     if (row < 0 || row >= hidden_rows) return;
     // a row that does not count gets zeros: the sum of no runs
     const bool counts = stats[i].x != INFINITY;
-    sum_splits(part + i * dp, counts ? splits : 0, np * dp, width, counts ? *alpha : 0.f, out + row * ldo);
+    const float a = listed_again(owner, row) ? __int_as_float(0x7fc00000) : counts ? *alpha : 0.f;
+    sum_splits(part + i * dp, counts ? splits : 0, np * dp, width, a, out + row * ldo);
 }
 
 // ---------------------------------------------------------------------------
@@ -1780,10 +1807,11 @@ struct BwdSpace {
     uint16_t *hp, *wp, *G;
     float *dh, *dw, *bias, *alpha, *scale;
     uint32_t* most;
+    int32_t* owner;  // see listed_again
 };
 
 template <typename A>
-void bwd_space(A& a, const Shape& s, BwdSpace* f) {
+void bwd_space(A& a, const Shape& s, const grws_head* h, BwdSpace* f) {
     auto take = [&](auto*& p, int64_t n) {
         using T = std::remove_reference_t<decltype(*p)>;
         if constexpr (std::is_same_v<A, Sizer>) a.template take<T>((size_t)n);
@@ -1798,6 +1826,7 @@ void bwd_space(A& a, const Shape& s, BwdSpace* f) {
     take(f->alpha, 1);
     take(f->scale, s.n);
     take(f->most, 1);
+    if (h->rows) take(f->owner, h->hidden_rows);
 }
 
 // whether 8 elements of a row may be read as 16-byte vectors
@@ -1806,17 +1835,17 @@ bool rows_of_16(const void* p, int64_t ld, int32_t dtype) {
 }
 
 int pack_hidden(const grws_head* h, const Shape& s, const Targets& t, uint16_t* hp, const Alpha& alpha,
-                int32_t* done, hipStream_t stream) {
+                int32_t* done, int32_t* owner, hipStream_t stream) {
     const dim3 grid((unsigned)ceil_div(s.np, 4));
     const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype);
     if (s.split)
         hipLaunchKernelGGL((head_pack_hidden_kernel<float, true>), grid, dim3(256), 0, stream, t,
                            static_cast<const float*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp, alpha,
-                           done);
+                           done, owner);
     else
         hipLaunchKernelGGL((head_pack_hidden_kernel<uint16_t, false>), grid, dim3(256), 0, stream, t,
                            static_cast<const uint16_t*>(h->hidden), h->ld_hidden, s.n, s.np, s.D, s.dp, vec, hp, alpha,
-                           done);
+                           done, owner);
     GRWS_LAUNCH_CHECK();
     return GRWS_OK;
 }
@@ -1945,7 +1974,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* row_stats, float* target
         else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 0>(h, a, stream)));
         else GRWS_TRY((launch_few<__hip_bfloat16, 0>(h, a, stream)));
     } else {
-        GRWS_TRY(pack_hidden(h, s, t, f.hp, Alpha{}, f.done, stream));
+        GRWS_TRY(pack_hidden(h, s, t, f.hp, Alpha{}, f.done, nullptr, stream));
     }
     for (int64_t v0 = 0; v0 < s.V && !s.few; v0 += s.vp) {
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
@@ -1980,7 +2009,7 @@ extern "C" size_t grws_head_bwd_workspace_bytes(const grws_head* h) {
     Sizer z;
     BwdSpace f{};
     const Shape s = shape_of(h, true);
-    bwd_space(z, s, &f);
+    bwd_space(z, s, h, &f);
     return z.used;
 }
 
@@ -2008,7 +2037,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
     const Targets t = targets_of(h);
     Carver cv(workspace, workspace_bytes);
     BwdSpace f{};
-    bwd_space(cv, s, &f);
+    bwd_space(cv, s, h, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
     const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
@@ -2025,7 +2054,13 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
         row_scale = f.scale;
     }
     const Alpha alpha{f.alpha, dloss, counts, per_row ? f.most : nullptr, h->temperature / gscale};
-    GRWS_TRY(pack_hidden(h, s, t, f.hp, alpha, nullptr, stream));
+    int32_t* owner = d_hidden ? f.owner : nullptr;
+    GRWS_TRY(pack_hidden(h, s, t, f.hp, alpha, nullptr, owner, stream));
+    if (owner) {
+        hipLaunchKernelGGL(head_repeated_kernel, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows, s.n,
+                           h->hidden_rows, owner);
+        GRWS_LAUNCH_CHECK();
+    }
     const int64_t plane = s.np * s.ldg;
     const size_t esz = dtype_size(h->dtype);
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
@@ -2137,7 +2172,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
             const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
             HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc, s.gplanes), f.dh, s.np, s.dp, v0 == 0,
                          s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
-                         h->hidden_rows, h->rows, stats};
+                         h->hidden_rows, h->rows, stats, owner};
             if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
             else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
             else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
@@ -2147,7 +2182,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
-                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, f.alpha, static_cast<T*>(d_hidden), ld_dh)
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, owner, f.alpha, static_cast<T*>(d_hidden), ld_dh)
         if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
         else GRWS_HEAD_DH(__hip_bfloat16);

@@ -70,9 +70,11 @@ def train_epoch_head(model, head, graphs_for_model, features: torch.Tensor, labe
                      teacher_weight: float = 0.5, temperature: float = 2.0, sync: bool = True):
     """One full-graph training step of a model with a LinearHead over many
     classes on its output rows, whose logits are never kept: cross entropy of
-    the rows train_idx (distinct) against labels, and with teacher = (values,
-    classes) [len(train_idx), k], the lists of a teacher's head (head.top),
+    the rows train_idx against labels, and with teacher = (values, classes)
+    [len(train_idx), k], the lists of a teacher's head (head.top),
     (1 - teacher_weight) of it plus teacher_weight of the distillation loss.
+    Strictly ascending int64 rows (train_idx from a mask is; checked once per
+    tensor) are read in place; any others, repeated ones too, are gathered.
     optimizer holds the parameters of both.  Returns (loss, acc) as
     train_epoch_full does."""
     model.train()
@@ -80,12 +82,13 @@ def train_epoch_head(model, head, graphs_for_model, features: torch.Tensor, labe
     if features.device != device:
         features = features.to(device)
     optimizer.zero_grad()
-    hidden = model(graphs_for_model, features)
-    loss, counts = head.loss(hidden, labels[train_idx], rows=train_idx)
-    n = train_idx.numel()
+    targets = labels[train_idx]
+    hidden, rows = _head_rows(model(graphs_for_model, features), train_idx)
+    loss, counts = head.loss(hidden, targets, rows=rows)
+    n = targets.numel()
     if teacher is not None:
         values, classes = teacher
-        kd, _ = head.distill(hidden, classes, values, rows=train_idx, temperature=temperature)
+        kd, _ = head.distill(hidden, classes, values, rows=rows, temperature=temperature)
         loss = (1.0 - teacher_weight) * loss + teacher_weight * kd
     acc = counts[0] / n if n > 0 else 0.0
     loss.backward()
@@ -96,15 +99,27 @@ def train_epoch_head(model, head, graphs_for_model, features: torch.Tensor, labe
     return loss.item(), acc
 
 
+def _head_rows(hidden, idx):
+    """(hidden, idx), or the gathered rows and None where a classifier's
+    gradient cannot be written to the rows idx in place."""
+    from ..layers.fused import rows_distinct
+    if idx.dtype == torch.int64 and idx.dim() == 1 and idx.device == hidden.device and rows_distinct(idx):
+        return hidden, idx
+    if idx.dtype == torch.bool:  # a model's rows can be padded to whole windows
+        hidden = hidden[:idx.shape[0]]
+    return hidden[idx], None
+
+
 @torch.no_grad()
 def evaluate_head(model, head, bcsr_full, features: torch.Tensor, labels: torch.Tensor, eval_idx: torch.Tensor):
     """(mean loss, accuracy) of a full-graph inference with a LinearHead on
-    the rows eval_idx (distinct)."""
+    the rows eval_idx."""
     model.eval()
     head.eval()
-    hidden = model.inference(bcsr_full, features)
-    loss, counts = head.loss(hidden, labels[eval_idx], rows=eval_idx)
-    n = eval_idx.numel()
+    targets = labels[eval_idx]
+    hidden, rows = _head_rows(model.inference(bcsr_full, features), eval_idx)
+    loss, counts = head.loss(hidden, targets, rows=rows)
+    n = targets.numel()
     return loss.item(), (counts[0] / n).item() if n > 0 else 0.0
 
 

@@ -78,8 +78,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     bias against labels.
 
     hidden [N, D], weight [V, D], bias [V] (one dtype of f32, f16, bf16),
-    labels int64 [n] (-100: the row does not count), rows int64 [n], distinct
-    (None = the first n rows).  reduction "mean": the f32 mean over counted
+    labels int64 [n] (-100: the row does not count), rows int64 [n] (None =
+    the first n rows; distinct ones where hidden needs a gradient, which is
+    NaN at a row listed twice: gather such rows first).  reduction "mean": the f32 mean over counted
     rows, NaN when none counts or a label or row id is out of range; "none":
     f32 [n], 0 for rows that do not count.  counts: int64 [3] on the device,
     {rows whose label is the first largest logit, counted rows, bad input}.

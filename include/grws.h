@@ -848,7 +848,8 @@ int grws_cross_entropy_bwd(const void* logits, int32_t dtype, int64_t ld, int64_
 /* not both); counts int64 [3] = {rows                                       */
 /* whose label is the first largest logit (k = 0), counted rows, bad input}. */
 /* Backward of dloss (f32 scalar of the mean, or with per_row [n] of         */
-/* row_loss): d_hidden (rows of `rows`; zero the others first), d_weight and */
+/* row_loss): d_hidden (rows of `rows`; zero the others first; NaN for a row */
+/* that `rows` lists twice, which the losses allow), d_weight and            */
 /* d_bias in `dtype`; NULL skips one.  A row that does not count reaches no  */
 /* gradient, whatever it holds.  Same inputs, same bits.                     */
 /* ------------------------------------------------------------------------ */

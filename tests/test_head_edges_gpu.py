@@ -260,3 +260,34 @@ def test_rows_far_apart(cuda_device, dt):
         out.append((loss.detach(), *torch.autograd.grad(loss, [x, y])))
     for x, y in zip(*out):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,width", [(9, 40), (200, 40), (6000, 300)])
+def test_repeated_rows(cuda_device, dt, n, width):
+    """A row listed twice: losses and the other gradients count both, its own
+    hidden gradient is NaN and no other row's is."""
+    print(f"case repeated {dt} {n}x{width}", flush=True)
+    classes, nodes = 300, 7000
+    h, w, b, labels, _, _ = _inputs(cuda_device, n, width, classes, dt, 3, nodes=nodes)
+    rows = torch.randperm(nodes, device=cuda_device)[:n]
+    labels[::5] = -100
+    single = rows.clone()
+    rows[5], rows[7] = rows[1], rows[1]
+    rows[6] = rows[0]  # one of the two does not count
+    out = []
+    for r in (rows, None):
+        x = h if r is not None else h[rows]
+        params = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        loss, counts = linear_cross_entropy(params[0], params[1], labels, bias=params[2], rows=r)
+        out.append([loss.detach(), counts, *torch.autograd.grad(loss, params)])
+    (loss, counts, dh, dw, db), (loss2, counts2, dx, dw2, db2) = out
+    assert torch.equal(loss, loss2) and torch.equal(counts, counts2)
+    assert torch.equal(dw, dw2) and torch.equal(db, db2)
+    nan = torch.isnan(dh).any(1)
+    assert sorted(nan.nonzero()[:, 0].tolist()) == sorted({int(rows[1]), int(rows[0])})
+    assert bool(torch.isnan(dh[nan]).all())
+    want = torch.zeros_like(dh)
+    want[rows] = dx
+    assert torch.equal(dh[~nan], want[~nan])
+    assert single.unique().numel() == n

@@ -86,3 +86,37 @@ def test_head_top_in_batches(cuda_device):
     v, c = torch.sort(torch.cat([head(x[i:i + 16]) for i in range(0, 70, 16)]).detach(), dim=1, descending=True,
                       stable=True)
     assert torch.equal(values, v[:, :6]) and torch.equal(classes.long(), c[:, :6])
+
+
+@pytest.mark.parametrize("kind", ["repeated", "shuffled", "mask"])
+def test_step_with_other_indices(cuda_device, kind):
+    """Rows listed twice, in any order, or a mask train as torch's ops do."""
+    graph, features, labels, idx, model, head = _problem(cuda_device)
+    if kind == "repeated":
+        idx = torch.cat([idx, idx[::3], idx[:5]])
+    elif kind == "shuffled":
+        idx = idx[torch.randperm(idx.numel(), device=cuda_device)]
+    else:
+        idx = torch.zeros(features.shape[0], dtype=torch.bool, device=cuda_device).index_fill(0, idx, True)
+    at = idx.nonzero()[:, 0] if kind == "mask" else idx
+    n = at.numel()
+    values, classes = LinearHead(48, 777).to(cuda_device).top(torch.randn(n, 48, device=cuda_device), 9)
+    twin, twin_head = copy.deepcopy(model), copy.deepcopy(head)
+    params = [*model.parameters(), *head.parameters()]
+    loss, acc = train_epoch_head(model, head, model._ensure_graph_list(graph), features, labels, idx,
+                                 torch.optim.SGD(params, lr=0.0), cuda_device, teacher=(values, classes))
+    logits = twin_head(twin(twin._ensure_graph_list(graph), features)[at])
+    q = torch.softmax(values / 2.0, 1)
+    logp = torch.log_softmax(logits / 2.0, 1).gather(1, classes.long())
+    want = 0.5 * F.cross_entropy(logits, labels[at]) + 0.5 * 4.0 * (q * (q.log() - logp)).sum(1).mean()
+    twins = [*twin.parameters(), *twin_head.parameters()]
+    grads = torch.autograd.grad(want, twins)
+    assert abs(loss - float(want.detach())) <= 1e-5 * abs(float(want.detach()))
+    assert round(float(acc) * n) == int((logits.argmax(1) == labels[at]).sum())
+    norm = torch.sqrt(sum((g.double() ** 2).sum() for g in grads))
+    scale = min(1.0, 1.0 / (float(norm) + 1e-6))
+    for p, g in zip(params, grads):
+        assert float((p.grad - scale * g).abs().max()) <= 1e-4 * float((scale * g).abs().max())
+    loss, acc = evaluate_head(model, head, graph, features, labels, idx)
+    logits = head(model.inference(graph, features)[at])
+    assert abs(loss - float(F.cross_entropy(logits, labels[at]))) <= 1e-5 * loss
