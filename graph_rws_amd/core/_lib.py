@@ -253,6 +253,7 @@ _PROTOS = {
     "grws_head_fwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(HeadView)]),
     "grws_head_fwd": (ctypes.c_int, [ctypes.POINTER(HeadView), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                      ctypes.c_size_t, _vp]),
+    "grws_head_plan": (ctypes.c_int, [ctypes.POINTER(HeadView), ctypes.c_int32, _c_i64p]),
     "grws_head_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(HeadView)]),
     "grws_head_bwd": (ctypes.c_int, [ctypes.POINTER(HeadView), _vp, _vp, _vp, _vp, _vp, ctypes.c_int32, _vp,
                                      ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, ctypes.c_size_t, _vp]),

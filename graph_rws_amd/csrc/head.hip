@@ -657,8 +657,9 @@ struct WeightArgs {
     void* out;  // first class of the piece
     int64_t ldo, classes, width;  // classes of the piece
     int32_t vec;  // rows of the output take 4-element stores
-    float* part;  // [splits][vp][dp], with splits > 1
+    float* part;  // [splits][vp][dp], or NULL: this one run is all of the sum
     int64_t vp, dp;
+    int32_t first;  // the first block of rows stores, the others add
 };
 
 template <int DT, int OT, int BP, int BQ, int WP, int WQ>
@@ -674,7 +675,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
     float4_t acc[TP][TQ];
     C::zero(acc);
     C::run(a.g, tp, tq, kb, ke, p0, q0, p1, q1, acc);
-    if (a.g.splits > 1) {
+    if (a.part) {
         float* out = a.part + sp * a.vp * a.dp;
 #pragma unroll
         for (int j = 0; j < TQ; ++j) {
@@ -682,7 +683,9 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
 #pragma unroll
             for (int i = 0; i < TP; ++i) {
                 const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + C::p_of(i, lane);
-                if (d < a.dp && v < a.classes) *reinterpret_cast<float4_t*>(out + v * a.dp + d) = acc[i][j];
+                if (d >= a.dp || v >= a.classes) continue;
+                float4_t* o = reinterpret_cast<float4_t*>(out + v * a.dp + d);
+                *o = a.first ? acc[i][j] : *o + acc[i][j];
             }
         }
         return;
@@ -917,14 +920,14 @@ __device__ __forceinline__ void load8(const T* x, int64_t c, int64_t width, bool
 // The student's logits at the teacher's entries, a wave per 4 entries of a
 // row (16 lanes share a dot product): n k rows of W are read, from beyond the
 // L2 (8,192 x 64 rows of 2 KB: 213 us, 5.0 TB/s).  The row's first wave also makes the teacher's probabilities: prob
-// [n k] (0 where an entry is not listed) and, after it, coef [n k], what the
+// [n k] (0 where an entry is not listed) and coef [n k], what the
 // gradient subtracts at the entry's class: the sum over the entries that list
 // the class, at the first of them; -1 at every other entry.
 template <typename T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* __restrict__ hidden, int64_t ldh,
                                                            const T* __restrict__ w, int64_t ldw, const T* bias,
                                                            int64_t n, int64_t width, int32_t vec, float inv_t,
-                                                           float* __restrict__ prob,
+                                                           float* __restrict__ prob, float* __restrict__ coef,
                                                            float* __restrict__ y, int32_t* __restrict__ state) {
     const int lane = threadIdx.x & 63;
     const int groups = (t.k + 3) / 4;
@@ -996,7 +999,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
         }
         if (k < t.k) {
             prob[i * t.k + k] = q;
-            prob[(n + i) * t.k + k] = idx >= 0 && first ? sum : -1.f;
+            coef[i * t.k + k] = idx >= 0 && first ? sum : -1.f;
         }
     }
 }
@@ -1458,6 +1461,15 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
     finish_loss(part_loss, part_cnt, gridDim.x, lane, loss_out, counts);
 }
 
+// owner[rows[i]] = i, where the rows are packed a block at a time
+__global__ __launch_bounds__(256) void head_owner_kernel(const int64_t* __restrict__ rows, int64_t n,
+                                                         int64_t hidden_rows, int32_t* owner) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i < n ? rows[i] : -1;
+    if (row < 0 || row >= hidden_rows) return;
+    __hip_atomic_store(owner + row, (int32_t)i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Of a row that is listed again, all but one listing find another's number.
 __global__ __launch_bounds__(256) void head_repeated_kernel(const int64_t* __restrict__ rows, int64_t n,
                                                             int64_t hidden_rows, int32_t* owner) {
@@ -1562,10 +1574,12 @@ __global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __r
     }
 }
 
-// 16 waves share 64 columns
+// 16 waves share 64 columns.  sum: NULL, or [vc] of the blocks of rows before,
+// in their order (first: none); only the last block writes the gradient.
 template <typename T>
 __global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict__ part, int64_t nparts, int64_t vp,
                                                          int64_t vc, const float* __restrict__ alpha,
+                                                         float* __restrict__ sum, int32_t first, int32_t last,
                                                          T* __restrict__ out) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1581,7 +1595,9 @@ __global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict
     s = 0.f;
 #pragma unroll
     for (int w = 0; w < 16; ++w) s += red[w][lane];
-    out[c] = from_float<T>(s * *alpha);
+    if (!first) s += sum[c];
+    if (last) out[c] = from_float<T>(s * *alpha);
+    else sum[c] = s;
 }
 
 // Adds the splits' sums in order and applies alpha, 4 columns a lane: dW of a
@@ -1638,6 +1654,14 @@ constexpr int64_t kJoinBlocks = 128;
 // 256 MiB, 4.70 with 512 and 4.54 with 1 GiB (fewer, fuller launches); at
 // 8,192 x 131,072 x 4,096 it makes 1%.
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
+// Rows are taken in blocks where the scratch would otherwise grow with rows x
+// classes: the strips' statistics of a forward block stay within kPartBytes
+// (8 bytes a row and strip), and a backward block leaves G room for
+// kLeastPiece classes a piece.  At most kBlockRows rows, so that no launch
+// has 2^32 threads.
+constexpr int64_t kPartBytes = (int64_t)512 << 20;
+constexpr int64_t kLeastPiece = 4096;
+constexpr int64_t kBlockRows = (int64_t)1 << 20;
 constexpr int64_t kFewClasses = 1024;  // up to here G has a second plane
 // Rows up to which head_few_kernel makes the logits.  32,000 x 2,048, against
 // the products on packed W: f32 1 row 79 against 485 us, 64 rows 121 against
@@ -1676,11 +1700,12 @@ Plan plan(int64_t p, int64_t q, int64_t stages, int64_t most_splits, double besi
 // Sizes of a call, the same for the workspace query and the launch.
 struct Shape {
     int64_t n, D, V;
+    int64_t blocks, nb;  // blocks of rows, rows of a block
     int planes, gplanes;  // of the operands, of G
     bool split;       // f32 operands in three planes
     bool pack_w;      // W goes through a packed copy
     bool few;         // few rows: head_few_kernel makes the logits
-    int64_t np, dp, vp;  // padded rows and width; classes of a piece
+    int64_t np, dp, vp;  // padded rows of a block, and width; classes of a piece
     int64_t ldg;         // pitch of G: rows start 256 bytes apart mod 4 KiB
     Plan logits, weight, hidden;
     int64_t strips, strip_classes;  // the forward's
@@ -1704,16 +1729,30 @@ Shape shape_of(const grws_head* h, bool backward) {
     s.gplanes = s.split ? 3 : s.V <= kFewClasses ? 2 : 1;
     s.pack_w = !weight_in_place(h);
     s.few = s.n <= (s.split ? kFewF32 : s.pack_w ? kFewPacked : kFewRows);
-    s.np = pad(s.n);
     s.dp = up(s.D, kK);
     s.vp = pad(s.V);
+    int64_t rows = kBlockRows;
+    auto limit = [&](int64_t bytes, int64_t row_bytes) {
+        if (rows > bytes / row_bytes) rows = bytes / row_bytes;
+    };
+    limit(kPieceBytes, 2 * s.planes * s.dp);                                     // the packed rows
+    if (backward) limit(kPieceBytes, 2 * s.gplanes * ((s.vp < kLeastPiece ? s.vp : kLeastPiece) + 128));
+    else limit(kPartBytes, 8 * (s.vp / 64));
+    limit((int64_t)1 << 31, 64 * ceil_div(h->k, 4) + 1);                         // threads of head_targets_kernel
+    rows = rows < 256 ? 256 : rows / 256 * 256;
+    s.blocks = ceil_div(s.n, rows);
+    s.nb = s.blocks == 1 ? s.n : up(ceil_div(s.n, s.blocks), 256);
+    s.blocks = ceil_div(s.n, s.nb);
+    s.np = pad(s.nb);
     auto bound = [&](int64_t bytes, int64_t column_bytes) {
         int64_t most = bytes / column_bytes / 256 * 256;
         if (most < 256) most = 256;
         if (s.vp > most) s.vp = most;
     };
     if (backward) bound(kPieceBytes, 2 * s.gplanes * s.np);
+    if (backward && s.blocks > 1) bound(kPieceBytes, 4 * s.dp);  // dW's sums over the blocks
     if (s.pack_w) bound(kPackBytes, 2 * s.planes * s.dp);
+    bound((int64_t)1 << 29, 1);  // a launch's threads
     const int64_t seg = s.split ? 6 : 1, gseg = s.split ? 6 : s.gplanes;
     // the pieces: as few and as equal as the bound allows, or up to three
     // more where the tiles then fill the rounds better
@@ -1726,7 +1765,7 @@ Shape shape_of(const grws_head* h, bool backward) {
         Plan w{}, d{};
         if (backward) {
             w = plan(s.D, vp, gseg * s.np / kK, ceil_div(s.np / kK, 4), 4);
-            d = plan(s.dp, s.np, gseg * vp / kK, ceil_div(vp / kK, 4), 4);
+            d = plan(s.dp, s.np, gseg * vp / kK, s.blocks > 1 ? 1 : ceil_div(vp / kK, 4), 4);
         }
         const double t = (double)ceil_div(s.V, vp) * (l.cost + w.cost + d.cost + 6);
         if (t < least) {
@@ -1748,6 +1787,33 @@ Shape shape_of(const grws_head* h, bool backward) {
     s.strips = pad(s.V) / s.strip_classes;
     s.ldg = s.vp + 128;
     return s;
+}
+
+// Rows r0.. of a call (n of them) as a call of their own.
+grws_head rows_of(const grws_head* h, int64_t r0, int64_t n) {
+    grws_head b = *h;
+    b.n = n;
+    if (h->rows) {
+        b.rows += r0;
+    } else {
+        b.hidden = static_cast<const char*>(h->hidden) + r0 * h->ld_hidden * dtype_size(h->dtype);
+        b.hidden_rows -= r0;
+    }
+    if (h->k == 0) {
+        b.labels += r0;
+    } else {
+        b.teacher_index = static_cast<const char*>(h->teacher_index) + r0 * h->k * (h->index_is_i64 ? 8 : 4);
+        b.teacher_logits += r0 * h->k;
+    }
+    return b;
+}
+
+// The shape of a call's block of rows from r0 on.
+Shape block_of(const Shape& s, int64_t r0) {
+    Shape b = s;
+    b.n = s.n - r0 < s.nb ? s.n - r0 : s.nb;
+    if (s.blocks > 1) b.np = up(b.n, 256);
+    return b;
 }
 
 int check_head(const grws_head* h) {
@@ -1797,7 +1863,7 @@ void fwd_space(A& a, const Shape& s, FwdSpace* f) {
     if (!s.few) take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w && !s.few) take(f->wp, s.planes * s.vp * s.dp);
     take(f->part, s.strips * s.np);
-    take(f->flags, s.n);
+    take(f->flags, s.nb);
     take(f->pl, s.n <= 8 ? 8 : ceil_div(s.n, 4));
     take(f->pc, s.n <= 8 ? 24 : 3 * ceil_div(s.n, 4));
     take(f->done, 1);
@@ -1805,7 +1871,7 @@ void fwd_space(A& a, const Shape& s, FwdSpace* f) {
 
 struct BwdSpace {
     uint16_t *hp, *wp, *G;
-    float *dh, *dw, *bias, *alpha, *scale;
+    float *dh, *dw, *bias, *bias_sum, *alpha, *scale;
     uint32_t* most;
     int32_t* owner;  // see listed_again
 };
@@ -1820,9 +1886,11 @@ void bwd_space(A& a, const Shape& s, const grws_head* h, BwdSpace* f) {
     take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w && !(s.few && s.split)) take(f->wp, s.planes * s.vp * s.dp);
     take(f->G, s.gplanes * s.np * s.ldg);
-    if (s.hidden.splits > 1 || s.vp < s.V) take(f->dh, s.hidden.splits * s.np * s.dp);
-    if (s.weight.splits > 1) take(f->dw, s.weight.splits * s.vp * s.dp);
+    // several pieces: of all rows; several runs (of one block only): of each
+    if (s.hidden.splits > 1 || s.vp < s.V) take(f->dh, s.hidden.splits * s.blocks * s.np * s.dp);
+    if (s.weight.splits > 1 || s.blocks > 1) take(f->dw, s.weight.splits * s.vp * s.dp);
     take(f->bias, s.np / kBiasRows * s.vp);
+    if (s.blocks > 1) take(f->bias_sum, s.vp);
     take(f->alpha, 1);
     take(f->scale, s.n);
     take(f->most, 1);
@@ -1909,7 +1977,7 @@ int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
 // NAME<..., BP, BQ, WP, WQ> at a plan's tile
 #define GRWS_HEAD_LAUNCH(PLAN, NAME, ARGS, ...)                                                                      \
     do {                                                                                                             \
-        GRWS_CHECK_ARG((int64_t)ARGS.g.tp * ARGS.g.tq < INT32_MAX, "head: more than 2^31 tiles");                    \
+        GRWS_CHECK_ARG((int64_t)ARGS.g.tp * ARGS.g.tq * 512 < (int64_t)1 << 32, "head: 2^32 threads or more");       \
         const dim3 grid_((unsigned)(ARGS.g.tp * ARGS.g.tq), (unsigned)ARGS.g.splits);                                \
         if (PLAN.tile == 256)                                                                                        \
             hipLaunchKernelGGL((NAME<__VA_ARGS__, 256, 256, 2, 4>), grid_, dim3(512), 0, stream, ARGS);              \
@@ -1917,6 +1985,128 @@ int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
             hipLaunchKernelGGL((NAME<__VA_ARGS__, 128, 128, 2, 2>), grid_, dim3(256), 0, stream, ARGS);              \
         GRWS_LAUNCH_CHECK();                                                                                         \
     } while (0)
+
+// G of a piece of the classes and a block of the rows, and what the two
+// products add of it to dW and dH.
+int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_t v0, int64_t vc, int64_t r0,
+                   RowStats all_stats, const float* target_logit, const float* target_prob, bool per_row,
+                   const Alpha& alpha, const int32_t* owner, float c1, float gscale, void* d_hidden, int64_t ld_dh,
+                   void* d_weight, int64_t ld_dw, void* d_bias, hipStream_t stream) {
+    const Shape sb = block_of(s, r0);
+    const grws_head hb = rows_of(h, r0, sb.n);
+    const Targets t = targets_of(&hb);
+    const size_t esz = dtype_size(h->dtype);
+    const RowStats stats = all_stats + r0;
+    const float* row_scale = per_row ? f.scale + r0 : nullptr;
+    const bool first_rows = r0 == 0, last_rows = r0 + sb.n == s.n;
+    const int64_t plane = sb.np * s.ldg;
+    const int64_t vt = up(vc, s.few ? 128 : s.logits.tile);  // G's columns that are written
+    if (s.blocks > 1) GRWS_TRY(pack_hidden(&hb, sb, t, f.hp, alpha, nullptr, nullptr, stream));
+    Opnd W;
+#define GRWS_HEAD_PLANES(X)                                  \
+    do {                                                     \
+        if (s.split) X(GRWS_BF16, 3);                        \
+        else if (h->dtype == GRWS_F16 && s.gplanes == 1) X(GRWS_F16, 1); \
+        else if (h->dtype == GRWS_F16) X(GRWS_F16, 2);       \
+        else if (s.gplanes == 1) X(GRWS_BF16, 1);            \
+        else X(GRWS_BF16, 2);                                \
+    } while (0)
+    if (s.few) {
+        FewArgs a{};
+        a.t = t;
+        a.hidden = h->hidden, a.weight = h->weight, a.bias = h->bias;
+        a.ldh = h->ld_hidden, a.ldw = h->ld_weight, a.n = s.n, a.np = s.np, a.width = s.D;
+        a.v0 = v0, a.vend = v0 + vc, a.classes = s.V, a.c1 = c1;
+        a.stats = stats, a.row_scale = row_scale, a.gscale = gscale, a.G = f.G, a.ldg = s.ldg, a.plane = plane;
+        a.bias_part = d_bias && h->k == 0 ? f.bias : nullptr, a.vt = vt;
+        if (s.split) GRWS_TRY((launch_few<float, 3>(h, a, stream)));
+        else if (h->dtype == GRWS_F16 && s.gplanes == 1) GRWS_TRY((launch_few<_Float16, 1>(h, a, stream)));
+        else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 2>(h, a, stream)));
+        else if (s.gplanes == 1) GRWS_TRY((launch_few<__hip_bfloat16, 1>(h, a, stream)));
+        else GRWS_TRY((launch_few<__hip_bfloat16, 2>(h, a, stream)));
+    } else {
+        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, first_rows, stream));
+        GradArgs a{gemm_of(s, s.logits, W, hidden_operand(sb, f.hp, false), vc, sb.np, s.dp, s.planes),
+                   v0, s.V, sb.n, c1, h->bias,
+                   h->dtype, stats, hb.labels, row_scale, gscale, f.G, s.ldg, plane,
+                   d_bias && h->k == 0 ? f.bias : nullptr, vt};
+#define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
+        GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
+#undef GRWS_HEAD_GRAD
+    }
+    if (h->k > 0) {
+        const dim3 grid((unsigned)ceil_div(sb.n * h->k, 256));
+        const float *y = target_logit + r0 * h->k, *coef = target_prob + (s.n + r0) * h->k;
+#define GRWS_HEAD_SUB(DT, PL)                                                                                      \
+    hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, stats, y, coef, row_scale, gscale, \
+                       c1, sb.n, v0, vc, f.G, s.ldg, plane)
+        GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
+#undef GRWS_HEAD_SUB
+        GRWS_LAUNCH_CHECK();
+    }
+    const char* gp = reinterpret_cast<const char*>(f.G);
+    if (d_bias) {
+        const int64_t nparts = sb.np / kBiasRows;
+        if (h->k > 0) {  // with labels head_grad_kernel has made the parts
+            const dim3 grid((unsigned)nparts, (unsigned)ceil_div(vt, 512));
+#define GRWS_HEAD_BIAS_PART(DT, PL)                                                                               \
+    hipLaunchKernelGGL((head_bias_part_kernel<DT, PL>), grid, dim3(256), 0, stream, f.G, s.ldg, plane, vt, f.bias)
+            GRWS_HEAD_PLANES(GRWS_HEAD_BIAS_PART);
+#undef GRWS_HEAD_BIAS_PART
+            GRWS_LAUNCH_CHECK();
+        }
+        const dim3 cg((unsigned)ceil_div(vc, 64));
+        char* db = static_cast<char*>(d_bias) + v0 * esz;
+#define GRWS_HEAD_BIAS(T)                                                                               \
+    hipLaunchKernelGGL(head_bias_kernel<T>, cg, dim3(1024), 0, stream, f.bias, nparts, vt, vc, f.alpha, \
+                       f.bias_sum, first_rows, last_rows, reinterpret_cast<T*>(db))
+        if (h->dtype == GRWS_F32) GRWS_HEAD_BIAS(float);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS(_Float16);
+        else GRWS_HEAD_BIAS(__hip_bfloat16);
+#undef GRWS_HEAD_BIAS
+        GRWS_LAUNCH_CHECK();
+    }
+#undef GRWS_HEAD_PLANES
+    if (d_weight) {
+        char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
+        const int32_t vec = reinterpret_cast<uintptr_t>(d_weight) % (4 * esz) == 0 && ld_dw % 4 == 0;
+        const Opnd G{gp, s.ldg * 2, plane * 2, s.ldg, sb.np};
+        WeightArgs w{gemm_of(s, s.weight, hidden_operand(sb, f.hp, true), G, s.D, vc, sb.np, s.gplanes),
+                     f.alpha, out, ld_dw, vc, s.D, vec, s.weight.splits > 1 || s.blocks > 1 ? f.dw : nullptr,
+                     s.vp, s.dp, first_rows};
+        if (s.split) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_F16, GRWS_F16);
+        else GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_BF16);
+    }
+    if (d_hidden && s.few && s.split) {
+        const FewHiddenArgs d{static_cast<const float*>(h->weight) + v0 * h->ld_weight, h->ld_weight, s.D, s.dp, s.n,
+                              s.np, vc, f.G, s.ldg, plane, f.dh, (int32_t)s.hidden.splits, v0 == 0};
+        const bool vec = rows_of_16(h->weight, h->ld_weight, h->dtype);
+        const dim3 grid((unsigned)(s.dp / 64), (unsigned)ceil_div(s.hidden.splits, 4), (unsigned)ceil_div(s.n, 64));
+#define GRWS_HEAD_FEW_DH(NQ)                                                                                     \
+    do {                                                                                                         \
+        if (vec) hipLaunchKernelGGL((head_few_dhidden_kernel<NQ, true>), grid, dim3(256), 0, stream, d);          \
+        else hipLaunchKernelGGL((head_few_dhidden_kernel<NQ, false>), grid, dim3(256), 0, stream, d);             \
+    } while (0)
+        if (s.n <= 16) GRWS_HEAD_FEW_DH(1);
+        else if (s.n <= 32) GRWS_HEAD_FEW_DH(2);
+        else GRWS_HEAD_FEW_DH(4);
+#undef GRWS_HEAD_FEW_DH
+        GRWS_LAUNCH_CHECK();
+    } else if (d_hidden) {
+        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, s.few, stream));
+        const Opnd G{gp, s.ldg * 2, plane * 2, sb.np, vt};
+        char* out = static_cast<char*>(d_hidden) + (h->rows ? 0 : r0 * ld_dh * esz);
+        const int32_t vec = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ld_dh % 4 == 0;
+        HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, sb.np, vc, s.gplanes), f.dh + (s.vp < s.V ? r0 * s.dp : 0),
+                     sb.np, s.dp, v0 == 0, s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, out, ld_dh, sb.n, s.D,
+                     hb.hidden_rows, hb.rows, stats, owner};
+        if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
+        else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
+    }
+    return GRWS_OK;
+}
 
 }  // namespace
 }  // namespace grws
@@ -1946,61 +2136,81 @@ extern "C" int grws_head_fwd(const grws_head* h, float* row_stats, float* target
     }
     GRWS_CHECK_ARG(row_stats && target_logit && (h->k == 0 || target_prob), "head: null output");
     const Shape s = shape_of(h, false);
-    const Targets t = targets_of(h);
     Carver cv(workspace, workspace_bytes);
     FwdSpace f{};
     fwd_space(cv, s, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
-    if (h->k > 0) {
-        const dim3 grid((unsigned)ceil_div(s.n * ((h->k + 3) / 4), 4));
-        const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype) &&
-                            rows_of_16(h->weight, h->ld_weight, h->dtype);
-#define GRWS_HEAD_TARGETS(T)                                                                                         \
-    hipLaunchKernelGGL(head_targets_kernel<T>, grid, dim3(256), 0, stream, t, static_cast<const T*>(h->hidden),      \
+    const int64_t join_rows = s.n <= 8 ? 1 : s.n <= 512 ? 4 : 16, joins = ceil_div(s.n, join_rows);
+    const bool one = s.blocks == 1 && joins <= kJoinBlocks;
+    for (int64_t r0 = 0; r0 < s.n; r0 += s.nb) {
+        const Shape sb = block_of(s, r0);
+        const grws_head hb = rows_of(h, r0, sb.n);
+        const Targets t = targets_of(&hb);
+        float* y = target_logit + r0 * (h->k > 0 ? h->k : 1);
+        float* prob = h->k > 0 ? target_prob + r0 * h->k : nullptr;
+        if (h->k > 0) {
+            const dim3 grid((unsigned)ceil_div(sb.n * ((h->k + 3) / 4), 4));
+            const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype) &&
+                                rows_of_16(h->weight, h->ld_weight, h->dtype);
+#define GRWS_HEAD_TARGETS(T)                                                                                        \
+    hipLaunchKernelGGL(head_targets_kernel<T>, grid, dim3(256), 0, stream, t, static_cast<const T*>(hb.hidden),     \
                        h->ld_hidden, static_cast<const T*>(h->weight), h->ld_weight, static_cast<const T*>(h->bias), \
-                       s.n, s.D, vec, 1.f / h->temperature, target_prob, target_logit, f.flags)
-        if (h->dtype == GRWS_F32) GRWS_HEAD_TARGETS(float);
-        else if (h->dtype == GRWS_F16) GRWS_HEAD_TARGETS(_Float16);
-        else GRWS_HEAD_TARGETS(__hip_bfloat16);
+                       sb.n, s.D, vec, 1.f / h->temperature, prob, prob + s.n * h->k, y, f.flags)
+            if (h->dtype == GRWS_F32) GRWS_HEAD_TARGETS(float);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_TARGETS(_Float16);
+            else GRWS_HEAD_TARGETS(__hip_bfloat16);
 #undef GRWS_HEAD_TARGETS
-        GRWS_LAUNCH_CHECK();
-    }
-    if (s.few) {
-        FewArgs a{t, h->hidden, h->weight, h->bias, h->ld_hidden, h->ld_weight, s.n, s.np, s.D, 0, s.V, s.V, c1,
-                  f.flags, f.part, target_logit, f.flags, f.done};
-        a.vt = pad(s.V);
-        if (h->dtype == GRWS_F32) GRWS_TRY((launch_few<float, 0>(h, a, stream)));
-        else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 0>(h, a, stream)));
-        else GRWS_TRY((launch_few<__hip_bfloat16, 0>(h, a, stream)));
-    } else {
-        GRWS_TRY(pack_hidden(h, s, t, f.hp, Alpha{}, f.done, nullptr, stream));
-    }
-    for (int64_t v0 = 0; v0 < s.V && !s.few; v0 += s.vp) {
-        const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
-        Opnd W;
-        GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-        StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes),
-                    v0, s.V, s.n, s.np, c1,
-                    h->bias, h->dtype, h->labels, f.part, target_logit, f.flags};
-        if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
-        else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
-    }
-    const int64_t rows = s.n <= 8 ? 1 : s.n <= 512 ? 4 : 16, blocks = ceil_div(s.n, rows);
+            GRWS_LAUNCH_CHECK();
+        }
+        if (s.few) {
+            FewArgs a{t, h->hidden, h->weight, h->bias, h->ld_hidden, h->ld_weight, s.n, s.np, s.D, 0, s.V, s.V, c1,
+                      f.flags, f.part, y, f.flags, f.done};
+            a.vt = pad(s.V);
+            if (h->dtype == GRWS_F32) GRWS_TRY((launch_few<float, 0>(h, a, stream)));
+            else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 0>(h, a, stream)));
+            else GRWS_TRY((launch_few<__hip_bfloat16, 0>(h, a, stream)));
+        } else {
+            GRWS_TRY(pack_hidden(&hb, sb, t, f.hp, Alpha{}, f.done, nullptr, stream));
+        }
+        for (int64_t v0 = 0; v0 < s.V && !s.few; v0 += s.vp) {
+            const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
+            Opnd W;
+            // W in one piece stays packed for the blocks to come
+            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, r0 == 0 || s.vp < s.V, stream));
+            StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(sb, f.hp, false), vc, sb.np, s.dp, s.planes),
+                        v0, s.V, sb.n, sb.np, c1,
+                        h->bias, h->dtype, hb.labels, f.part, y, f.flags};
+            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
+            else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
+        }
+        const int64_t at = r0 / join_rows;  // blocks are multiples of 256 rows
 #define GRWS_HEAD_JOIN(R)                                                                                            \
-    hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)blocks), dim3(512), 0, stream, t, f.part,                 \
-                       ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, s.n, s.np, h->temperature, c1,      \
-                       target_logit, target_prob, f.flags, reinterpret_cast<float2*>(row_stats), row_loss, f.pl, f.pc, \
-                       blocks <= kJoinBlocks ? f.done : nullptr, loss, counts)
-    if (rows == 1) GRWS_HEAD_JOIN(1);
-    else if (rows == 4) GRWS_HEAD_JOIN(4);
-    else GRWS_HEAD_JOIN(16);
+    hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)ceil_div(sb.n, R)), dim3(512), 0, stream, t, f.part,      \
+                       ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, sb.n, sb.np, h->temperature, c1, y, \
+                       prob, f.flags, reinterpret_cast<float2*>(row_stats) + r0, row_loss ? row_loss + r0 : nullptr, \
+                       f.pl + at, f.pc + 3 * at, one ? f.done : nullptr, loss, counts)
+        if (join_rows == 1) GRWS_HEAD_JOIN(1);
+        else if (join_rows == 4) GRWS_HEAD_JOIN(4);
+        else GRWS_HEAD_JOIN(16);
 #undef GRWS_HEAD_JOIN
-    GRWS_LAUNCH_CHECK();
-    if (blocks > kJoinBlocks) {
-        hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(64), 0, stream, f.pl, f.pc, blocks, loss, counts);
         GRWS_LAUNCH_CHECK();
     }
+    if (!one) {
+        hipLaunchKernelGGL(head_finish_kernel, dim3(1), dim3(64), 0, stream, f.pl, f.pc, joins, loss, counts);
+        GRWS_LAUNCH_CHECK();
+    }
+    return GRWS_OK;
+}
+
+extern "C" int grws_head_plan(const grws_head* h, int32_t backward, int64_t* out) {
+    clear_error();
+    GRWS_TRY(check_head(h));
+    GRWS_CHECK_ARG(out && h->n > 0, "head: nothing to plan");
+    const Shape s = shape_of(h, backward != 0);
+    const int64_t v[GRWS_HEAD_PLAN] = {s.blocks, s.nb, ceil_div(s.V, s.vp), s.vp, s.few, s.few ? 0 : s.logits.tile,
+                                       s.weight.tile, s.weight.splits, s.hidden.tile, s.hidden.splits};
+    for (int i = 0; i < GRWS_HEAD_PLAN; ++i) out[i] = v[i];
     return GRWS_OK;
 }
 
@@ -2034,16 +2244,13 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
     GRWS_CHECK_ARG(row_stats && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
     if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
     const Shape s = shape_of(h, true);
-    const Targets t = targets_of(h);
     Carver cv(workspace, workspace_bytes);
     BwdSpace f{};
     bwd_space(cv, s, h, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
     const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
-    const float* coef = target_prob ? target_prob + s.n * h->k : nullptr;
     const RowStats stats = reinterpret_cast<RowStats>(row_stats);
-    const float* row_scale = nullptr;
     if (per_row) {
         GRWS_TRY(fill_i32(reinterpret_cast<int32_t*>(f.most), 1, 0, stream));
         const dim3 grid((unsigned)ceil_div(s.n, 256));
@@ -2051,138 +2258,46 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
         GRWS_LAUNCH_CHECK();
         hipLaunchKernelGGL(head_row_scale_kernel, grid, dim3(256), 0, stream, dloss, stats, s.n, f.most, f.scale);
         GRWS_LAUNCH_CHECK();
-        row_scale = f.scale;
     }
     const Alpha alpha{f.alpha, dloss, counts, per_row ? f.most : nullptr, h->temperature / gscale};
     int32_t* owner = d_hidden ? f.owner : nullptr;
-    GRWS_TRY(pack_hidden(h, s, t, f.hp, alpha, nullptr, owner, stream));
+    if (s.blocks == 1) {
+        GRWS_TRY(pack_hidden(h, s, targets_of(h), f.hp, alpha, nullptr, owner, stream));
+    } else if (owner) {
+        hipLaunchKernelGGL(head_owner_kernel, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows, s.n,
+                           h->hidden_rows, owner);
+        GRWS_LAUNCH_CHECK();
+    }
     if (owner) {
         hipLaunchKernelGGL(head_repeated_kernel, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows, s.n,
                            h->hidden_rows, owner);
         GRWS_LAUNCH_CHECK();
     }
-    const int64_t plane = s.np * s.ldg;
     const size_t esz = dtype_size(h->dtype);
+    // pieces of the classes, and of each the blocks of rows: W's piece is
+    // packed once, dW's is complete after its blocks
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
-        const int64_t vt = up(vc, s.few ? 128 : s.logits.tile);  // G's columns that are written
-        Opnd W;
-#define GRWS_HEAD_PLANES(X)                                  \
-    do {                                                     \
-        if (s.split) X(GRWS_BF16, 3);                        \
-        else if (h->dtype == GRWS_F16 && s.gplanes == 1) X(GRWS_F16, 1); \
-        else if (h->dtype == GRWS_F16) X(GRWS_F16, 2);       \
-        else if (s.gplanes == 1) X(GRWS_BF16, 1);            \
-        else X(GRWS_BF16, 2);                                \
-    } while (0)
-        if (s.few) {
-            FewArgs a{};
-            a.t = t;
-            a.hidden = h->hidden, a.weight = h->weight, a.bias = h->bias;
-            a.ldh = h->ld_hidden, a.ldw = h->ld_weight, a.n = s.n, a.np = s.np, a.width = s.D;
-            a.v0 = v0, a.vend = v0 + vc, a.classes = s.V, a.c1 = c1;
-            a.stats = stats, a.row_scale = row_scale, a.gscale = gscale, a.G = f.G, a.ldg = s.ldg, a.plane = plane;
-            a.bias_part = d_bias && h->k == 0 ? f.bias : nullptr, a.vt = vt;
-            if (s.split) GRWS_TRY((launch_few<float, 3>(h, a, stream)));
-            else if (h->dtype == GRWS_F16 && s.gplanes == 1) GRWS_TRY((launch_few<_Float16, 1>(h, a, stream)));
-            else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 2>(h, a, stream)));
-            else if (s.gplanes == 1) GRWS_TRY((launch_few<__hip_bfloat16, 1>(h, a, stream)));
-            else GRWS_TRY((launch_few<__hip_bfloat16, 2>(h, a, stream)));
-        } else {
-            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, true, stream));
-            GradArgs a{gemm_of(s, s.logits, W, hidden_operand(s, f.hp, false), vc, s.np, s.dp, s.planes),
-                       v0, s.V, s.n, c1, h->bias,
-                       h->dtype, stats, h->labels, row_scale, gscale, f.G, s.ldg, plane,
-                       d_bias && h->k == 0 ? f.bias : nullptr, vt};
-#define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
-            GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
-#undef GRWS_HEAD_GRAD
-        }
-        if (h->k > 0) {
-            const dim3 grid((unsigned)ceil_div(s.n * h->k, 256));
-#define GRWS_HEAD_SUB(DT, PL)                                                                                 \
-    hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, stats, target_logit, coef, \
-                       row_scale, gscale, c1, s.n, v0, vc, f.G, s.ldg, plane)
-            GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
-#undef GRWS_HEAD_SUB
-            GRWS_LAUNCH_CHECK();
-        }
-        const char* gp = reinterpret_cast<const char*>(f.G);
-        if (d_bias) {
-            const int64_t nparts = s.np / kBiasRows;
-            if (h->k > 0) {  // with labels head_grad_kernel has made the parts
-                const dim3 grid((unsigned)nparts, (unsigned)ceil_div(vt, 512));
-#define GRWS_HEAD_BIAS_PART(DT, PL)                                                                               \
-    hipLaunchKernelGGL((head_bias_part_kernel<DT, PL>), grid, dim3(256), 0, stream, f.G, s.ldg, plane, vt, f.bias)
-                GRWS_HEAD_PLANES(GRWS_HEAD_BIAS_PART);
-#undef GRWS_HEAD_BIAS_PART
-                GRWS_LAUNCH_CHECK();
-            }
-            const dim3 cg((unsigned)ceil_div(vc, 64));
-            char* db = static_cast<char*>(d_bias) + v0 * esz;
-#define GRWS_HEAD_BIAS(T) \
-    hipLaunchKernelGGL(head_bias_kernel<T>, cg, dim3(1024), 0, stream, f.bias, nparts, vt, vc, f.alpha, \
-                       reinterpret_cast<T*>(db))
-            if (h->dtype == GRWS_F32) GRWS_HEAD_BIAS(float);
-            else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS(_Float16);
-            else GRWS_HEAD_BIAS(__hip_bfloat16);
-#undef GRWS_HEAD_BIAS
-            GRWS_LAUNCH_CHECK();
-        }
-        if (d_weight) {
+        for (int64_t r0 = 0; r0 < s.n; r0 += s.nb)
+            GRWS_TRY(backward_block(h, s, f, v0, vc, r0, stats, target_logit, target_prob, per_row, alpha, owner, c1,
+                                    gscale, d_hidden, ld_dh, d_weight, ld_dw, d_bias, stream));
+        if (d_weight && (s.weight.splits > 1 || s.blocks > 1)) {
             char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
-            const int32_t vec = reinterpret_cast<uintptr_t>(d_weight) % (4 * esz) == 0 && ld_dw % 4 == 0;
-            const Opnd G{gp, s.ldg * 2, plane * 2, s.ldg, s.np};
-            WeightArgs w{gemm_of(s, s.weight, hidden_operand(s, f.hp, true), G, s.D, vc, s.np, s.gplanes),
-                         f.alpha, out, ld_dw,
-                         vc, s.D, vec, f.dw, s.vp, s.dp};
-            if (s.split) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
-            else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_F16, GRWS_F16);
-            else GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_BF16);
-            if (s.weight.splits > 1) {
 #define GRWS_HEAD_DW(T)                                                                                             \
     hipLaunchKernelGGL(head_weight_out_kernel<T>, dim3((unsigned)vc), dim3(256), 0, stream, f.dw, s.weight.splits,  \
                        s.vp, s.dp, s.D, f.alpha, reinterpret_cast<T*>(out), ld_dw)
-                if (h->dtype == GRWS_F32) GRWS_HEAD_DW(float);
-                else if (h->dtype == GRWS_F16) GRWS_HEAD_DW(_Float16);
-                else GRWS_HEAD_DW(__hip_bfloat16);
+            if (h->dtype == GRWS_F32) GRWS_HEAD_DW(float);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_DW(_Float16);
+            else GRWS_HEAD_DW(__hip_bfloat16);
 #undef GRWS_HEAD_DW
-                GRWS_LAUNCH_CHECK();
-            }
-        }
-        if (d_hidden && s.few && s.split) {
-            const FewHiddenArgs d{static_cast<const float*>(h->weight) + v0 * h->ld_weight, h->ld_weight, s.D, s.dp, s.n,
-                                  s.np, vc, f.G, s.ldg, plane, f.dh, (int32_t)s.hidden.splits, v0 == 0};
-            const bool vec = rows_of_16(h->weight, h->ld_weight, h->dtype);
-            const dim3 grid((unsigned)(s.dp / 64), (unsigned)ceil_div(s.hidden.splits, 4),
-                            (unsigned)ceil_div(s.n, 64));
-#define GRWS_HEAD_FEW_DH(NQ)                                                                                     \
-    do {                                                                                                         \
-        if (vec) hipLaunchKernelGGL((head_few_dhidden_kernel<NQ, true>), grid, dim3(256), 0, stream, d);          \
-        else hipLaunchKernelGGL((head_few_dhidden_kernel<NQ, false>), grid, dim3(256), 0, stream, d);             \
-    } while (0)
-            if (s.n <= 16) GRWS_HEAD_FEW_DH(1);
-            else if (s.n <= 32) GRWS_HEAD_FEW_DH(2);
-            else GRWS_HEAD_FEW_DH(4);
-#undef GRWS_HEAD_FEW_DH
             GRWS_LAUNCH_CHECK();
-        } else if (d_hidden) {
-            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, true, &W, s.few, stream));
-            const Opnd G{gp, s.ldg * 2, plane * 2, s.np, vt};
-            const int32_t vec = reinterpret_cast<uintptr_t>(d_hidden) % (4 * esz) == 0 && ld_dh % 4 == 0;
-            HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, s.np, vc, s.gplanes), f.dh, s.np, s.dp, v0 == 0,
-                         s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, d_hidden, ld_dh, s.n, s.D,
-                         h->hidden_rows, h->rows, stats, owner};
-            if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
-            else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
-            else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
         }
     }
-#undef GRWS_HEAD_PLANES
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
-                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, owner, f.alpha, static_cast<T*>(d_hidden), ld_dh)
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, owner, f.alpha,         \
+                       static_cast<T*>(d_hidden), ld_dh)
         if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
         else GRWS_HEAD_DH(__hip_bfloat16);

@@ -871,6 +871,13 @@ size_t grws_head_fwd_workspace_bytes(const grws_head* head);
 int grws_head_fwd(const grws_head* head, float* row_stats, float* target_logit, float* target_prob, float* row_loss,
                   float* loss, int64_t* counts, void* workspace, size_t workspace_bytes, void* stream);
 size_t grws_head_bwd_workspace_bytes(const grws_head* head);
+/* How a call is cut up, for reports and tests (host only): {blocks of rows, */
+/* rows of one, pieces of the classes, classes of one, whether the kernels   */
+/* of few rows make the logits, tile of the logits' product (0: those),      */
+/* tile and runs along k of dW's, tile and runs of dH's}; the last four of   */
+/* the backward only.                                                        */
+#define GRWS_HEAD_PLAN 10
+int grws_head_plan(const grws_head* head, int32_t backward, int64_t* out);
 int grws_head_bwd(const grws_head* head, const float* row_stats, const float* target_logit, const float* target_prob,
                   const int64_t* counts, const float* dloss, int32_t per_row, void* d_hidden, int64_t ld_dh,
                   void* d_weight, int64_t ld_dw, void* d_bias, void* workspace, size_t workspace_bytes,

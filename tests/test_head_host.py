@@ -106,3 +106,45 @@ def test_products_use_no_scratch(tmp_path):
     for k, v in kernels.items():
         assert v.get("private_segment_fixed_size", 0) == 0 and v.get("vgpr_spill_count", 0) == 0, f"{k}: {v}"
         assert v["vgpr_count"] <= 256, f"{k} leaves fewer than two waves per SIMD: {v}"
+
+
+@pytest.mark.parametrize("dtype", [L.GRWS_F32, L.GRWS_F16, L.GRWS_BF16])
+@pytest.mark.parametrize("k", [0, 32])
+def test_both_workspaces_are_bounded_in_rows_and_classes(dtype, k):
+    """What grows with rows x classes is taken in blocks of rows and pieces of
+    classes: 1 GiB of G, 1 of packed rows, half of statistics, 0.25 of packed
+    weight, 0.27 of runs at most; beyond it the scratch grows with the hidden
+    rows (their f32 sums) and with nothing else."""
+    lib = L.load()
+    for n, width, classes in [(100, 64, 1000), (8192, 4096, 131072), (30000, 1024, 1000000), (1, 4096, 2000000),
+                              (2449029, 100, 47), (2449029, 256, 100003), (1600000, 256, 131072), (111059956, 128, 172),
+                              (50000, 65536, 50000), (300, 65536, 2000000000), (20000000, 8, 1000)]:
+        h = _head(n=n, hidden_rows=n, width=width, ld_hidden=width, ld_weight=width, classes=classes, dtype=dtype)
+        if k:
+            h = _head(n=n, hidden_rows=n, width=width, ld_hidden=width, ld_weight=width, classes=classes, dtype=dtype,
+                      k=k, labels=None, teacher_index=8, teacher_logits=8)
+        padded = (width + 63) // 64 * 64
+        # 256 rows are the least, and a row has a loss of its own in the join
+        fwd = 7 << 28 if 8 * classes // 64 * 256 < 1 << 29 else (5 << 28) + 8 * classes // 64 * 256 + (1 << 20)
+        assert lib.grws_head_fwd_workspace_bytes(ctypes.byref(h)) <= fwd + 8 * n
+        assert lib.grws_head_bwd_workspace_bytes(ctypes.byref(h)) <= (4 << 30) + n * (4 + 4 * padded)
+
+
+def _plan(backward, **kw):
+    out = (ctypes.c_int64 * 10)()
+    assert L.load().grws_head_plan(ctypes.byref(_head(**kw)), backward, out) == L.GRWS_OK
+    return list(out)
+
+
+def test_blocks_of_rows_cover_the_rows():
+    for n in (1, 128, 129, 300, 100000, 5000001, 2 ** 31 - 1):
+        for classes in (1, 47, 5000, 10 ** 6):
+            for backward in (0, 1):
+                blocks, rows, pieces, some = _plan(backward, n=n, hidden_rows=n, classes=classes)[:4]
+                assert (blocks - 1) * rows < n <= blocks * rows and (blocks == 1 or rows % 256 == 0)
+                assert (pieces - 1) * some < classes <= pieces * some and some % 128 == 0
+                assert rows <= 1 << 20
+    lib = L.load()
+    out = (ctypes.c_int64 * 10)()
+    assert lib.grws_head_plan(ctypes.byref(_head(n=0)), 0, out) == L.GRWS_E_INVALID
+    assert lib.grws_head_plan(ctypes.byref(_head()), 0, None) == L.GRWS_E_INVALID
