@@ -403,6 +403,8 @@ __global__ __launch_bounds__(kT) void top_join_kernel(const T* __restrict__ logi
     write_best(p, k, bits, class_bits, logits + r * ld, values + r * k, index + r * k);
 }
 
+constexpr int64_t kMostRows = 1 << 23;  // of a launch (they need no stretches)
+
 // Stretches of a row: one when the rows alone fill the chip (4 work-groups
 // on each of 256 CUs), else as many as that takes, of at least 4,096 logits
 // and 4 k.
@@ -442,6 +444,15 @@ extern "C" int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, in
     GRWS_CHECK_ARG(logits && values && index, "top_logits: null pointer");
     int32_t class_bits = 1;
     while ((1ll << class_bits) < classes) ++class_bits;
+    if (rows > kMostRows) {  // a work-group of 256 a row: 2^32 threads are not launched
+        const size_t e = dtype_size(dtype);
+        for (int64_t r = 0; r < rows; r += kMostRows)
+            GRWS_TRY(grws_top_logits(static_cast<const char*>(logits) + r * ld * e, dtype, ld,
+                                     rows - r < kMostRows ? rows - r : kMostRows, classes, k,
+                                     static_cast<char*>(values) + r * k * e, index + r * k, workspace,
+                                     workspace_bytes, stream_));
+        return GRWS_OK;
+    }
     if (classes <= kWaveClasses && k <= kWaveK) {
         const dim3 blocks((unsigned)((rows + kWaves - 1) / kWaves));
 #define GRWS_TOP_WAVE(T, PER)                                                                                    \
