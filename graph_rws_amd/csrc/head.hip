@@ -1518,12 +1518,19 @@ __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __rest
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.
 // (A label's place is known to the product's epilogue: one for a row.)
+// sums (or NULL): the classes' sums of q in units of 2^-31, whole numbers, so
+// that the order of the atomics does not matter; with the p that the epilogue
+// has summed they make the bias gradient of unrounded p - q.  What is not
+// finite goes into the class's sum of p instead.
+constexpr float kSumUnit = 2147483648.f;
 template <int DT, int PLANES>
 __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats stats,
                                                             const float* __restrict__ y,
                                                             const float* __restrict__ coef,
                                                             const float* __restrict__ row_scale, float gscale,
-                                                            float c1, int64_t n, int64_t v0, int64_t vc, uint16_t* G,
+                                                            float c1, int64_t n, int64_t v0, int64_t vc,
+                                                            unsigned long long* sums, float* bias_part, int64_t vt,
+                                                            uint16_t* G,
                                                             int64_t ldg, int64_t plane) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (at >= n * t.k) return;
@@ -1537,49 +1544,22 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats 
     planes_of<DT, PLANES>((exp2f(fmaf(y[at], c, -(m * c))) * stats[i].y - q) * s, h);
 #pragma unroll
     for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
-}
-
-// Column sums of a piece of G over runs of kBiasRows rows, 4 waves of 16 rows,
-// 8 columns a lane: after head_subtract_kernel (with labels the gradient
-// product's epilogue has made them).
-
-template <int DT, int PLANES>
-__global__ __launch_bounds__(256) void head_bias_part_kernel(const uint16_t* __restrict__ G, int64_t ldg,
-                                                             int64_t plane, int64_t vp, float* __restrict__ part) {
-    __shared__ float red[4][512];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.y * 512 + lane * 8;
-    const int64_t r0 = (int64_t)blockIdx.x * kBiasRows + wave * (kBiasRows / 4);
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < vp) {
-#pragma unroll 4
-        for (int64_t r = r0; r < r0 + kBiasRows / 4; ++r) {
-#pragma unroll
-            for (int z = PLANES - 1; z >= 0; --z) {
-                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(G + z * plane + r * ldg + c);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint16_t h = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-                    s[e] += from16<DT>(h);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) red[wave][lane * 8 + e] = s[e];
-    __syncthreads();
-    for (int x = threadIdx.x; x < 512; x += 256) {
-        const int64_t col = (int64_t)blockIdx.y * 512 + x;
-        if (col < vp) part[blockIdx.x * vp + col] = (red[0][x] + red[1][x]) + (red[2][x] + red[3][x]);
-    }
+    if (!sums) return;
+    const float u = row_scale ? q * row_scale[i] : q;
+    if (fabsf(u) < INFINITY)
+        atomicAdd(sums + (v - v0), (unsigned long long)__float2ll_rn(u * kSumUnit));
+    else
+        bias_part[i / kBiasRows * vt + (v - v0)] = __int_as_float(0x7fc00000);
 }
 
 // 16 waves share 64 columns.  sum: NULL, or [vc] of the blocks of rows before,
-// in their order (first: none); only the last block writes the gradient.
+// in their order (first: none); only the last block writes the gradient,
+// after taking off the targets' sums (NULL: they are in the parts).
 template <typename T>
 __global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict__ part, int64_t nparts, int64_t vp,
                                                          int64_t vc, const float* __restrict__ alpha,
                                                          float* __restrict__ sum, int32_t first, int32_t last,
+                                                         const int64_t* __restrict__ targets, float gscale,
                                                          T* __restrict__ out) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1596,6 +1576,7 @@ __global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict
 #pragma unroll
     for (int w = 0; w < 16; ++w) s += red[w][lane];
     if (!first) s += sum[c];
+    if (last && targets) s -= gscale * (float)((double)targets[c] / (double)kSumUnit);
     if (last) out[c] = from_float<T>(s * *alpha);
     else sum[c] = s;
 }
@@ -1873,6 +1854,7 @@ struct BwdSpace {
     uint16_t *hp, *wp, *G;
     float *dh, *dw, *bias, *bias_sum, *alpha, *scale;
     uint32_t* most;
+    int64_t* targets;  // see head_subtract_kernel
     int32_t* owner;  // see listed_again
 };
 
@@ -1894,6 +1876,7 @@ void bwd_space(A& a, const Shape& s, const grws_head* h, BwdSpace* f) {
     take(f->alpha, 1);
     take(f->scale, s.n);
     take(f->most, 1);
+    if (h->k > 0) take(f->targets, s.vp);
     if (h->rows) take(f->owner, h->hidden_rows);
 }
 
@@ -2018,7 +2001,7 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
         a.ldh = h->ld_hidden, a.ldw = h->ld_weight, a.n = s.n, a.np = s.np, a.width = s.D;
         a.v0 = v0, a.vend = v0 + vc, a.classes = s.V, a.c1 = c1;
         a.stats = stats, a.row_scale = row_scale, a.gscale = gscale, a.G = f.G, a.ldg = s.ldg, a.plane = plane;
-        a.bias_part = d_bias && h->k == 0 ? f.bias : nullptr, a.vt = vt;
+        a.bias_part = d_bias ? f.bias : nullptr, a.vt = vt;
         if (s.split) GRWS_TRY((launch_few<float, 3>(h, a, stream)));
         else if (h->dtype == GRWS_F16 && s.gplanes == 1) GRWS_TRY((launch_few<_Float16, 1>(h, a, stream)));
         else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 2>(h, a, stream)));
@@ -2029,7 +2012,7 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
         GradArgs a{gemm_of(s, s.logits, W, hidden_operand(sb, f.hp, false), vc, sb.np, s.dp, s.planes),
                    v0, s.V, sb.n, c1, h->bias,
                    h->dtype, stats, hb.labels, row_scale, gscale, f.G, s.ldg, plane,
-                   d_bias && h->k == 0 ? f.bias : nullptr, vt};
+                   d_bias ? f.bias : nullptr, vt};
 #define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
         GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
 #undef GRWS_HEAD_GRAD
@@ -2037,9 +2020,11 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
     if (h->k > 0) {
         const dim3 grid((unsigned)ceil_div(sb.n * h->k, 256));
         const float *y = target_logit + r0 * h->k, *coef = target_prob + (s.n + r0) * h->k;
+        auto* sums = d_bias ? reinterpret_cast<unsigned long long*>(f.targets) : nullptr;
+        if (sums && first_rows) GRWS_TRY(fill_i64(f.targets, vc, 0, stream));
 #define GRWS_HEAD_SUB(DT, PL)                                                                                      \
     hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, stats, y, coef, row_scale, gscale, \
-                       c1, sb.n, v0, vc, f.G, s.ldg, plane)
+                       c1, sb.n, v0, vc, sums, f.bias, vt, f.G, s.ldg, plane)
         GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
 #undef GRWS_HEAD_SUB
         GRWS_LAUNCH_CHECK();
@@ -2047,19 +2032,12 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
     const char* gp = reinterpret_cast<const char*>(f.G);
     if (d_bias) {
         const int64_t nparts = sb.np / kBiasRows;
-        if (h->k > 0) {  // with labels head_grad_kernel has made the parts
-            const dim3 grid((unsigned)nparts, (unsigned)ceil_div(vt, 512));
-#define GRWS_HEAD_BIAS_PART(DT, PL)                                                                               \
-    hipLaunchKernelGGL((head_bias_part_kernel<DT, PL>), grid, dim3(256), 0, stream, f.G, s.ldg, plane, vt, f.bias)
-            GRWS_HEAD_PLANES(GRWS_HEAD_BIAS_PART);
-#undef GRWS_HEAD_BIAS_PART
-            GRWS_LAUNCH_CHECK();
-        }
         const dim3 cg((unsigned)ceil_div(vc, 64));
         char* db = static_cast<char*>(d_bias) + v0 * esz;
 #define GRWS_HEAD_BIAS(T)                                                                               \
     hipLaunchKernelGGL(head_bias_kernel<T>, cg, dim3(1024), 0, stream, f.bias, nparts, vt, vc, f.alpha, \
-                       f.bias_sum, first_rows, last_rows, reinterpret_cast<T*>(db))
+                       f.bias_sum, first_rows, last_rows, h->k > 0 ? f.targets : nullptr, gscale,    \
+                       reinterpret_cast<T*>(db))
         if (h->dtype == GRWS_F32) GRWS_HEAD_BIAS(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS(_Float16);
         else GRWS_HEAD_BIAS(__hip_bfloat16);

@@ -291,3 +291,34 @@ def test_repeated_rows(cuda_device, dt, n, width):
     want[rows] = dx
     assert torch.equal(dh[~nan], want[~nan])
     assert single.unique().numel() == n
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_bias_gradient_of_lists(cuda_device, dt):
+    """A uniform student of 2,048 classes, each of which 6 of 4,096 rows list
+    with a probability of 1/3: the bias gradient 4,096 / 2,048 - 6 / 3 is 0,
+    to 2^-21 of the two probabilities' sums of 2 and the fp32 sums' rounding
+    (128 terms one after the other, 2^-24 of at most 4 each)."""
+    n, classes = 4096, 2048
+    h = torch.randn(n, 16, device=cuda_device).to(dt)
+    w = torch.zeros(classes, 16, device=cuda_device).to(dt)
+    b = torch.zeros(classes, device=cuda_device, dtype=dt).requires_grad_(True)
+    index = (torch.arange(n, device=cuda_device)[:, None] * 3 + torch.arange(3, device=cuda_device)) % classes
+    loss, _ = linear_distill(h, w, index, torch.zeros(n, 3, device=cuda_device), bias=b, reduction="none")
+    db = torch.autograd.grad(loss.sum(), [b])[0].float()
+    assert float(db.abs().max()) <= 4 * 2.0 ** -21 + 128 * 4 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("n", [9, 200])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_bias_gradient_of_a_spoiled_list(cuda_device, dt, n):
+    """A NaN among a list's logits is seen in its classes' bias gradients."""
+    h, w, b, _, lists, teacher = _inputs(cuda_device, n, 24, 2000, dt, 8)
+    teacher[3, 1] = math.nan
+    b.requires_grad_(True)
+    loss, _ = linear_distill(h, w, lists, teacher, bias=b)
+    db = torch.autograd.grad(loss, [b])[0]
+    assert bool(torch.isnan(loss)) and bool(torch.isnan(db[lists[3].long()]).all())
+    other = torch.ones(2000, dtype=torch.bool, device=cuda_device)
+    other[lists[3].long()] = False
+    assert bool(torch.isfinite(db[other]).all())
