@@ -123,3 +123,54 @@ def test_blocks_of_rows_and_repeated_rows(cuda_device):
     want[rows] = dx
     dh[rows[3]] = want[rows[3]]
     assert torch.equal(dh, want)
+
+
+@pytest.mark.parametrize("dt,n,width,classes", [
+    (torch.bfloat16, 66000, 16, 9300), (torch.float16, 66000, 16, 9300),  # pieces, runs
+    (torch.bfloat16, 66000, 256, 9300),  # pieces of one run: the last adds and writes
+    (torch.float32, 40000, 256, 6000)])
+def test_pieces_of_classes(cuda_device, dt, n, width, classes):
+    """G of all the classes passes its bound: the hidden gradient is added up
+    over the pieces."""
+    print(f"case pieces {dt} {n}x{width}x{classes}", flush=True)
+    p = plan(1, torch.empty(n, width, device=cuda_device, dtype=dt),
+             torch.empty(classes, width, device=cuda_device, dtype=dt), n)
+    assert p["blocks"] == 1 and p["pieces"] > 1, p
+    assert (p["dh_runs"] == 1 and p["dh_tile"] == 256) or width != 256 or dt == torch.float32, p
+    _check(cuda_device, dt, n, width, classes, 5, scale=4096.0)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("k", [0, 4])
+def test_large_tiles_of_one_run(cuda_device, dt, k):
+    """256-tiles of both gradients, each all of its sum (f32: of two pieces,
+    which the hidden gradient adds up, and two runs of the weight gradient)."""
+    n, width, classes = 16384 - 5, 1000, 16384 - 3
+    print(f"case tiles {dt} k={k}", flush=True)
+    p = plan(1, torch.empty(n, width, device=cuda_device, dtype=dt),
+             torch.empty(classes, width, device=cuda_device, dtype=dt), n, k)
+    assert (p["tile"], p["dw_tile"], p["dh_tile"], p["dh_runs"]) == (256, 256, 256, 1), p
+    assert p["dw_runs"] == p["pieces"] == (2 if dt == torch.float32 else 1), p
+    _check(cuda_device, dt, n, width, classes, 6, k=k, scale=4096.0)
+
+
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_pieces_of_packed_weight(cuda_device, n):
+    """f32 weight in several packed pieces, forward and backward (few rows
+    read it as it lies, but take the same pieces backward)."""
+    width, classes, dt = 1030, 50000, torch.float32
+    h, w = torch.empty(n, width, device=cuda_device), torch.empty(classes, width, device=cuda_device)
+    f, b = plan(0, h, w, n), plan(1, h, w, n)
+    assert b["pieces"] > 1 and f["few"] == b["few"] == (n <= 128) and (n <= 128 or f["pieces"] > 1), (f, b)
+    _check(cuda_device, dt, n, width, classes, 7)
+    _check(cuda_device, dt, n, width, classes, 8, nodes=2 * n, k=4)
+
+
+@pytest.mark.parametrize("n", [20, 300])
+def test_pieces_of_unaligned_weight(cuda_device, n):
+    """The same of a 16-bit weight whose rows are not 16-byte aligned."""
+    width, classes, dt = 1030, 140000, torch.bfloat16
+    h, w = (torch.empty(x, width, device=cuda_device, dtype=dt) for x in (n, classes))
+    f, b = plan(0, h, w, n), plan(1, h, w, n)
+    assert b["pieces"] > 1 and f["few"] == (n <= 32) and (n <= 32 or f["pieces"] > 1), (f, b)
+    _check(cuda_device, dt, n, width, classes, 9)
