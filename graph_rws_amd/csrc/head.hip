@@ -1518,19 +1518,12 @@ __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __rest
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.
 // (A label's place is known to the product's epilogue: one for a row.)
-// sums (or NULL): the classes' sums of q in units of 2^-31, whole numbers, so
-// that the order of the atomics does not matter; with the p that the epilogue
-// has summed they make the bias gradient of unrounded p - q.  What is not
-// finite goes into the class's sum of p instead.
-constexpr float kSumUnit = 2147483648.f;
 template <int DT, int PLANES>
 __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats stats,
                                                             const float* __restrict__ y,
                                                             const float* __restrict__ coef,
                                                             const float* __restrict__ row_scale, float gscale,
-                                                            float c1, int64_t n, int64_t v0, int64_t vc,
-                                                            unsigned long long* sums, float* bias_part, int64_t vt,
-                                                            uint16_t* G,
+                                                            float c1, int64_t n, int64_t v0, int64_t vc, uint16_t* G,
                                                             int64_t ldg, int64_t plane) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (at >= n * t.k) return;
@@ -1544,22 +1537,58 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats 
     planes_of<DT, PLANES>((exp2f(fmaf(y[at], c, -(m * c))) * stats[i].y - q) * s, h);
 #pragma unroll
     for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
-    if (!sums) return;
-    const float u = row_scale ? q * row_scale[i] : q;
-    if (fabsf(u) < INFINITY)
-        atomicAdd(sums + (v - v0), (unsigned long long)__float2ll_rn(u * kSumUnit));
-    else
-        bias_part[i / kBiasRows * vt + (v - v0)] = __int_as_float(0x7fc00000);
+}
+
+// The teacher's share of a part of the bias gradient (kBiasRows rows): the
+// epilogue has summed p, this takes off q, unrounded both.  A work-group adds
+// the part's entries in kBiasClasses of the classes in LDS, in whole units of
+// 2^-40, so that the order does not matter (global atomics, of 200,000 rows of
+// 5 entries in 47 classes, took 1.5 ms; this 40 us).
+constexpr int kBiasClasses = 4096;
+constexpr float kBiasUnit = 1099511627776.f;
+
+__global__ __launch_bounds__(256) void head_bias_targets_kernel(Targets t, RowStats stats,
+                                                                const float* __restrict__ coef,
+                                                                const float* __restrict__ row_scale, float gscale,
+                                                                int64_t n, int64_t v0, int64_t vc, int64_t vt,
+                                                                float* __restrict__ part) {
+    __shared__ unsigned long long sum[kBiasClasses];
+    __shared__ int bad;
+    const int64_t first = (int64_t)blockIdx.x * kBiasRows, c0 = (int64_t)blockIdx.y * kBiasClasses;
+    const int classes = (int)(vc - c0 < kBiasClasses ? vc - c0 : kBiasClasses);
+    const int rows = (int)(n - first < kBiasRows ? n - first : kBiasRows);  // none, of a padding part
+    for (int c = threadIdx.x; c < classes; c += 256) sum[c] = 0;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    float* out = part + blockIdx.x * vt + c0;
+    auto entries = [&](auto use) {
+        for (int e = threadIdx.x; e < rows * t.k; e += 256) {
+            const int64_t i = first + e / t.k, at = first * t.k + e;
+            const int64_t c = teacher_at(t, i, e % t.k) - v0 - c0;
+            if (c < 0 || c >= classes || coef[at] < 0.f || stats[i].x == INFINITY) continue;
+            use((int)c, row_scale ? coef[at] * row_scale[i] : coef[at]);
+        }
+    };
+    entries([&](int c, float q) {
+        if (fabsf(q) < INFINITY) atomicAdd(sum + c, (unsigned long long)__float2ll_rn(q * kBiasUnit));
+        else bad = 1;
+    });
+    __syncthreads();
+    for (int c = threadIdx.x; c < classes; c += 256)
+        if (sum[c]) out[c] -= gscale * (float)((double)(long long)sum[c] / (double)kBiasUnit);
+    if (!bad) return;  // uniform
+    __syncthreads();
+    entries([&](int c, float q) {
+        if (!(fabsf(q) < INFINITY)) out[c] = __int_as_float(0x7fc00000);
+    });
 }
 
 // 16 waves share 64 columns.  sum: NULL, or [vc] of the blocks of rows before,
-// in their order (first: none); only the last block writes the gradient,
-// after taking off the targets' sums (NULL: they are in the parts).
+// in their order (first: none); only the last block writes the gradient.
 template <typename T>
 __global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict__ part, int64_t nparts, int64_t vp,
                                                          int64_t vc, const float* __restrict__ alpha,
                                                          float* __restrict__ sum, int32_t first, int32_t last,
-                                                         const int64_t* __restrict__ targets, float gscale,
                                                          T* __restrict__ out) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1576,7 +1605,6 @@ __global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict
 #pragma unroll
     for (int w = 0; w < 16; ++w) s += red[w][lane];
     if (!first) s += sum[c];
-    if (last && targets) s -= gscale * (float)((double)targets[c] / (double)kSumUnit);
     if (last) out[c] = from_float<T>(s * *alpha);
     else sum[c] = s;
 }
@@ -1854,7 +1882,6 @@ struct BwdSpace {
     uint16_t *hp, *wp, *G;
     float *dh, *dw, *bias, *bias_sum, *alpha, *scale;
     uint32_t* most;
-    int64_t* targets;  // see head_subtract_kernel
     int32_t* owner;  // see listed_again
 };
 
@@ -1876,7 +1903,6 @@ void bwd_space(A& a, const Shape& s, const grws_head* h, BwdSpace* f) {
     take(f->alpha, 1);
     take(f->scale, s.n);
     take(f->most, 1);
-    if (h->k > 0) take(f->targets, s.vp);
     if (h->rows) take(f->owner, h->hidden_rows);
 }
 
@@ -2020,14 +2046,18 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
     if (h->k > 0) {
         const dim3 grid((unsigned)ceil_div(sb.n * h->k, 256));
         const float *y = target_logit + r0 * h->k, *coef = target_prob + (s.n + r0) * h->k;
-        auto* sums = d_bias ? reinterpret_cast<unsigned long long*>(f.targets) : nullptr;
-        if (sums && first_rows) GRWS_TRY(fill_i64(f.targets, vc, 0, stream));
 #define GRWS_HEAD_SUB(DT, PL)                                                                                      \
     hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, stats, y, coef, row_scale, gscale, \
-                       c1, sb.n, v0, vc, sums, f.bias, vt, f.G, s.ldg, plane)
+                       c1, sb.n, v0, vc, f.G, s.ldg, plane)
         GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
 #undef GRWS_HEAD_SUB
         GRWS_LAUNCH_CHECK();
+        if (d_bias) {
+            const dim3 parts((unsigned)(sb.np / kBiasRows), (unsigned)ceil_div(vc, kBiasClasses));
+            hipLaunchKernelGGL(head_bias_targets_kernel, parts, dim3(256), 0, stream, t, stats, coef, row_scale, gscale,
+                               sb.n, v0, vc, vt, f.bias);
+            GRWS_LAUNCH_CHECK();
+        }
     }
     const char* gp = reinterpret_cast<const char*>(f.G);
     if (d_bias) {
@@ -2036,8 +2066,7 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
         char* db = static_cast<char*>(d_bias) + v0 * esz;
 #define GRWS_HEAD_BIAS(T)                                                                               \
     hipLaunchKernelGGL(head_bias_kernel<T>, cg, dim3(1024), 0, stream, f.bias, nparts, vt, vc, f.alpha, \
-                       f.bias_sum, first_rows, last_rows, h->k > 0 ? f.targets : nullptr, gscale,    \
-                       reinterpret_cast<T*>(db))
+                       f.bias_sum, first_rows, last_rows, reinterpret_cast<T*>(db))
         if (h->dtype == GRWS_F32) GRWS_HEAD_BIAS(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_BIAS(_Float16);
         else GRWS_HEAD_BIAS(__hip_bfloat16);
