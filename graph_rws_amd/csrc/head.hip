@@ -748,18 +748,26 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
     C::zero(acc);
     C::run(a.g, tp, tq, kb, ke, p0, q0, p1, q1, acc);
     float* out = a.part + sp * a.np * a.dp;
+    // the rows' places and factors, all of them asked for at once: 0 for a row
+    // that does not count, NaN for one listed again
+    int64_t place[TQ];
+    float factor[TQ];
     const float alpha = a.last ? *a.alpha : 0.f;
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
-        int64_t to = -1;
-        bool counts = false;
-        if (a.last && row < a.n) {
-            to = a.rows ? a.rows[row] : row;
-            if (to >= a.hidden_rows) to = -1;
-            counts = a.stats[row].x != INFINITY;
-        }
-        const bool again = to >= 0 && listed_again(a.owner, to);
+        const bool live = a.last && row < a.n;
+        place[j] = !live ? -1 : a.rows ? a.rows[row] : row;
+        factor[j] = live && a.stats[row].x != INFINITY ? alpha : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        if (place[j] >= a.hidden_rows) place[j] = -1;
+        if (place[j] >= 0 && listed_again(a.owner, place[j])) factor[j] = __int_as_float(0x7fc00000);
+    }
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15), to = place[j];
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
             const int64_t d = (int64_t)tp * BP + (wave % WP) * (TP * 16) + C::p_of(i, lane);
@@ -768,8 +776,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
             const float4_t v = a.first ? acc[i][j] : *o + acc[i][j];
             if (!a.last) *o = v;
             else if (to >= 0 && d < a.width)
-                store4<OT>(a.out, to * a.ldo + d,
-                           again ? v * __int_as_float(0x7fc00000) : counts ? v * alpha : float4_t{0.f, 0.f, 0.f, 0.f},
+                store4<OT>(a.out, to * a.ldo + d, factor[j] != 0.f ? v * factor[j] : float4_t{0.f, 0.f, 0.f, 0.f},
                            a.width - d, a.vec);
         }
     }
