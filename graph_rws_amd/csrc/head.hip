@@ -545,6 +545,13 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
     tile_of(a.g, tp, tq);
     float4_t acc[TP][TQ];
     const int64_t pfirst = (int64_t)tp * BP + (wave % WP) * (TP * 16);
+    // the rows' statistics are here when the product is (asked for behind it,
+    // 16,384 x 20,224 of 256 takes 322 us, not 300); run() has barriers
+    __shared__ float2 row_stats[BQ];
+    if (threadIdx.x < BQ) {
+        const int64_t row = (int64_t)tq * BQ + threadIdx.x;
+        row_stats[threadIdx.x] = row < a.n ? a.stats[row] : make_float2(INFINITY, 0.f);
+    }
     begin_logits<C>(acc, a.v0 + pfirst, a.classes, a.bias, a.bias_dt, lane);
     C::run(a.g, tp, tq, 0, a.g.ksteps, p0, q0, p1, q1, acc);
 #pragma unroll
@@ -552,7 +559,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
         // of a row that does not count, whose largest logit is given as +inf,
         // all are 2^-inf (its hidden row is zeros, so a logit is its bias)
-        const float2 st = row < a.n ? a.stats[row] : make_float2(INFINITY, 0.f);
+        const float2 st = row_stats[row - (int64_t)tq * BQ];
         const float m = st.x, c1 = base2(m, a.c1), ref = m * c1;
         const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
         const bool stray = row >= a.n || (m == INFINITY && st.y != 0.f);
@@ -2091,6 +2098,16 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
         if (s.split) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_F32);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_F16, GRWS_F16);
         else GRWS_HEAD_LAUNCH(s.weight, head_dweight_kernel, w, GRWS_BF16, GRWS_BF16);
+        if (w.part && last_rows) {  // before dH, whose operands would push the runs out of the L2
+#define GRWS_HEAD_DW(T)                                                                                             \
+    hipLaunchKernelGGL(head_weight_out_kernel<T>, dim3((unsigned)vc), dim3(256), 0, stream, f.dw, s.weight.splits,  \
+                       s.vp, s.dp, s.D, f.alpha, reinterpret_cast<T*>(out), ld_dw)
+            if (h->dtype == GRWS_F32) GRWS_HEAD_DW(float);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_DW(_Float16);
+            else GRWS_HEAD_DW(__hip_bfloat16);
+#undef GRWS_HEAD_DW
+            GRWS_LAUNCH_CHECK();
+        }
     }
     if (d_hidden && s.few && s.split) {
         const FewHiddenArgs d{static_cast<const float*>(h->weight) + v0 * h->ld_weight, h->ld_weight, s.D, s.dp, s.n,
@@ -2295,17 +2312,6 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
         for (int64_t r0 = 0; r0 < s.n; r0 += s.nb)
             GRWS_TRY(backward_block(h, s, f, v0, vc, r0, stats, target_logit, target_prob, per_row, alpha, owner, c1,
                                     gscale, d_hidden, ld_dh, d_weight, ld_dw, d_bias, stream));
-        if (d_weight && (s.weight.splits > 1 || s.blocks > 1)) {
-            char* out = static_cast<char*>(d_weight) + v0 * ld_dw * esz;
-#define GRWS_HEAD_DW(T)                                                                                             \
-    hipLaunchKernelGGL(head_weight_out_kernel<T>, dim3((unsigned)vc), dim3(256), 0, stream, f.dw, s.weight.splits,  \
-                       s.vp, s.dp, s.D, f.alpha, reinterpret_cast<T*>(out), ld_dw)
-            if (h->dtype == GRWS_F32) GRWS_HEAD_DW(float);
-            else if (h->dtype == GRWS_F16) GRWS_HEAD_DW(_Float16);
-            else GRWS_HEAD_DW(__hip_bfloat16);
-#undef GRWS_HEAD_DW
-            GRWS_LAUNCH_CHECK();
-        }
     }
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
