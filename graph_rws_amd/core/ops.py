@@ -1900,10 +1900,10 @@ class HeadCall:
                                L.dtype_code(hidden.dtype), self.k, i64, float(temperature))
 
     def saved_pointers(self, saved: torch.Tensor):
-        """Addresses of the rows' statistics, the targets' logits and the
-        teacher's probabilities in the buffer that head_fwd saves."""
+        """Addresses of lse, the targets' logits and the teacher's
+        probabilities in the buffer that head_fwd saves."""
         p, n = saved.data_ptr(), self.n
-        return p, p + 8 * n, p + 4 * n * (2 + self.k) if self.k else None
+        return p, p + 4 * n, p + 4 * n * (1 + self.k) if self.k else None
 
 
 def _on_device(dev: torch.device):
@@ -1919,15 +1919,15 @@ def head_fwd(call: HeadCall, per_row: bool):
     n, k = call.n, call.k
     out = torch.empty((n,) if per_row else (), dtype=torch.float32, device=dev)
     counts = torch.empty(3, dtype=torch.int64, device=dev)
-    # the rows' statistics [2 * n], the targets' logits [n * max(k, 1)], the teacher's probabilities [2 * n * k]
-    saved = torch.empty(n * (2 + max(k, 1) + 2 * k), dtype=torch.float32, device=dev)
-    stats, logit, prob = call.saved_pointers(saved)
+    # lse [n], the targets' logits [n * max(k, 1)], the teacher's probabilities [2 * n * k]
+    saved = torch.empty(n * (1 + max(k, 1) + 2 * k), dtype=torch.float32, device=dev)
+    lse, logit, prob = call.saved_pointers(saved)
     ref = ctypes.byref(call.view)
     lib = L.load()
     wsb = lib.grws_head_fwd_workspace_bytes(ref)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     with _on_device(dev):
-        L.call("grws_head_fwd", ref, stats, logit, prob, out.data_ptr() if per_row else None,
+        L.call("grws_head_fwd", ref, lse, logit, prob, out.data_ptr() if per_row else None,
                None if per_row else out.data_ptr(), counts.data_ptr(), ws.data_ptr(), wsb, L.stream_of(dev))
     return out, counts, saved
 
@@ -1937,7 +1937,7 @@ def head_bwd(call: HeadCall, saved: torch.Tensor, counts: torch.Tensor, dloss: t
     """(d_hidden, d_weight, d_bias), None where not needed, of head_fwd's
     loss (dloss a scalar, or [n] per row)."""
     dev = call.hidden.device
-    stats, logit, prob = call.saved_pointers(saved)
+    lse, logit, prob = call.saved_pointers(saved)
     dl = dloss.float().contiguous()
     dh = dw = db = None
     if need[0]:
@@ -1953,7 +1953,7 @@ def head_bwd(call: HeadCall, saved: torch.Tensor, counts: torch.Tensor, dloss: t
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     width = call.hidden.shape[1]
     with _on_device(dev):
-        L.call("grws_head_bwd", ref, stats, logit, prob, counts.data_ptr(), dl.data_ptr(), int(dloss.dim() == 1),
+        L.call("grws_head_bwd", ref, lse, logit, prob, counts.data_ptr(), dl.data_ptr(), int(dloss.dim() == 1),
                L.ptr(dh), width, L.ptr(dw), width, L.ptr(db), ws.data_ptr(), wsb, L.stream_of(dev))
     return dh, dw, db
 

@@ -452,12 +452,28 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
     }
 }
 
-// What the forward leaves of a row for the gradients: the largest logit m
-// and one over the sum of the exponentials, so p = 2^(z c - ref) times that.
-// (Of one log-sum, m c1 + log2 s rounded, nothing would be left of s beside a
-// large m.)  A row that does not count has m = +inf and a factor of zero, or
-// NaN where its zeros met a weight that is not finite.
-typedef const float2* RowStats;
+// What the forward leaves of a row for the gradients, p = 2^(z c - ref) factor:
+//   lse = m c1 + log2 s rounded (m the largest logit, s the sum against it),
+//     +inf for a row that does not count; -inf where m c1 overflows, as for
+//     logits that are all masks of the type's lowest value;
+//   factor: 2^(lse - m c1) / s, what the rounding took (up to 4% of p beside
+//     an m of 10^6); 1 / s where lse is -inf.  Of a row that does not count 0,
+//     or NaN where its zeros met a weight that is not finite.
+// factor lies `stride` apart: in the place of a label's logit, or of a list's
+// first probability, which nothing needs after the forward.
+struct RowStats {
+    const float* lse;
+    const float* factor;
+    int64_t stride;
+    __device__ __forceinline__ float2 of(int64_t i) const { return make_float2(lse[i], factor[i * stride]); }
+    RowStats from(int64_t r0) const { return RowStats{lse + r0, factor + r0 * stride, stride}; }
+};
+
+// c and ref of a row.  (Where lse is -inf every logit that is not -inf itself
+// is of the largest one's size: a c of 2^-149 makes one of it.)
+__device__ __forceinline__ float2 base_of(float lse, float c1) {
+    return lse == -INFINITY ? make_float2(__uint_as_float(1), 0.f) : make_float2(c1, lse);
+}
 
 struct GradArgs {
     Gemm g;
@@ -550,19 +566,19 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
     __shared__ float2 row_stats[BQ];
     if (threadIdx.x < BQ) {
         const int64_t row = (int64_t)tq * BQ + threadIdx.x;
-        row_stats[threadIdx.x] = row < a.n ? a.stats[row] : make_float2(INFINITY, 0.f);
+        row_stats[threadIdx.x] = row < a.n ? a.stats.of(row) : make_float2(INFINITY, 0.f);
     }
     begin_logits<C>(acc, a.v0 + pfirst, a.classes, a.bias, a.bias_dt, lane);
     C::run(a.g, tp, tq, 0, a.g.ksteps, p0, q0, p1, q1, acc);
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
-        // of a row that does not count, whose largest logit is given as +inf,
-        // all are 2^-inf (its hidden row is zeros, so a logit is its bias)
+        // of a row that does not count, whose lse is +inf, all are 2^-inf
+        // (its hidden row is zeros, so a logit is its bias)
         const float2 st = row_stats[row - (int64_t)tq * BQ];
-        const float m = st.x, c1 = base2(m, a.c1), ref = m * c1;
+        const float lse = st.x, c1 = base_of(lse, a.c1).x, ref = base_of(lse, a.c1).y;
         const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
-        const bool stray = row >= a.n || (m == INFINITY && st.y != 0.f);
+        const bool stray = row >= a.n || (lse == INFINITY && st.y != 0.f);
         const float f = stray ? 0.f : st.y * s;
         if (__any(stray)) {
 #pragma unroll
@@ -577,7 +593,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
 #pragma unroll
         for (int i = 0; i < TP; ++i) acc[i][j] *= f;
         if (a.labels) {
-            const int64_t lab = m != INFINITY ? a.labels[row] - a.v0 - pfirst : -1;
+            const int64_t lab = lse != INFINITY ? a.labels[row] - a.v0 - pfirst : -1;
             const bool here = lab >= 0 && lab < TP * 16;
             if (__any(here)) {
                 const int at = here ? (int)lab : -1;
@@ -765,7 +781,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
         const bool live = a.last && row < a.n;
         place[j] = !live ? -1 : a.rows ? a.rows[row] : row;
-        factor[j] = live && a.stats[row].x != INFINITY ? alpha : 0.f;
+        factor[j] = live && a.stats.lse[row] != INFINITY ? alpha : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
@@ -1063,7 +1079,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
         const int64_t row = first + 16 * j + r;
-        if constexpr (GRAD) live[j] = row < a.n && a.stats[row].x != INFINITY;
+        if constexpr (GRAD) live[j] = row < a.n && a.stats.lse[row] != INFINITY;
         else live[j] = row < a.n && (a.t.labels ? row_state<1>(a.t, row, 0) : a.states[row]) == 1;
         h[j] = static_cast<const T*>(a.hidden) + (live[j] ? (a.t.rows ? a.t.rows[row] : row) * a.ldh : 0);
     }
@@ -1175,8 +1191,8 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                 }
             }
         } else {
-            const float2 st = live[j] ? a.stats[row] : make_float2(INFINITY, 0.f);
-            const float m = st.x, c1 = base2(m, a.c1), ref = m * c1;
+            const float2 st = live[j] ? a.stats.of(row) : make_float2(INFINITY, 0.f);
+            const float c1 = base_of(st.x, a.c1).x, ref = base_of(st.x, a.c1).y;
             const float sc = a.row_scale && live[j] ? a.row_scale[row] * a.gscale : a.gscale;
             const float f = st.y * sc;
 #pragma unroll
@@ -1363,9 +1379,9 @@ __device__ __forceinline__ void finish_loss(const double* part_loss, const int32
 template <int R>
 __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2* __restrict__ part, int64_t strips,
                                                         int32_t strip_classes, int64_t n, int64_t np,
-                                                        float temperature, float c1, const float* __restrict__ y,
-                                                        const float* __restrict__ prob,
-                                                        const int32_t* __restrict__ flags, float2* __restrict__ stats,
+                                                        float temperature, float c1, float* __restrict__ y,
+                                                        float* __restrict__ prob,
+                                                        const int32_t* __restrict__ flags, float* __restrict__ lse,
                                                         float* __restrict__ row_loss, double* part_loss,
                                                         int32_t* part_cnt, int32_t* done,
                                                         float* __restrict__ loss_out, int64_t* __restrict__ counts) {
@@ -1445,9 +1461,17 @@ __global__ __launch_bounds__(512) void head_join_kernel(Targets t, const float2*
             bad = 1;
             v = __int_as_float(0x7fc00000);
         }
-        // a live row with a logit of +inf has nothing but NaN
-        stats[i] = make_float2(st != 1 ? INFINITY : m == INFINITY ? __int_as_float(0x7fc00000) : m,
-                               st == 1 ? past_rounding(m, c1) / s : s == s ? 0.f : s);
+        // see RowStats.  (A live row with a logit of +inf, or a largest one
+        // whose m c1 is +inf, has nothing but NaN.)
+        const float nan = __int_as_float(0x7fc00000);
+        float l = INFINITY, f = s == s ? 0.f : s;
+        if (st == 1) {
+            l = fmaf(m, c1, log2f(s));
+            f = l == -INFINITY ? (s > 0.f ? 1.f / s : nan) : __builtin_amdgcn_exp2f(-fmaf(m, c1, -l)) / s;
+            if (l == INFINITY) l = nan;
+        }
+        lse[i] = l;
+        (t.labels ? y : prob)[i * (t.labels ? 1 : t.k)] = f;
         if (row_loss) row_loss[i] = v;
     }
 #pragma unroll
@@ -1508,7 +1532,7 @@ __global__ __launch_bounds__(256) void head_most_kernel(const float* __restrict_
     // order of the atomics does not matter.  Infinities and NaN are left out:
     // they are their rows' own shares, not a factor of every row
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    uint32_t m = i < n && stats[i].x != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
+    uint32_t m = i < n && stats.lse[i] != INFINITY ? __float_as_uint(fabsf(dloss[i])) : 0u;
     if (m >= 0x7f800000u) m = 0u;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -1527,7 +1551,7 @@ __global__ __launch_bounds__(256) void head_row_scale_kernel(const float* __rest
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const float m = __uint_as_float(*most);
-    scale[i] = stats[i].x == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : dloss[i] * 0.f;
+    scale[i] = stats.lse[i] == INFINITY ? 0.f : m > 0.f ? dloss[i] / m : dloss[i] * 0.f;
 }
 
 // G at a teacher's entries: the rounded p - q, q the entry's coefficient.
@@ -1544,11 +1568,12 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats 
     const int64_t i = at / t.k;
     const int64_t v = teacher_at(t, i, (int)(at - i * t.k));
     if (v < v0 || v >= v0 + vc) return;
-    const float q = coef[at], m = stats[i].x, c = base2(m, c1);
-    if (q < 0.f || m == INFINITY) return;
+    const float q = coef[at];
+    const float2 st = stats.of(i), b = base_of(st.x, c1);
+    if (q < 0.f || st.x == INFINITY) return;
     const float s = row_scale ? row_scale[i] * gscale : gscale;
     uint16_t h[PLANES];
-    planes_of<DT, PLANES>((exp2f(fmaf(y[at], c, -(m * c))) * stats[i].y - q) * s, h);
+    planes_of<DT, PLANES>((exp2f(fmaf(y[at], b.x, -b.y)) * st.y - q) * s, h);
 #pragma unroll
     for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
 }
@@ -1579,7 +1604,7 @@ __global__ __launch_bounds__(256) void head_bias_targets_kernel(Targets t, RowSt
         for (int e = threadIdx.x; e < rows * t.k; e += 256) {
             const int64_t i = first + e / t.k, at = first * t.k + e;
             const int64_t c = teacher_at(t, i, e % t.k) - v0 - c0;
-            if (c < 0 || c >= classes || coef[at] < 0.f || stats[i].x == INFINITY) continue;
+            if (c < 0 || c >= classes || coef[at] < 0.f || stats.lse[i] == INFINITY) continue;
             use((int)c, row_scale ? coef[at] * row_scale[i] : coef[at]);
         }
     };
@@ -1658,7 +1683,7 @@ __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __res
     const int64_t row = rows ? rows[i] : i;
     if (row < 0 || row >= hidden_rows) return;
     // a row that does not count gets zeros: the sum of no runs
-    const bool counts = stats[i].x != INFINITY;
+    const bool counts = stats.lse[i] != INFINITY;
     const float a = listed_again(owner, row) ? __int_as_float(0x7fc00000) : counts ? *alpha : 0.f;
     sum_splits(part + i * dp, counts ? splits : 0, np * dp, width, a, out + row * ldo);
 }
@@ -2012,14 +2037,14 @@ int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
 // G of a piece of the classes and a block of the rows, and what the two
 // products add of it to dW and dH.
 int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_t v0, int64_t vc, int64_t r0,
-                   RowStats all_stats, const float* target_logit, const float* target_prob, bool per_row,
+                   const RowStats& all_stats, const float* target_logit, const float* target_prob, bool per_row,
                    const Alpha& alpha, const int32_t* owner, float c1, float gscale, void* d_hidden, int64_t ld_dh,
                    void* d_weight, int64_t ld_dw, void* d_bias, hipStream_t stream) {
     const Shape sb = block_of(s, r0);
     const grws_head hb = rows_of(h, r0, sb.n);
     const Targets t = targets_of(&hb);
     const size_t esz = dtype_size(h->dtype);
-    const RowStats stats = all_stats + r0;
+    const RowStats stats = all_stats.from(r0);
     const float* row_scale = per_row ? f.scale + r0 : nullptr;
     const bool first_rows = r0 == 0, last_rows = r0 + sb.n == s.n;
     const int64_t plane = sb.np * s.ldg;
@@ -2152,7 +2177,7 @@ extern "C" size_t grws_head_fwd_workspace_bytes(const grws_head* h) {
     return z.used;
 }
 
-extern "C" int grws_head_fwd(const grws_head* h, float* row_stats, float* target_logit, float* target_prob,
+extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit, float* target_prob,
                              float* row_loss, float* loss, int64_t* counts, void* workspace, size_t workspace_bytes,
                              void* stream_) {
     clear_error();
@@ -2165,7 +2190,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* row_stats, float* target
         GRWS_LAUNCH_CHECK();
         return GRWS_OK;
     }
-    GRWS_CHECK_ARG(row_stats && target_logit && (h->k == 0 || target_prob), "head: null output");
+    GRWS_CHECK_ARG(lse && target_logit && (h->k == 0 || target_prob), "head: null output");
     const Shape s = shape_of(h, false);
     Carver cv(workspace, workspace_bytes);
     FwdSpace f{};
@@ -2219,7 +2244,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* row_stats, float* target
 #define GRWS_HEAD_JOIN(R)                                                                                            \
     hipLaunchKernelGGL(head_join_kernel<R>, dim3((unsigned)ceil_div(sb.n, R)), dim3(512), 0, stream, t, f.part,      \
                        ceil_div(s.V, s.strip_classes), (int32_t)s.strip_classes, sb.n, sb.np, h->temperature, c1, y, \
-                       prob, f.flags, reinterpret_cast<float2*>(row_stats) + r0, row_loss ? row_loss + r0 : nullptr, \
+                       prob, f.flags, lse + r0, row_loss ? row_loss + r0 : nullptr,                                 \
                        f.pl + at, f.pc + 3 * at, one ? f.done : nullptr, loss, counts)
         if (join_rows == 1) GRWS_HEAD_JOIN(1);
         else if (join_rows == 4) GRWS_HEAD_JOIN(4);
@@ -2254,7 +2279,7 @@ extern "C" size_t grws_head_bwd_workspace_bytes(const grws_head* h) {
     return z.used;
 }
 
-extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const float* target_logit,
+extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* target_logit,
                              const float* target_prob, const int64_t* counts, const float* dloss, int32_t per_row,
                              void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw, void* d_bias,
                              void* workspace, size_t workspace_bytes, void* stream_) {
@@ -2272,7 +2297,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
         if (d_bias) GRWS_TRY(fill_bytes_zero(d_bias, h->classes * e, stream));
         return GRWS_OK;
     }
-    GRWS_CHECK_ARG(row_stats && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
+    GRWS_CHECK_ARG(lse && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
     if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
     const Shape s = shape_of(h, true);
     Carver cv(workspace, workspace_bytes);
@@ -2281,7 +2306,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* row_stats, const f
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
     const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
-    const RowStats stats = reinterpret_cast<RowStats>(row_stats);
+    const RowStats stats = h->k > 0 ? RowStats{lse, target_prob, h->k} : RowStats{lse, target_logit, 1};
     if (per_row) {
         GRWS_TRY(fill_i32(reinterpret_cast<int32_t*>(f.most), 1, 0, stream));
         const dim3 grid((unsigned)ceil_div(s.n, 256));

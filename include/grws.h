@@ -838,10 +838,9 @@ int grws_cross_entropy_bwd(const void* logits, int32_t dtype, int64_t ld, int64_
 /* Losses: cross entropy lse_i - z_i,label; distillation T^2 KL(softmax of   */
 /* the listed teacher logits / T || softmax(z_i / T)).                       */
 /*                                                                           */
-/* Forward, no sync: row_stats f32 [n x 2], 8-byte aligned (a row's largest  */
-/* logit, +inf when it does not count, and the reciprocal of its sum of      */
-/* exponentials) and target_logit f32 [n * max(k, 1)], target_prob f32       */
-/* [2 x n x k] (k > 0), which the backward takes; row_loss                   */
+/* Forward, no sync: lse f32 [n] (log2 of the sum of 2^(z log2(e) / T), +inf */
+/* for rows that do not count) and target_logit f32 [n * max(k, 1)],         */
+/* target_prob f32 [2 x n x k] (k > 0), which the backward takes; row_loss   */
 /* f32 [n] (0 for rows that do not count, NaN for bad input); loss f32 scalar,   */
 /* the mean over counted rows (NaN when none counts or an input is bad: a    */
 /* label, class index or row id out of range; loss or row_loss may be NULL,  */
@@ -868,7 +867,7 @@ typedef struct grws_head {
 } grws_head;
 
 size_t grws_head_fwd_workspace_bytes(const grws_head* head);
-int grws_head_fwd(const grws_head* head, float* row_stats, float* target_logit, float* target_prob, float* row_loss,
+int grws_head_fwd(const grws_head* head, float* lse, float* target_logit, float* target_prob, float* row_loss,
                   float* loss, int64_t* counts, void* workspace, size_t workspace_bytes, void* stream);
 size_t grws_head_bwd_workspace_bytes(const grws_head* head);
 /* How a call is cut up, for reports and tests (host only): {blocks of rows, */
@@ -878,7 +877,7 @@ size_t grws_head_bwd_workspace_bytes(const grws_head* head);
 /* the backward only.                                                        */
 #define GRWS_HEAD_PLAN 10
 int grws_head_plan(const grws_head* head, int32_t backward, int64_t* out);
-int grws_head_bwd(const grws_head* head, const float* row_stats, const float* target_logit, const float* target_prob,
+int grws_head_bwd(const grws_head* head, const float* lse, const float* target_logit, const float* target_prob,
                   const int64_t* counts, const float* dloss, int32_t per_row, void* d_hidden, int64_t ld_dh,
                   void* d_weight, int64_t ld_dw, void* d_bias, void* workspace, size_t workspace_bytes,
                   void* stream);

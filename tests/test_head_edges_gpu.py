@@ -322,3 +322,30 @@ def test_bias_gradient_of_a_spoiled_list(cuda_device, dt, n):
     other = torch.ones(2000, dtype=torch.bool, device=cuda_device)
     other[lists[3].long()] = False
     assert bool(torch.isfinite(db[other]).all())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [9, 200])
+@pytest.mark.parametrize("kind", ["labels", "lists"])
+def test_saved_statistics(cuda_device, dt, n, kind):
+    """lse as the header has it, within the buffer it asks for, and a second
+    backward of the same forward has the same bits."""
+    h, w, b, labels, lists, teacher = _inputs(cuda_device, n, 40, 300, dt, 5)
+    labels[::4] = -100
+    lists[::4] = -1
+    t = 1.0 if kind == "labels" else 2.0
+    call = (ops.HeadCall(h, w, b, None, labels) if kind == "labels"
+            else ops.HeadCall(h, w, b, None, None, lists, teacher, t))
+    loss, counts, saved = ops.head_fwd(call, True)
+    assert saved.numel() == n * (2 if kind == "labels" else 16)
+    z = (h.double() @ w.double().t() + b.double()) / t * math.log2(math.e)
+    live = torch.ones(n, dtype=torch.bool, device=cuda_device)
+    live[::4] = False
+    assert bool((saved[:n][~live] == math.inf).all())
+    want = torch.logsumexp(z * math.log(2), 1) / math.log(2)
+    # 48 2^-23 of the summed magnitudes (20 at most), and lse's own rounding
+    assert float((saved[:n][live].double() - want[live]).abs().max()) <= 2e-4
+    up = torch.randn(n, device=cuda_device)
+    first = ops.head_bwd(call, saved, counts, up)
+    for x, y in zip(first, ops.head_bwd(call, saved, counts, up)):
+        assert torch.equal(x, y)
