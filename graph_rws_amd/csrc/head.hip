@@ -732,15 +732,6 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
 // so the order is fixed).  8,192 x 4,096 over 65,536 classes: 3.28 ms (1,343
 // TFLOP/s).
 
-// Whether `rows` lists the row more than once: owner, which holds a listing's
-// number for every listed row, has kAgain there.  Each listing has a gradient
-// of its own and only one of them could be kept: the row gets NaN, which is
-// seen, and not one of them, which is not.
-constexpr int32_t kAgain = -1;
-__device__ __forceinline__ bool listed_again(const int32_t* owner, int64_t row) {
-    return owner && owner[row] == kAgain;
-}
-
 struct HiddenArgs {
     Gemm g;
     float* part;  // [splits][np][dp]
@@ -754,7 +745,6 @@ struct HiddenArgs {
     int64_t ldo, n, width, hidden_rows;
     const int64_t* rows;
     RowStats stats;  // a row that does not count gets zeros, whatever alpha and W hold
-    const int32_t* owner;  // NULL, or see listed_again
 };
 
 template <int DT, int OT, int BP, int BQ, int WP, int WQ>
@@ -771,8 +761,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
     C::zero(acc);
     C::run(a.g, tp, tq, kb, ke, p0, q0, p1, q1, acc);
     float* out = a.part + sp * a.np * a.dp;
-    // the rows' places and factors, all of them asked for at once: 0 for a row
-    // that does not count, NaN for one listed again
+    // the rows' places and factors (0: does not count), all asked for at once
     int64_t place[TQ];
     float factor[TQ];
     const float alpha = a.last ? *a.alpha : 0.f;
@@ -781,12 +770,8 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dhidden_kernel(HiddenArgs a
         const int64_t row = (int64_t)tq * BQ + (wave / WP) * (TQ * 16) + 16 * j + (lane & 15);
         const bool live = a.last && row < a.n;
         place[j] = !live ? -1 : a.rows ? a.rows[row] : row;
-        factor[j] = live && a.stats.lse[row] != INFINITY ? alpha : 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < TQ; ++j) {
         if (place[j] >= a.hidden_rows) place[j] = -1;
-        if (place[j] >= 0 && listed_again(a.owner, place[j])) factor[j] = __int_as_float(0x7fc00000);
+        factor[j] = live && a.stats.lse[row] != INFINITY ? alpha : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < TQ; ++j) {
@@ -1508,14 +1493,17 @@ __global__ __launch_bounds__(256) void head_owner_kernel(const int64_t* __restri
     __hip_atomic_store(owner + row, (int32_t)i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Of a row that is listed again, all but one listing find another's number.
+// d_hidden of a row that is listed more than once: each listing has a gradient
+// of its own and one of them was kept.  All but one find another's number in
+// owner and put NaN there, which is seen, and the one that was kept is not.
+template <typename T>
 __global__ __launch_bounds__(256) void head_repeated_kernel(const int64_t* __restrict__ rows, int64_t n,
-                                                            int64_t hidden_rows, int32_t* owner) {
+                                                            int64_t hidden_rows, const int32_t* __restrict__ owner,
+                                                            int64_t width, T* out, int64_t ldo) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t row = i < n ? rows[i] : -1;
-    if (row < 0 || row >= hidden_rows) return;
-    if (__hip_atomic_load(owner + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (int32_t)i)
-        __hip_atomic_store(owner + row, kAgain, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (row < 0 || row >= hidden_rows || owner[row] == (int32_t)i) return;
+    for (int64_t d = 0; d < width; ++d) out[row * ldo + d] = from_float<T>(__int_as_float(0x7fc00000));
 }
 
 // finish_loss in a launch of its own (also of no rows at all)
@@ -1652,14 +1640,14 @@ __global__ __launch_bounds__(1024) void head_bias_kernel(const float* __restrict
 // piece (rows in place), or dH (to the rows they belong to)
 template <typename T>
 __device__ __forceinline__ void sum_splits(const float* __restrict__ part, int64_t splits, int64_t stride,
-                                           int64_t width, float a, T* __restrict__ out) {
+                                           int64_t width, float a, bool keep, T* __restrict__ out) {
     for (int64_t d = threadIdx.x * 4; d < width; d += blockDim.x * 4) {
         float4_t s{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int64_t k = 0; k < splits; ++k) s += *reinterpret_cast<const float4_t*>(part + k * stride + d);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (d + e < width) out[d + e] = from_float<T>(s[e] * a);
+            if (d + e < width) out[d + e] = from_float<T>(keep ? s[e] * a : 0.f);
     }
 }
 
@@ -1669,23 +1657,21 @@ __global__ __launch_bounds__(256) void head_weight_out_kernel(const float* __res
                                                               const float* __restrict__ alpha, T* __restrict__ out,
                                                               int64_t ldo) {
     const int64_t v = blockIdx.x;
-    sum_splits(part + v * dp, splits, vp * dp, width, *alpha, out + v * ldo);
+    sum_splits(part + v * dp, splits, vp * dp, width, *alpha, true, out + v * ldo);
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __restrict__ part, int64_t splits,
                                                               int64_t np, int64_t dp, int64_t width,
                                                               const int64_t* __restrict__ rows, int64_t hidden_rows,
-                                                              RowStats stats, const int32_t* __restrict__ owner,
+                                                              RowStats stats,
                                                               const float* __restrict__ alpha, T* __restrict__ out,
                                                               int64_t ldo) {
     const int64_t i = blockIdx.x;
     const int64_t row = rows ? rows[i] : i;
     if (row < 0 || row >= hidden_rows) return;
-    // a row that does not count gets zeros: the sum of no runs
-    const bool counts = stats.lse[i] != INFINITY;
-    const float a = listed_again(owner, row) ? __int_as_float(0x7fc00000) : counts ? *alpha : 0.f;
-    sum_splits(part + i * dp, counts ? splits : 0, np * dp, width, a, out + row * ldo);
+    const bool keep = stats.lse[i] != INFINITY;  // a row that does not count gets zeros
+    sum_splits(part + i * dp, splits, np * dp, width, *alpha, keep, out + row * ldo);
 }
 
 // ---------------------------------------------------------------------------
@@ -1921,7 +1907,7 @@ struct BwdSpace {
     uint16_t *hp, *wp, *G;
     float *dh, *dw, *bias, *bias_sum, *alpha, *scale;
     uint32_t* most;
-    int32_t* owner;  // see listed_again
+    int32_t* owner;  // see head_repeated_kernel
 };
 
 template <typename A>
@@ -2038,7 +2024,7 @@ int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
 // products add of it to dW and dH.
 int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_t v0, int64_t vc, int64_t r0,
                    const RowStats& all_stats, const float* target_logit, const float* target_prob, bool per_row,
-                   const Alpha& alpha, const int32_t* owner, float c1, float gscale, void* d_hidden, int64_t ld_dh,
+                   const Alpha& alpha, float c1, float gscale, void* d_hidden, int64_t ld_dh,
                    void* d_weight, int64_t ld_dw, void* d_bias, hipStream_t stream) {
     const Shape sb = block_of(s, r0);
     const grws_head hb = rows_of(h, r0, sb.n);
@@ -2156,7 +2142,7 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
         const int32_t vec = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ld_dh % 4 == 0;
         HiddenArgs d{gemm_of(s, s.hidden, W, G, s.dp, sb.np, vc, s.gplanes), f.dh + (s.vp < s.V ? r0 * s.dp : 0),
                      sb.np, s.dp, v0 == 0, s.hidden.splits == 1 && v0 + vc == s.V, vec, f.alpha, out, ld_dh, sb.n, s.D,
-                     hb.hidden_rows, hb.rows, stats, owner};
+                     hb.hidden_rows, hb.rows, stats};
         if (s.split) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_F32);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_F16, GRWS_F16);
         else GRWS_HEAD_LAUNCH(s.hidden, head_dhidden_kernel, d, GRWS_BF16, GRWS_BF16);
@@ -2324,29 +2310,34 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
                            h->hidden_rows, owner);
         GRWS_LAUNCH_CHECK();
     }
-    if (owner) {
-        hipLaunchKernelGGL(head_repeated_kernel, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows, s.n,
-                           h->hidden_rows, owner);
-        GRWS_LAUNCH_CHECK();
-    }
     const size_t esz = dtype_size(h->dtype);
     // pieces of the classes, and of each the blocks of rows: W's piece is
     // packed once, dW's is complete after its blocks
     for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
         const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
         for (int64_t r0 = 0; r0 < s.n; r0 += s.nb)
-            GRWS_TRY(backward_block(h, s, f, v0, vc, r0, stats, target_logit, target_prob, per_row, alpha, owner, c1,
+            GRWS_TRY(backward_block(h, s, f, v0, vc, r0, stats, target_logit, target_prob, per_row, alpha, c1,
                                     gscale, d_hidden, ld_dh, d_weight, ld_dw, d_bias, stream));
     }
     if (d_hidden && s.hidden.splits > 1) {
 #define GRWS_HEAD_DH(T)                                                                                              \
     hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
-                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, owner, f.alpha,         \
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, f.alpha,                \
                        static_cast<T*>(d_hidden), ld_dh)
         if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
         else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
         else GRWS_HEAD_DH(__hip_bfloat16);
 #undef GRWS_HEAD_DH
+        GRWS_LAUNCH_CHECK();
+    }
+    if (owner) {
+#define GRWS_HEAD_REPEATED(T)                                                                                        \
+    hipLaunchKernelGGL(head_repeated_kernel<T>, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows,   \
+                       s.n, h->hidden_rows, owner, s.D, static_cast<T*>(d_hidden), ld_dh)
+        if (h->dtype == GRWS_F32) GRWS_HEAD_REPEATED(float);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_REPEATED(_Float16);
+        else GRWS_HEAD_REPEATED(__hip_bfloat16);
+#undef GRWS_HEAD_REPEATED
         GRWS_LAUNCH_CHECK();
     }
     return GRWS_OK;
