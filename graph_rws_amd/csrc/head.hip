@@ -13,21 +13,26 @@
 // where q of cross entropy is 1 at the label.
 //
 // Forward: one product whose epilogue reduces each 16 TP classes of a row to
-// (max, sum of 2^(y - max)) in registers; a second kernel joins them.
+// (m, sum of 2^(y - m)) in registers; a second kernel joins them.
 // Backward: pieces of the classes.  For each piece the product is made again
-// and its epilogue writes G = 2^(y - L) in 16 bits to a scratch matrix (less
-// one at the label; a small kernel subtracts a teacher's entries), and two
-// products read G: dW's rows of the piece (complete), and dH (added up over
-// the pieces in fp32).  Few rows have a kernel of their own for the logits.
+// and its epilogue writes G = p - q, p = 2^(y - L), in 16 bits to a scratch
+// matrix (a small kernel puts a teacher's entries in place), and two products
+// read G: dW's rows of the piece (complete), and dH (added up over the pieces
+// in fp32).  Few rows have a kernel of their own for the logits.  Many rows go
+// through in blocks, so that neither the strips' (m, sum) nor G grow with rows
+// x classes.
 //
 // G is rounded to the operands' 16-bit type because the matrix cores take no
 // wider one; p - q is formed in fp32 and rounded once.  Its factor s_i T is
 // applied to the fp32 sums instead (f16: G carries 2^15, so that
-// probabilities down to 2^-29 stay normal numbers).  Up to kFewClasses classes
-// G keeps a second plane, what the rounding left over: there a handful of its
-// entries make most of a sum and the rounding shows (0.0027 of a bf16 gradient
-// against 0.0017 for rounding the gradient alone), and the second product is
-// short.
+// probabilities down to 2^-29 stay normal numbers).  That rounding shows at
+// any number of classes: against 64 bits a bf16 gradient is off by 0.0018 to
+// 0.0024 of its norm, where rounding the gradient alone is 0.0017 (f16:
+// 0.00025-0.0003 against 0.0002; 4,096 rows of 47 to 65,536 classes).  Up to
+// kFewClasses classes G keeps a second plane, what the rounding left over, and
+// only the gradient's own rounding remains.  It costs nothing for 1,024 rows
+// and, for 16,384 rows of width 256, 11% of a call at 172 classes and 25% at
+// 1,024; at 2,048 it would be 40%, which is where it stops.
 //
 // F32 operands: x = a + b + c with three bf16 (the top, middle and low 8 of
 // 24 significant bits, truncated, so the split is exact and never
@@ -384,13 +389,13 @@ struct StatsArgs {
     int32_t* earlier;       // [n]: an earlier class of the label's strip has the label's logit
 };
 
-// Bound by the matrix cores for wide D (8,192 x 131,072 x 4,096 bf16: 6.48 ms,
-// 1,357 TFLOP/s; the library's plain product reaches 1,300) and by the
-// exponentials, a quarter of the vector rate, for narrow D (16,384 x 100,003 x
-// 256: 1.05 ms, 800 TFLOP/s; a tile's 8,200 MFMA cycles and about 9,000 VALU
-// cycles follow one another).  p are classes and q rows, so a lane holds
-// 4 TP classes of TQ rows and the reduction over classes takes two
-// cross-lane steps a row.
+// Bound by the matrix cores for wide D (8,192 x 131,072 x 4,096 bf16: 6.6 ms,
+// 1,330 TFLOP/s, MFMA busy 65% of the time; the library's plain product of
+// 8,192^3 reaches 1,295) and by the exponentials, a quarter of the vector rate,
+// for narrow D (16,384 x 100,003 x 256: 1.03-1.08 ms, 800 TFLOP/s; a tile's
+// 8,200 MFMA cycles and about 9,000 VALU cycles follow one another).  p are
+// classes and q rows, so a lane holds 4 TP classes of TQ rows and the
+// reduction over classes takes two cross-lane steps a row.
 template <int DT, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
     using C = Core<DT, false, false, BP, BQ, WP, WQ>;
@@ -548,8 +553,8 @@ __device__ __forceinline__ float rotate(float x) {
 
 constexpr int kBiasRows = 64;  // rows of a part of the bias gradient's sums
 
-// The same product, leaving G.  8,192 x 65,536 of 4,096: 3.47 ms (1,270
-// TFLOP/s); 16,384 x 20,224 of 256: 324 us (524), where 660 MB of G go out
+// The same product, leaving G.  8,192 x 65,536 of 4,096: 3.52 ms (1,250
+// TFLOP/s); 16,384 x 20,224 of 256: 304 us (558), where 660 MB of G go out
 // beside the exponentials.
 template <int DT, int PLANES, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
@@ -672,7 +677,7 @@ __device__ __forceinline__ void store4(void* out, int64_t at, float4_t v, int64_
 // dW rows of a piece: p are columns of H, q the piece's classes, k the rows,
 // cut into `splits` runs when the tiles alone leave CUs idle (their fp32 sums
 // are added in order by head_weight_out_kernel).  65,536 x 4,096 over 8,192
-// rows: 3.62 ms (1,214 TFLOP/s; both operands take two 8-byte LDS reads where
+// rows: 3.63 ms (1,212 TFLOP/s; both operands take two 8-byte LDS reads where
 // the others take one of 16 bytes).
 struct WeightArgs {
     Gemm g;
@@ -729,7 +734,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_dweight_kernel(WeightArgs a
 
 // dH of a piece: p are columns of W, q the rows, k the piece's classes, cut
 // into `splits` runs; each run adds to its own fp32 sums (piece after piece,
-// so the order is fixed).  8,192 x 4,096 over 65,536 classes: 3.28 ms (1,343
+// so the order is fixed).  8,192 x 4,096 over 65,536 classes: 3.33 ms (1,320
 // TFLOP/s).
 
 struct HiddenArgs {
@@ -934,7 +939,7 @@ __device__ __forceinline__ void load8(const T* x, int64_t c, int64_t width, bool
 
 // The student's logits at the teacher's entries, a wave per 4 entries of a
 // row (16 lanes share a dot product): n k rows of W are read, from beyond the
-// L2 (8,192 x 64 rows of 2 KB: 213 us, 5.0 TB/s).  The row's first wave also makes the teacher's probabilities: prob
+// L2 (8,192 x 64 rows of 2 KB: 225 us, 4.8 TB/s).  The row's first wave also makes the teacher's probabilities: prob
 // [n k] (0 where an entry is not listed) and coef [n k], what the
 // gradient subtracts at the entry's class: the sum over the entries that list
 // the class, at the first of them; -1 at every other entry.
@@ -1232,8 +1237,8 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
 // 64 columns of 16 NQ rows over a run of classes, 16 at a time: lane (g, r)
 // reads columns 4 r .. + 3 of classes 4 g .. + 3 (256 bytes a class), which are
 // the operands of four tiles with columns 4 r + c.  1 row x 32,000 x 2,048 with
-// gradients: 702 -> 468 us against dH from packed planes of W, 64 rows 791 ->
-// 669, 128 rows 895 -> 859.
+// gradients: 702 -> 463 us against dH from packed planes of W, 64 rows 791 ->
+// 667, 128 rows 895 -> 865.
 struct FewHiddenArgs {
     const float* weight;  // first class of the piece
     int64_t ldw, width, dp, n, np, vc;
@@ -1570,7 +1575,7 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats 
 // epilogue has summed p, this takes off q, unrounded both.  A work-group adds
 // the part's entries in kBiasClasses of the classes in LDS, in whole units of
 // 2^-40, so that the order does not matter (global atomics, of 200,000 rows of
-// 5 entries in 47 classes, took 1.5 ms; this 40 us).
+// 5 entries in 47 classes, took 1.5 ms; this 12 us).
 constexpr int kBiasClasses = 4096;
 constexpr float kBiasUnit = 1099511627776.f;
 
@@ -1697,11 +1702,12 @@ constexpr int64_t kPartBytes = (int64_t)512 << 20;
 constexpr int64_t kLeastPiece = 4096;
 constexpr int64_t kBlockRows = (int64_t)1 << 20;
 constexpr int64_t kFewClasses = 1024;  // up to here G has a second plane
-// Rows up to which head_few_kernel makes the logits.  32,000 x 2,048, against
-// the products on packed W: f32 1 row 79 against 485 us, 64 rows 121 against
-// 487 (two readings of W for 128 rows); 16-bit rows that are not 16-byte
-// aligned 57 against 116 at 1 row and 127 against 119 at 64; aligned ones,
-// which need no packing, 34 against 49 at 1 row, 38 against 52 at 16.
+// Rows up to which head_few_kernel makes the logits.  Forward calls on 32,000 x
+// 2,048, replayed in a graph, against the products (on packed W, where it has
+// to be): f32 1 row 73 against 479 us, 64 rows 110 against 486, 128 (two
+// readings of W) 227 against 486; 16-bit rows that are not 16-byte aligned 54
+// against 117 at 1 row, 71 against 120 at 32; aligned ones, which need no
+// packing, 33 against 50 at 1 row, 40 against 51 at 16.
 constexpr int64_t kFewRows = 16, kFewPacked = 32, kFewF32 = 128;
 constexpr int64_t kPackBytes = (int64_t)256 << 20;  // a packed piece of W
 
