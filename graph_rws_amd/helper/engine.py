@@ -100,10 +100,11 @@ def train_epoch_head(model, head, graphs_for_model, features: torch.Tensor, labe
 
 
 def _head_rows(hidden, idx):
-    """(hidden, idx), or the gathered rows and None where a classifier's
-    gradient cannot be written to the rows idx in place."""
+    """(hidden, idx), or the gathered rows and None where the classifier
+    cannot read the rows idx in place, or not write their gradient there."""
     from ..layers.fused import rows_distinct
-    if idx.dtype == torch.int64 and idx.dim() == 1 and idx.device == hidden.device and rows_distinct(idx):
+    if (idx.dtype == torch.int64 and idx.dim() == 1 and idx.device == hidden.device
+            and (not hidden.requires_grad or rows_distinct(idx))):
         return hidden, idx
     if idx.dtype == torch.bool:  # a model's rows can be padded to whole windows
         hidden = hidden[:idx.shape[0]]
