@@ -9,8 +9,10 @@ from .ops import (  # noqa: F401
     pack_tiles,
     SpmmPlan,
     build_spmm_plan,
+    clip_grads,
     csr_to_bcsr_cpu,
     default_slabs,
+    grad_norm,
     SamplingTimingResult,
     reindex_bcsr,
     relabel,
@@ -50,4 +52,6 @@ __all__ = [
     "SamplingTimingResult",
     "window_seeds",
     "top_logits",
+    "grad_norm",
+    "clip_grads",
 ]

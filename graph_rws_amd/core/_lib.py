@@ -260,6 +260,9 @@ _PROTOS = {
     "grws_top_logits_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
     "grws_top_logits": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_int32, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "grws_clip_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32]),
+    "grws_clip_grads": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int32, ctypes.c_float, _vp, _vp, _vp,
+                                       ctypes.c_size_t, _vp]),
     "grws_relabel_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
     "grws_relabel": (ctypes.c_int, [_vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int64,
                                     _vp, _vp, ctypes.c_int64, _vp, ctypes.c_size_t, _c_i64p,

@@ -1980,3 +1980,91 @@ def top_logits(logits: torch.Tensor, k: int):
         L.call("grws_top_logits", L.ptr(x), code, _row_pitch(x), n, classes, k, L.ptr(values), L.ptr(index),
                L.ptr(ws), wsb, L.stream_of(dev))
     return values, index
+
+
+# ---------------------------------------------------------------------------
+# global gradient norm and clipping (csrc/clip.hip)
+# ---------------------------------------------------------------------------
+def _one_run(t: torch.Tensor) -> bool:
+    """Whether t's elements lie next to each other, in whatever order of its
+    dimensions."""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != size:
+            return False
+        size *= n
+    return True
+
+
+def _clip_call(who: str, grads, outs, max_norm: float, scale: Optional[torch.Tensor]) -> torch.Tensor:
+    dev = grads[0].device
+    L.require_device(who, dev, scale, *grads)
+    if scale is not None and (scale.numel() != 1 or scale.dtype != torch.float32):
+        raise ValueError(f"{who}: scale must be one float32")
+    m = len(grads)
+    ptrs, ints, sizes = ctypes.c_void_p * m, ctypes.c_int32 * m, ctypes.c_int64 * m
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    wsb = int(L.load().grws_clip_workspace_bytes(m))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        L.call("grws_clip_grads", ptrs(*[g.data_ptr() for g in grads]),
+               ints(*[L.dtype_code(g.dtype) for g in grads]), sizes(*[g.numel() for g in grads]),
+               ptrs(*[o.data_ptr() for o in outs]) if outs is not None else None,
+               ints(*[L.dtype_code(o.dtype) for o in outs]) if outs is not None else None, m, float(max_norm),
+               L.ptr(scale), norm.data_ptr(), ws.data_ptr(), wsb, L.stream_of(dev))
+    return norm
+
+
+def _clip_list(who: str, grads):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        raise ValueError(f"{who}: no gradients")
+    for g in grads:
+        if g.layout != torch.strided:
+            raise TypeError(f"{who}: gradients must be dense tensors (got {g.layout})")
+    return [g.detach() for g in grads]
+
+
+def grad_norm(grads, scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The 2-norm of all the gradients together (f32 scalar on their device,
+    squares summed in 64 bits), of scale * gradient where scale (a float32 on
+    the device, the inverse of a loss scale) is given.  A list of dense F32 /
+    F16 / BF16 tensors of any strides on one GPU; no host sync."""
+    grads = [g if _one_run(g) else g.contiguous() for g in _clip_list("grad_norm", grads)]
+    return _clip_call("grad_norm", grads, None, 0.0, scale)
+
+
+def clip_grads(grads, max_norm: float, out=None, scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradients times scale * min(1, max_norm / (norm + 1e-6)), norm as
+    grad_norm has it, which is returned; in place, or into `out`: a list of
+    tensors of the gradients' shapes, each of its gradient's dtype or float32
+    (what an optimizer with float32 copies of 16-bit parameters reads).  A
+    norm that is not finite makes zeros and NaN of the gradients, as
+    torch.nn.utils.clip_grad_norm_ does.  Tensors that share memory are an
+    error; no host sync."""
+    grads = _clip_list("clip_grads", grads)
+    if not float(max_norm) >= 0.0:
+        raise ValueError(f"clip_grads: max_norm must not be negative (got {max_norm})")
+    if out is None:
+        flat = [g if _one_run(g) else g.contiguous() for g in grads]
+        norm = _clip_call("clip_grads", flat, flat, max_norm, scale)
+        for g, f in zip(grads, flat):
+            if f is not g:
+                g.copy_(f)
+    else:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
+            raise ValueError("clip_grads: out must have the gradients' shapes")
+        L.require_device("clip_grads", grads[0].device, *out)
+        for o, g in zip(out, grads):
+            if o.dtype not in (g.dtype, torch.float32):
+                raise TypeError(f"clip_grads: out must be of the gradient's dtype or float32 (got {o.dtype} for "
+                                f"{g.dtype})")
+            if not o.is_contiguous() and (o.stride() != g.stride() or not _one_run(o)):
+                raise ValueError("clip_grads: out must be contiguous or have its gradient's strides")
+        flat = [g if o.stride() == g.stride() and _one_run(g) else g.contiguous() for o, g in zip(out, grads)]
+        norm = _clip_call("clip_grads", flat, out, max_norm, scale)
+    torch.autograd.graph.increment_version(grads if out is None else out)
+    return norm

@@ -7,6 +7,7 @@ from .timer import (  # noqa: F401
     reset_spmm_timings,
 )
 from .engine import (  # noqa: F401
+    clip_grad_norm_,
     compute_loss_and_metrics,
     evaluate,
     evaluate_head,

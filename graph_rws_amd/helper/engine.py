@@ -10,6 +10,22 @@ import torch
 import torch.nn.functional as F
 
 
+def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_(parameters, max_norm) of the 2-norm in
+    two launches (core.clip_grads); torch's own where the gradients are not
+    dense F32 / F16 / BF16 tensors of one GPU, each listed once."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads or any(g.layout != torch.strided or not g.is_cuda or g.device != grads[0].device
+                        or g.dtype not in _CLIPPED for g in grads) or len({id(g) for g in grads}) != len(grads):
+        return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
+    from ..core import clip_grads
+    return clip_grads(grads, max_norm)
+
+
+_CLIPPED = (torch.float32, torch.float16, torch.bfloat16)
+
+
 def compute_loss_and_metrics(logits, labels):
     """(loss, correct_count tensor, num_samples) (engine.py:22-41)."""
     if labels.dim() > 1:
@@ -58,7 +74,7 @@ def train_epoch_full(model, graphs_for_model, features: torch.Tensor, labels: to
     loss, correct, n = loss_and_metrics_rows(logits, train_idx, labels[train_idx])
     acc = correct / n if n > 0 else 0.0
     loss.backward()
-    torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)
+    clip_grad_norm_(model.parameters(), max_norm=1.0)
     optimizer.step()
     if not sync:
         return loss.detach(), acc
@@ -92,7 +108,7 @@ def train_epoch_head(model, head, graphs_for_model, features: torch.Tensor, labe
         loss = (1.0 - teacher_weight) * loss + teacher_weight * kd
     acc = counts[0] / n if n > 0 else 0.0
     loss.backward()
-    torch.nn.utils.clip_grad_norm_(list(model.parameters()) + list(head.parameters()), max_norm=1.0)
+    clip_grad_norm_(list(model.parameters()) + list(head.parameters()), max_norm=1.0)
     optimizer.step()
     if not sync:
         return loss.detach(), acc
@@ -314,7 +330,7 @@ def train_epoch_node_sampling(model, graphs_for_model, features: torch.Tensor,
         loss, correct, n = loss_and_metrics_rows(logits, rows, labels[seeds], check_rows=False)
         loss.backward()
         timer.record("Bwd")
-        torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)
+        clip_grad_norm_(model.parameters(), max_norm=1.0)
         optimizer.step()
         timer.record("Step")
         with torch.no_grad():

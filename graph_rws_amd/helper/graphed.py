@@ -232,7 +232,7 @@ class GraphedBlockStep:
                 blocks[0].tile_cols, feats.dtype, blocks[0].values_condensed.dtype)
 
     def _eager(self, bk):
-        from .engine import loss_and_metrics_rows
+        from .engine import clip_grad_norm_, loss_and_metrics_rows
         self.model.train()
         self.opt.zero_grad()
         if self.dtype is None:
@@ -242,7 +242,7 @@ class GraphedBlockStep:
                 logits = self.model(bk.graphs, bk.X)
         loss, correct, _ = loss_and_metrics_rows(logits, None, bk.labels)
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(self.model.parameters(), max_norm=1.0)
+        clip_grad_norm_(self.model.parameters(), max_norm=1.0)
         self.opt.step()
         return loss.detach(), correct
 

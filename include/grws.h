@@ -894,6 +894,25 @@ int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, int64_t rows,
                     void* values, int32_t* index, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* The global norm of `count` gradients and clipping by it, what ends the   */
+/* reference's training steps (helper/engine.py:44-83).  Tensor i: sizes[i] */
+/* consecutive elements of dtypes[i] at grads[i], any alignment; the lists  */
+/* are on the host.  norm (f32 device scalar, may be NULL with outs) =      */
+/* |scale| sqrt(sum of squares), squares summed in 64 bits; scale: f32      */
+/* device scalar (the inverse of a loss scale) or NULL for 1.               */
+/* outs[i] = grads[i] scale min(1, max_norm / (norm + 1e-6)) in             */
+/* out_dtypes[i]: the gradient's dtype or f32 (NULL: the gradient's);       */
+/* outs[i] may be grads[i] in the same dtype, tensors do not overlap        */
+/* otherwise.  outs NULL: the norm alone.  A norm that is not finite makes  */
+/* zeros and NaN of the gradients, as the formula does.  Same inputs, same  */
+/* bits.                                                                    */
+/* ------------------------------------------------------------------------ */
+size_t grws_clip_workspace_bytes(int32_t count);
+int grws_clip_grads(const void* const* grads, const int32_t* dtypes, const int64_t* sizes, void* const* outs,
+                    const int32_t* out_dtypes, int32_t count, float max_norm, const float* scale, float* norm,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Measurement only: no counterpart in the reference.  The random row-      */
 /* gather ceiling that bounds the SpMM's X reads, for benchmark reports.    */
 /* n_idx row indices (int32, a multiple of 8; values outside [0, rows)      */
