@@ -260,6 +260,13 @@ _PROTOS = {
     "grws_top_logits_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
     "grws_top_logits": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_int32, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "grws_log_probs_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
+    "grws_log_probs_fwd": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp,
+                                          ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _vp, _vp,
+                                          _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "grws_log_probs_bwd": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp,
+                                          ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _vp, _vp, _vp, _vp, _vp,
+                                          ctypes.c_int64, _vp]),
     "grws_clip_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32]),
     "grws_clip_grads": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int32, ctypes.c_float, _vp, _vp, _vp,
                                        ctypes.c_size_t, _vp]),

@@ -1983,6 +1983,81 @@ def top_logits(logits: torch.Tensor, k: int):
 
 
 # ---------------------------------------------------------------------------
+# log probabilities of given classes, entropy and alternatives (csrc/logp.hip)
+# ---------------------------------------------------------------------------
+def _check_given(who: str, index: torch.Tensor, classes: int, temperature: float, top: int):
+    """(n, k) of the given classes [n] or [n, k]."""
+    if index.dim() not in (1, 2) or index.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{who}: index must be int32 or int64 [n] or [n, k]")
+    n, k = index.shape[0], index.shape[1] if index.dim() == 2 else 1
+    if not 1 <= k <= 1024:
+        raise ValueError(f"{who}: 1 to 1024 given classes a row (got {k})")
+    if not 0.0 < float(temperature) < float("inf"):
+        raise ValueError(f"{who}: the temperature must be positive (got {temperature})")
+    if not 0 <= top <= min(classes, 1024):
+        raise ValueError(f"{who}: top must be 0..{min(classes, 1024)} (got {top})")
+    return n, k
+
+
+def check_log_probs(logits, index, temperature: float, top: int) -> None:
+    """Raises unless the arguments are log_probs_fwd's: logits [n, classes],
+    index int32 or int64 [n] or [n, k], all on one GPU."""
+    L.require_device("log_probs", logits.device, index)
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"log_probs: logits must be [rows, classes] (got {tuple(logits.shape)})")
+    L.dtype_code(logits.dtype)
+    n, _ = _check_given("log_probs", index, logits.shape[1], temperature, top)
+    if n != logits.shape[0]:
+        raise ValueError(f"log_probs: {n} rows of classes for {logits.shape[0]} rows of logits")
+
+
+def _top_outputs(n: int, top: int, dev):
+    if not top:
+        return None, None
+    return (torch.empty((n, top), dtype=torch.float32, device=dev),
+            torch.empty((n, top), dtype=torch.int32, device=dev))
+
+
+def log_probs_fwd(logits: torch.Tensor, index: torch.Tensor, temperature: float, top: int, save: bool):
+    """(logp as index, entropy [n], saved f32 [n, 2] or None, top_logp, top_index
+    [n, top] or None) of arguments that check_log_probs takes; logits with
+    unit column stride, index contiguous."""
+    n, classes = logits.shape
+    dev = logits.device
+    logp = torch.empty(index.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(n, dtype=torch.float32, device=dev)
+    saved = torch.empty((n, 2), dtype=torch.float32, device=dev) if save else None
+    top_logp, top_index = _top_outputs(n, top, dev)
+    wsb = L.load().grws_log_probs_workspace_bytes(n, classes, top)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    k = index.shape[1] if index.dim() == 2 else 1
+    with _on_device(dev):
+        L.call("grws_log_probs_fwd", logits.data_ptr(), L.dtype_code(logits.dtype), _row_pitch(logits), n, classes,
+               index.data_ptr(), int(index.dtype == torch.int64), k, top, temperature, logp.data_ptr(),
+               entropy.data_ptr(), L.ptr(saved), L.ptr(top_logp), L.ptr(top_index), L.ptr(ws), wsb, L.stream_of(dev))
+    return logp, entropy, saved, top_logp, top_index
+
+
+def _f32_rows(t: Optional[torch.Tensor]):
+    return t.float().contiguous() if t is not None else None
+
+
+def log_probs_bwd(logits: torch.Tensor, index: torch.Tensor, temperature: float, saved: torch.Tensor,
+                  entropy: torch.Tensor, dlogp: Optional[torch.Tensor], dentropy: Optional[torch.Tensor]):
+    """The logits' gradient of log_probs_fwd's logp and entropy (None: zeros)."""
+    n, classes = logits.shape
+    dev = logits.device
+    grad = torch.empty((n, classes), dtype=logits.dtype, device=dev)
+    dlogp, dentropy = _f32_rows(dlogp), _f32_rows(dentropy)
+    k = index.shape[1] if index.dim() == 2 else 1
+    with _on_device(dev):
+        L.call("grws_log_probs_bwd", logits.data_ptr(), L.dtype_code(logits.dtype), _row_pitch(logits), n, classes,
+               index.data_ptr(), int(index.dtype == torch.int64), k, temperature, saved.data_ptr(),
+               entropy.data_ptr(), L.ptr(dlogp), L.ptr(dentropy), grad.data_ptr(), classes, L.stream_of(dev))
+    return grad
+
+
+# ---------------------------------------------------------------------------
 # global gradient norm and clipping (csrc/clip.hip)
 # ---------------------------------------------------------------------------
 def _one_run(t: torch.Tensor) -> bool:

@@ -39,6 +39,7 @@ SOURCES = [
     "fused.hip",
     "head.hip",
     "top.hip",
+    "logp.hip",
     "clip.hip",
     "probe.hip",
 ]

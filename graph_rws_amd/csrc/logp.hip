@@ -1,0 +1,542 @@
+// Log probabilities of given classes, entropy and top alternatives of rows of
+// logits in memory, and their gradient (gfx950).
+//
+//   y_v = z_v log2(e) / T     m the largest z, u_v = (z_v - m) log2(e) / T
+//   s = sum 2^u, t = sum 2^u u       log2 p_v = u_v - log2 s
+//   logp_j = ln2 log2 p_cj           H = ln2 (log2 s - t / s)
+//   dz_v = (sum_j a_j [v = c_j] - p_v (A + b (ln p_v + H))) / T
+// with a_j the upstream gradient of logp_j, b that of H, A the sum of a_j.
+// t <= 0 and s >= 1, so H adds two terms of one sign and nothing cancels.  The
+// largest logit is taken off before the factor: masks of the type's lowest
+// value leave zero and do not overflow.
+//
+// Forward: one pass.  Every thread keeps its own (m, s, t) and moves them to a
+// new m when a step of 32 logits has a larger one (rare after the first
+// steps); the work-group joins them at the end, in a fixed order.  Top logits
+// come from the same registers (top_pool.h).  Few rows are cut into stretches
+// and joined, short ones take a wave each.
+#include "top_pool.h"
+
+namespace grws {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// (m, s, t) of some of a row's logits; nothing of them: m = -inf, s = t = 0.
+struct Stats {
+    float m, s, t;
+};
+
+__device__ __forceinline__ Stats no_stats() { return Stats{-INFINITY, 0.f, 0.f}; }
+
+// 2^u u and 2^d (s d + t) below -200 are zero: infinities would leave NaN
+__device__ __forceinline__ float reach(float u) { return fmaxf(u, -200.f); }
+
+// s and t seen from a larger m, d = (old m - new m) log2(e) / T further down
+// (-inf where there was nothing)
+__device__ __forceinline__ void move(Stats& a, float d) {
+    d = reach(d);
+    const float f = __builtin_amdgcn_exp2f(d);
+    a.t = fmaf(d, a.s, a.t) * f;
+    a.s *= f;
+}
+
+__device__ __forceinline__ Stats join(Stats a, Stats b, float c1) {
+    // a NaN logit shows in s; largest values are compared without it
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return Stats{m, a.s + b.s, a.t + b.t};  // zeros, or NaN
+    move(a, (a.m - m) * c1);
+    move(b, (b.m - m) * c1);
+    return Stats{m, a.s + b.s, a.t + b.t};
+}
+
+__device__ __forceinline__ void add(Stats& a, float z, float m, float c1) {
+    const float u = (z - m) * c1, e = __builtin_amdgcn_exp2f(u);
+    a.s += e;
+    a.t = fmaf(e, reach(u), a.t);
+}
+
+// joins lanes d apart, d = 32..1: every lane has the wave's
+__device__ __forceinline__ Stats join_wave(Stats a, float c1) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const Stats b{__shfl_xor(a.m, d, kWave), __shfl_xor(a.s, d, kWave), __shfl_xor(a.t, d, kWave)};
+        // both sides in one order, so the lanes agree
+        a = (threadIdx.x & d) ? join(b, a, c1) : join(a, b, c1);
+    }
+    return a;
+}
+
+// The classes whose log probabilities are asked for: k a row; a negative
+// one asks for nothing (0), one past the last is an error (NaN).
+struct Given {
+    const void* index;
+    int32_t k, i64;
+    __device__ __forceinline__ int64_t at(int64_t r, int j) const {
+        return i64 ? static_cast<const int64_t*>(index)[r * k + j]
+                   : (int64_t) static_cast<const int32_t*>(index)[r * k + j];
+    }
+};
+
+struct Outputs {
+    float* logp;      // [rows k]
+    float* entropy;   // [rows]
+    float2* saved;    // [rows]: m, log2 s; or NULL
+    float* top_logp;  // [rows top]
+    int32_t* top_index;
+};
+
+// The factors of T: c1 = log2(e) / T.
+struct Scale {
+    float c1, inv_t;
+};
+
+// What a row's statistics say of logit z (in natural units: a mask of the
+// type's lowest value stays finite).
+struct Row {
+    float m, l2, inv_t;  // largest logit, log2 s
+    __device__ __forceinline__ float logp(float z) const { return fmaf(z - m, inv_t, -kLn2 * l2); }
+};
+
+__device__ __forceinline__ Row row_of(const Stats& a, const Scale& sc) {
+    return Row{a.m, a.m == -INFINITY ? __int_as_float(0x7fc00000) : log2f(a.s), sc.inv_t};
+}
+
+// The row's outputs, `lanes` threads of which this is `sub`.
+template <typename T>
+__device__ __forceinline__ void put_row(const Stats& a, const Scale& sc, const T* row, int64_t r, int32_t classes,
+                                        const Given& g, const Outputs& o, int sub, int lanes) {
+    const Row q = row_of(a, sc);
+    for (int j = sub; j < g.k; j += lanes) {
+        const int64_t c = g.at(r, j);
+        float v = 0.f;
+        if (c >= classes) v = __int_as_float(0x7fc00000);
+        else if (c >= 0) v = q.logp(to_float(row[c]));
+        o.logp[r * g.k + j] = v;
+    }
+    if (sub != 0) return;
+    o.entropy[r] = kLn2 * (q.l2 - a.t / a.s);
+    if (o.saved) o.saved[r] = make_float2(q.m, q.l2);
+}
+
+template <typename T>
+__device__ __forceinline__ void add_chunk(Stats& a, const Chunk<T>& v, float c1) {
+    float z[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) z[i] = v.in(i) ? to_float(v.get(i)) : -INFINITY;
+    float m = z[0];
+#pragma unroll
+    for (int i = 1; i < kMine; ++i) m = fmaxf(m, z[i]);
+    if (m > a.m) {
+        move(a, (a.m - m) * c1);
+        a.m = m;
+    }
+    m = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) add(a, z[i], m, c1);
+}
+
+// A work-group a row, or a stretch of one (FINAL false: its statistics and
+// keys go to `part` and `best`).  MAXK 0: no alternatives.
+template <typename T, bool FINAL, int MAXK>
+__global__ __launch_bounds__(kT) void logp_rows_kernel(const T* __restrict__ logits, int64_t ld, int64_t r0,
+                                                       int32_t classes, int32_t class_bits, int32_t top,
+                                                       int32_t stretch, Scale sc, Given g, Outputs o,
+                                                       float4* __restrict__ part, uint64_t* __restrict__ best) {
+    __shared__ Pool<MAXK ? MAXK : 1> p;
+    __shared__ float sm[kWaves], ss[kWaves], st[kWaves];
+    const int64_t r = r0 + blockIdx.x;
+    const T* row = logits + r * ld;
+    const int32_t first = (int32_t)blockIdx.y * stretch;
+    const int32_t end = classes - first < stretch ? classes : first + stretch;
+    const int bits = (int)sizeof(T) * 8 + class_bits;
+    if (MAXK && threadIdx.x == 0) p.count = 0;
+    uint64_t bound = 0;
+    float least = -INFINITY;
+    Stats a = no_stats();
+    for (int32_t c = first; c < end; c += kChunk) {
+        Chunk<T> v;
+        v.load(row, c, end);
+        add_chunk(a, v, sc.c1);
+        if constexpr (MAXK) offer_chunk<MAXK>(p, v, row, c, first, end, class_bits, top, bound, least);
+    }
+    a = join_wave(a, sc.c1);
+    if ((threadIdx.x & 63) == 0) {
+        sm[threadIdx.x >> 6] = a.m;
+        ss[threadIdx.x >> 6] = a.s;
+        st[threadIdx.x >> 6] = a.t;
+    }
+    __syncthreads();
+    a = Stats{sm[0], ss[0], st[0]};
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) a = join(a, Stats{sm[w], ss[w], st[w]}, sc.c1);
+    if constexpr (FINAL) {
+        put_row(a, sc, row, r, classes, g, o, threadIdx.x, kT);
+        if constexpr (MAXK) {
+            const Row q = row_of(a, sc);
+            put_best(p, top, bits, class_bits, [&](int at, int32_t cls) {
+                o.top_index[r * top + at] = cls;
+                o.top_logp[r * top + at] = q.logp(to_float(row[cls]));
+            });
+        }
+    } else {
+        const int64_t at = blockIdx.x * (int64_t)gridDim.y + blockIdx.y;
+        if (threadIdx.x == 0) part[at] = make_float4(a.m, a.s, a.t, 0.f);
+        if constexpr (MAXK) {
+            keep_best(p, top, bits);
+            __syncthreads();
+            const int n = p.count < top ? p.count : top;
+            for (int j = threadIdx.x; j < top; j += kT) best[at * top + j] = j < n ? p.keys[j] : 0;
+        }
+    }
+}
+
+// Joins the stretches of a row.
+template <typename T, int MAXK>
+__global__ __launch_bounds__(kT) void logp_join_kernel(const T* __restrict__ logits, int64_t ld, int64_t r0,
+                                                       int32_t classes, int32_t class_bits, int32_t top,
+                                                       int32_t stretches, Scale sc, Given g, Outputs o,
+                                                       const float4* __restrict__ part,
+                                                       const uint64_t* __restrict__ best) {
+    __shared__ Pool<MAXK ? MAXK : 1> p;
+    const int64_t r = r0 + blockIdx.x;
+    const T* row = logits + r * ld;
+    Stats a = no_stats();
+    // every wave joins them all, in one order
+    for (int w = threadIdx.x & 63; w < stretches; w += 64) {
+        const float4 x = part[blockIdx.x * (int64_t)stretches + w];
+        a = join(a, Stats{x.x, x.y, x.z}, sc.c1);
+    }
+    a = join_wave(a, sc.c1);
+    put_row(a, sc, row, r, classes, g, o, threadIdx.x, kT);
+    if constexpr (MAXK) {
+        if (threadIdx.x == 0) p.count = 0;
+        constexpr int OFFER = Sizes<MAXK>::OFFER;
+        const int bits = (int)sizeof(T) * 8 + class_bits;
+        const int64_t count = (int64_t)stretches * top;
+        uint64_t bound = 0;
+        for (int64_t c = 0; c < count; c += kT * OFFER) {
+            uint64_t x[OFFER];
+#pragma unroll
+            for (int i = 0; i < OFFER; ++i) {
+                const int64_t at = c + i * kT + threadIdx.x;
+                x[i] = at < count ? best[blockIdx.x * count + at] : 0;
+            }
+            offer(p, x, top, bits, bound);
+        }
+        const Row q = row_of(a, sc);
+        put_best(p, top, bits, class_bits, [&](int at, int32_t cls) {
+            o.top_index[r * top + at] = cls;
+            o.top_logp[r * top + at] = q.logp(to_float(row[cls]));
+        });
+    }
+}
+
+// Short rows: a wave holds a row in its registers; the alternatives as in
+// top_wave_kernel, the largest key `top` times.
+constexpr int kWaveClasses = 1024;
+constexpr int kWaveTop = 16;
+
+template <typename T, int PER>
+__global__ __launch_bounds__(kT) void logp_wave_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows,
+                                                       int32_t classes, int32_t class_bits, int32_t top, Scale sc,
+                                                       Given g, Outputs o) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    if (r >= rows) return;  // uniform over the wave
+    const T* row = logits + r * ld;
+    T x[PER];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = i * 64 + lane;
+        x[i] = c < classes ? row[c] : from_float<T>(-INFINITY);
+        m = fmaxf(m, to_float(x[i]));
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
+    Stats a{m, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) add(a, to_float(x[i]), m == -INFINITY ? 0.f : m, sc.c1);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        a.s += __shfl_xor(a.s, d, kWave);
+        a.t += __shfl_xor(a.t, d, kWave);
+    }
+    put_row(a, sc, row, r, classes, g, o, lane, 64);
+    if (top == 0) return;
+    const Row q = row_of(a, sc);
+    const uint64_t low = (1ull << class_bits) - 1;
+    uint64_t key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = i * 64 + lane;
+        key[i] = c < classes ? ((uint64_t)order_of<T>(x[i]) << class_bits) | (low - (uint32_t)c) : 0;
+    }
+    for (int n = 0; n < top; ++n) {
+        uint64_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) best = key[i] > best ? key[i] : best;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            const uint64_t other = __shfl_xor((unsigned long long)best, d, kWave);
+            best = other > best ? other : best;
+        }
+        const int c = (int)(low - (best & low));
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (key[i] == best) {  // one lane's: keys are distinct
+                key[i] = 0;
+                o.top_index[r * top + n] = c;
+                o.top_logp[r * top + n] = q.logp(to_float(x[i]));
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// the gradient
+// ---------------------------------------------------------------------------
+struct Upstream {
+    const float* dlogp;     // [rows k], or NULL: zeros
+    const float* dentropy;  // [rows], or NULL: zeros
+};
+
+// The sum of a_j of a row's given classes, `LANES` lanes of a wave together.
+__device__ __forceinline__ float given_sum(const Given& g, const Upstream& up, int64_t r, int32_t classes, int lane) {
+    float s = 0.f;
+    if (!up.dlogp) return s;
+    for (int j = lane; j < g.k; j += 64) {
+        const int64_t c = g.at(r, j);
+        if (c >= 0 && c < classes) s += up.dlogp[r * g.k + j];
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, kWave);
+    return s;
+}
+
+// dz of a logit that is not given: -p (A + b (ln p + H)) / T.  A row of
+// nothing but -inf has no p: zeros, so that it can be left out of a loss.
+struct Slope {
+    float m, l2, c1, k, b2, inv_t;  // k = (A + b H), b2 = b ln2
+    __device__ __forceinline__ float of(float z) const {
+        if (m == -INFINITY) return 0.f;  // uniform
+        const float u = fmaf(z - m, c1, -l2);
+        return -__builtin_amdgcn_exp2f(u) * fmaf(b2, reach(u), k) * inv_t;
+    }
+};
+
+// Elements at a time of a row's stretch; ROWS rows a work-group (a wave each)
+// or one.  Given classes are put in place after the rest: each wave's stores
+// have left before its own threads (ONE: the work-group's, behind a barrier)
+// write the same places again.
+template <typename T, bool ONE>
+__global__ __launch_bounds__(kT) void logp_grad_kernel(const T* __restrict__ logits, int64_t ld, int64_t r0,
+                                                       int64_t rows, int32_t classes, int32_t stretch, float c1,
+                                                       float inv_t, Given g, Upstream up,
+                                                       const float2* __restrict__ saved,
+                                                       const float* __restrict__ entropy, T* __restrict__ out,
+                                                       int64_t ldo) {
+    constexpr int N = ONE ? kT : 64;  // threads of a row
+    const int sub = ONE ? threadIdx.x : threadIdx.x & 63;
+    const int64_t r = r0 + (ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6));
+    if (r >= rows) return;  // uniform over the row's threads
+    const int32_t first = (int32_t)blockIdx.y * stretch;
+    const int32_t end = classes - first < stretch ? classes : first + stretch;
+    const T* row = logits + r * ld;
+    T* to = out + r * ldo;
+    const float2 s = saved[r];
+    const float b = up.dentropy ? up.dentropy[r] : 0.f;
+    const float A = given_sum(g, up, r, classes, threadIdx.x & 63);
+    const Slope f{s.x, s.y, c1, up.dentropy ? fmaf(b, entropy[r], A) : A, b * kLn2, inv_t};
+    struct Vec {
+        T x[kVec];
+    };
+    for (int32_t c = first + sub * kVec; c < end; c += N * kVec) {
+        Vec v;
+        if (c + kVec <= end) {
+            __builtin_memcpy(&v, row + c, sizeof(v));
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) v.x[e] = from_float<T>(f.of(to_float(v.x[e])));
+            __builtin_memcpy(to + c, &v, sizeof(v));
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+                if (c + e < end) to[c + e] = from_float<T>(f.of(to_float(row[c + e])));
+        }
+    }
+    if (!up.dlogp || f.m == -INFINITY) return;  // uniform
+    __threadfence_block();
+    if constexpr (ONE) __syncthreads();
+    for (int j = sub; j < g.k; j += N) {
+        const int64_t c = g.at(r, j);
+        if (c < first || c >= end) continue;
+        float a = up.dlogp[r * g.k + j];
+        bool again = false;  // an earlier entry has the class: it adds this one
+        for (int o = 0; o < j && !again; ++o) again = g.at(r, o) == c;
+        if (again) continue;
+        for (int o = j + 1; o < g.k; ++o)
+            if (g.at(r, o) == c) a += up.dlogp[r * g.k + o];
+        to[c] = from_float<T>(fmaf(a, inv_t, f.of(to_float(row[c]))));
+    }
+}
+
+constexpr int64_t kMostBlocks = 1 << 23;  // of a launch: 2^31 threads
+constexpr int32_t kGradStretch = kChunk;
+
+// Stretches of a row: as many as it takes to fill the chip when there are few
+// rows, of at least 2,048 logits and 4 `top`.
+int32_t stretches(int64_t rows, int64_t classes, int64_t top) {
+    int64_t n = (1024 + rows - 1) / rows;
+    const int64_t least = 4 * top > 2048 ? 4 * top : 2048;
+    const int64_t most = classes / least;
+    if (n > most) n = most;
+    return n < 1 ? 1 : (int32_t)n;
+}
+
+bool by_wave(int64_t classes, int64_t top) { return classes <= kWaveClasses && top <= kWaveTop; }
+
+int check(const char* what, int32_t dtype, int64_t ld, int64_t rows, int64_t classes, int32_t k, float temperature) {
+    if (dtype != GRWS_F32 && dtype != GRWS_F16 && dtype != GRWS_BF16)
+        return set_error(GRWS_E_DTYPE, "%s: unsupported dtype %d", what, dtype);
+    GRWS_CHECK_ARG(rows >= 0 && rows <= INT32_MAX && classes > 0 && classes <= INT32_MAX - 65536 && ld >= classes,
+                   "%s: bad sizes", what);
+    GRWS_CHECK_ARG(k >= 1 && k <= 1024, "%s: 1 to 1024 given classes a row", what);
+    GRWS_CHECK_ARG(temperature > 0.f && temperature < INFINITY && kLog2e / temperature < INFINITY,
+                   "%s: the temperature must be positive", what);
+    return GRWS_OK;
+}
+
+int32_t bits_of(int64_t classes) {
+    int32_t b = 1;
+    while ((1ll << b) < classes) ++b;
+    return b;
+}
+
+template <typename T>
+int forward(const T* x, int64_t ld, int64_t rows, int32_t classes, int32_t top, const Scale& sc, const Given& g,
+            const Outputs& o, float4* part, uint64_t* best, hipStream_t stream) {
+    const int32_t cb = bits_of(classes);
+    if (by_wave(classes, top)) {
+        const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves));
+        if (classes <= 256)
+            hipLaunchKernelGGL((logp_wave_kernel<T, 4>), grid, dim3(kT), 0, stream, x, ld, rows, classes, cb, top, sc,
+                               g, o);
+        else
+            hipLaunchKernelGGL((logp_wave_kernel<T, 16>), grid, dim3(kT), 0, stream, x, ld, rows, classes, cb, top,
+                               sc, g, o);
+        GRWS_LAUNCH_CHECK();
+        return GRWS_OK;
+    }
+    const int32_t n = stretches(rows, classes, top);
+    const int32_t stretch = (int32_t)(((int64_t)classes + n - 1) / n + 63) / 64 * 64;  // (the last may be empty)
+    for (int64_t r0 = 0; r0 < rows; r0 += kMostBlocks) {  // (with several stretches there are fewer than 1,024 rows)
+        const dim3 grid((unsigned)(rows - r0 < kMostBlocks ? rows - r0 : kMostBlocks), (unsigned)n);
+#define GRWS_LOGP(MAXK)                                                                                              \
+    do {                                                                                                             \
+        if (n == 1) {                                                                                                \
+            hipLaunchKernelGGL((logp_rows_kernel<T, true, MAXK>), grid, dim3(kT), 0, stream, x, ld, r0, classes, cb, \
+                               top, stretch, sc, g, o, part, best);                                                  \
+        } else {                                                                                                     \
+            hipLaunchKernelGGL((logp_rows_kernel<T, false, MAXK>), grid, dim3(kT), 0, stream, x, ld, r0, classes,    \
+                               cb, top, stretch, sc, g, o, part, best);                                              \
+            GRWS_LAUNCH_CHECK();                                                                                     \
+            hipLaunchKernelGGL((logp_join_kernel<T, MAXK>), dim3(grid.x), dim3(kT), 0, stream, x, ld, r0, classes,   \
+                               cb, top, n, sc, g, o, part, best);                                                    \
+        }                                                                                                            \
+    } while (0)
+        if (top == 0) GRWS_LOGP(0);
+        else if (top <= kSmallK) GRWS_LOGP(kSmallK);
+        else GRWS_LOGP(kMaxK);
+#undef GRWS_LOGP
+        GRWS_LAUNCH_CHECK();
+    }
+    return GRWS_OK;
+}
+
+template <typename T>
+int backward(const T* x, int64_t ld, int64_t rows, int32_t classes, float c1, float inv_t, const Given& g,
+             const Upstream& up, const float2* saved, const float* entropy, T* out, int64_t ldo, hipStream_t stream) {
+    if (classes <= kWaveClasses) {
+        const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves));
+        hipLaunchKernelGGL((logp_grad_kernel<T, false>), grid, dim3(kT), 0, stream, x, ld, (int64_t)0, rows, classes,
+                           classes, c1, inv_t, g, up, saved, entropy, out, ldo);
+        GRWS_LAUNCH_CHECK();
+        return GRWS_OK;
+    }
+    // (at most 2^18 stretches of a row, so 2^13 rows or more of 2^31 threads)
+    const int64_t n = ((int64_t)classes + kGradStretch - 1) / kGradStretch;
+    const int64_t most = kMostBlocks / n < 1 ? 1 : kMostBlocks / n;
+    for (int64_t r0 = 0; r0 < rows; r0 += most) {
+        const dim3 grid((unsigned)(rows - r0 < most ? rows - r0 : most), (unsigned)n);
+        hipLaunchKernelGGL((logp_grad_kernel<T, true>), grid, dim3(kT), 0, stream, x, ld, r0, rows, classes,
+                           kGradStretch, c1, inv_t, g, up, saved, entropy, out, ldo);
+        GRWS_LAUNCH_CHECK();
+    }
+    return GRWS_OK;
+}
+
+}  // namespace
+}  // namespace grws
+
+using namespace grws;
+
+extern "C" size_t grws_log_probs_workspace_bytes(int64_t rows, int64_t classes, int32_t top) {
+    if (rows <= 0 || classes <= 0 || top < 0 || by_wave(classes, top)) return 0;
+    const int32_t n = stretches(rows, classes, top);
+    if (n == 1) return 0;
+    Sizer s;
+    s.take<float4>((size_t)rows * n);
+    s.take<uint64_t>((size_t)rows * n * top);
+    return s.used;
+}
+
+extern "C" int grws_log_probs_fwd(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t classes,
+                                  const void* index, int32_t index_is_i64, int32_t k, int32_t top, float temperature,
+                                  float* logp, float* entropy, float* saved, float* top_logp, int32_t* top_index,
+                                  void* workspace, size_t workspace_bytes, void* stream_) {
+    clear_error();
+    hipStream_t stream = as_stream(stream_);
+    GRWS_TRY(check("log_probs", dtype, ld, rows, classes, k, temperature));
+    GRWS_CHECK_ARG(top >= 0 && top <= kMaxK && top <= classes, "log_probs: top must be 0..min(classes, 1024)");
+    if (rows == 0) return GRWS_OK;
+    GRWS_CHECK_ARG(logits && index && logp && entropy && (top == 0 || (top_logp && top_index)),
+                   "log_probs: null pointer");
+    const int32_t n = by_wave(classes, top) ? 1 : stretches(rows, classes, top);
+    Carver cv(workspace, workspace_bytes);
+    float4* part = n > 1 ? cv.take<float4>((size_t)rows * n) : nullptr;
+    uint64_t* best = n > 1 ? cv.take<uint64_t>((size_t)rows * n * top) : nullptr;
+    if (!cv.ok)
+        return set_error(GRWS_E_CAPACITY, "log_probs: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
+    const Given g{index, k, index_is_i64};
+    const Outputs o{logp, entropy, reinterpret_cast<float2*>(saved), top_logp, top_index};
+    const Scale sc{kLog2e / temperature, 1.f / temperature};
+#define GRWS_LOGP_FWD(T)                                                                                         \
+    return forward(static_cast<const T*>(logits), ld, rows, (int32_t)classes, top, sc, g, o, part, best, stream)
+    if (dtype == GRWS_F32) GRWS_LOGP_FWD(float);
+    if (dtype == GRWS_F16) GRWS_LOGP_FWD(_Float16);
+    GRWS_LOGP_FWD(__hip_bfloat16);
+#undef GRWS_LOGP_FWD
+}
+
+extern "C" int grws_log_probs_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t classes,
+                                  const void* index, int32_t index_is_i64, int32_t k, float temperature,
+                                  const float* saved, const float* entropy, const float* dlogp,
+                                  const float* dentropy, void* grad, int64_t ldg, void* stream_) {
+    clear_error();
+    hipStream_t stream = as_stream(stream_);
+    GRWS_TRY(check("log_probs", dtype, ld, rows, classes, k, temperature));
+    GRWS_CHECK_ARG(ldg >= classes, "log_probs: bad sizes");
+    if (rows == 0) return GRWS_OK;
+    GRWS_CHECK_ARG(logits && index && saved && entropy && grad, "log_probs: null pointer");
+    const Given g{index, k, index_is_i64};
+    const Upstream up{dlogp, dentropy};
+    const float c1 = kLog2e / temperature;
+#define GRWS_LOGP_BWD(T)                                                                                     \
+    return backward(static_cast<const T*>(logits), ld, rows, (int32_t)classes, c1, 1.f / temperature, g, up, \
+                    reinterpret_cast<const float2*>(saved), entropy, static_cast<T*>(grad), ldg, stream)
+    if (dtype == GRWS_F32) GRWS_LOGP_BWD(float);
+    if (dtype == GRWS_F16) GRWS_LOGP_BWD(_Float16);
+    GRWS_LOGP_BWD(__hip_bfloat16);
+#undef GRWS_LOGP_BWD
+}

@@ -894,6 +894,31 @@ int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, int64_t rows,
                     void* values, int32_t* index, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Log probabilities of softmax(logits / T) of given classes, the entropy   */
+/* and the largest logits' log probabilities of each row of logits [rows x  */
+/* ld] (any alignment).  index (int32, or int64 with index_is_i64)          */
+/* [rows x k], 1 <= k <= 1024: the given classes; a negative one asks for   */
+/* nothing (0), one past the last is an error (NaN).  logp f32 [rows x k],  */
+/* entropy f32 [rows] (natural logarithms), saved f32 [rows x 2] (what the  */
+/* backward takes; may be NULL).  top > 0 (at most min(classes, 1024)):     */
+/* top_logp f32 and top_index int32 [rows x top], largest first, of equal   */
+/* logits the lowest class first, NaN as the largest.  A class of -inf has  */
+/* no probability; a row of nothing but -inf, or with NaN or +inf, is NaN.  */
+/* Backward of dlogp [rows x k] and dentropy [rows] (NULL: zeros): grad     */
+/* [rows x ldg] in dtype, every element written; a class given twice gets   */
+/* both; zeros in a row of nothing but -inf.  Same inputs, same bits.       */
+/* ------------------------------------------------------------------------ */
+size_t grws_log_probs_workspace_bytes(int64_t rows, int64_t classes, int32_t top);
+int grws_log_probs_fwd(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t classes,
+                       const void* index, int32_t index_is_i64, int32_t k, int32_t top, float temperature,
+                       float* logp, float* entropy, float* saved, float* top_logp, int32_t* top_index,
+                       void* workspace, size_t workspace_bytes, void* stream);
+int grws_log_probs_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t classes,
+                       const void* index, int32_t index_is_i64, int32_t k, float temperature, const float* saved,
+                       const float* entropy, const float* dlogp, const float* dentropy, void* grad, int64_t ldg,
+                       void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* The global norm of `count` gradients and clipping by it, what ends the   */
 /* reference's training steps (helper/engine.py:44-83).  Tensor i: sizes[i] */
 /* consecutive elements of dtypes[i] at grads[i], any alignment; the lists  */
