@@ -257,6 +257,12 @@ _PROTOS = {
     "grws_head_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(HeadView)]),
     "grws_head_bwd": (ctypes.c_int, [ctypes.POINTER(HeadView), _vp, _vp, _vp, _vp, _vp, ctypes.c_int32, _vp,
                                      ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, ctypes.c_size_t, _vp]),
+    "grws_head_log_probs_fwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(HeadView), ctypes.c_int32]),
+    "grws_head_log_probs_fwd": (ctypes.c_int, [ctypes.POINTER(HeadView), ctypes.c_int32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                               ctypes.c_size_t, _vp]),
+    "grws_head_log_probs_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(HeadView)]),
+    "grws_head_log_probs_bwd": (ctypes.c_int, [ctypes.POINTER(HeadView), _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64,
+                                               _vp, ctypes.c_int64, _vp, _vp, ctypes.c_size_t, _vp]),
     "grws_top_logits_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
     "grws_top_logits": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_int32, _vp, _vp, _vp, ctypes.c_size_t, _vp]),

@@ -1848,16 +1848,7 @@ def check_head(hidden, weight, bias=None, rows=None, labels=None, teacher_index=
     temperature), all on one GPU."""
     who = "linear_cross_entropy" if labels is not None else "linear_distill"
     L.require_device(who, hidden.device, weight, bias, rows, labels, teacher_index, teacher_logits)
-    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] or weight.numel() == 0:
-        raise ValueError(f"{who}: hidden must be [rows, width] and weight [classes, width] (got "
-                         f"{tuple(hidden.shape)} and {tuple(weight.shape)})")
-    L.dtype_code(hidden.dtype)
-    if weight.dtype != hidden.dtype or (bias is not None and bias.dtype != hidden.dtype):
-        raise TypeError(f"{who}: hidden, weight and bias must have one dtype")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError(f"{who}: bias must be [classes]")
-    if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int64):
-        raise ValueError(f"{who}: rows must be int64 [n]")
+    _check_head_operands(who, hidden, weight, bias, rows)
     if labels is not None:
         if labels.dim() != 1 or labels.dtype != torch.int64:
             raise ValueError(f"{who}: labels must be int64 [n]")
@@ -1871,6 +1862,23 @@ def check_head(hidden, weight, bias=None, rows=None, labels=None, teacher_index=
             raise ValueError(f"{who}: 1 to 1024 teacher entries a row (got {k})")
         if not 0.0 < float(temperature) < float("inf"):
             raise ValueError(f"{who}: the temperature must be positive (got {temperature})")
+    _check_head_rows(who, hidden, rows, n)
+
+
+def _check_head_operands(who, hidden, weight, bias, rows) -> None:
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] or weight.numel() == 0:
+        raise ValueError(f"{who}: hidden must be [rows, width] and weight [classes, width] (got "
+                         f"{tuple(hidden.shape)} and {tuple(weight.shape)})")
+    L.dtype_code(hidden.dtype)
+    if weight.dtype != hidden.dtype or (bias is not None and bias.dtype != hidden.dtype):
+        raise TypeError(f"{who}: hidden, weight and bias must have one dtype")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"{who}: bias must be [classes]")
+    if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int64):
+        raise ValueError(f"{who}: rows must be int64 [n]")
+
+
+def _check_head_rows(who, hidden, rows, n: int) -> None:
     if rows is not None and rows.shape[0] != n:
         raise ValueError(f"{who}: {rows.shape[0]} rows for {n} targets")
     if rows is None and n > hidden.shape[0]:
@@ -1879,7 +1887,8 @@ def check_head(hidden, weight, bias=None, rows=None, labels=None, teacher_index=
 
 class HeadCall:
     """The library's view of one classifier call (arguments as check_head
-    takes them), with the tensors that it points to."""
+    takes them; of log probabilities the given classes are labels or, without
+    logits, teacher_index), with the tensors that it points to."""
 
     def __init__(self, hidden, weight, bias=None, rows=None, labels=None, teacher_index=None, teacher_logits=None,
                  temperature: float = 1.0):
@@ -1891,7 +1900,8 @@ class HeadCall:
             self.n, self.k, i64 = labels.shape[0], 0, 0
         else:
             self.labels = None
-            self.index, self.logits = teacher_index.contiguous(), teacher_logits.float().contiguous()
+            self.index = teacher_index.contiguous()
+            self.logits = teacher_logits.float().contiguous() if teacher_logits is not None else None
             self.n, self.k = teacher_index.shape
             i64 = int(teacher_index.dtype == torch.int64)
         self.view = L.HeadView(self.hidden.data_ptr(), self.weight.data_ptr(), L.ptr(self.bias), L.ptr(self.rows),
@@ -1932,13 +1942,10 @@ def head_fwd(call: HeadCall, per_row: bool):
     return out, counts, saved
 
 
-def head_bwd(call: HeadCall, saved: torch.Tensor, counts: torch.Tensor, dloss: torch.Tensor,
-             need=(True, True, True)):
-    """(d_hidden, d_weight, d_bias), None where not needed, of head_fwd's
-    loss (dloss a scalar, or [n] per row)."""
+def _head_grads(call: HeadCall, need):
+    """Buffers for d_hidden (zeros where rows are left out), d_weight and
+    d_bias, None where not needed."""
     dev = call.hidden.device
-    lse, logit, prob = call.saved_pointers(saved)
-    dl = dloss.float().contiguous()
     dh = dw = db = None
     if need[0]:
         some = call.rows is not None or call.n < call.hidden.shape[0]
@@ -1947,6 +1954,17 @@ def head_bwd(call: HeadCall, saved: torch.Tensor, counts: torch.Tensor, dloss: t
         dw = torch.empty(call.weight.shape, dtype=call.weight.dtype, device=dev)
     if need[2] and call.bias is not None:
         db = torch.empty(call.bias.shape, dtype=call.bias.dtype, device=dev)
+    return dh, dw, db
+
+
+def head_bwd(call: HeadCall, saved: torch.Tensor, counts: torch.Tensor, dloss: torch.Tensor,
+             need=(True, True, True)):
+    """(d_hidden, d_weight, d_bias), None where not needed, of head_fwd's
+    loss (dloss a scalar, or [n] per row)."""
+    dev = call.hidden.device
+    lse, logit, prob = call.saved_pointers(saved)
+    dl = dloss.float().contiguous()
+    dh, dw, db = _head_grads(call, need)
     ref = ctypes.byref(call.view)
     lib = L.load()
     wsb = lib.grws_head_bwd_workspace_bytes(ref)
@@ -2040,6 +2058,58 @@ def log_probs_fwd(logits: torch.Tensor, index: torch.Tensor, temperature: float,
 
 def _f32_rows(t: Optional[torch.Tensor]):
     return t.float().contiguous() if t is not None else None
+
+
+def check_linear_log_probs(hidden, weight, index, bias, rows, temperature: float, top: int) -> None:
+    """Raises unless the arguments are linear_log_probs': those of a classifier
+    call (check_head) and index int32 or int64 [n] or [n, k], all on one GPU."""
+    who = "linear_log_probs"
+    L.require_device(who, hidden.device, weight, index, bias, rows)
+    _check_head_operands(who, hidden, weight, bias, rows)
+    n, _ = _check_given(who, index, weight.shape[0], temperature, top)
+    _check_head_rows(who, hidden, rows, n)
+
+
+def given_call(hidden, weight, index, bias, rows, temperature: float) -> HeadCall:
+    """The HeadCall of linear_log_probs: one class a row goes as its label (found
+    in the product's own registers), several as a list."""
+    if index.dim() == 1 or index.shape[1] == 1:
+        return HeadCall(hidden, weight, bias, rows, labels=index.reshape(-1).long(), temperature=temperature)
+    return HeadCall(hidden, weight, bias, rows, teacher_index=index, temperature=temperature)
+
+
+def head_log_probs_fwd(call: HeadCall, shape, top: int):
+    """(logp of `shape`, entropy [n], saved f32 [2, n], top_logp, top_index
+    [n, top] or None) of a given_call (csrc/head.hip).  No host sync."""
+    dev, n = call.hidden.device, call.n
+    logp = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(n, dtype=torch.float32, device=dev)
+    saved = torch.empty((2, n), dtype=torch.float32, device=dev)
+    top_logp, top_index = _top_outputs(n, top, dev)
+    ref = ctypes.byref(call.view)
+    wsb = L.load().grws_head_log_probs_fwd_workspace_bytes(ref, top)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        L.call("grws_head_log_probs_fwd", ref, top, logp.data_ptr(), entropy.data_ptr(), saved.data_ptr(),
+               L.ptr(top_logp), L.ptr(top_index), ws.data_ptr(), wsb, L.stream_of(dev))
+    return logp, entropy, saved, top_logp, top_index
+
+
+def head_log_probs_bwd(call: HeadCall, saved: torch.Tensor, logp: torch.Tensor, entropy: torch.Tensor,
+                       dlogp: Optional[torch.Tensor], dentropy: Optional[torch.Tensor], need=(True, True, True)):
+    """(d_hidden, d_weight, d_bias), None where not needed, of
+    head_log_probs_fwd's logp and entropy (upstream None: zeros)."""
+    dev = call.hidden.device
+    dlogp, dentropy = _f32_rows(dlogp), _f32_rows(dentropy)
+    dh, dw, db = _head_grads(call, need)
+    ref = ctypes.byref(call.view)
+    wsb = L.load().grws_head_log_probs_bwd_workspace_bytes(ref)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    width = call.hidden.shape[1]
+    with _on_device(dev):
+        L.call("grws_head_log_probs_bwd", ref, saved.data_ptr(), logp.data_ptr(), entropy.data_ptr(), L.ptr(dlogp),
+               L.ptr(dentropy), L.ptr(dh), width, L.ptr(dw), width, L.ptr(db), ws.data_ptr(), wsb, L.stream_of(dev))
+    return dh, dw, db
 
 
 def log_probs_bwd(logits: torch.Tensor, index: torch.Tensor, temperature: float, saved: torch.Tensor,

@@ -49,7 +49,8 @@
 // a b128 read of 16 rows spreads over all banks) or strided along k (rows of
 // BP or BQ columns, 32-byte chunks XORed with the row, read by gfx950's
 // transposing LDS read, two per 32 k).
-#include "grws_internal.h"
+#include "logp.h"
+#include "top_pool.h"
 
 namespace grws {
 namespace {
@@ -69,8 +70,6 @@ typedef __attribute__((address_space(3))) char lds_char_t;
 
 constexpr int kK = 64;               // k of a stage; the operands' k is padded to whole stages
 constexpr int64_t kIgnoreLabel = -100;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kPastEnd = 0x80000000u;  // past every resource: the load returns zeros
 
 // An operand in memory.  Contiguous along k: `rows` rows of `k` elements.
@@ -376,6 +375,24 @@ __device__ __forceinline__ float past_rounding(float m, float c1) {
     return fabsf(ref) == INFINITY ? 1.f : __builtin_amdgcn_exp2f(-fmaf(m, c1, -ref));
 }
 
+// Log probabilities and entropies: (m, s, t) of each row's strips, s and t
+// against the rounded m c1, and the logits themselves where alternatives are
+// looked for.
+struct Strips {
+    float4* part;
+    int64_t row, strip;  // entries from a row, a strip, to the next
+    float* z;            // [np][ldz], or NULL
+    int64_t ldz;
+};
+
+// What strip (m, s, t) is against m c1 itself.
+__device__ __forceinline__ Stats exact_strip(const float4& v, float c1) {
+    Stats a{v.x, v.y, v.z};
+    const float ref = a.m * c1;
+    if (fabsf(ref) != INFINITY) move(a, -fmaf(a.m, c1, -ref));
+    return a;
+}
+
 struct StatsArgs {
     Gemm g;
     int64_t v0, classes;  // first class of the piece, all classes
@@ -387,6 +404,7 @@ struct StatsArgs {
     float2* part;           // [strips][np]: largest logit m, sum of 2^(z c1 - the rounded m c1)
     float* ylabel;          // [n]: the label's logit
     int32_t* earlier;       // [n]: an earlier class of the label's strip has the label's logit
+    Strips strips;          // instead of part
 };
 
 // Bound by the matrix cores for wide D (8,192 x 131,072 x 4,096 bf16: 6.6 ms,
@@ -396,7 +414,7 @@ struct StatsArgs {
 // 8,200 MFMA cycles and about 9,000 VALU cycles follow one another).  p are
 // classes and q rows, so a lane holds 4 TP classes of TQ rows and the
 // reduction over classes takes two cross-lane steps a row.
-template <int DT, int BP, int BQ, int WP, int WQ>
+template <int DT, bool GIVEN, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
     using C = Core<DT, false, false, BP, BQ, WP, WQ>;
     constexpr int TP = C::TP, TQ = C::TQ;
@@ -420,14 +438,29 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
         m = fmaxf(m, __shfl_xor(m, 16, kWave));
         m = fmaxf(m, __shfl_xor(m, 32, kWave));
         const float c1 = base2(m, a.c1), ref = m == -INFINITY ? 0.f : m * c1;  // nothing but -inf: a sum of zeros
-        float s = 0.f;
+        float s = 0.f, t = 0.f;
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref));
+            for (int e = 0; e < 4; ++e) {
+                const float u = fmaf(acc[i][j][e], c1, -ref), x = __builtin_amdgcn_exp2f(u);
+                s += x;
+                if constexpr (GIVEN) t = fmaf(x, reach(u), t);
+            }
         s += __shfl_xor(s, 16, kWave);
         s += __shfl_xor(s, 32, kWave);
-        if (lane < 16) a.part[strip * a.np + row] = make_float2(m, s);
+        if constexpr (GIVEN) {
+            t += __shfl_xor(t, 16, kWave);
+            t += __shfl_xor(t, 32, kWave);
+            if (lane < 16) a.strips.part[strip * a.strips.strip + row * a.strips.row] = make_float4(m, s, t, 0.f);
+            if (a.strips.z) {  // uniform
+                float* z = a.strips.z + row * a.strips.ldz + vfirst;
+#pragma unroll
+                for (int i = 0; i < TP; ++i) *reinterpret_cast<float4_t*>(z + C::p_of(i, lane)) = acc[i][j];
+            }
+        } else {
+            if (lane < 16) a.part[strip * a.np + row] = make_float2(m, s);
+        }
         if (a.labels) {
             const int64_t lab = row < a.n ? a.labels[row] - vfirst : -1;
             const bool here = lab >= 0 && lab < TP * 16 && lab + vfirst < a.classes;
@@ -439,17 +472,16 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y = C::p_of(i, lane) + e == l ? acc[i][j][e] : y;
                 y = __shfl(y, (((l >> 3) & 3) << 4) | (lane & 15), kWave);  // its lane: p_of's
-                int tie = 0;
+                if (here && lane < 16) a.ylabel[row] = y;
+                if constexpr (!GIVEN) {
+                    int tie = 0;
 #pragma unroll
-                for (int i = 0; i < TP; ++i)
+                    for (int i = 0; i < TP; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        tie |= acc[i][j][e] == y && C::p_of(i, lane) + e < l;
-                tie |= __shfl_xor(tie, 16, kWave);
-                tie |= __shfl_xor(tie, 32, kWave);
-                if (here && lane < 16) {
-                    a.ylabel[row] = y;
-                    a.earlier[row] = tie;
+                        for (int e = 0; e < 4; ++e) tie |= acc[i][j][e] == y && C::p_of(i, lane) + e < l;
+                    tie |= __shfl_xor(tie, 16, kWave);
+                    tie |= __shfl_xor(tie, 32, kWave);
+                    if (here && lane < 16) a.earlier[row] = tie;
                 }
             }
         }
@@ -480,6 +512,18 @@ __device__ __forceinline__ float2 base_of(float lse, float c1) {
     return lse == -INFINITY ? make_float2(__uint_as_float(1), 0.f) : make_float2(c1, lse);
 }
 
+// The gradient of log probabilities of given classes c_j and of an entropy,
+// with a_j and b theirs and A = sum a_j:
+//   dz_v = (sum_j a_j [v = c_j] - p_v (A + b (ln p_v + H))) / T
+// of which G holds dz T gscale / most (see Alpha; |dz T| <= sum |a_j| + |b|
+// (H + 1), whose largest is `most`).  With p = 2^u factor (RowStats) the
+// bracket is slope + bend u.
+struct GivenRow {
+    float slope, bend;  // (A + b (H + ln factor)) / most, b ln2 / most
+    float a;            // of one given class: a / most
+    float pad;
+};
+
 struct GradArgs {
     Gemm g;
     int64_t v0, classes, n;
@@ -494,6 +538,7 @@ struct GradArgs {
     int64_t ldg, plane;
     float* bias_part;  // [np / kBiasRows][vt]: column sums, or NULL
     int64_t vt;
+    const GivenRow* given;  // [n]: log probabilities' and entropies'
 };
 
 __device__ __forceinline__ uint16_t top16(float x) { return (uint16_t)(__float_as_uint(x) >> 16); }
@@ -556,7 +601,7 @@ constexpr int kBiasRows = 64;  // rows of a part of the bias gradient's sums
 // The same product, leaving G.  8,192 x 65,536 of 4,096: 3.52 ms (1,250
 // TFLOP/s); 16,384 x 20,224 of 256: 304 us (558), where 660 MB of G go out
 // beside the exponentials.
-template <int DT, int PLANES, int BP, int BQ, int WP, int WQ>
+template <int DT, int PLANES, bool GIVEN, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
     using C = Core<DT, false, false, BP, BQ, WP, WQ>;
     constexpr int TP = C::TP, TQ = C::TQ;
@@ -569,9 +614,11 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
     // the rows' statistics are here when the product is (asked for behind it,
     // 16,384 x 20,224 of 256 takes 322 us, not 300); run() has barriers
     __shared__ float2 row_stats[BQ];
+    __shared__ GivenRow row_given[GIVEN ? BQ : 1];
     if (threadIdx.x < BQ) {
         const int64_t row = (int64_t)tq * BQ + threadIdx.x;
         row_stats[threadIdx.x] = row < a.n ? a.stats.of(row) : make_float2(INFINITY, 0.f);
+        if constexpr (GIVEN) row_given[threadIdx.x] = row < a.n ? a.given[row] : GivenRow{0.f, 0.f, 0.f, 0.f};
     }
     begin_logits<C>(acc, a.v0 + pfirst, a.classes, a.bias, a.bias_dt, lane);
     C::run(a.g, tp, tq, 0, a.g.ksteps, p0, q0, p1, q1, acc);
@@ -582,9 +629,11 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
         // (its hidden row is zeros, so a logit is its bias)
         const float2 st = row_stats[row - (int64_t)tq * BQ];
         const float lse = st.x, c1 = base_of(lse, a.c1).x, ref = base_of(lse, a.c1).y;
-        const float s = a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
+        GivenRow given;
+        if constexpr (GIVEN) given = row_given[row - (int64_t)tq * BQ];
+        const float s = !GIVEN && a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
         const bool stray = row >= a.n || (lse == INFINITY && st.y != 0.f);
-        const float f = stray ? 0.f : st.y * s;
+        const float f = stray ? 0.f : GIVEN ? -st.y * s : st.y * s;
         if (__any(stray)) {
 #pragma unroll
             for (int i = 0; i < TP; ++i)
@@ -594,10 +643,15 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref));
+            for (int e = 0; e < 4; ++e) {
+                const float u = fmaf(acc[i][j][e], c1, -ref);
+                acc[i][j][e] = __builtin_amdgcn_exp2f(u);
+                if constexpr (GIVEN) acc[i][j][e] *= fmaf(given.bend, reach(u), given.slope);
+            }
 #pragma unroll
         for (int i = 0; i < TP; ++i) acc[i][j] *= f;
         if (a.labels) {
+            const float at_label = GIVEN ? -given.a * s : s;
             const int64_t lab = lse != INFINITY ? a.labels[row] - a.v0 - pfirst : -1;
             const bool here = lab >= 0 && lab < TP * 16;
             if (__any(here)) {
@@ -605,7 +659,7 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
 #pragma unroll
                 for (int i = 0; i < TP; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= at == C::p_of(i, lane) + e ? s : 0.f;
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= at == C::p_of(i, lane) + e ? at_label : 0.f;
             }
         }
 #pragma unroll
@@ -807,6 +861,7 @@ struct Targets {
     const int64_t* rows;
     int64_t hidden_rows, classes;
     int32_t k, i64;
+    int32_t given;  // labels or tindex are the classes of log probabilities: every row with a place in hidden counts
 };
 
 __device__ __forceinline__ int64_t teacher_at(const Targets& t, int64_t i, int k) {
@@ -816,7 +871,7 @@ __device__ __forceinline__ int64_t teacher_at(const Targets& t, int64_t i, int k
 
 // an entry of weight zero (a logit of -inf) is not listed
 __device__ __forceinline__ bool teacher_listed(const Targets& t, int64_t i, int k, int64_t idx) {
-    return idx >= 0 && idx < t.classes && t.tlogit[i * t.k + k] != -INFINITY;
+    return idx >= 0 && idx < t.classes && (t.given || t.tlogit[i * t.k + k] != -INFINITY);
 }
 
 // `lanes` lanes of a wave, of which this is `sub`, ask together (all of them
@@ -825,6 +880,7 @@ template <int LANES>
 __device__ __forceinline__ int row_state(const Targets& t, int64_t i, int sub) {
     const int64_t row = t.rows ? t.rows[i] : i;
     if (row < 0 || row >= t.hidden_rows) return 2;
+    if (t.given) return 1;
     if (t.labels) {
         const int64_t l = t.labels[i];
         if (l == kIgnoreLabel) return 0;
@@ -983,6 +1039,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets t, const T* _
     }
     if (k0 != 0) return;
     if (lane == 0) state[i] = st;
+    if (t.given) return;
     float m = -INFINITY;
     for (int k = lane; k < t.k && live; k += 64)
         if (teacher_listed(t, i, k, teacher_at(t, i, k))) m = fmaxf(m, t.tlogit[i * t.k + k] * inv_t);
@@ -1047,16 +1104,19 @@ struct FewArgs {
     int64_t ldg, plane;
     float* bias_part;
     int64_t vt;
+    // log probabilities
+    Strips strips;          // forward, instead of part
+    const GivenRow* given;  // backward
 };
 
-template <typename T, int NQ, int PLANES, bool VEC>
+template <typename T, int NQ, int PLANES, bool GIVEN, bool VEC>
 __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     constexpr bool GRAD = PLANES > 0;
     constexpr int DT = std::is_same_v<T, _Float16> ? GRWS_F16 : GRWS_BF16;
     constexpr int E = 16 / sizeof(T);  // elements of a 16-byte load
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int64_t first = (int64_t)blockIdx.y * (16 * NQ);  // row
-    if (!GRAD && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.done = 0;
+    if (!GRAD && !GIVEN && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.done = 0;
     const int64_t vfirst = a.v0 + ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
     const T* w[2];
     const T* h[NQ];
@@ -1070,7 +1130,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     for (int j = 0; j < NQ; ++j) {
         const int64_t row = first + 16 * j + r;
         if constexpr (GRAD) live[j] = row < a.n && a.stats.lse[row] != INFINITY;
-        else live[j] = row < a.n && (a.t.labels ? row_state<1>(a.t, row, 0) : a.states[row]) == 1;
+        else live[j] = row < a.n && (GIVEN || a.t.labels ? row_state<1>(a.t, row, 0) : a.states[row]) == 1;
         h[j] = static_cast<const T*>(a.hidden) + (live[j] ? (a.t.rows ? a.t.rows[row] : row) * a.ldh : 0);
     }
     float4_t acc[2][NQ];
@@ -1160,17 +1220,33 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
             m = fmaxf(m, __shfl_xor(m, 32, kWave));
             y = __shfl(y, (((l >> 2) & 3) << 4) | r, kWave);
             const float c1 = base2(m, a.c1), ref = m == -INFINITY ? 0.f : m * c1;
-            float s = 0.f;
+            float s = 0.f, t = 0.f;
             int tie = 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref));
+                    const float u = fmaf(acc[i][j][e], c1, -ref), x = __builtin_amdgcn_exp2f(u);
+                    s += x;
+                    if constexpr (GIVEN) t = fmaf(x, reach(u), t);
                     tie |= acc[i][j][e] == y && 16 * i + 4 * g + e < l;
                 }
             s += __shfl_xor(s, 16, kWave);
             s += __shfl_xor(s, 32, kWave);
+            if constexpr (GIVEN) {
+                t += __shfl_xor(t, 16, kWave);
+                t += __shfl_xor(t, 32, kWave);
+                if (a.strips.z && row < a.n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<float4_t*>(a.strips.z + row * a.strips.ldz + vfirst + 16 * i + 4 * g) =
+                            acc[i][j];
+                if (g == 0) {
+                    a.strips.part[vfirst / 32 * a.strips.strip + row * a.strips.row] = make_float4(m, s, t, 0.f);
+                    if (here) a.ylabel[row] = y;
+                }
+                continue;
+            }
             tie |= __shfl_xor(tie, 16, kWave);
             tie |= __shfl_xor(tie, 32, kWave);
             if (g == 0) {
@@ -1183,15 +1259,21 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
         } else {
             const float2 st = live[j] ? a.stats.of(row) : make_float2(INFINITY, 0.f);
             const float c1 = base_of(st.x, a.c1).x, ref = base_of(st.x, a.c1).y;
-            const float sc = a.row_scale && live[j] ? a.row_scale[row] * a.gscale : a.gscale;
-            const float f = st.y * sc;
+            const float sc = !GIVEN && a.row_scale && live[j] ? a.row_scale[row] * a.gscale : a.gscale;
+            const float f = GIVEN ? -st.y * sc : st.y * sc;
+            GivenRow given{0.f, 0.f, 0.f, 0.f};
+            if (GIVEN && live[j]) given = a.given[row];
+            const float at_label = GIVEN ? -given.a * sc : sc;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 uint16_t x[4][PLANES > 0 ? PLANES : 1];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float p = live[j] ? __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c1, -ref)) * f : 0.f;
-                    p = 16 * i + 4 * g + e == l ? p - sc : p;
+                    const float u = fmaf(acc[i][j][e], c1, -ref);
+                    float p = __builtin_amdgcn_exp2f(u);
+                    if constexpr (GIVEN) p *= fmaf(given.bend, reach(u), given.slope);
+                    p = live[j] ? p * f : 0.f;
+                    p = 16 * i + 4 * g + e == l ? p - at_label : p;
                     sums[i][e] += p;
                     planes_of<DT, PLANES>(p, x[e]);
                 }
@@ -1579,7 +1661,9 @@ __global__ __launch_bounds__(256) void head_subtract_kernel(Targets t, RowStats 
 constexpr int kBiasClasses = 4096;
 constexpr float kBiasUnit = 1099511627776.f;
 
+// place: NULL, or the classes of given lists, whose coefficients are added.
 __global__ __launch_bounds__(256) void head_bias_targets_kernel(Targets t, RowStats stats,
+                                                                const int32_t* __restrict__ place,
                                                                 const float* __restrict__ coef,
                                                                 const float* __restrict__ row_scale, float gscale,
                                                                 int64_t n, int64_t v0, int64_t vc, int64_t vt,
@@ -1596,9 +1680,9 @@ __global__ __launch_bounds__(256) void head_bias_targets_kernel(Targets t, RowSt
     auto entries = [&](auto use) {
         for (int e = threadIdx.x; e < rows * t.k; e += 256) {
             const int64_t i = first + e / t.k, at = first * t.k + e;
-            const int64_t c = teacher_at(t, i, e % t.k) - v0 - c0;
-            if (c < 0 || c >= classes || coef[at] < 0.f || stats.lse[i] == INFINITY) continue;
-            use((int)c, row_scale ? coef[at] * row_scale[i] : coef[at]);
+            const int64_t c = (place ? place[at] : teacher_at(t, i, e % t.k)) - v0 - c0;
+            if (c < 0 || c >= classes || (!place && coef[at] < 0.f) || stats.lse[i] == INFINITY) continue;
+            use((int)c, place ? -coef[at] : row_scale ? coef[at] * row_scale[i] : coef[at]);
         }
     };
     entries([&](int c, float q) {
@@ -1677,6 +1761,295 @@ __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __res
     if (row < 0 || row >= hidden_rows) return;
     const bool keep = stats.lse[i] != INFINITY;  // a row that does not count gets zeros
     sum_splits(part + i * dp, splits, np * dp, width, *alpha, keep, out + row * ldo);
+}
+
+// ---------------------------------------------------------------------------
+// log probabilities of given classes and entropies
+// ---------------------------------------------------------------------------
+// What a call returns and keeps of each row (see RowStats for lse, factor).
+struct GivenOut {
+    float* logp;     // [n k]
+    float* entropy;  // [n]
+    float* lse;      // [n]
+    float* factor;   // [n]
+};
+
+// A row's statistics to lse, factor and entropy, by one thread.  Entropies of
+// rows without a place in hidden, of nothing but -inf (neither counts in the
+// gradient) or with a NaN or +inf are NaN.
+__device__ __forceinline__ void put_given_row(const Stats& a, float c1, bool live, const GivenOut& o, int64_t i) {
+    const float nan = __int_as_float(0x7fc00000);
+    float l = INFINITY, f = a.s == a.s ? 0.f : a.s, h = nan;
+    if (live && a.m != -INFINITY) {
+        const float l2 = log2f(a.s);
+        l = fmaf(a.m, c1, l2);
+        f = l == -INFINITY ? (a.s > 0.f ? 1.f / a.s : nan) : __builtin_amdgcn_exp2f(-fmaf(a.m, c1, -l)) / a.s;
+        if (l == INFINITY) l = nan;
+        h = kLn2 * (l2 - a.t / a.s);
+    }
+    o.lse[i] = l;
+    o.factor[i] = f;
+    o.entropy[i] = h;
+}
+
+// log p of a given class (0 where none is) whose logit is z
+__device__ __forceinline__ float given_logp(const Stats& a, bool live, int64_t cls, int64_t classes, float z,
+                                            float inv_t) {
+    if (!live || cls >= classes || a.m == -INFINITY) return __int_as_float(0x7fc00000);
+    return cls < 0 ? 0.f : fmaf(z - a.m, inv_t, -kLn2 * log2f(a.s));
+}
+
+__device__ __forceinline__ int64_t given_at(const Targets& t, int64_t i, int k) {
+    return t.labels ? t.labels[i] : teacher_at(t, i, k);
+}
+
+// Joins the strips of R rows (512 / R at a time).  y: the given classes'
+// logits [n max(k, 1)].
+template <int R>
+__global__ __launch_bounds__(512) void head_given_join_kernel(Targets t, Strips part, int64_t strips, int64_t n,
+                                                              float c1, float inv_t, const float* __restrict__ y,
+                                                              GivenOut o) {
+    __shared__ float sm[8][R], ss[8][R], st[8][R];
+    constexpr int G = 64 / R;  // lanes of a wave that share a row
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane % R, g = lane / R;
+    const int64_t i = (int64_t)blockIdx.x * R + r;
+    Stats a = no_stats();
+    auto join_lanes = [&]() {
+#pragma unroll
+        for (int d = R; d < 64; d <<= 1) {
+            const Stats b{__shfl_xor(a.m, d, kWave), __shfl_xor(a.s, d, kWave), __shfl_xor(a.t, d, kWave)};
+            a = lane & d ? join(b, a, c1) : join(a, b, c1);  // both sides in one order
+        }
+    };
+    if (i < n) {
+#pragma unroll 4
+        for (int64_t k = wave * G + g; k < strips; k += 8 * G)
+            a = join(a, exact_strip(part.part[k * part.strip + i * part.row], c1), c1);
+    }
+    join_lanes();
+    if (g == 0) {
+        sm[wave][r] = a.m;
+        ss[wave][r] = a.s;
+        st[wave][r] = a.t;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    a = no_stats();
+    for (int w = g; w < 8; w += G) a = join(a, Stats{sm[w][r], ss[w][r], st[w][r]}, c1);
+    join_lanes();
+    if (i >= n) return;
+    const bool live = row_state<1>(t, i, 0) == 1;
+    const int k = t.labels ? 1 : t.k;
+    for (int j = g; j < k; j += G) o.logp[i * k + j] = given_logp(a, live, given_at(t, i, j), t.classes, y[i * k + j], inv_t);
+    if (g == 0) put_given_row(a, c1, live, o, i);
+}
+
+// A work-group a row: joins its strips, reads the given classes' logits, and
+// finds the `top` largest.  They lie in the `top` strips with the largest
+// maxima (of equal ones the first: each holds a logit in front of any that is
+// left out), so of z no more than those is read, and of those what reaches the
+// last one's maximum is looked at.
+template <int MAXK>
+__global__ __launch_bounds__(kT) void head_top_kernel(Targets t, Strips part, int32_t strips, int32_t strip_classes,
+                                                      int32_t strip_bits, int32_t class_bits, int32_t top, float c1,
+                                                      float inv_t, GivenOut o, float* __restrict__ top_logp,
+                                                      int32_t* __restrict__ top_index) {
+    __shared__ Pool<MAXK> p;
+    __shared__ float sm[kWaves], ss[kWaves], st[kWaves];
+    __shared__ int32_t chosen[MAXK];
+    __shared__ uint32_t reached;
+    constexpr int OFFER = Sizes<MAXK>::OFFER;
+    const int64_t i = blockIdx.x;
+    const float4* mine = part.part + i * part.row;
+    const float* z = part.z + i * part.ldz;
+    const uint64_t low = (1ull << strip_bits) - 1;
+    if (threadIdx.x == 0) {
+        p.count = 0;
+        reached = ~0u;
+    }
+    Stats a = no_stats();
+    uint64_t bound = 0;
+    for (int32_t c = 0; c < strips; c += kT * OFFER) {
+        uint64_t x[OFFER];
+#pragma unroll
+        for (int e = 0; e < OFFER; ++e) {
+            const int32_t k = c + e * kT + (int32_t)threadIdx.x;
+            x[e] = 0;
+            if (k < strips) {
+                const float4 v = mine[k];
+                a = join(a, exact_strip(v, c1), c1);
+                // a sum that is not a number: a NaN in the strip, larger than everything
+                x[e] = ((uint64_t)order_of<float>(v.y == v.y ? v.x : v.y) << strip_bits) | (low - (uint32_t)k);
+            }
+        }
+        offer(p, x, top, 32 + strip_bits, bound);
+    }
+    a = join_wave(a, c1);
+    if ((threadIdx.x & 63) == 0) {
+        sm[threadIdx.x >> 6] = a.m;
+        ss[threadIdx.x >> 6] = a.s;
+        st[threadIdx.x >> 6] = a.t;
+    }
+    keep_best(p, top, 32 + strip_bits);
+    __syncthreads();
+    a = Stats{sm[0], ss[0], st[0]};
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) a = join(a, Stats{sm[w], ss[w], st[w]}, c1);
+    const bool live = row_state<1>(t, i, 0) == 1;
+    const int k = t.labels ? 1 : t.k;
+    for (int j = threadIdx.x; j < k; j += kT) {
+        const int64_t cls = given_at(t, i, j);
+        o.logp[i * k + j] =
+            given_logp(a, live, cls, t.classes, z[cls < 0 || cls >= t.classes ? 0 : cls], inv_t);
+    }
+    if (threadIdx.x == 0) put_given_row(a, c1, live, o, i);
+    const int n = p.count < top ? p.count : top;
+    for (int j = threadIdx.x; j < n; j += kT) {
+        const uint64_t key = p.keys[j];
+        chosen[j] = (int32_t)(low - (key & low));
+        if (n == top) atomicMin(&reached, (uint32_t)(key >> strip_bits));  // whole numbers: no order
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) p.count = 0;
+    // (strips with a NaN or an infinity: everything in them is looked at)
+    bound = n == top && reached != ~0u ? ((uint64_t)reached << class_bits) - 1 : 0;
+    const uint64_t all = (1ull << class_bits) - 1;
+    const int32_t count = n * strip_classes;
+    for (int32_t c = 0; c < count; c += kT * OFFER) {
+        uint64_t x[OFFER];
+#pragma unroll
+        for (int e = 0; e < OFFER; ++e) {
+            const int32_t at = c + e * kT + (int32_t)threadIdx.x;
+            x[e] = 0;
+            if (at < count) {
+                const int64_t cls = (int64_t)chosen[at / strip_classes] * strip_classes + at % strip_classes;
+                if (cls < t.classes) x[e] = ((uint64_t)order_of<float>(z[cls]) << class_bits) | (all - (uint32_t)cls);
+            }
+        }
+        offer(p, x, top, 32 + class_bits, bound);
+    }
+    put_best(p, top, 32 + class_bits, class_bits, [&](int at, int32_t cls) {
+        top_index[i * top + at] = cls;
+        top_logp[i * top + at] = given_logp(a, live, cls, t.classes, z[cls], inv_t);
+    });
+}
+
+// The rows' parts of the gradient before `most` is known (a row that does not
+// count: zeros), a wave a row; of lists also place (the class, at the first
+// entry that lists it; -1 at any other) and coef (its sum).  most: of each
+// work-group the largest finite bound of |dz T|.
+constexpr int kGivenBlocks = 1024;
+
+__global__ __launch_bounds__(256) void head_given_rows_kernel(Targets t, RowStats stats, int64_t n,
+                                                              const float* __restrict__ entropy,
+                                                              const float* __restrict__ dlogp,
+                                                              const float* __restrict__ dentropy,
+                                                              GivenRow* __restrict__ out,
+                                                              int32_t* __restrict__ place, float* __restrict__ coef,
+                                                              float* __restrict__ most) {
+    __shared__ float red[4];
+    const int lane = threadIdx.x & 63;
+    const int k = t.labels ? 1 : t.k;
+    float best = 0.f;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+        const float2 st = stats.of(i);
+        const bool live = st.x != INFINITY;
+        auto entry = [&](int j, int64_t* cls) {
+            *cls = live && dlogp && j < k ? given_at(t, i, j) : -1;
+            if (*cls >= t.classes) *cls = -1;
+            return *cls >= 0 ? dlogp[i * k + j] : 0.f;
+        };
+        float sum = 0.f, mag = 0.f;
+        for (int jb = 0; jb < k; jb += 64) {
+            const int j = jb + lane;
+            int64_t cls;
+            const float x = entry(j, &cls);
+            sum += x;
+            mag += fabsf(x);
+            if (!place) continue;
+            float both = x;
+            bool first = cls >= 0;
+            for (int ob = 0; ob < k; ob += 64) {
+                int64_t ocls;
+                const float ox = entry(ob + lane, &ocls);
+                const int many = k - ob < 64 ? k - ob : 64;
+                for (int o = 0; o < many; ++o) {
+                    const int other = __shfl((int)ocls, o, kWave);
+                    const float y = __shfl(ox, o, kWave);
+                    if (ob + o != j && other == (int)cls) {
+                        both += y;
+                        first = first && ob + o > j;
+                    }
+                }
+            }
+            if (j < k) {
+                place[i * k + j] = first ? (int32_t)cls : -1;
+                coef[i * k + j] = both;
+            }
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            sum += __shfl_xor(sum, d, kWave);
+            mag += __shfl_xor(mag, d, kWave);
+        }
+        const float b = live && dentropy ? dentropy[i] : 0.f, h = live && dentropy ? entropy[i] : 0.f;
+        mag += fabsf(b) * (h + 1.f);
+        if (mag < INFINITY) best = fmaxf(best, mag);
+        if (lane == 0)
+            out[i] = live ? GivenRow{dentropy ? fmaf(b, fmaf(kLn2, log2f(st.y), h), sum) : sum, b * kLn2, sum, 0.f}
+                          : GivenRow{0.f, 0.f, 0.f, 0.f};
+    }
+    if (lane == 0) red[threadIdx.x >> 6] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) most[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// Divides by the largest of them (where all are zero, nothing but what is not
+// finite is left), and the factor of the sums: most T' with T' = 1 / (T gscale).
+__global__ __launch_bounds__(256) void head_given_scale_kernel(const float* __restrict__ most, int32_t blocks,
+                                                               int64_t n, int64_t entries, float factor,
+                                                               GivenRow* __restrict__ rows,
+                                                               float* __restrict__ coef, float* __restrict__ alpha) {
+    __shared__ float red[4];
+    float m = 0.f;
+    for (int k = threadIdx.x; k < blocks; k += 256) m = fmaxf(m, most[k]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    auto share = [&](float x) { return m > 0.f ? x / m : x * 0.f; };
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+    if (first == 0) *alpha = m * factor;
+    for (int64_t at = first; at < n; at += step) {
+        const GivenRow r = rows[at];
+        rows[at] = GivenRow{share(r.slope), share(r.bend), share(r.a), 0.f};
+    }
+    for (int64_t at = first; at < entries; at += step) coef[at] = share(coef[at]);
+}
+
+// G at the given classes of lists (one of a row is known to the epilogue).
+template <int DT, int PLANES>
+__global__ __launch_bounds__(256) void head_given_entries_kernel(int32_t k, RowStats stats,
+                                                                 const GivenRow* __restrict__ rows,
+                                                                 const float* __restrict__ logp,
+                                                                 const int32_t* __restrict__ place,
+                                                                 const float* __restrict__ coef, float gscale,
+                                                                 int64_t n, int64_t v0, int64_t vc, uint16_t* G,
+                                                                 int64_t ldg, int64_t plane) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= n * k) return;
+    const int64_t i = at / k, v = place[at];
+    if (v < v0 || v >= v0 + vc) return;
+    const GivenRow r = rows[i];
+    // u of the epilogue, from log p
+    const float u = reach(fmaf(logp[at], kLog2e, -log2f(stats.of(i).y)));
+    const float p = __builtin_amdgcn_exp2f(logp[at] * kLog2e);
+    uint16_t h[PLANES];
+    planes_of<DT, PLANES>((coef[at] - p * fmaf(r.bend, u, r.slope)) * gscale, h);
+#pragma unroll
+    for (int z = 0; z < PLANES; ++z) G[z * plane + i * ldg + (v - v0)] = h[z];
 }
 
 // ---------------------------------------------------------------------------
@@ -1759,7 +2132,12 @@ bool weight_in_place(const grws_head* h) {
 // to whole 128-tiles, or 256-tiles where there is more than one of 128
 int64_t pad(int64_t x) { return x <= 128 ? 128 : up(x, 256); }
 
-Shape shape_of(const grws_head* h, bool backward) {
+// Pitch of kept logits: rows start 256 bytes apart mod 4 KiB.
+int64_t z_pitch(int64_t classes) { return pad(classes) + 64; }
+
+// part_bytes: of a row's strip, forward; keep_z: the logits are kept for a
+// block of the rows.
+Shape shape_of(const grws_head* h, bool backward, int64_t part_bytes = 8, bool keep_z = false) {
     Shape s{};
     s.n = h->n;
     s.D = h->width;
@@ -1777,7 +2155,8 @@ Shape shape_of(const grws_head* h, bool backward) {
     };
     limit(kPieceBytes, 2 * s.planes * s.dp);                                     // the packed rows
     if (backward) limit(kPieceBytes, 2 * s.gplanes * ((s.vp < kLeastPiece ? s.vp : kLeastPiece) + 128));
-    else limit(kPartBytes, 8 * (s.vp / 64));
+    else limit(kPartBytes, part_bytes * (s.vp / 64));
+    if (keep_z) limit(kPieceBytes, 4 * z_pitch(s.V));
     limit((int64_t)1 << 31, 64 * ceil_div(h->k, 4) + 1);                         // threads of head_targets_kernel
     rows = rows < 256 ? 256 : rows / 256 * 256;
     s.blocks = ceil_div(s.n, rows);
@@ -1843,7 +2222,7 @@ grws_head rows_of(const grws_head* h, int64_t r0, int64_t n) {
         b.labels += r0;
     } else {
         b.teacher_index = static_cast<const char*>(h->teacher_index) + r0 * h->k * (h->index_is_i64 ? 8 : 4);
-        b.teacher_logits += r0 * h->k;
+        if (h->teacher_logits) b.teacher_logits += r0 * h->k;
     }
     return b;
 }
@@ -1856,7 +2235,8 @@ Shape block_of(const Shape& s, int64_t r0) {
     return b;
 }
 
-int check_head(const grws_head* h) {
+// given: the targets are the classes of log probabilities
+int check_head(const grws_head* h, bool given = false) {
     GRWS_CHECK_ARG(h != nullptr, "head: null description");
     if (h->dtype != GRWS_F32 && h->dtype != GRWS_F16 && h->dtype != GRWS_BF16)
         return set_error(GRWS_E_DTYPE, "head: unsupported dtype %d", h->dtype);
@@ -1867,10 +2247,14 @@ int check_head(const grws_head* h) {
                        h->ld_weight <= (1 << 21),
                    "head: leading dimensions must be the width at least and 2^21 at most");
     GRWS_CHECK_ARG(h->k >= 0 && h->k <= 1024, "head: at most 1024 teacher entries a row");
-    GRWS_CHECK_ARG(h->temperature > 0.f && h->temperature < INFINITY, "head: the temperature must be positive");
+    GRWS_CHECK_ARG(h->temperature > 0.f && h->temperature < INFINITY && kLog2e / h->temperature < INFINITY,
+                   "head: the temperature must be positive");
     if (h->n > 0) {
         GRWS_CHECK_ARG(h->hidden && h->weight, "head: null pointer");
-        if (h->k == 0) {
+        if (given) {
+            GRWS_CHECK_ARG(h->k == 0 ? h->labels != nullptr : h->teacher_index && !h->labels,
+                           "head: null classes");
+        } else if (h->k == 0) {
             GRWS_CHECK_ARG(h->labels != nullptr, "head: null labels");
             GRWS_CHECK_ARG(h->temperature == 1.f, "head: labels take no temperature");
         } else {
@@ -1880,21 +2264,23 @@ int check_head(const grws_head* h) {
     return GRWS_OK;
 }
 
-Targets targets_of(const grws_head* h) {
+Targets targets_of(const grws_head* h, bool given = false) {
     return Targets{h->labels, h->teacher_index, h->teacher_logits, h->rows, h->hidden_rows, h->classes,
-                   h->k, h->index_is_i64};
+                   h->k, h->index_is_i64, given};
 }
 
 struct FwdSpace {
     uint16_t *hp, *wp;
     float2* part;
+    float4* strips;  // log probabilities, instead of part, and the rest
+    float *z, *y;
     int32_t* flags;  // labels: StatsArgs::earlier; a teacher's lists: the rows' states
     double* pl;
     int32_t *pc, *done;
 };
 
 template <typename A>
-void fwd_space(A& a, const Shape& s, FwdSpace* f) {
+void fwd_space(A& a, const Shape& s, const grws_head* h, bool given, int32_t top, FwdSpace* f) {
     auto take = [&](auto*& p, int64_t n) {
         using T = std::remove_reference_t<decltype(*p)>;
         if constexpr (std::is_same_v<A, Sizer>) a.template take<T>((size_t)n);
@@ -1902,6 +2288,13 @@ void fwd_space(A& a, const Shape& s, FwdSpace* f) {
     };
     if (!s.few) take(f->hp, s.planes * s.np * s.dp);
     if (s.pack_w && !s.few) take(f->wp, s.planes * s.vp * s.dp);
+    if (given) {
+        take(f->strips, s.strips * s.np);
+        if (top) take(f->z, (s.few ? s.n : s.np) * z_pitch(s.V));
+        else take(f->y, s.nb * (h->k > 0 ? h->k : 1));
+        take(f->flags, s.nb);
+        return;
+    }
     take(f->part, s.strips * s.np);
     take(f->flags, s.nb);
     take(f->pl, s.n <= 8 ? 8 : ceil_div(s.n, 4));
@@ -1914,10 +2307,14 @@ struct BwdSpace {
     float *dh, *dw, *bias, *bias_sum, *alpha, *scale;
     uint32_t* most;
     int32_t* owner;  // see head_repeated_kernel
+    // log probabilities: see head_given_rows_kernel
+    GivenRow* given;
+    int32_t* place;
+    float *coef, *given_most;
 };
 
 template <typename A>
-void bwd_space(A& a, const Shape& s, const grws_head* h, BwdSpace* f) {
+void bwd_space(A& a, const Shape& s, const grws_head* h, bool given, BwdSpace* f) {
     auto take = [&](auto*& p, int64_t n) {
         using T = std::remove_reference_t<decltype(*p)>;
         if constexpr (std::is_same_v<A, Sizer>) a.template take<T>((size_t)n);
@@ -1932,8 +2329,15 @@ void bwd_space(A& a, const Shape& s, const grws_head* h, BwdSpace* f) {
     take(f->bias, s.np / kBiasRows * s.vp);
     if (s.blocks > 1) take(f->bias_sum, s.vp);
     take(f->alpha, 1);
-    take(f->scale, s.n);
-    take(f->most, 1);
+    if (given) {
+        take(f->given, s.n);
+        take(f->place, s.n * h->k);
+        take(f->coef, s.n * h->k);
+        take(f->given_most, kGivenBlocks);
+    } else {
+        take(f->scale, s.n);
+        take(f->most, 1);
+    }
     if (h->rows) take(f->owner, h->hidden_rows);
 }
 
@@ -1997,14 +2401,14 @@ Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64
                 (int32_t)ceil_div(nq, pl.tile), (int32_t)pl.splits};
 }
 
-template <typename T, int PLANES>
+template <typename T, int PLANES, bool GIVEN>
 int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
     const bool vec = rows_of_16(h->weight, h->ld_weight, h->dtype) && rows_of_16(h->hidden, h->ld_hidden, h->dtype);
     const dim3 grid((unsigned)ceil_div(a.vt, 128), (unsigned)ceil_div(a.n, 64));
 #define GRWS_HEAD_FEW(NQ)                                                                                         \
     do {                                                                                                          \
-        if (vec) hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, true>), grid, dim3(256), 0, stream, a);        \
-        else hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, false>), grid, dim3(256), 0, stream, a);           \
+        if (vec) hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, GIVEN, true>), grid, dim3(256), 0, stream, a);        \
+        else hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, GIVEN, false>), grid, dim3(256), 0, stream, a);           \
     } while (0)
     if (a.n <= 16) GRWS_HEAD_FEW(1);
     else if (a.n <= 32) GRWS_HEAD_FEW(2);
@@ -2028,13 +2432,17 @@ int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
 
 // G of a piece of the classes and a block of the rows, and what the two
 // products add of it to dW and dH.
+// logp: NULL, or of log probabilities (target_prob is then NULL, and
+// target_logit not looked at).
 int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_t v0, int64_t vc, int64_t r0,
                    const RowStats& all_stats, const float* target_logit, const float* target_prob, bool per_row,
-                   const Alpha& alpha, float c1, float gscale, void* d_hidden, int64_t ld_dh,
+                   const float* logp, const Alpha& alpha, float c1, float gscale, void* d_hidden, int64_t ld_dh,
                    void* d_weight, int64_t ld_dw, void* d_bias, hipStream_t stream) {
     const Shape sb = block_of(s, r0);
     const grws_head hb = rows_of(h, r0, sb.n);
-    const Targets t = targets_of(&hb);
+    const bool given = logp != nullptr;
+    const Targets t = targets_of(&hb, given);
+    const GivenRow* given_rows = given ? f.given + r0 : nullptr;
     const size_t esz = dtype_size(h->dtype);
     const RowStats stats = all_stats.from(r0);
     const float* row_scale = per_row ? f.scale + r0 : nullptr;
@@ -2059,34 +2467,51 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
         a.v0 = v0, a.vend = v0 + vc, a.classes = s.V, a.c1 = c1;
         a.stats = stats, a.row_scale = row_scale, a.gscale = gscale, a.G = f.G, a.ldg = s.ldg, a.plane = plane;
         a.bias_part = d_bias ? f.bias : nullptr, a.vt = vt;
-        if (s.split) GRWS_TRY((launch_few<float, 3>(h, a, stream)));
-        else if (h->dtype == GRWS_F16 && s.gplanes == 1) GRWS_TRY((launch_few<_Float16, 1>(h, a, stream)));
-        else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 2>(h, a, stream)));
-        else if (s.gplanes == 1) GRWS_TRY((launch_few<__hip_bfloat16, 1>(h, a, stream)));
-        else GRWS_TRY((launch_few<__hip_bfloat16, 2>(h, a, stream)));
+        a.given = given_rows;
+#define GRWS_HEAD_FEW_GRAD(T, PL)                                   \
+    do {                                                            \
+        if (given) GRWS_TRY((launch_few<T, PL, true>(h, a, stream))); \
+        else GRWS_TRY((launch_few<T, PL, false>(h, a, stream)));    \
+    } while (0)
+        if (s.split) GRWS_HEAD_FEW_GRAD(float, 3);
+        else if (h->dtype == GRWS_F16 && s.gplanes == 1) GRWS_HEAD_FEW_GRAD(_Float16, 1);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_FEW_GRAD(_Float16, 2);
+        else if (s.gplanes == 1) GRWS_HEAD_FEW_GRAD(__hip_bfloat16, 1);
+        else GRWS_HEAD_FEW_GRAD(__hip_bfloat16, 2);
+#undef GRWS_HEAD_FEW_GRAD
     } else {
         GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, first_rows, stream));
         GradArgs a{gemm_of(s, s.logits, W, hidden_operand(sb, f.hp, false), vc, sb.np, s.dp, s.planes),
                    v0, s.V, sb.n, c1, h->bias,
                    h->dtype, stats, hb.labels, row_scale, gscale, f.G, s.ldg, plane,
-                   d_bias ? f.bias : nullptr, vt};
-#define GRWS_HEAD_GRAD(DT, PL) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL)
+                   d_bias ? f.bias : nullptr, vt, given_rows};
+#define GRWS_HEAD_GRAD(DT, PL)                                                   \
+    do {                                                                         \
+        if (given) GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL, true); \
+        else GRWS_HEAD_LAUNCH(s.logits, head_grad_kernel, a, DT, PL, false);     \
+    } while (0)
         GRWS_HEAD_PLANES(GRWS_HEAD_GRAD);
 #undef GRWS_HEAD_GRAD
     }
     if (h->k > 0) {
         const dim3 grid((unsigned)ceil_div(sb.n * h->k, 256));
-        const float *y = target_logit + r0 * h->k, *coef = target_prob + (s.n + r0) * h->k;
-#define GRWS_HEAD_SUB(DT, PL)                                                                                      \
-    hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, stats, y, coef, row_scale, gscale, \
-                       c1, sb.n, v0, vc, f.G, s.ldg, plane)
-        GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
+        const int32_t* place = given ? f.place + r0 * h->k : nullptr;
+        const float* coef = given ? f.coef + r0 * h->k : target_prob + (s.n + r0) * h->k;
+#define GRWS_HEAD_SUB(DT, PL)                                                                                        \
+    hipLaunchKernelGGL((head_subtract_kernel<DT, PL>), grid, dim3(256), 0, stream, t, stats, target_logit + r0 * h->k, \
+                       coef, row_scale, gscale, c1, sb.n, v0, vc, f.G, s.ldg, plane)
+#define GRWS_HEAD_ENTRIES(DT, PL)                                                                                   \
+    hipLaunchKernelGGL((head_given_entries_kernel<DT, PL>), grid, dim3(256), 0, stream, h->k, stats, given_rows,    \
+                       logp + r0 * h->k, place, coef, gscale, sb.n, v0, vc, f.G, s.ldg, plane)
+        if (given) GRWS_HEAD_PLANES(GRWS_HEAD_ENTRIES);
+        else GRWS_HEAD_PLANES(GRWS_HEAD_SUB);
+#undef GRWS_HEAD_ENTRIES
 #undef GRWS_HEAD_SUB
         GRWS_LAUNCH_CHECK();
         if (d_bias) {
             const dim3 parts((unsigned)(sb.np / kBiasRows), (unsigned)ceil_div(vc, kBiasClasses));
-            hipLaunchKernelGGL(head_bias_targets_kernel, parts, dim3(256), 0, stream, t, stats, coef, row_scale, gscale,
-                               sb.n, v0, vc, vt, f.bias);
+            hipLaunchKernelGGL(head_bias_targets_kernel, parts, dim3(256), 0, stream, t, stats, place, coef, row_scale,
+                               gscale, sb.n, v0, vc, vt, f.bias);
             GRWS_LAUNCH_CHECK();
         }
     }
@@ -2156,6 +2581,63 @@ int backward_block(const grws_head* h, const Shape& s, const BwdSpace& f, int64_
     return GRWS_OK;
 }
 
+// The gradients of a call whose rows' factors are there.
+int backward_all(const grws_head* h, const Shape& s, const BwdSpace& f, const RowStats& stats,
+                 const float* target_logit, const float* target_prob, bool per_row, const float* logp,
+                 const Alpha& alpha, float c1, float gscale, void* d_hidden, int64_t ld_dh, void* d_weight,
+                 int64_t ld_dw, void* d_bias, hipStream_t stream) {
+    int32_t* owner = d_hidden ? f.owner : nullptr;
+    if (s.blocks == 1) {
+        GRWS_TRY(pack_hidden(h, s, targets_of(h, logp != nullptr), f.hp, alpha, nullptr, owner, stream));
+    } else if (owner) {
+        hipLaunchKernelGGL(head_owner_kernel, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows, s.n,
+                           h->hidden_rows, owner);
+        GRWS_LAUNCH_CHECK();
+    }
+    const size_t esz = dtype_size(h->dtype);
+    // pieces of the classes, and of each the blocks of rows: W's piece is
+    // packed once, dW's is complete after its blocks
+    for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
+        const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
+        for (int64_t r0 = 0; r0 < s.n; r0 += s.nb)
+            GRWS_TRY(backward_block(h, s, f, v0, vc, r0, stats, target_logit, target_prob, per_row, logp, alpha, c1,
+                                    gscale, d_hidden, ld_dh, d_weight, ld_dw, d_bias, stream));
+    }
+    if (d_hidden && s.hidden.splits > 1) {
+#define GRWS_HEAD_DH(T)                                                                                              \
+    hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
+                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, f.alpha,                \
+                       static_cast<T*>(d_hidden), ld_dh)
+        if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
+        else GRWS_HEAD_DH(__hip_bfloat16);
+#undef GRWS_HEAD_DH
+        GRWS_LAUNCH_CHECK();
+    }
+    if (owner) {
+#define GRWS_HEAD_REPEATED(T)                                                                                        \
+    hipLaunchKernelGGL(head_repeated_kernel<T>, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows,   \
+                       s.n, h->hidden_rows, owner, s.D, static_cast<T*>(d_hidden), ld_dh)
+        if (h->dtype == GRWS_F32) GRWS_HEAD_REPEATED(float);
+        else if (h->dtype == GRWS_F16) GRWS_HEAD_REPEATED(_Float16);
+        else GRWS_HEAD_REPEATED(__hip_bfloat16);
+#undef GRWS_HEAD_REPEATED
+        GRWS_LAUNCH_CHECK();
+    }
+    return GRWS_OK;
+}
+
+// The gradients of no rows at all.
+int backward_none(const grws_head* h, void* d_weight, int64_t ld_dw, void* d_bias, hipStream_t stream) {
+    const size_t e = dtype_size(h->dtype);
+    if (d_weight)
+        for (int64_t v = 0; v < (ld_dw == h->width ? 1 : h->classes); ++v)
+            GRWS_TRY(fill_bytes_zero(static_cast<char*>(d_weight) + v * ld_dw * e,
+                                     (ld_dw == h->width ? h->classes : 1) * h->width * e, stream));
+    if (d_bias) GRWS_TRY(fill_bytes_zero(d_bias, h->classes * e, stream));
+    return GRWS_OK;
+}
+
 }  // namespace
 }  // namespace grws
 
@@ -2165,7 +2647,7 @@ extern "C" size_t grws_head_fwd_workspace_bytes(const grws_head* h) {
     if (check_head(h) != GRWS_OK || h->n == 0) return 0;
     Sizer z;
     FwdSpace f{};
-    fwd_space(z, shape_of(h, false), &f);
+    fwd_space(z, shape_of(h, false), h, false, 0, &f);
     return z.used;
 }
 
@@ -2186,7 +2668,7 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
     const Shape s = shape_of(h, false);
     Carver cv(workspace, workspace_bytes);
     FwdSpace f{};
-    fwd_space(cv, s, &f);
+    fwd_space(cv, s, h, false, 0, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
     const int64_t join_rows = s.n <= 8 ? 1 : s.n <= 512 ? 4 : 16, joins = ceil_div(s.n, join_rows);
@@ -2215,9 +2697,9 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
             FewArgs a{t, h->hidden, h->weight, h->bias, h->ld_hidden, h->ld_weight, s.n, s.np, s.D, 0, s.V, s.V, c1,
                       f.flags, f.part, y, f.flags, f.done};
             a.vt = pad(s.V);
-            if (h->dtype == GRWS_F32) GRWS_TRY((launch_few<float, 0>(h, a, stream)));
-            else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 0>(h, a, stream)));
-            else GRWS_TRY((launch_few<__hip_bfloat16, 0>(h, a, stream)));
+            if (h->dtype == GRWS_F32) GRWS_TRY((launch_few<float, 0, false>(h, a, stream)));
+            else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 0, false>(h, a, stream)));
+            else GRWS_TRY((launch_few<__hip_bfloat16, 0, false>(h, a, stream)));
         } else {
             GRWS_TRY(pack_hidden(&hb, sb, t, f.hp, Alpha{}, f.done, nullptr, stream));
         }
@@ -2229,8 +2711,8 @@ extern "C" int grws_head_fwd(const grws_head* h, float* lse, float* target_logit
             StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(sb, f.hp, false), vc, sb.np, s.dp, s.planes),
                         v0, s.V, sb.n, sb.np, c1,
                         h->bias, h->dtype, hb.labels, f.part, y, f.flags};
-            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16);
-            else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16);
+            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16, false);
+            else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16, false);
         }
         const int64_t at = r0 / join_rows;  // blocks are multiples of 256 rows
 #define GRWS_HEAD_JOIN(R)                                                                                            \
@@ -2267,7 +2749,7 @@ extern "C" size_t grws_head_bwd_workspace_bytes(const grws_head* h) {
     Sizer z;
     BwdSpace f{};
     const Shape s = shape_of(h, true);
-    bwd_space(z, s, h, &f);
+    bwd_space(z, s, h, false, &f);
     return z.used;
 }
 
@@ -2280,21 +2762,13 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
     GRWS_TRY(check_head(h));
     GRWS_CHECK_ARG((!d_hidden || ld_dh >= h->width) && (!d_weight || ld_dw >= h->width),
                    "head: gradients' leading dimensions must be the width at least");
-    if (h->n == 0) {
-        const size_t e = dtype_size(h->dtype);
-        if (d_weight)
-            for (int64_t v = 0; v < (ld_dw == h->width ? 1 : h->classes); ++v)
-                GRWS_TRY(fill_bytes_zero(static_cast<char*>(d_weight) + v * ld_dw * e,
-                                         (ld_dw == h->width ? h->classes : 1) * h->width * e, stream));
-        if (d_bias) GRWS_TRY(fill_bytes_zero(d_bias, h->classes * e, stream));
-        return GRWS_OK;
-    }
+    if (h->n == 0) return backward_none(h, d_weight, ld_dw, d_bias, stream);
     GRWS_CHECK_ARG(lse && target_logit && counts && dloss && (h->k == 0 || target_prob), "head: null pointer");
     if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
     const Shape s = shape_of(h, true);
     Carver cv(workspace, workspace_bytes);
     BwdSpace f{};
-    bwd_space(cv, s, h, &f);
+    bwd_space(cv, s, h, false, &f);
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     const float c1 = kLog2e / h->temperature;
     const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
@@ -2308,43 +2782,160 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
         GRWS_LAUNCH_CHECK();
     }
     const Alpha alpha{f.alpha, dloss, counts, per_row ? f.most : nullptr, h->temperature / gscale};
-    int32_t* owner = d_hidden ? f.owner : nullptr;
-    if (s.blocks == 1) {
-        GRWS_TRY(pack_hidden(h, s, targets_of(h), f.hp, alpha, nullptr, owner, stream));
-    } else if (owner) {
-        hipLaunchKernelGGL(head_owner_kernel, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows, s.n,
-                           h->hidden_rows, owner);
-        GRWS_LAUNCH_CHECK();
-    }
-    const size_t esz = dtype_size(h->dtype);
-    // pieces of the classes, and of each the blocks of rows: W's piece is
-    // packed once, dW's is complete after its blocks
-    for (int64_t v0 = 0; v0 < s.V; v0 += s.vp) {
-        const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
-        for (int64_t r0 = 0; r0 < s.n; r0 += s.nb)
-            GRWS_TRY(backward_block(h, s, f, v0, vc, r0, stats, target_logit, target_prob, per_row, alpha, c1,
-                                    gscale, d_hidden, ld_dh, d_weight, ld_dw, d_bias, stream));
-    }
-    if (d_hidden && s.hidden.splits > 1) {
-#define GRWS_HEAD_DH(T)                                                                                              \
-    hipLaunchKernelGGL(head_hidden_out_kernel<T>, dim3((unsigned)s.n), dim3(256), 0, stream, f.dh,               \
-                       s.hidden.splits, s.np, s.dp, s.D, h->rows, h->hidden_rows, stats, f.alpha,                \
-                       static_cast<T*>(d_hidden), ld_dh)
-        if (h->dtype == GRWS_F32) GRWS_HEAD_DH(float);
-        else if (h->dtype == GRWS_F16) GRWS_HEAD_DH(_Float16);
-        else GRWS_HEAD_DH(__hip_bfloat16);
-#undef GRWS_HEAD_DH
-        GRWS_LAUNCH_CHECK();
-    }
-    if (owner) {
-#define GRWS_HEAD_REPEATED(T)                                                                                        \
-    hipLaunchKernelGGL(head_repeated_kernel<T>, dim3((unsigned)ceil_div(s.n, 256)), dim3(256), 0, stream, h->rows,   \
-                       s.n, h->hidden_rows, owner, s.D, static_cast<T*>(d_hidden), ld_dh)
-        if (h->dtype == GRWS_F32) GRWS_HEAD_REPEATED(float);
-        else if (h->dtype == GRWS_F16) GRWS_HEAD_REPEATED(_Float16);
-        else GRWS_HEAD_REPEATED(__hip_bfloat16);
-#undef GRWS_HEAD_REPEATED
+    return backward_all(h, s, f, stats, target_logit, target_prob, per_row, nullptr, alpha, c1, gscale, d_hidden, ld_dh,
+                        d_weight, ld_dw, d_bias, stream);
+}
+
+// ---------------------------------------------------------------------------
+// log probabilities
+// ---------------------------------------------------------------------------
+namespace grws {
+namespace {
+
+Shape given_shape(const grws_head* h, int32_t top) { return shape_of(h, false, 16, top > 0); }
+
+int check_given(const grws_head* h, int32_t top) {
+    GRWS_TRY(check_head(h, true));
+    GRWS_CHECK_ARG(top >= 0 && top <= kMaxK && top <= h->classes, "head: top must be 0..min(classes, 1024)");
+    return GRWS_OK;
+}
+
+int32_t bits_for(int64_t n) {
+    int32_t b = 1;
+    while ((1ll << b) < n) ++b;
+    return b;
+}
+
+}  // namespace
+}  // namespace grws
+
+extern "C" size_t grws_head_log_probs_fwd_workspace_bytes(const grws_head* h, int32_t top) {
+    if (check_given(h, top) != GRWS_OK || h->n == 0) return 0;
+    Sizer z;
+    FwdSpace f{};
+    fwd_space(z, given_shape(h, top), h, true, top, &f);
+    return z.used;
+}
+
+extern "C" int grws_head_log_probs_fwd(const grws_head* h, int32_t top, float* logp, float* entropy, float* saved,
+                                       float* top_logp, int32_t* top_index, void* workspace, size_t workspace_bytes,
+                                       void* stream_) {
+    clear_error();
+    hipStream_t stream = as_stream(stream_);
+    GRWS_TRY(check_given(h, top));
+    if (h->n == 0) return GRWS_OK;
+    GRWS_CHECK_ARG(logp && entropy && saved && (top == 0 || (top_logp && top_index)), "head: null output");
+    const Shape s = given_shape(h, top);
+    Carver cv(workspace, workspace_bytes);
+    FwdSpace f{};
+    fwd_space(cv, s, h, true, top, &f);
+    if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
+    const float c1 = kLog2e / h->temperature, inv_t = 1.f / h->temperature;
+    const int64_t k = h->k > 0 ? h->k : 1;
+    for (int64_t r0 = 0; r0 < s.n; r0 += s.nb) {
+        const Shape sb = block_of(s, r0);
+        const grws_head hb = rows_of(h, r0, sb.n);
+        const Targets t = targets_of(&hb, true);
+        const int64_t strips = ceil_div(s.V, s.strip_classes);
+        // alternatives: a row's strips lie together
+        const Strips part = top ? Strips{f.strips, s.strips, 1, f.z, z_pitch(s.V)}
+                                : Strips{f.strips, 1, sb.np, nullptr, 0};
+        const int64_t* labels = top ? nullptr : hb.labels;  // kept logits are read at the given classes
+        if (h->k > 0 && !top) {
+            const dim3 grid((unsigned)ceil_div(sb.n * ((h->k + 3) / 4), 4));
+            const int32_t vec = rows_of_16(h->hidden, h->ld_hidden, h->dtype) &&
+                                rows_of_16(h->weight, h->ld_weight, h->dtype);
+#define GRWS_HEAD_TARGETS(T)                                                                                        \
+    hipLaunchKernelGGL(head_targets_kernel<T>, grid, dim3(256), 0, stream, t, static_cast<const T*>(hb.hidden),     \
+                       h->ld_hidden, static_cast<const T*>(h->weight), h->ld_weight, static_cast<const T*>(h->bias), \
+                       sb.n, s.D, vec, inv_t, nullptr, nullptr, f.y, f.flags)
+            if (h->dtype == GRWS_F32) GRWS_HEAD_TARGETS(float);
+            else if (h->dtype == GRWS_F16) GRWS_HEAD_TARGETS(_Float16);
+            else GRWS_HEAD_TARGETS(__hip_bfloat16);
+#undef GRWS_HEAD_TARGETS
+            GRWS_LAUNCH_CHECK();
+        }
+        if (s.few) {
+            FewArgs a{};
+            a.t = t;
+            a.t.labels = labels;
+            a.hidden = h->hidden, a.weight = h->weight, a.bias = h->bias;
+            a.ldh = h->ld_hidden, a.ldw = h->ld_weight, a.n = s.n, a.np = s.np, a.width = s.D;
+            a.vend = s.V, a.classes = s.V, a.c1 = c1, a.ylabel = f.y, a.vt = pad(s.V), a.strips = part;
+            if (h->dtype == GRWS_F32) GRWS_TRY((launch_few<float, 0, true>(h, a, stream)));
+            else if (h->dtype == GRWS_F16) GRWS_TRY((launch_few<_Float16, 0, true>(h, a, stream)));
+            else GRWS_TRY((launch_few<__hip_bfloat16, 0, true>(h, a, stream)));
+        } else {
+            GRWS_TRY(pack_hidden(&hb, sb, t, f.hp, Alpha{}, nullptr, nullptr, stream));
+        }
+        for (int64_t v0 = 0; v0 < s.V && !s.few; v0 += s.vp) {
+            const int64_t vc = s.V - v0 < s.vp ? s.V - v0 : s.vp;
+            Opnd W;
+            GRWS_TRY(weight_piece(h, s, v0, vc, f.wp, false, &W, r0 == 0 || s.vp < s.V, stream));
+            StatsArgs a{gemm_of(s, s.logits, W, hidden_operand(sb, f.hp, false), vc, sb.np, s.dp, s.planes),
+                        v0, s.V, sb.n, sb.np, c1, h->bias, h->dtype, labels, nullptr, f.y, nullptr, part};
+            if (h->dtype == GRWS_F16) GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_F16, true);
+            else GRWS_HEAD_LAUNCH(s.logits, head_stats_kernel, a, GRWS_BF16, true);
+        }
+        const GivenOut o{logp + r0 * k, entropy + r0, saved + r0, saved + s.n + r0};
+        if (top) {
+#define GRWS_HEAD_TOP(MAXK)                                                                                           \
+    hipLaunchKernelGGL(head_top_kernel<MAXK>, dim3((unsigned)sb.n), dim3(kT), 0, stream, t, part, (int32_t)strips,    \
+                       (int32_t)s.strip_classes, bits_for(strips), bits_for(s.V), top, c1, inv_t, o,                  \
+                       top_logp + r0 * top, top_index + r0 * top)
+            if (top <= kSmallK) GRWS_HEAD_TOP(kSmallK);
+            else GRWS_HEAD_TOP(kMaxK);
+#undef GRWS_HEAD_TOP
+        } else {
+#define GRWS_HEAD_JOIN(R)                                                                                           \
+    hipLaunchKernelGGL(head_given_join_kernel<R>, dim3((unsigned)ceil_div(sb.n, R)), dim3(512), 0, stream, t, part, \
+                       strips, sb.n, c1, inv_t, f.y, o)
+            if (s.n <= 8) GRWS_HEAD_JOIN(1);
+            else if (s.n <= 512) GRWS_HEAD_JOIN(4);
+            else GRWS_HEAD_JOIN(16);
+#undef GRWS_HEAD_JOIN
+        }
         GRWS_LAUNCH_CHECK();
     }
     return GRWS_OK;
+}
+
+extern "C" size_t grws_head_log_probs_bwd_workspace_bytes(const grws_head* h) {
+    if (check_head(h, true) != GRWS_OK || h->n == 0) return 0;
+    Sizer z;
+    BwdSpace f{};
+    bwd_space(z, shape_of(h, true), h, true, &f);
+    return z.used;
+}
+
+extern "C" int grws_head_log_probs_bwd(const grws_head* h, const float* saved, const float* logp,
+                                       const float* entropy, const float* dlogp, const float* dentropy,
+                                       void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw, void* d_bias,
+                                       void* workspace, size_t workspace_bytes, void* stream_) {
+    clear_error();
+    hipStream_t stream = as_stream(stream_);
+    GRWS_TRY(check_head(h, true));
+    GRWS_CHECK_ARG((!d_hidden || ld_dh >= h->width) && (!d_weight || ld_dw >= h->width),
+                   "head: gradients' leading dimensions must be the width at least");
+    if (h->n == 0) return backward_none(h, d_weight, ld_dw, d_bias, stream);
+    GRWS_CHECK_ARG(saved && logp && entropy, "head: null pointer");
+    if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
+    const Shape s = shape_of(h, true);
+    Carver cv(workspace, workspace_bytes);
+    BwdSpace f{};
+    bwd_space(cv, s, h, true, &f);
+    if (!cv.ok) return set_error(GRWS_E_CAPACITY, "head: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
+    const float gscale = h->dtype == GRWS_F16 ? 32768.f : 1.f;
+    const RowStats stats{saved, saved + s.n, 1};
+    const int64_t blocks = ceil_div(s.n, 4) < kGivenBlocks ? ceil_div(s.n, 4) : kGivenBlocks;
+    hipLaunchKernelGGL(head_given_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, targets_of(h, true), stats,
+                       s.n, entropy, dlogp, dentropy, f.given, h->k > 0 ? f.place : nullptr, f.coef, f.given_most);
+    GRWS_LAUNCH_CHECK();
+    const int64_t parts = ceil_div(h->k > 1 ? s.n * h->k : s.n, 256);
+    hipLaunchKernelGGL(head_given_scale_kernel, dim3((unsigned)(parts < 2048 ? parts : 2048)), dim3(256), 0, stream,
+                       f.given_most, (int32_t)blocks, s.n, s.n * h->k, 1.f / (h->temperature * gscale), f.given, f.coef,
+                       f.alpha);
+    GRWS_LAUNCH_CHECK();
+    return backward_all(h, s, f, stats, nullptr, nullptr, false, logp, Alpha{}, kLog2e / h->temperature, gscale,
+                        d_hidden, ld_dh, d_weight, ld_dw, d_bias, stream);
 }

@@ -15,58 +15,11 @@
 // steps); the work-group joins them at the end, in a fixed order.  Top logits
 // come from the same registers (top_pool.h).  Few rows are cut into stretches
 // and joined, short ones take a wave each.
+#include "logp.h"
 #include "top_pool.h"
 
 namespace grws {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-// (m, s, t) of some of a row's logits; nothing of them: m = -inf, s = t = 0.
-struct Stats {
-    float m, s, t;
-};
-
-__device__ __forceinline__ Stats no_stats() { return Stats{-INFINITY, 0.f, 0.f}; }
-
-// 2^u u and 2^d (s d + t) below -200 are zero: infinities would leave NaN
-__device__ __forceinline__ float reach(float u) { return fmaxf(u, -200.f); }
-
-// s and t seen from a larger m, d = (old m - new m) log2(e) / T further down
-// (-inf where there was nothing)
-__device__ __forceinline__ void move(Stats& a, float d) {
-    d = reach(d);
-    const float f = __builtin_amdgcn_exp2f(d);
-    a.t = fmaf(d, a.s, a.t) * f;
-    a.s *= f;
-}
-
-__device__ __forceinline__ Stats join(Stats a, Stats b, float c1) {
-    // a NaN logit shows in s; largest values are compared without it
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return Stats{m, a.s + b.s, a.t + b.t};  // zeros, or NaN
-    move(a, (a.m - m) * c1);
-    move(b, (b.m - m) * c1);
-    return Stats{m, a.s + b.s, a.t + b.t};
-}
-
-__device__ __forceinline__ void add(Stats& a, float z, float m, float c1) {
-    const float u = (z - m) * c1, e = __builtin_amdgcn_exp2f(u);
-    a.s += e;
-    a.t = fmaf(e, reach(u), a.t);
-}
-
-// joins lanes d apart, d = 32..1: every lane has the wave's
-__device__ __forceinline__ Stats join_wave(Stats a, float c1) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const Stats b{__shfl_xor(a.m, d, kWave), __shfl_xor(a.s, d, kWave), __shfl_xor(a.t, d, kWave)};
-        // both sides in one order, so the lanes agree
-        a = (threadIdx.x & d) ? join(b, a, c1) : join(a, b, c1);
-    }
-    return a;
-}
 
 // The classes whose log probabilities are asked for: k a row; a negative
 // one asks for nothing (0), one past the last is an error (NaN).

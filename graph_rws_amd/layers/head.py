@@ -21,6 +21,7 @@ import torch
 from torch.autograd import Function
 
 from ..core import ops as _ops
+from .logp import linear_log_probs
 
 _REDUCTIONS = ("mean", "none")
 
@@ -134,6 +135,10 @@ class LinearHead(torch.nn.Module):
         """linear_distill of this classifier (the student)."""
         return linear_distill(hidden, self.weight, teacher_index, teacher_logits, self.bias, rows, temperature,
                               reduction)
+
+    def log_probs(self, hidden, index, rows=None, temperature: float = 1.0, top: int = 0):
+        """linear_log_probs of this classifier."""
+        return linear_log_probs(hidden, self.weight, index, self.bias, rows, temperature, top)
 
     @torch.no_grad()
     def top(self, hidden, k: int, rows_at_once: int = 8192):

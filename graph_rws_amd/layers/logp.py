@@ -2,7 +2,12 @@
 gradients: what training by rewards, on pseudo labels or towards sure answers
 takes of a classifier, and what scoring with one reports.
 
-``log_probs`` reads logits in memory (csrc/logp.hip).
+``log_probs`` reads logits in memory (csrc/logp.hip).  ``linear_log_probs``
+makes those of a classifier, log_probs(F.linear(hidden[rows], weight, bias),
+index), without keeping them (csrc/head.hip): its forward reduces them in the
+product's epilogue, its backward makes them again piece by piece of the
+classes.  Under autocast hidden, weight and bias are taken in the autocast
+dtype, as ``F.linear`` takes them.
 """
 from __future__ import annotations
 
@@ -77,3 +82,49 @@ def log_probs(logits: torch.Tensor, index: torch.Tensor, temperature: float = 1.
     derivative."""
     _ops.check_log_probs(logits, index, temperature, top)
     return LogProbs(*_LogProbs.apply(logits, index, float(temperature), int(top)))
+
+
+class _LinearLogProbs(Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, rows, index, temperature, top):
+        ctx.set_materialize_grads(False)
+        call = _ops.given_call(hidden, weight, index, bias, rows, temperature)
+        logp, entropy, saved, top_logp, top_index = _ops.head_log_probs_fwd(call, index.shape, top)
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(hidden, weight, bias, rows, index, logp, entropy, saved)
+            ctx.temperature = temperature
+        if top:
+            ctx.mark_non_differentiable(top_logp, top_index)
+        return logp, entropy, top_logp, top_index
+
+    @staticmethod
+    def backward(ctx, dlogp, dentropy, _dtop, _dindex):
+        if dlogp is None and dentropy is None:
+            return (None,) * 7
+        hidden, weight, bias, rows, index, logp, entropy, saved = ctx.saved_tensors
+        call = _ops.given_call(hidden, weight, index, bias, rows, ctx.temperature)
+        grads = _ops.head_log_probs_bwd(call, saved, logp, entropy, dlogp, dentropy, ctx.needs_input_grad[:3])
+        if torch.is_grad_enabled():  # create_graph=True
+            owners = [t for t in (hidden, weight, bias, dlogp, dentropy) if t is not None]
+            grads = _Once.apply(len(owners), *owners, *grads)
+        return (*grads, None, None, None, None)
+
+
+def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, index: torch.Tensor,
+                     bias: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None,
+                     temperature: float = 1.0, top: int = 0) -> LogProbs:
+    """LogProbs of softmax((hidden[rows] @ weight.T + bias) / temperature).
+
+    hidden [N, D], weight [V, D], bias [V] (one dtype of f32, f16, bf16), rows
+    int64 [n] (None = the first n rows; distinct ones where hidden needs a
+    gradient, which is NaN at a row listed twice: gather such rows first).
+    index int32 or int64 [n] or [n, k] (k <= 1024), the given classes, and
+    what is not a number as in log_probs; a row id out of range is an error
+    (NaN in its row, no gradient).  top > 0 (for scoring) keeps the logits of
+    up to 1 GiB, or 256 rows, at a time.  No host sync; no second derivative."""
+    if hidden.is_cuda and torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(dt), weight.to(dt)
+        bias = bias.to(dt) if bias is not None else None
+    _ops.check_linear_log_probs(hidden, weight, index, bias, rows, temperature, top)
+    return LogProbs(*_LinearLogProbs.apply(hidden, weight, bias, rows, index, float(temperature), int(top)))

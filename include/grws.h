@@ -883,6 +883,32 @@ int grws_head_bwd(const grws_head* head, const float* lse, const float* target_l
                   void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Log probabilities of softmax(z / T) of given classes, and its entropy,    */
+/* for the same z = H W^T + b of n rows, which is not kept.  Of `head`:      */
+/* the given classes are labels int64 [n] (k = 0) or teacher_index [n x k]   */
+/* (teacher_logits NULL); any temperature; a negative class asks for nothing */
+/* (log probability 0), one past the last is an error (NaN).  A row whose id */
+/* is out of range, or of nothing but -inf, is NaN and reaches no gradient;  */
+/* one with a NaN or +inf is NaN.  Outputs: logp f32 [n * max(k, 1)],        */
+/* entropy f32 [n] (natural logarithms), saved f32 [2 x n] (what the         */
+/* backward takes); top > 0 (at most min(classes, 1024)): top_logp f32 and   */
+/* top_index int32 [n x top] of the largest logits, largest first, of equal  */
+/* ones the lowest class first (the logits of a block of rows, 1 GiB or 256  */
+/* rows of them, are then in the workspace).  Backward of dlogp and dentropy */
+/* (shaped alike; NULL: zeros): gradients as of grws_head_bwd.  No sync;     */
+/* same inputs, same bits.                                                   */
+/* ------------------------------------------------------------------------ */
+size_t grws_head_log_probs_fwd_workspace_bytes(const grws_head* head, int32_t top);
+int grws_head_log_probs_fwd(const grws_head* head, int32_t top, float* logp, float* entropy, float* saved,
+                            float* top_logp, int32_t* top_index, void* workspace, size_t workspace_bytes,
+                            void* stream);
+size_t grws_head_log_probs_bwd_workspace_bytes(const grws_head* head);
+int grws_head_log_probs_bwd(const grws_head* head, const float* saved, const float* logp, const float* entropy,
+                            const float* dlogp, const float* dentropy, void* d_hidden, int64_t ld_dh,
+                            void* d_weight, int64_t ld_dw, void* d_bias, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* The k largest logits of each row of logits [rows x ld], largest first,   */
 /* with their classes: values [rows x k] in dtype, index int32 [rows x k].  */
 /* Of equal logits the lowest class comes first; NaN counts as the largest. */

@@ -1,10 +1,12 @@
 """Host side of log_probs: refusals before any launch, and workspace sizes
 (CPU tier: nothing here touches a GPU)."""
+import ctypes
+
 import pytest
 import torch
 
 from graph_rws_amd.core import _lib as L
-from graph_rws_amd.layers import log_probs
+from graph_rws_amd.layers import linear_log_probs, log_probs
 
 P = 1 << 20  # never read
 
@@ -61,3 +63,70 @@ def test_python_refusals():
     z, i = torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="CUDA"):
         log_probs(z, i)
+
+
+# ---------------------------------------------------------------------------
+# of a classifier whose logits are not kept
+# ---------------------------------------------------------------------------
+def _head(**kw):
+    v = dict(hidden=P, weight=P, bias=None, rows=None, labels=P, teacher_index=None, teacher_logits=None,
+             ld_hidden=64, ld_weight=64, hidden_rows=100, n=100, width=64, classes=1000, dtype=L.GRWS_BF16, k=0,
+             index_is_i64=0, temperature=1.5)
+    v.update(kw)
+    return L.HeadView(*(v[name] for name, _ in L.HeadView._fields_))
+
+
+def _head_fwd(head, top=0, logp=P, saved=P, top_index=P, ws_bytes=1 << 40):
+    return L.load().grws_head_log_probs_fwd(ctypes.byref(head), top, logp, P, saved, P, top_index, P, ws_bytes, None)
+
+
+def _head_bwd(head, saved=P, logp=P, ld=64, ws_bytes=1 << 40):
+    return L.load().grws_head_log_probs_bwd(ctypes.byref(head), saved, logp, P, P, P, P, ld, P, 64, P, P, ws_bytes,
+                                            None)
+
+
+LISTS = dict(labels=None, teacher_index=P, k=4)
+
+
+@pytest.mark.parametrize("kw,call,status,word", [
+    (dict(dtype=7), {}, L.GRWS_E_DTYPE, b"dtype"), (dict(n=-1), {}, L.GRWS_E_INVALID, b"row count"),
+    (dict(labels=None), {}, L.GRWS_E_INVALID, b"classes"), (dict(k=4), {}, L.GRWS_E_INVALID, b"classes"),
+    (dict(LISTS, labels=P), {}, L.GRWS_E_INVALID, b"classes"),
+    (dict(temperature=0.0), {}, L.GRWS_E_INVALID, b"temperature"),
+    (dict(temperature=1e-42), {}, L.GRWS_E_INVALID, b"temperature"),
+    (dict(weight=None), {}, L.GRWS_E_INVALID, b"null"),
+    (dict(k=1025, labels=None, teacher_index=P), {}, L.GRWS_E_INVALID, b"1024"),
+    ({}, dict(top=-1), L.GRWS_E_INVALID, b"top"), ({}, dict(top=1001), L.GRWS_E_INVALID, b"top"),
+    (dict(classes=5000), dict(top=1025), L.GRWS_E_INVALID, b"top"),
+    ({}, dict(logp=None), L.GRWS_E_INVALID, b"null"), ({}, dict(saved=None), L.GRWS_E_INVALID, b"null"),
+    ({}, dict(top=2, top_index=None), L.GRWS_E_INVALID, b"null"),
+])
+def test_head_refuses(kw, call, status, word):
+    assert _head_fwd(_head(**kw), **call) == status
+    assert word in L.load().grws_last_error()
+
+
+def test_head_workspaces():
+    lib = L.load()
+    for kw in ({}, LISTS):
+        h = _head(**kw)
+        for top in (0, 8):
+            need = lib.grws_head_log_probs_fwd_workspace_bytes(ctypes.byref(h), top)
+            assert need > 0 and _head_fwd(h, top=top, ws_bytes=need - 1) == L.GRWS_E_CAPACITY
+        need = lib.grws_head_log_probs_bwd_workspace_bytes(ctypes.byref(h))
+        assert need > 0 and _head_bwd(h, ws_bytes=need - 1) == L.GRWS_E_CAPACITY
+        assert _head_bwd(h, ld=63) == L.GRWS_E_INVALID and _head_bwd(h, saved=None) == L.GRWS_E_INVALID
+        assert _head_bwd(h, logp=None) == L.GRWS_E_INVALID
+    assert lib.grws_head_log_probs_fwd_workspace_bytes(ctypes.byref(_head(dtype=9)), 0) == 0
+    # kept logits: a block of the rows
+    for n, classes in ((8192, 131072), (30000, 1000000), (1, 2000000)):
+        h = _head(n=n, hidden_rows=n, classes=classes)
+        assert lib.grws_head_log_probs_fwd_workspace_bytes(ctypes.byref(h), 8) < 3 << 29
+        assert lib.grws_head_log_probs_fwd_workspace_bytes(ctypes.byref(h), 0) < 1 << 30
+    assert _head_fwd(_head(n=0)) == L.GRWS_OK
+
+
+def test_linear_python_refusals():
+    h, w, i = torch.zeros(3, 5), torch.zeros(7, 5), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        linear_log_probs(h, w, i)
