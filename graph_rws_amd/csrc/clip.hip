@@ -20,12 +20,14 @@
 namespace grws {
 namespace {
 
-constexpr int kT = 256;             // threads of a work-group
-constexpr int kVec = 8;             // elements of a load (two loads of f32)
-constexpr int kLoads = 2;           // loads a thread has in flight
-constexpr int kChunk = kT * kVec * kLoads;  // elements of a work-group's step
+constexpr int kT = 256;      // threads of a work-group
+constexpr int kChunk = 8192;  // elements of a work-group's step
 constexpr int kTensors = 64;        // of a launch: what fits into its arguments
 constexpr int kBlocks = 1024;       // work-groups of a launch: 4 a CU
+// What the last cache (256 MB) keeps for the second pass, or with the outputs
+// for what follows; beyond it loads and stores go past the caches (of 5e8 bf16
+// the squares 164 us against 180, of 5e7 f32 norm and clipping CLIP1).
+constexpr int64_t kCached = (int64_t)192 << 20;
 
 struct Tensors {
     const void* src[kTensors];
@@ -36,20 +38,33 @@ struct Tensors {
     int32_t count;
 };
 
-template <typename T>
+template <typename T, int N>
 struct Vec {
-    T x[kVec];
+    T x[N];
 };
 
-// elements at + 0..7 of x, zeros from `size` on; any alignment
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* x, int64_t at, int64_t size) {
-    Vec<T> v;
-    if (at + kVec <= size) {
-        __builtin_memcpy(&v, x + at, sizeof(v));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2), aligned(2)));
+
+// elements at.. of x, zeros from `size` on; any alignment.  ONCE: past the
+// caches.
+template <bool ONCE, int N, typename T>
+__device__ __forceinline__ Vec<T, N> load_vec(const T* x, int64_t at, int64_t size) {
+    typedef std::conditional_t<N * sizeof(T) % 16 == 0, u32x4_t, u32x2_t> W;
+    constexpr int C = N * sizeof(T) / sizeof(W);
+    Vec<T, N> v;
+    if (at + N <= size) {
+        W w[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const W* p = reinterpret_cast<const W*>(x + at) + i;
+            if constexpr (ONCE) w[i] = __builtin_nontemporal_load(p);
+            else w[i] = *p;
+        }
+        __builtin_memcpy(&v, w, sizeof(v));
     } else {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) v.x[e] = at + e < size ? x[at + e] : from_float<T>(0.f);
+        for (int e = 0; e < N; ++e) v.x[e] = at + e < size ? x[at + e] : from_float<T>(0.f);
     }
     return v;
 }
@@ -76,44 +91,46 @@ __device__ __forceinline__ int tensor_of(const Tensors& a, int64_t c) {
     return lo;
 }
 
-// use(tensor, first element of the work-group's chunk) for a run of the
-// chunks; the dtype of a chunk is uniform.
+// use(tensor, first element of the chunk) for every gridDim-th chunk (the
+// work-groups read neighbouring memory; runs of it a work-group: 772 us against
+// 741 for 5e8 bf16); the dtype of a chunk is uniform.
 template <typename F>
 __device__ __forceinline__ void for_chunks(const Tensors& a, F use) {
     const int64_t n = a.first[a.count];
-    const int64_t b = n * blockIdx.x / gridDim.x, e = n * (blockIdx.x + 1) / gridDim.x;
-    if (b >= e) return;
-    int t = tensor_of(a, b);
-    for (int64_t c = b; c < e; ++c) {
+    if (blockIdx.x >= n) return;
+    int t = tensor_of(a, blockIdx.x);
+    for (int64_t c = blockIdx.x; c < n; c += gridDim.x) {
         while (c >= a.first[t + 1]) ++t;
         use(t, (c - a.first[t]) * kChunk);
     }
 }
 
-template <typename T>
+template <bool ONCE, typename T>
 __device__ __forceinline__ double squares(const void* src, int64_t from, int64_t size) {
+    constexpr int N = 16 / sizeof(T), LOADS = kChunk / (kT * N);
     const T* x = static_cast<const T*>(src);
-    Vec<T> v[kLoads];
+    Vec<T, N> v[LOADS];
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) v[l] = load_vec(x, from + ((int64_t)l * kT + threadIdx.x) * kVec, size);
+    for (int l = 0; l < LOADS; ++l) v[l] = load_vec<ONCE, N>(x, from + ((int64_t)l * kT + threadIdx.x) * N, size);
     double s = 0.0;
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l)
+    for (int l = 0; l < LOADS; ++l)
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
+        for (int e = 0; e < N; ++e) {
             const double g = (double)to_float(v[l].x[e]);
             s = __builtin_fma(g, g, s);
         }
     return s;
 }
 
+template <bool ONCE>
 __global__ __launch_bounds__(kT) void clip_squares_kernel(Tensors a, double* __restrict__ part) {
     __shared__ double red[kT / kWave];
     double s = 0.0;
     for_chunks(a, [&](int t, int64_t from) {
-        if (a.src_dt[t] == GRWS_F32) s += squares<float>(a.src[t], from, a.size[t]);
-        else if (a.src_dt[t] == GRWS_F16) s += squares<_Float16>(a.src[t], from, a.size[t]);
-        else s += squares<__hip_bfloat16>(a.src[t], from, a.size[t]);
+        if (a.src_dt[t] == GRWS_F32) s += squares<ONCE, float>(a.src[t], from, a.size[t]);
+        else if (a.src_dt[t] == GRWS_F16) s += squares<ONCE, _Float16>(a.src[t], from, a.size[t]);
+        else s += squares<ONCE, __hip_bfloat16>(a.src[t], from, a.size[t]);
     });
     s = block_sum(s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -134,24 +151,31 @@ __global__ __launch_bounds__(kT) void clip_norm_kernel(const double* __restrict_
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
-template <typename T, typename O>
+// (A lane stores 16 bytes next to its neighbour's, so it reads 8 of 16-bit
+// gradients that go to f32.)
+template <bool ONCE, typename T, typename O>
 __device__ __forceinline__ void scale_chunk(const void* src, void* dst, int64_t from, int64_t size, float f) {
+    constexpr int N = 16 / sizeof(O), LOADS = kChunk / (kT * N);
     const T* x = static_cast<const T*>(src);
     O* o = static_cast<O*>(dst);
-    Vec<T> v[kLoads];
+    Vec<T, N> v[LOADS];
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) v[l] = load_vec(x, from + ((int64_t)l * kT + threadIdx.x) * kVec, size);
+    for (int l = 0; l < LOADS; ++l) v[l] = load_vec<ONCE, N>(x, from + ((int64_t)l * kT + threadIdx.x) * N, size);
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) {
-        const int64_t at = from + ((int64_t)l * kT + threadIdx.x) * kVec;
-        Vec<O> w;
+    for (int l = 0; l < LOADS; ++l) {
+        const int64_t at = from + ((int64_t)l * kT + threadIdx.x) * N;
+        Vec<O, N> w;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) w.x[e] = from_float<O>(to_float(v[l].x[e]) * f);
-        if (at + kVec <= size) {
-            __builtin_memcpy(o + at, &w, sizeof(w));
+        for (int e = 0; e < N; ++e) w.x[e] = from_float<O>(to_float(v[l].x[e]) * f);
+        if (at + N <= size) {
+            u32x4_t x4;
+            __builtin_memcpy(&x4, &w, sizeof(w));
+            u32x4_t* p = reinterpret_cast<u32x4_t*>(o + at);
+            if constexpr (ONCE) __builtin_nontemporal_store(x4, p);
+            else *p = x4;
         } else {
 #pragma unroll
-            for (int e = 0; e < kVec; ++e)
+            for (int e = 0; e < N; ++e)
                 if (at + e < size) o[at + e] = w.x[e];
         }
     }
@@ -159,6 +183,7 @@ __device__ __forceinline__ void scale_chunk(const void* src, void* dst, int64_t 
 
 // A factor of exactly one leaves gradients that are clipped in place as they
 // are (in_place), without reading them a second time.
+template <bool ONCE>
 __global__ __launch_bounds__(kT) void clip_scale_kernel(Tensors a, const double* __restrict__ part, int parts,
                                                         float max_norm, const float* scale, int32_t in_place,
                                                         float* __restrict__ norm) {
@@ -175,13 +200,13 @@ __global__ __launch_bounds__(kT) void clip_scale_kernel(Tensors a, const double*
         const int64_t size = a.size[t];
         const int s = a.src_dt[t], d = a.dst_dt[t];
         if (d == s) {
-            if (s == GRWS_F32) scale_chunk<float, float>(x, o, from, size, f);
-            else if (s == GRWS_F16) scale_chunk<_Float16, _Float16>(x, o, from, size, f);
-            else scale_chunk<__hip_bfloat16, __hip_bfloat16>(x, o, from, size, f);
+            if (s == GRWS_F32) scale_chunk<ONCE, float, float>(x, o, from, size, f);
+            else if (s == GRWS_F16) scale_chunk<ONCE, _Float16, _Float16>(x, o, from, size, f);
+            else scale_chunk<ONCE, __hip_bfloat16, __hip_bfloat16>(x, o, from, size, f);
         } else if (s == GRWS_F16) {
-            scale_chunk<_Float16, float>(x, o, from, size, f);
+            scale_chunk<ONCE, _Float16, float>(x, o, from, size, f);
         } else {
-            scale_chunk<__hip_bfloat16, float>(x, o, from, size, f);
+            scale_chunk<ONCE, __hip_bfloat16, float>(x, o, from, size, f);
         }
     });
 }
@@ -267,6 +292,7 @@ extern "C" int grws_clip_grads(const void* const* grads, const int32_t* dtypes, 
     GRWS_CHECK_ARG(norm || outs, "clip: nothing to compute");
     GRWS_CHECK_ARG(!outs || max_norm >= 0.f, "clip: max_norm must not be negative");
     int32_t in_place = 1;
+    int64_t bytes = 0, all_bytes = 0;
     for (int32_t i = 0; i < count; ++i) {
         const int32_t d = out_dtypes ? out_dtypes[i] : dtypes[i];
         if (!known(dtypes[i]) || !known(d))
@@ -276,6 +302,8 @@ extern "C" int grws_clip_grads(const void* const* grads, const int32_t* dtypes, 
         GRWS_CHECK_ARG(sizes[i] >= 0, "clip: negative size");
         if (sizes[i] == 0) continue;
         GRWS_CHECK_ARG(grads[i] && (!outs || outs[i]), "clip: null tensor");
+        bytes += sizes[i] * (int64_t)dtype_size(dtypes[i]);
+        all_bytes += sizes[i] * (int64_t)(dtype_size(dtypes[i]) + (outs ? dtype_size(d) : 0));
         if (outs && outs[i] != grads[i]) in_place = 0;
         GRWS_CHECK_ARG(!outs || outs[i] != grads[i] || d == dtypes[i], "clip: in place is in one dtype");
     }
@@ -285,7 +313,8 @@ extern "C" int grws_clip_grads(const void* const* grads, const int32_t* dtypes, 
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "clip: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     int parts = 0;
     GRWS_TRY(for_launches(grads, dtypes, sizes, outs, out_dtypes, count, [&](const Tensors& a, unsigned blocks) -> int {
-        hipLaunchKernelGGL(clip_squares_kernel, dim3(blocks), dim3(kT), 0, stream, a, part + parts);
+        if (bytes > kCached) hipLaunchKernelGGL(clip_squares_kernel<true>, dim3(blocks), dim3(kT), 0, stream, a, part + parts);
+        else hipLaunchKernelGGL(clip_squares_kernel<false>, dim3(blocks), dim3(kT), 0, stream, a, part + parts);
         GRWS_LAUNCH_CHECK();
         parts += (int)blocks;
         return GRWS_OK;
@@ -299,8 +328,12 @@ extern "C" int grws_clip_grads(const void* const* grads, const int32_t* dtypes, 
     }
     float* first = norm;
     return for_launches(grads, dtypes, sizes, outs, out_dtypes, count, [&](const Tensors& a, unsigned blocks) -> int {
-        hipLaunchKernelGGL(clip_scale_kernel, dim3(blocks), dim3(kT), 0, stream, a, part, parts, max_norm, scale,
-                           in_place, first);
+        if (all_bytes > kCached)
+            hipLaunchKernelGGL(clip_scale_kernel<true>, dim3(blocks), dim3(kT), 0, stream, a, part, parts, max_norm,
+                               scale, in_place, first);
+        else
+            hipLaunchKernelGGL(clip_scale_kernel<false>, dim3(blocks), dim3(kT), 0, stream, a, part, parts, max_norm,
+                               scale, in_place, first);
         GRWS_LAUNCH_CHECK();
         first = nullptr;
         return GRWS_OK;

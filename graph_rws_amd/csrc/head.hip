@@ -361,14 +361,7 @@ __device__ __forceinline__ void begin_logits(float4_t (&acc)[TP][TQ], int64_t vf
 }
 
 // The maxima stay logits: two of them can be one float when multiplied by c1,
-// and a hit is a matter of which is larger.  The exponentials of a row are
-// 2^(z c - ref), ref the rounded m c, of a largest logit m.  c is c1, but a
-// half where m c1 overflows (m a mask of the type's lowest value): floats of
-// that size lie so far apart that any c leaves zero of a z other than m, and
-// with a power of two m c is exact and leaves one of m.
-__device__ __forceinline__ float base2(float m, float c1) {
-    return fabsf(m * c1) == INFINITY && fabsf(m) != INFINITY ? 0.5f : c1;
-}
+// and a hit is a matter of which is larger (base2 in logp.h).
 // what makes a strip's sum one against m c1 itself
 __device__ __forceinline__ float past_rounding(float m, float c1) {
     const float ref = m * c1;
@@ -1929,9 +1922,10 @@ __global__ __launch_bounds__(kT) void head_top_kernel(Targets t, Strips part, in
         }
         offer(p, x, top, 32 + class_bits, bound);
     }
-    put_best(p, top, 32 + class_bits, class_bits, [&](int at, int32_t cls) {
+    put_ranked(p, top, 32 + class_bits, [&](int at, uint64_t key) {
+        const int32_t cls = (int32_t)(all - (key & all));
         top_index[i * top + at] = cls;
-        top_logp[i * top + at] = given_logp(a, live, cls, t.classes, z[cls], inv_t);
+        top_logp[i * top + at] = given_logp(a, live, cls, t.classes, value_of<float>((uint32_t)(key >> class_bits)), inv_t);
     });
 }
 

@@ -47,13 +47,25 @@ __device__ __forceinline__ void add(Stats& a, float z, float m, float c1) {
     a.t = fmaf(e, reach(u), a.t);
 }
 
-// joins lanes d apart, d = 32..1: every lane has the wave's
+// The exponentials are 2^(z c - ref), ref the rounded m c, of a largest logit m.
+// c is c1, but a half where m c1 overflows (m a mask of the type's lowest
+// value): floats of that size lie so far apart that any c leaves zero of a z
+// other than m, and with a power of two m c is exact and leaves one of m.
+__device__ __forceinline__ float base2(float m, float c1) {
+    return fabsf(m * c1) == INFINITY && fabsf(m) != INFINITY ? 0.5f : c1;
+}
+
+// The wave's, in every lane: the largest m first, then sums against it.
 __device__ __forceinline__ Stats join_wave(Stats a, float c1) {
+    float m = a.m;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
+    if (m != -INFINITY) move(a, (a.m - m) * c1);
+    a.m = m;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
-        const Stats b{__shfl_xor(a.m, d, kWave), __shfl_xor(a.s, d, kWave), __shfl_xor(a.t, d, kWave)};
-        // both sides in one order, so the lanes agree
-        a = (threadIdx.x & d) ? join(b, a, c1) : join(a, b, c1);
+        a.s += __shfl_xor(a.s, d, kWave);
+        a.t += __shfl_xor(a.t, d, kWave);
     }
     return a;
 }

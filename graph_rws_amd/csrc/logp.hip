@@ -56,16 +56,31 @@ __device__ __forceinline__ Row row_of(const Stats& a, const Scale& sc) {
     return Row{a.m, a.m == -INFINITY ? __int_as_float(0x7fc00000) : log2f(a.s), sc.inv_t};
 }
 
+// A thread's first given class and its logit, asked for before the pass over
+// the row: two reads that follow one another.
+struct Early {
+    int64_t cls;
+    float z;
+};
+
+template <typename T>
+__device__ __forceinline__ Early early_given(const T* row, int64_t r, int32_t classes, const Given& g, int sub) {
+    Early e{-1, 0.f};
+    if (sub < g.k) e.cls = g.at(r, sub);
+    if (e.cls >= 0 && e.cls < classes) e.z = to_float(row[e.cls]);
+    return e;
+}
+
 // The row's outputs, `lanes` threads of which this is `sub`.
 template <typename T>
 __device__ __forceinline__ void put_row(const Stats& a, const Scale& sc, const T* row, int64_t r, int32_t classes,
-                                        const Given& g, const Outputs& o, int sub, int lanes) {
+                                        const Given& g, Early e, const Outputs& o, int sub, int lanes) {
     const Row q = row_of(a, sc);
     for (int j = sub; j < g.k; j += lanes) {
-        const int64_t c = g.at(r, j);
+        if (j != sub) e = early_given(row, r, classes, g, j);
         float v = 0.f;
-        if (c >= classes) v = __int_as_float(0x7fc00000);
-        else if (c >= 0) v = q.logp(to_float(row[c]));
+        if (e.cls >= classes) v = __int_as_float(0x7fc00000);
+        else if (e.cls >= 0) v = q.logp(e.z);
         o.logp[r * g.k + j] = v;
     }
     if (sub != 0) return;
@@ -73,48 +88,204 @@ __device__ __forceinline__ void put_row(const Stats& a, const Scale& sc, const T
     if (o.saved) o.saved[r] = make_float2(q.m, q.l2);
 }
 
-template <typename T>
-__device__ __forceinline__ void add_chunk(Stats& a, const Chunk<T>& v, float c1) {
-    float z[kMine];
+// The pool's alternatives; a key holds its logit.
+template <typename T, int MAXK>
+__device__ __forceinline__ void put_top(Pool<MAXK>& p, const Row& q, int64_t r, int32_t class_bits, int32_t top,
+                                        const Outputs& o) {
+    const uint64_t low = (1ull << class_bits) - 1;
+    put_ranked(p, top, (int)sizeof(T) * 8 + class_bits, [&](int at, uint64_t key) {
+        o.top_index[r * top + at] = (int32_t)(low - (key & low));
+        o.top_logp[r * top + at] = q.logp(value_of<T>((uint32_t)(key >> class_bits)));
+    });
+}
+
+// What a thread has added: s and t against ref, the rounded m c (see base2),
+// and what that rounding took.
+struct Running {
+    Stats a = no_stats();
+    float c = 1.f, ref = 0.f, past = 0.f;
+
+    // Adds N logits; the largest of them.
+    template <int N>
+    __device__ __forceinline__ float add(const float (&z)[N], float c1) {
+        float m = z[0];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) z[i] = v.in(i) ? to_float(v.get(i)) : -INFINITY;
-    float m = z[0];
+        for (int i = 1; i < N; ++i) m = fmaxf(m, z[i]);
+        if (m > a.m) {
+            const float to = base2(m, c1), r = m * to, p = fabsf(r) == INFINITY ? 0.f : fmaf(-m, to, r);
+            move(a, (a.m - m) * c1 + (past - p));
+            a.m = m;
+            c = to;
+            ref = r;
+            past = p;
+        }
+        const float s = a.s, t = a.t;
 #pragma unroll
-    for (int i = 1; i < kMine; ++i) m = fmaxf(m, z[i]);
-    if (m > a.m) {
-        move(a, (a.m - m) * c1);
-        a.m = m;
+        for (int i = 0; i < N; ++i) {
+            const float u = fmaf(z[i], c, -ref), e = __builtin_amdgcn_exp2f(u);
+            a.s += e;
+            a.t = fmaf(e, u, a.t);
+        }
+        if (a.t != a.t && a.s == a.s) {  // a zero times an infinity: again
+            a.s = s;
+            a.t = t;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float u = fmaf(z[i], c, -ref), e = __builtin_amdgcn_exp2f(u);
+                a.s += e;
+                a.t = fmaf(e, reach(u), a.t);
+            }
+        }
+        return m;
     }
-    m = a.m == -INFINITY ? 0.f : a.m;
+    // Adds a step's logits; the largest of them.
+    template <typename T>
+    __device__ __forceinline__ float add(const Chunk<T>& v, float c1) {
+        float m = -INFINITY;
+        if (v.whole) {
+            // in halves: fewer registers, so one wave more a SIMD
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) add(a, z[i], m, c1);
+            for (int h = 0; h < 2; ++h) {
+                float z[kMine / 2];
+#pragma unroll
+                for (int i = 0; i < kMine / 2; ++i) z[i] = to_float(v.get(h * (kMine / 2) + i));
+                m = fmaxf(m, add(z, c1));
+            }
+            return m;
+        }
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) {
+            if (v.at - (int)(threadIdx.x & 63) * kVec + l * kT * kVec >= v.c1) break;  // nothing of the wave's: uniform
+            float z[kVec];
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) z[e] = v.in(l * kVec + e) ? to_float(v.get(l * kVec + e)) : -INFINITY;
+            m = fmaxf(m, add(z, c1));
+        }
+        return m;
+    }
+    // against m c itself
+    __device__ __forceinline__ Stats stats() {
+        move(a, past);
+        return a;
+    }
+};
+
+// Where the alternatives of small `top` are: every thread leaves the largest
+// logit of each of its runs of steps, at least `top` threads' largest
+// reach a first bound, and only runs that reach it are looked at again.  So the
+// pass over the row has no barrier and no candidates (8,192 x 50,021 bf16 with
+// 16 alternatives: 470 us with a pool that every step offers to).
+template <typename T>
+struct Runs {
+    typedef std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> Order;
+    static constexpr int GROUPS = 32 / sizeof(T);  // of a thread: 8 KB a work-group
+    Order most[GROUPS][kT];
+};
+
+template <typename T, int MAXK>
+__device__ __forceinline__ void offer_runs(Pool<MAXK>& p, Runs<T>& runs, int32_t groups, int32_t steps, const T* row,
+                                           int32_t first, int32_t end, int32_t class_bits, int32_t top) {
+    constexpr int VB = sizeof(T) * 8, OFFER = Sizes<MAXK>::OFFER, GROUPS = Runs<T>::GROUPS;
+    constexpr uint32_t ALL = VB == 16 ? 0xffffu : 0xffffffffu;
+    const uint64_t low = (1ull << class_bits) - 1;
+    uint32_t order[GROUPS], mine = 0;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        order[g] = g < groups ? runs.most[g][threadIdx.x] : 0;
+        mine = order[g] > mine ? order[g] : mine;
+    }
+    // (a NaN, or an infinity whose sum is one, stands for the largest: where
+    // they are the bound, all runs are looked at)
+    uint32_t reach = top <= kT / 2 ? first_bound(p, mine, top, VB) : 0;
+    if ((reach >> (VB - 16)) >= (ALL >> (VB - 16))) reach = 0;
+    __syncthreads();
+    if (threadIdx.x == 0) p.first = 0;
+    __syncthreads();
+    uint32_t in = 0;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+        if (g < groups && order[g] >= reach) in |= 1u << g;
+    uint16_t* chosen = reinterpret_cast<uint16_t*>(runs.most);  // every thread has read its runs
+    if (in) {
+        int at = (int)atomicAdd(&p.first, (uint32_t)__builtin_popcount(in));
+        for (uint32_t m = in; m; m &= m - 1) chosen[at++] = (uint16_t)(__builtin_ctz(m) * kT + (int)threadIdx.x);
+    }
+    __syncthreads();
+    uint64_t bound = reach > 0 ? ((uint64_t)reach << class_bits) - 1 : 0;
+    const int32_t run = steps * kMine;
+    const int64_t count = (int64_t)p.first * run;
+    for (int64_t c = 0; c < count; c += kT * OFFER) {
+        uint64_t x[OFFER];
+#pragma unroll
+        for (int e = 0; e < OFFER; ++e) {
+            const int64_t at = c + e * kT + (int)threadIdx.x;
+            x[e] = 0;
+            if (at < count) {
+                const int32_t k = (int32_t)(at / run), i = (int32_t)(at - (int64_t)k * run);  // logit i of the run
+                const int32_t cls = first + (chosen[k] / kT) * steps * kChunk + i / kVec * kT * kVec +
+                                    chosen[k] % kT * kVec + i % kVec;
+                if (cls < end) x[e] = ((uint64_t)order_of<T>(row[cls]) << class_bits) | (low - (uint32_t)cls);
+            }
+        }
+        offer(p, x, top, VB + class_bits, bound);
+    }
 }
 
 // A work-group a row, or a stretch of one (FINAL false: its statistics and
 // keys go to `part` and `best`).  MAXK 0: no alternatives.
-template <typename T, bool FINAL, int MAXK>
+template <typename T, bool FINAL, int MAXK, bool ONCE>
 __global__ __launch_bounds__(kT) void logp_rows_kernel(const T* __restrict__ logits, int64_t ld, int64_t r0,
                                                        int32_t classes, int32_t class_bits, int32_t top,
                                                        int32_t stretch, Scale sc, Given g, Outputs o,
                                                        float4* __restrict__ part, uint64_t* __restrict__ best) {
+    constexpr bool RUNS = MAXK == kSmallK;
     __shared__ Pool<MAXK ? MAXK : 1> p;
+    __shared__ std::conditional_t<RUNS, Runs<T>, int> runs;
     __shared__ float sm[kWaves], ss[kWaves], st[kWaves];
     const int64_t r = r0 + blockIdx.x;
     const T* row = logits + r * ld;
     const int32_t first = (int32_t)blockIdx.y * stretch;
     const int32_t end = classes - first < stretch ? classes : first + stretch;
     const int bits = (int)sizeof(T) * 8 + class_bits;
-    if (MAXK && threadIdx.x == 0) p.count = 0;
     uint64_t bound = 0;
     float least = -INFINITY;
-    Stats a = no_stats();
-    for (int32_t c = first; c < end; c += kChunk) {
-        Chunk<T> v;
-        v.load(row, c, end);
-        add_chunk(a, v, sc.c1);
-        if constexpr (MAXK) offer_chunk<MAXK>(p, v, row, c, first, end, class_bits, top, bound, least);
+    Running sum;
+    Early early{-1, 0.f};
+    if constexpr (FINAL) early = early_given(row, r, classes, g, threadIdx.x);
+    // what lies before a whole 16 bytes: a logit a thread
+    const int32_t head = end > first ? before_aligned(row + first, end - first) : 0, begin = first + head;
+    if ((int32_t)threadIdx.x < head) {
+        const float z[1] = {to_float(row[first + threadIdx.x])};
+        sum.add(z, sc.c1);
     }
-    a = join_wave(a, sc.c1);
+    const int32_t all_steps = end > begin ? (end - begin + kChunk - 1) / kChunk : 0;
+    const int32_t steps = (all_steps + Runs<T>::GROUPS - 1) / Runs<T>::GROUPS;  // of a run
+    float run = -INFINITY;
+    int32_t group = 0, left = steps;
+    if constexpr (MAXK) {
+        __syncthreads();
+        if ((int32_t)threadIdx.x < head)
+            p.keys[threadIdx.x] = ((uint64_t)order_of<T>(row[first + threadIdx.x]) << class_bits) |
+                                  (((1ull << class_bits) - 1) - (uint32_t)(first + threadIdx.x));
+        if (threadIdx.x == 0) p.count = head;
+        __syncthreads();
+    }
+    for (int32_t c = begin; c < end; c += kChunk) {
+        Chunk<T> v;
+        v.template load<ONCE>(row, c, end);
+        const float m = sum.add(v, sc.c1);
+        if constexpr (RUNS) {
+            run = fmaxf(run, m);
+            if (--left == 0 || c + kChunk >= end) {
+                runs.most[group++][threadIdx.x] = order_of<T>(from_float<T>(sum.a.s == sum.a.s ? run : sum.a.s));
+                run = -INFINITY;
+                left = steps;
+            }
+        } else if constexpr (MAXK) {
+            offer_chunk<MAXK>(p, v, row, c, begin, end, class_bits, top, bound, least);
+        }
+    }
+    Stats a = join_wave(sum.stats(), sc.c1);
     if ((threadIdx.x & 63) == 0) {
         sm[threadIdx.x >> 6] = a.m;
         ss[threadIdx.x >> 6] = a.s;
@@ -124,23 +295,18 @@ __global__ __launch_bounds__(kT) void logp_rows_kernel(const T* __restrict__ log
     a = Stats{sm[0], ss[0], st[0]};
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) a = join(a, Stats{sm[w], ss[w], st[w]}, sc.c1);
+    if constexpr (RUNS) offer_runs<T>(p, runs, group, steps, row, begin, end, class_bits, top);
     if constexpr (FINAL) {
-        put_row(a, sc, row, r, classes, g, o, threadIdx.x, kT);
+        put_row(a, sc, row, r, classes, g, early, o, threadIdx.x, kT);
         if constexpr (MAXK) {
-            const Row q = row_of(a, sc);
-            put_best(p, top, bits, class_bits, [&](int at, int32_t cls) {
-                o.top_index[r * top + at] = cls;
-                o.top_logp[r * top + at] = q.logp(to_float(row[cls]));
-            });
+            put_top<T>(p, row_of(a, sc), r, class_bits, top, o);
         }
     } else {
         const int64_t at = blockIdx.x * (int64_t)gridDim.y + blockIdx.y;
         if (threadIdx.x == 0) part[at] = make_float4(a.m, a.s, a.t, 0.f);
         if constexpr (MAXK) {
-            keep_best(p, top, bits);
-            __syncthreads();
-            const int n = p.count < top ? p.count : top;
-            for (int j = threadIdx.x; j < top; j += kT) best[at * top + j] = j < n ? p.keys[j] : 0;
+            for (int j = threadIdx.x; j < top; j += kT) best[at * top + j] = 0;  // (a barrier follows)
+            put_ranked(p, top, bits, [&](int j, uint64_t key) { best[at * top + j] = key; });
         }
     }
 }
@@ -155,6 +321,7 @@ __global__ __launch_bounds__(kT) void logp_join_kernel(const T* __restrict__ log
     __shared__ Pool<MAXK ? MAXK : 1> p;
     const int64_t r = r0 + blockIdx.x;
     const T* row = logits + r * ld;
+    const Early early = early_given(row, r, classes, g, threadIdx.x);
     Stats a = no_stats();
     // every wave joins them all, in one order
     for (int w = threadIdx.x & 63; w < stretches; w += 64) {
@@ -162,7 +329,7 @@ __global__ __launch_bounds__(kT) void logp_join_kernel(const T* __restrict__ log
         a = join(a, Stats{x.x, x.y, x.z}, sc.c1);
     }
     a = join_wave(a, sc.c1);
-    put_row(a, sc, row, r, classes, g, o, threadIdx.x, kT);
+    put_row(a, sc, row, r, classes, g, early, o, threadIdx.x, kT);
     if constexpr (MAXK) {
         if (threadIdx.x == 0) p.count = 0;
         constexpr int OFFER = Sizes<MAXK>::OFFER;
@@ -178,11 +345,7 @@ __global__ __launch_bounds__(kT) void logp_join_kernel(const T* __restrict__ log
             }
             offer(p, x, top, bits, bound);
         }
-        const Row q = row_of(a, sc);
-        put_best(p, top, bits, class_bits, [&](int at, int32_t cls) {
-            o.top_index[r * top + at] = cls;
-            o.top_logp[r * top + at] = q.logp(to_float(row[cls]));
-        });
+        put_top<T>(p, row_of(a, sc), r, class_bits, top, o);
     }
 }
 
@@ -199,6 +362,7 @@ __global__ __launch_bounds__(kT) void logp_wave_kernel(const T* __restrict__ log
     const int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
     if (r >= rows) return;  // uniform over the wave
     const T* row = logits + r * ld;
+    const Early early = early_given(row, r, classes, g, lane);
     T x[PER];
     float m = -INFINITY;
 #pragma unroll
@@ -217,7 +381,7 @@ __global__ __launch_bounds__(kT) void logp_wave_kernel(const T* __restrict__ log
         a.s += __shfl_xor(a.s, d, kWave);
         a.t += __shfl_xor(a.t, d, kWave);
     }
-    put_row(a, sc, row, r, classes, g, o, lane, 64);
+    put_row(a, sc, row, r, classes, g, early, o, lane, 64);
     if (top == 0) return;
     const Row q = row_of(a, sc);
     const uint64_t low = (1ull << class_bits) - 1;
@@ -279,11 +443,23 @@ struct Slope {
     }
 };
 
+template <bool ONCE, typename V>
+__device__ __forceinline__ void store_vec(void* p, const V& v) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+    u32x4 w[sizeof(V) / 16];
+    __builtin_memcpy(w, &v, sizeof(V));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / 16); ++i) {
+        if constexpr (ONCE) __builtin_nontemporal_store(w[i], static_cast<u32x4*>(p) + i);
+        else static_cast<u32x4*>(p)[i] = w[i];
+    }
+}
+
 // Elements at a time of a row's stretch; ROWS rows a work-group (a wave each)
 // or one.  Given classes are put in place after the rest: each wave's stores
 // have left before its own threads (ONE: the work-group's, behind a barrier)
 // write the same places again.
-template <typename T, bool ONE>
+template <typename T, bool ONE, bool ONCE>
 __global__ __launch_bounds__(kT) void logp_grad_kernel(const T* __restrict__ logits, int64_t ld, int64_t r0,
                                                        int64_t rows, int32_t classes, int32_t stretch, float c1,
                                                        float inv_t, Given g, Upstream up,
@@ -302,19 +478,19 @@ __global__ __launch_bounds__(kT) void logp_grad_kernel(const T* __restrict__ log
     const float b = up.dentropy ? up.dentropy[r] : 0.f;
     const float A = given_sum(g, up, r, classes, threadIdx.x & 63);
     const Slope f{s.x, s.y, c1, up.dentropy ? fmaf(b, entropy[r], A) : A, b * kLn2, inv_t};
+    constexpr int E = 16 / sizeof(T);  // a lane's 16 bytes lie next to its neighbour's
     struct Vec {
-        T x[kVec];
+        T x[E];
     };
-    for (int32_t c = first + sub * kVec; c < end; c += N * kVec) {
-        Vec v;
-        if (c + kVec <= end) {
-            __builtin_memcpy(&v, row + c, sizeof(v));
+    for (int32_t c = first + sub * E; c < end; c += N * E) {
+        if (c + E <= end) {
+            Vec v = load_vec<ONCE, Vec>(row + c);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) v.x[e] = from_float<T>(f.of(to_float(v.x[e])));
-            __builtin_memcpy(to + c, &v, sizeof(v));
+            for (int e = 0; e < E; ++e) v.x[e] = from_float<T>(f.of(to_float(v.x[e])));
+            store_vec<ONCE>(to + c, v);
         } else {
 #pragma unroll
-            for (int e = 0; e < kVec; ++e)
+            for (int e = 0; e < E; ++e)
                 if (c + e < end) to[c + e] = from_float<T>(f.of(to_float(row[c + e])));
         }
     }
@@ -346,6 +522,10 @@ int32_t stretches(int64_t rows, int64_t classes, int64_t top) {
     if (n > most) n = most;
     return n < 1 ? 1 : (int32_t)n;
 }
+
+// Whether logits are read past the caches: those that do not fit into the last
+// one (256 MB), where the backward would find them.
+bool streams(int64_t bytes) { return bytes > ((int64_t)192 << 20); }
 
 bool by_wave(int64_t classes, int64_t top) { return classes <= kWaveClasses && top <= kWaveTop; }
 
@@ -382,17 +562,22 @@ int forward(const T* x, int64_t ld, int64_t rows, int32_t classes, int32_t top, 
         return GRWS_OK;
     }
     const int32_t n = stretches(rows, classes, top);
+    const bool once = streams(rows * classes * (int64_t)sizeof(T));
     const int32_t stretch = (int32_t)(((int64_t)classes + n - 1) / n + 63) / 64 * 64;  // (the last may be empty)
     for (int64_t r0 = 0; r0 < rows; r0 += kMostBlocks) {  // (with several stretches there are fewer than 1,024 rows)
         const dim3 grid((unsigned)(rows - r0 < kMostBlocks ? rows - r0 : kMostBlocks), (unsigned)n);
 #define GRWS_LOGP(MAXK)                                                                                              \
     do {                                                                                                             \
         if (n == 1) {                                                                                                \
-            hipLaunchKernelGGL((logp_rows_kernel<T, true, MAXK>), grid, dim3(kT), 0, stream, x, ld, r0, classes, cb, \
-                               top, stretch, sc, g, o, part, best);                                                  \
+            if (once && MAXK != kMaxK)                                                                               \
+                hipLaunchKernelGGL((logp_rows_kernel<T, true, MAXK, MAXK != kMaxK>), grid, dim3(kT), 0, stream, x,   \
+                                   ld, r0, classes, cb, top, stretch, sc, g, o, part, best);                         \
+            else                                                                                                     \
+                hipLaunchKernelGGL((logp_rows_kernel<T, true, MAXK, false>), grid, dim3(kT), 0, stream, x, ld, r0,   \
+                                   classes, cb, top, stretch, sc, g, o, part, best);                                 \
         } else {                                                                                                     \
-            hipLaunchKernelGGL((logp_rows_kernel<T, false, MAXK>), grid, dim3(kT), 0, stream, x, ld, r0, classes,    \
-                               cb, top, stretch, sc, g, o, part, best);                                              \
+            hipLaunchKernelGGL((logp_rows_kernel<T, false, MAXK, false>), grid, dim3(kT), 0, stream, x, ld, r0,      \
+                               classes, cb, top, stretch, sc, g, o, part, best);                                     \
             GRWS_LAUNCH_CHECK();                                                                                     \
             hipLaunchKernelGGL((logp_join_kernel<T, MAXK>), dim3(grid.x), dim3(kT), 0, stream, x, ld, r0, classes,   \
                                cb, top, n, sc, g, o, part, best);                                                    \
@@ -412,7 +597,7 @@ int backward(const T* x, int64_t ld, int64_t rows, int32_t classes, float c1, fl
              const Upstream& up, const float2* saved, const float* entropy, T* out, int64_t ldo, hipStream_t stream) {
     if (classes <= kWaveClasses) {
         const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves));
-        hipLaunchKernelGGL((logp_grad_kernel<T, false>), grid, dim3(kT), 0, stream, x, ld, (int64_t)0, rows, classes,
+        hipLaunchKernelGGL((logp_grad_kernel<T, false, false>), grid, dim3(kT), 0, stream, x, ld, (int64_t)0, rows, classes,
                            classes, c1, inv_t, g, up, saved, entropy, out, ldo);
         GRWS_LAUNCH_CHECK();
         return GRWS_OK;
@@ -420,10 +605,15 @@ int backward(const T* x, int64_t ld, int64_t rows, int32_t classes, float c1, fl
     // (at most 2^18 stretches of a row, so 2^13 rows or more of 2^31 threads)
     const int64_t n = ((int64_t)classes + kGradStretch - 1) / kGradStretch;
     const int64_t most = kMostBlocks / n < 1 ? 1 : kMostBlocks / n;
+    const bool once = streams(rows * classes * (int64_t)sizeof(T));
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
         const dim3 grid((unsigned)(rows - r0 < most ? rows - r0 : most), (unsigned)n);
-        hipLaunchKernelGGL((logp_grad_kernel<T, true>), grid, dim3(kT), 0, stream, x, ld, r0, rows, classes,
-                           kGradStretch, c1, inv_t, g, up, saved, entropy, out, ldo);
+#define GRWS_LOGP_GRAD(ONCE)                                                                                         \
+    hipLaunchKernelGGL((logp_grad_kernel<T, true, ONCE>), grid, dim3(kT), 0, stream, x, ld, r0, rows, classes,       \
+                       kGradStretch, c1, inv_t, g, up, saved, entropy, out, ldo)
+        if (once) GRWS_LOGP_GRAD(true);
+        else GRWS_LOGP_GRAD(false);
+#undef GRWS_LOGP_GRAD
         GRWS_LAUNCH_CHECK();
     }
     return GRWS_OK;

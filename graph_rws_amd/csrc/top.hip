@@ -28,19 +28,102 @@ __global__ __launch_bounds__(kT, MAXK <= kSmallK ? 8 : 5) void top_rows_kernel(
     const T* __restrict__ logits, int64_t ld, int32_t classes, int32_t class_bits, int32_t k, int32_t stretch,
                                                       T* __restrict__ values, int32_t* __restrict__ index,
                                                       uint64_t* __restrict__ best) {
+    constexpr int VB = sizeof(T) * 8, CAP = Sizes<MAXK>::CAP, OFFER = Sizes<MAXK>::OFFER;
+    struct Vec {
+        uint32_t w[kVec * sizeof(T) / 4];
+    };
     __shared__ Pool<MAXK> p;
     const int64_t r = blockIdx.x;
     const T* row = logits + r * ld;
     const int32_t c0 = (int32_t)blockIdx.y * stretch;
     const int32_t c1 = classes - c0 < stretch ? classes : c0 + stretch;
-    const int bits = (int)sizeof(T) * 8 + class_bits;
+    const int bits = VB + class_bits;
+    const uint64_t low = (1ull << class_bits) - 1;
     if (threadIdx.x == 0) p.count = 0;
     uint64_t bound = 0;
     float least = -INFINITY;  // the bound's logit: smaller ones are not looked at
     for (int32_t c = c0; c < c1; c += kChunk) {
-        Chunk<T> v;
-        v.load(row, c, c1);
-        offer_chunk<MAXK>(p, v, row, c, c0, c1, class_bits, k, bound, least);
+        // load i of a thread: logits c + 2,048 i + 8 thread + 0..7
+        Vec v[kLoads];
+        const int32_t at = c + (int32_t)threadIdx.x * kVec;
+        const bool whole = c + kChunk <= c1;  // uniform
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int32_t f = at + i * kT * kVec;
+            if (whole || f + kVec <= c1) {
+                __builtin_memcpy(&v[i], row + f, sizeof(Vec));  // rows of any alignment
+            } else {
+                T x[kVec];
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) x[e] = f + e < c1 ? row[f + e] : from_float<T>(0.f);
+                __builtin_memcpy(&v[i], x, sizeof(Vec));
+            }
+        }
+        auto get = [&](int i) -> T {
+            const uint32_t w = v[i / kVec].w[(i % kVec) * (int)sizeof(T) / 4];
+            if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)(w >> (16 * (i & 1))));
+            else return __builtin_bit_cast(T, w);
+        };
+        auto cls = [&](int i) { return at + (i / kVec) * kT * kVec + i % kVec; };
+        // a candidate is read again (few are, from the L1 or L2) instead of
+        // holding 32 keys in registers
+        auto key = [&](int i) {
+            const int32_t x = cls(i);
+            return ((uint64_t)order_of<T>(row[x]) << class_bits) | (low - (uint32_t)x);
+        };
+        if (c == c0 && k <= kT / 2 && c1 - c0 >= 4 * kT) {  // uniform
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i)
+                if (cls(i) < c1) {
+                    const uint32_t o = order_of<T>(get(i));
+                    most = o > most ? o : most;
+                }
+            const uint32_t o = first_bound(p, most, k, VB);
+            if (o > 0) {
+                bound = ((uint64_t)o << class_bits) - 1;
+                least = value_of<T>(o);
+            }
+        }
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (!(to_float(get(i)) < least) && (whole || cls(i) < c1)) mask |= 1u << i;
+        // room for the wave's candidates; what does not fit shows in the count
+        __syncthreads();
+        const int before = p.count;
+        __syncthreads();
+        const int mine = __builtin_popcount(mask);
+        int incl = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d, kWave);
+            if ((int)(threadIdx.x & 63) >= d) incl += o;
+        }
+        int base = 0;
+        if ((threadIdx.x & 63) == 63 && incl) base = atomicAdd(&p.count, incl);
+        base = __shfl(base, 63, kWave) + incl - mine;
+        if (base + mine <= CAP) {
+#pragma unroll 1
+            for (uint32_t m = mask; m; m &= m - 1) {
+                const uint64_t x = key(__builtin_ctz(m));
+                // a logit equal to the bound's, of a later class, keeps its place as an empty key
+                p.keys[base++] = x > bound ? x : 0;
+            }
+        }
+        __syncthreads();
+        if (p.count > CAP) {  // uniform: again, a few a thread at a time
+            __syncthreads();
+            if (threadIdx.x == 0) p.count = before;
+#pragma unroll 1
+            for (int i = 0; i < kMine; i += OFFER) {
+                uint64_t x[OFFER];
+#pragma unroll
+                for (int e = 0; e < OFFER; ++e) x[e] = (mask >> (i + e)) & 1 ? key(i + e) : 0;
+                offer(p, x, k, bits, bound);
+            }
+            if (bound > 0) least = value_of<T>((uint32_t)((bound + 1) >> class_bits));
+        }
     }
     if constexpr (FINAL) {
         write_best(p, k, bits, class_bits, row, values + r * k, index + r * k);

@@ -190,6 +190,26 @@ __device__ __forceinline__ void put_best(Pool<MAXK>& p, int k, int bits, int cla
     }
 }
 
+// put(place, key) for the pool's k largest, by counting the larger ones: of few
+// keys all of them, without finding the k-th first.
+template <int MAXK, typename F>
+__device__ __forceinline__ void put_ranked(Pool<MAXK>& p, int k, int bits, F put) {
+    __syncthreads();
+    int n = p.count;
+    if (n > kT) {  // uniform
+        keep_best(p, k, bits);
+        __syncthreads();
+        n = p.count < k ? p.count : k;
+    }
+    for (int a = threadIdx.x; a < n; a += kT) {
+        const uint64_t key = p.keys[a];
+        int rank = 0;
+#pragma unroll 8
+        for (int b = 0; b < n; ++b) rank += p.keys[b] > key;
+        if (key != 0 && rank < k) put(rank, key);
+    }
+}
+
 // The first bound: order bits that at least k of the threads' maxima reach
 // (their upper 16 bits; the first wave, 4 maxima a lane).
 template <int MAXK>
@@ -214,7 +234,35 @@ __device__ __forceinline__ uint32_t first_bound(Pool<MAXK>& p, uint32_t most, in
     return p.first;
 }
 
-// A work-group's step through a row: thread's logit i is class at + 2,048 (i / 8) + i % 8.
+// A V from any address.  ONCE: what does not fit into the last cache goes past
+// them (8,192 x 50,048 bf16 forward 126 us against 141; of 16,384 x 5,003, which
+// do fit, 51 against 46).
+template <bool ONCE, typename V>
+__device__ __forceinline__ V load_vec(const void* p) {
+    static_assert(sizeof(V) % 16 == 0, "whole loads");
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+    u32x4 w[sizeof(V) / 16];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / 16); ++i)
+        if constexpr (ONCE) w[i] = __builtin_nontemporal_load(static_cast<const u32x4*>(p) + i);
+        else w[i] = static_cast<const u32x4*>(p)[i];
+    V v;
+    __builtin_memcpy(&v, w, sizeof(V));
+    return v;
+}
+
+// Elements before the first that lies at a whole 16 bytes, of `most`.  (Loads of
+// 16 bytes that do not take twice the time: 4,099 rows of 100,003 bf16, every
+// other one at an odd element, 219 us against 186.)
+template <typename T>
+__device__ __forceinline__ int32_t before_aligned(const T* p, int32_t most) {
+    const int32_t n = (int32_t)((0 - reinterpret_cast<uintptr_t>(p)) & 15) / (int32_t)sizeof(T);
+    return n < most ? n : most;
+}
+
+// A work-group's step through a row: load i of a thread has the logits from
+// at + 2,048 i on, kVec of them; where those go past the end, the last kVec of
+// the row, of which the first are not its own (rows have kVec logits or more).
 template <typename T>
 struct Chunk {
     struct Vec {
@@ -224,31 +272,27 @@ struct Chunk {
     int32_t at, c1;
     bool whole;  // uniform
 
-    // logits c.. of a stretch that ends at c1 (zeros past it)
+    // logits c.. of a stretch that ends at `end`
+    template <bool ONCE>
     __device__ __forceinline__ void load(const T* row, int32_t c, int32_t end) {
         at = c + (int32_t)threadIdx.x * kVec;
         c1 = end;
         whole = c + kChunk <= c1;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int32_t f = at + i * kT * kVec;
-            if (whole || f + kVec <= c1) {
-                __builtin_memcpy(&v[i], row + f, sizeof(Vec));  // rows of any alignment
-            } else {
-                T x[kVec];
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) x[e] = f + e < c1 ? row[f + e] : from_float<T>(0.f);
-                __builtin_memcpy(&v[i], x, sizeof(Vec));
-            }
-        }
+        for (int i = 0; i < kLoads; ++i) v[i] = load_vec<ONCE, Vec>(row + from(i));
+    }
+    // first class of load i
+    __device__ __forceinline__ int32_t from(int i) const {
+        const int32_t f = at + i * kT * kVec;
+        return whole || f + kVec <= c1 ? f : c1 - kVec;
     }
     __device__ __forceinline__ T get(int i) const {
         const uint32_t w = v[i / kVec].w[(i % kVec) * (int)sizeof(T) / 4];
         if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)(w >> (16 * (i & 1))));
         else return __builtin_bit_cast(T, w);
     }
-    __device__ __forceinline__ int32_t cls(int i) const { return at + (i / kVec) * kT * kVec + i % kVec; }
-    __device__ __forceinline__ bool in(int i) const { return whole || cls(i) < c1; }
+    __device__ __forceinline__ int32_t cls(int i) const { return from(i / kVec) + i % kVec; }
+    __device__ __forceinline__ bool in(int i) const { return whole || cls(i) >= at + i / kVec * kT * kVec; }
 };
 
 // Offers a step's logits to the pool.  c0: the stretch's first class; bound:
