@@ -449,7 +449,8 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
             if (a.strips.z) {  // uniform
                 float* z = a.strips.z + row * a.strips.ldz + vfirst;
 #pragma unroll
-                for (int i = 0; i < TP; ++i) *reinterpret_cast<float4_t*>(z + C::p_of(i, lane)) = acc[i][j];
+                for (int i = 0; i < TP; ++i)
+                    __builtin_nontemporal_store(acc[i][j], reinterpret_cast<float4_t*>(z + C::p_of(i, lane)));
             }
         } else {
             if (lane < 16) a.part[strip * a.np + row] = make_float2(m, s);
@@ -1839,44 +1840,51 @@ __global__ __launch_bounds__(512) void head_given_join_kernel(Targets t, Strips 
 }
 
 // A work-group a row: joins its strips, reads the given classes' logits, and
-// finds the `top` largest.  They lie in the `top` strips with the largest
-// maxima (of equal ones the first: each holds a logit in front of any that is
-// left out), so of z no more than those is read, and of those what reaches the
-// last one's maximum is looked at.
+// finds the `top` largest.  Where `top` strips' maxima reach a bound, so do the
+// `top` largest logits: only strips that reach it are read, and of those what
+// does.  The bound is the `top`-th largest of the threads' largest maxima, or
+// nothing where `top` is more than half of the threads (then it rises as the
+// logits go by).
+constexpr int kListed = 2048;  // strips that are looked at, at a time
+
 template <int MAXK>
 __global__ __launch_bounds__(kT) void head_top_kernel(Targets t, Strips part, int32_t strips, int32_t strip_classes,
-                                                      int32_t strip_bits, int32_t class_bits, int32_t top, float c1,
-                                                      float inv_t, GivenOut o, float* __restrict__ top_logp,
+                                                      int32_t class_bits, int32_t top, float c1, float inv_t,
+                                                      GivenOut o, float* __restrict__ top_logp,
                                                       int32_t* __restrict__ top_index) {
     __shared__ Pool<MAXK> p;
     __shared__ float sm[kWaves], ss[kWaves], st[kWaves];
-    __shared__ int32_t chosen[MAXK];
-    __shared__ uint32_t reached;
-    constexpr int OFFER = Sizes<MAXK>::OFFER;
+    __shared__ int32_t chosen[kListed];
+    __shared__ int32_t listed;
+    constexpr int OFFER = Sizes<MAXK>::OFFER, HELD = kListed / kT;
     const int64_t i = blockIdx.x;
     const float4* mine = part.part + i * part.row;
     const float* z = part.z + i * part.ldz;
-    const uint64_t low = (1ull << strip_bits) - 1;
-    if (threadIdx.x == 0) {
-        p.count = 0;
-        reached = ~0u;
-    }
+    const int k = t.labels ? 1 : t.k;
+    // the first given class's logit, while the strips are on their way
+    const int64_t cls0 = (int)threadIdx.x < k ? given_at(t, i, threadIdx.x) : -1;
+    const float z0 = cls0 >= 0 && cls0 < t.classes ? z[cls0] : 0.f;
+    if (threadIdx.x == 0) p.count = 0;
+    // a sum that is not a number: a NaN (or an infinity) in the strip, larger than everything
+    auto order = [&](const float4& v) { return order_of<float>(v.y == v.y ? v.x : v.y); };
     Stats a = no_stats();
-    uint64_t bound = 0;
-    for (int32_t c = 0; c < strips; c += kT * OFFER) {
-        uint64_t x[OFFER];
+    uint32_t held[HELD], most = 0;  // orders of the first strips
 #pragma unroll
-        for (int e = 0; e < OFFER; ++e) {
-            const int32_t k = c + e * kT + (int32_t)threadIdx.x;
-            x[e] = 0;
-            if (k < strips) {
-                const float4 v = mine[k];
-                a = join(a, exact_strip(v, c1), c1);
-                // a sum that is not a number: a NaN in the strip, larger than everything
-                x[e] = ((uint64_t)order_of<float>(v.y == v.y ? v.x : v.y) << strip_bits) | (low - (uint32_t)k);
-            }
+    for (int h = 0; h < HELD; ++h) {
+        const int32_t s = h * kT + (int32_t)threadIdx.x;
+        held[h] = 0;
+        if (s < strips) {
+            const float4 v = mine[s];
+            a = join(a, exact_strip(v, c1), c1);
+            held[h] = order(v);
+            most = held[h] > most ? held[h] : most;
         }
-        offer(p, x, top, 32 + strip_bits, bound);
+    }
+    for (int32_t s = kListed + (int32_t)threadIdx.x; s < strips; s += kT) {
+        const float4 v = mine[s];
+        a = join(a, exact_strip(v, c1), c1);
+        const uint32_t x = order(v);
+        most = x > most ? x : most;
     }
     a = join_wave(a, c1);
     if ((threadIdx.x & 63) == 0) {
@@ -1884,48 +1892,53 @@ __global__ __launch_bounds__(kT) void head_top_kernel(Targets t, Strips part, in
         ss[threadIdx.x >> 6] = a.s;
         st[threadIdx.x >> 6] = a.t;
     }
-    keep_best(p, top, 32 + strip_bits);
-    __syncthreads();
+    uint32_t reach = 0;
+    if (top <= kT / 2) reach = first_bound(p, most, top, 32);
+    else __syncthreads();
+    // (strips that are not a number at the bound: everything is looked at)
+    if (reach >= 0xffff0000u) reach = 0;
     a = Stats{sm[0], ss[0], st[0]};
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) a = join(a, Stats{sm[w], ss[w], st[w]}, c1);
     const bool live = row_state<1>(t, i, 0) == 1;
-    const int k = t.labels ? 1 : t.k;
     for (int j = threadIdx.x; j < k; j += kT) {
-        const int64_t cls = given_at(t, i, j);
-        o.logp[i * k + j] =
-            given_logp(a, live, cls, t.classes, z[cls < 0 || cls >= t.classes ? 0 : cls], inv_t);
+        const int64_t cls = j < kT ? cls0 : given_at(t, i, j);
+        const float x = j < kT ? z0 : z[cls < 0 || cls >= t.classes ? 0 : cls];
+        o.logp[i * k + j] = given_logp(a, live, cls, t.classes, x, inv_t);
     }
     if (threadIdx.x == 0) put_given_row(a, c1, live, o, i);
-    const int n = p.count < top ? p.count : top;
-    for (int j = threadIdx.x; j < n; j += kT) {
-        const uint64_t key = p.keys[j];
-        chosen[j] = (int32_t)(low - (key & low));
-        if (n == top) atomicMin(&reached, (uint32_t)(key >> strip_bits));  // whole numbers: no order
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) p.count = 0;
-    // (strips with a NaN or an infinity: everything in them is looked at)
-    bound = n == top && reached != ~0u ? ((uint64_t)reached << class_bits) - 1 : 0;
+    uint64_t bound = reach > 0 ? ((uint64_t)reach << class_bits) - 1 : 0;
     const uint64_t all = (1ull << class_bits) - 1;
-    const int32_t count = n * strip_classes;
-    for (int32_t c = 0; c < count; c += kT * OFFER) {
-        uint64_t x[OFFER];
+    for (int32_t s0 = 0; s0 < strips; s0 += kListed) {
+        __syncthreads();
+        if (threadIdx.x == 0) listed = 0;
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < OFFER; ++e) {
-            const int32_t at = c + e * kT + (int32_t)threadIdx.x;
-            x[e] = 0;
-            if (at < count) {
-                const int64_t cls = (int64_t)chosen[at / strip_classes] * strip_classes + at % strip_classes;
-                if (cls < t.classes) x[e] = ((uint64_t)order_of<float>(z[cls]) << class_bits) | (all - (uint32_t)cls);
-            }
+        for (int h = 0; h < HELD; ++h) {
+            const int32_t s = s0 + h * kT + (int32_t)threadIdx.x;
+            if (s < strips && (s0 == 0 ? held[h] : order(mine[s])) >= reach) chosen[atomicAdd(&listed, 1)] = s;
         }
-        offer(p, x, top, 32 + class_bits, bound);
+        __syncthreads();
+        const int32_t count = listed * strip_classes;
+        for (int32_t c = 0; c < count; c += kT * OFFER) {
+            uint64_t x[OFFER];
+#pragma unroll
+            for (int e = 0; e < OFFER; ++e) {
+                const int32_t at = c + e * kT + (int32_t)threadIdx.x;
+                x[e] = 0;
+                if (at < count) {
+                    const int64_t cls = (int64_t)chosen[at / strip_classes] * strip_classes + at % strip_classes;
+                    if (cls < t.classes)
+                        x[e] = ((uint64_t)order_of<float>(z[cls]) << class_bits) | (all - (uint32_t)cls);
+                }
+            }
+            offer(p, x, top, 32 + class_bits, bound);
+        }
     }
     put_ranked(p, top, 32 + class_bits, [&](int at, uint64_t key) {
-        const int32_t cls = (int32_t)(all - (key & all));
-        top_index[i * top + at] = cls;
-        top_logp[i * top + at] = given_logp(a, live, cls, t.classes, value_of<float>((uint32_t)(key >> class_bits)), inv_t);
+        top_index[i * top + at] = (int32_t)(all - (key & all));
+        top_logp[i * top + at] =
+            given_logp(a, live, 0, t.classes, value_of<float>((uint32_t)(key >> class_bits)), inv_t);
     });
 }
 
@@ -2875,7 +2888,7 @@ extern "C" int grws_head_log_probs_fwd(const grws_head* h, int32_t top, float* l
         if (top) {
 #define GRWS_HEAD_TOP(MAXK)                                                                                           \
     hipLaunchKernelGGL(head_top_kernel<MAXK>, dim3((unsigned)sb.n), dim3(kT), 0, stream, t, part, (int32_t)strips,    \
-                       (int32_t)s.strip_classes, bits_for(strips), bits_for(s.V), top, c1, inv_t, o,                  \
+                       (int32_t)s.strip_classes, bits_for(s.V), top, c1, inv_t, o,                                    \
                        top_logp + r0 * top, top_index + r0 * top)
             if (top <= kSmallK) GRWS_HEAD_TOP(kSmallK);
             else GRWS_HEAD_TOP(kMaxK);

@@ -336,6 +336,16 @@ __global__ __launch_bounds__(kT) void logp_join_kernel(const T* __restrict__ log
         const int bits = (int)sizeof(T) * 8 + class_bits;
         const int64_t count = (int64_t)stretches * top;
         uint64_t bound = 0;
+        if (top <= kT / 2) {  // what `top` of the threads' largest keys reach
+            constexpr int VB = sizeof(T) * 8;
+            uint32_t most = 0;
+            for (int64_t c = threadIdx.x; c < count; c += kT) {
+                const uint32_t x = (uint32_t)(best[blockIdx.x * count + c] >> class_bits);
+                most = x > most ? x : most;
+            }
+            const uint32_t reach = first_bound(p, most, top, VB);
+            if (reach > 0) bound = ((uint64_t)reach << class_bits) - 1;
+        }
         for (int64_t c = 0; c < count; c += kT * OFFER) {
             uint64_t x[OFFER];
 #pragma unroll
