@@ -1103,6 +1103,11 @@ struct FewArgs {
     const GivenRow* given;  // backward
 };
 
+// Log probabilities (GIVEN): the work-group's waves share 32 classes, a quarter
+// of the width each, and the first adds up their sums in order, where a loss's
+// have 32 classes each: four times the work-groups, and shorter streams (forward
+// calls of 21 f32 rows x 12,291 x 2,056: 52 us against 103; 8 bf16 rows x 8,000
+// x 4,096: 24 against 49; 1 row of 131,072 x 4,096: 200 against 252, 5.4 TB/s).
 template <typename T, int NQ, int PLANES, bool GIVEN, bool VEC>
 __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     constexpr bool GRAD = PLANES > 0;
@@ -1111,7 +1116,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int64_t first = (int64_t)blockIdx.y * (16 * NQ);  // row
     if (!GRAD && !GIVEN && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.done = 0;
-    const int64_t vfirst = a.v0 + ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
+    const int64_t vfirst = a.v0 + (GIVEN ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
     const T* w[2];
     const T* h[NQ];
     bool live[NQ];
@@ -1146,6 +1151,10 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
         return f;
     };
     constexpr int STEP = 4 * E;                       // k of a step: the four lane groups
+    // this wave's k
+    const int64_t share = GIVEN ? (a.width + 4 * STEP - 1) / (4 * STEP) * STEP : a.width;
+    const int64_t kb = GIVEN ? (int64_t)(threadIdx.x >> 6) * share : 0;
+    const int64_t ke = kb + share < a.width ? kb + share : a.width;
     constexpr int U = NQ == 1 ? 4 : NQ == 2 ? 3 : 2;  // steps whose loads are in flight
     auto multiply = [&](int64_t c, int steps, bool whole) {
         Frag x[U][2], y[U][NQ];
@@ -1179,10 +1188,27 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                 }
         }
     };
-    int64_t c = g * E;
-    for (; c - g * E + U * STEP <= a.width; c += U * STEP) multiply(c, U, true);
-    for (; c - g * E + STEP <= a.width; c += STEP) multiply(c, 1, true);
-    if (c - g * E < a.width) multiply(c, 1, false);
+    int64_t c = kb + g * E;
+    for (; c - g * E + U * STEP <= ke; c += U * STEP) multiply(c, U, true);
+    for (; c - g * E + STEP <= ke; c += STEP) multiply(c, 1, true);
+    if (c - g * E < ke) multiply(c, 1, false);
+    if constexpr (GIVEN) {
+        __shared__ float4_t sums[3][2 * NQ][64];
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+                if (wave > 0) sums[wave - 1][i * NQ + j][lane] = acc[i][j];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int x = 0; x < 3; ++x) acc[i][j] += sums[x][i * NQ + j][lane];
+    }
     // class vfirst + 16 i + 4 g + e
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -2082,6 +2108,14 @@ constexpr int64_t kPartBytes = (int64_t)512 << 20;
 constexpr int64_t kLeastPiece = 4096;
 constexpr int64_t kBlockRows = (int64_t)1 << 20;
 constexpr int64_t kFewClasses = 1024;  // up to here G has a second plane
+// Log probabilities' gradients have entries of both signs, whose roundings a
+// few rows, or hidden rows of few columns (nearly parallel rows of W), do not
+// average: one plane of G left 16-bit gradients 1.6 to 3.2 times as far from 64
+// bits as their own rounding at 3 to 300 rows, and 1.6 to 1.9 times at widths of
+// 16 and 32, where it is 1.4 to 1.5 otherwise.  Two planes cost 10 to 40% of the
+// backward there (3 rows x 12,000 x 512: 53 us against 48, 16 x 131,072 x 2,048:
+// 729 against 543), and 60 to 70% of many wide rows, which keep one.
+constexpr int64_t kFewGiven = 1024, kNarrow = 64;
 // Rows up to which head_few_kernel makes the logits.  Forward calls on 32,000 x
 // 2,048, replayed in a graph, against the products (on packed W, where it has
 // to be): f32 1 row 73 against 479 us, 64 rows 110 against 486, 128 (two
@@ -2142,16 +2176,16 @@ int64_t pad(int64_t x) { return x <= 128 ? 128 : up(x, 256); }
 // Pitch of kept logits: rows start 256 bytes apart mod 4 KiB.
 int64_t z_pitch(int64_t classes) { return pad(classes) + 64; }
 
-// part_bytes: of a row's strip, forward; keep_z: the logits are kept for a
-// block of the rows.
-Shape shape_of(const grws_head* h, bool backward, int64_t part_bytes = 8, bool keep_z = false) {
+// given: of log probabilities; keep_z: their logits are kept for a block of the
+// rows.
+Shape shape_of(const grws_head* h, bool backward, bool given = false, bool keep_z = false) {
     Shape s{};
     s.n = h->n;
     s.D = h->width;
     s.V = h->classes;
     s.split = h->dtype == GRWS_F32;
     s.planes = s.split ? 3 : 1;
-    s.gplanes = s.split ? 3 : s.V <= kFewClasses ? 2 : 1;
+    s.gplanes = s.split ? 3 : s.V <= kFewClasses || (given && (s.n <= kFewGiven || s.D < kNarrow)) ? 2 : 1;
     s.pack_w = !weight_in_place(h);
     s.few = s.n <= (s.split ? kFewF32 : s.pack_w ? kFewPacked : kFewRows);
     s.dp = up(s.D, kK);
@@ -2162,7 +2196,7 @@ Shape shape_of(const grws_head* h, bool backward, int64_t part_bytes = 8, bool k
     };
     limit(kPieceBytes, 2 * s.planes * s.dp);                                     // the packed rows
     if (backward) limit(kPieceBytes, 2 * s.gplanes * ((s.vp < kLeastPiece ? s.vp : kLeastPiece) + 128));
-    else limit(kPartBytes, part_bytes * (s.vp / 64));
+    else limit(kPartBytes, (given ? 16 : 8) * (s.vp / 64));
     if (keep_z) limit(kPieceBytes, 4 * z_pitch(s.V));
     limit((int64_t)1 << 31, 64 * ceil_div(h->k, 4) + 1);                         // threads of head_targets_kernel
     rows = rows < 256 ? 256 : rows / 256 * 256;
@@ -2411,11 +2445,11 @@ Gemm gemm_of(const Shape& s, const Plan& pl, const Opnd& P, const Opnd& Q, int64
 template <typename T, int PLANES, bool GIVEN>
 int launch_few(const grws_head* h, const FewArgs& a, hipStream_t stream) {
     const bool vec = rows_of_16(h->weight, h->ld_weight, h->dtype) && rows_of_16(h->hidden, h->ld_hidden, h->dtype);
-    const dim3 grid((unsigned)ceil_div(a.vt, 128), (unsigned)ceil_div(a.n, 64));
-#define GRWS_HEAD_FEW(NQ)                                                                                         \
-    do {                                                                                                          \
-        if (vec) hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, GIVEN, true>), grid, dim3(256), 0, stream, a);        \
-        else hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, GIVEN, false>), grid, dim3(256), 0, stream, a);           \
+    const dim3 grid((unsigned)ceil_div(a.vt, GIVEN ? 32 : 128), (unsigned)ceil_div(a.n, 64));
+#define GRWS_HEAD_FEW(NQ)                                                                                           \
+    do {                                                                                                            \
+        if (vec) hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, GIVEN, true>), grid, dim3(256), 0, stream, a);  \
+        else hipLaunchKernelGGL((head_few_kernel<T, NQ, PLANES, GIVEN, false>), grid, dim3(256), 0, stream, a);     \
     } while (0)
     if (a.n <= 16) GRWS_HEAD_FEW(1);
     else if (a.n <= 32) GRWS_HEAD_FEW(2);
@@ -2799,7 +2833,7 @@ extern "C" int grws_head_bwd(const grws_head* h, const float* lse, const float* 
 namespace grws {
 namespace {
 
-Shape given_shape(const grws_head* h, int32_t top) { return shape_of(h, false, 16, top > 0); }
+Shape given_shape(const grws_head* h, int32_t top) { return shape_of(h, false, true, top > 0); }
 
 int check_given(const grws_head* h, int32_t top) {
     GRWS_TRY(check_head(h, true));
@@ -2911,7 +2945,7 @@ extern "C" size_t grws_head_log_probs_bwd_workspace_bytes(const grws_head* h) {
     if (check_head(h, true) != GRWS_OK || h->n == 0) return 0;
     Sizer z;
     BwdSpace f{};
-    bwd_space(z, shape_of(h, true), h, true, &f);
+    bwd_space(z, shape_of(h, true, true), h, true, &f);
     return z.used;
 }
 
@@ -2927,7 +2961,7 @@ extern "C" int grws_head_log_probs_bwd(const grws_head* h, const float* saved, c
     if (h->n == 0) return backward_none(h, d_weight, ld_dw, d_bias, stream);
     GRWS_CHECK_ARG(saved && logp && entropy, "head: null pointer");
     if (!d_hidden && !d_weight && !d_bias) return GRWS_OK;
-    const Shape s = shape_of(h, true);
+    const Shape s = shape_of(h, true, true);
     Carver cv(workspace, workspace_bytes);
     BwdSpace f{};
     bwd_space(cv, s, h, true, &f);
