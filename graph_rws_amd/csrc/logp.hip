@@ -222,7 +222,7 @@ __device__ __forceinline__ void offer_runs(Pool<MAXK>& p, Runs<T>& runs, int32_t
             x[e] = 0;
             if (at < count) {
                 const int32_t k = (int32_t)(at / run), i = (int32_t)(at - (int64_t)k * run);  // logit i of the run
-                const int32_t cls = first + (chosen[k] / kT) * steps * kChunk + i / kVec * kT * kVec +
+                const int64_t cls = first + (int64_t)(chosen[k] / kT) * steps * kChunk + (int64_t)(i / kVec) * kT * kVec +
                                     chosen[k] % kT * kVec + i % kVec;
                 if (cls < end) x[e] = ((uint64_t)order_of<T>(row[cls]) << class_bits) | (low - (uint32_t)cls);
             }
@@ -365,11 +365,12 @@ constexpr int kWaveClasses = 1024;
 constexpr int kWaveTop = 16;
 
 template <typename T, int PER>
-__global__ __launch_bounds__(kT) void logp_wave_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows,
+__global__ __launch_bounds__(kT) void logp_wave_kernel(const T* __restrict__ logits, int64_t ld, int64_t r0,
+                                                       int64_t rows,
                                                        int32_t classes, int32_t class_bits, int32_t top, Scale sc,
                                                        Given g, Outputs o) {
     const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    const int64_t r = r0 + (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
     if (r >= rows) return;  // uniform over the wave
     const T* row = logits + r * ld;
     const Early early = early_given(row, r, classes, g, lane);
@@ -523,6 +524,12 @@ __global__ __launch_bounds__(kT) void logp_grad_kernel(const T* __restrict__ log
 constexpr int64_t kMostBlocks = 1 << 23;  // of a launch: 2^31 threads
 constexpr int32_t kGradStretch = kChunk;
 
+// Work-groups of the rows left, a wave a row, in one launch.
+unsigned wave_blocks(int64_t rows) {
+    const int64_t n = (rows + kWaves - 1) / kWaves;
+    return (unsigned)(n < kMostBlocks ? n : kMostBlocks);
+}
+
 // Stretches of a row: as many as it takes to fill the chip when there are few
 // rows, of at least 2,048 logits and 4 `top`.
 int32_t stretches(int64_t rows, int64_t classes, int64_t top) {
@@ -561,14 +568,16 @@ int forward(const T* x, int64_t ld, int64_t rows, int32_t classes, int32_t top, 
             const Outputs& o, float4* part, uint64_t* best, hipStream_t stream) {
     const int32_t cb = bits_of(classes);
     if (by_wave(classes, top)) {
-        const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves));
-        if (classes <= 256)
-            hipLaunchKernelGGL((logp_wave_kernel<T, 4>), grid, dim3(kT), 0, stream, x, ld, rows, classes, cb, top, sc,
-                               g, o);
-        else
-            hipLaunchKernelGGL((logp_wave_kernel<T, 16>), grid, dim3(kT), 0, stream, x, ld, rows, classes, cb, top,
-                               sc, g, o);
-        GRWS_LAUNCH_CHECK();
+        for (int64_t r0 = 0; r0 < rows; r0 += kMostBlocks * kWaves) {
+            const dim3 grid(wave_blocks(rows - r0));
+            if (classes <= 256)
+                hipLaunchKernelGGL((logp_wave_kernel<T, 4>), grid, dim3(kT), 0, stream, x, ld, r0, rows, classes, cb,
+                                   top, sc, g, o);
+            else
+                hipLaunchKernelGGL((logp_wave_kernel<T, 16>), grid, dim3(kT), 0, stream, x, ld, r0, rows, classes, cb,
+                                   top, sc, g, o);
+            GRWS_LAUNCH_CHECK();
+        }
         return GRWS_OK;
     }
     const int32_t n = stretches(rows, classes, top);
@@ -606,21 +615,24 @@ template <typename T>
 int backward(const T* x, int64_t ld, int64_t rows, int32_t classes, float c1, float inv_t, const Given& g,
              const Upstream& up, const float2* saved, const float* entropy, T* out, int64_t ldo, hipStream_t stream) {
     if (classes <= kWaveClasses) {
-        const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves));
-        hipLaunchKernelGGL((logp_grad_kernel<T, false, false>), grid, dim3(kT), 0, stream, x, ld, (int64_t)0, rows, classes,
-                           classes, c1, inv_t, g, up, saved, entropy, out, ldo);
-        GRWS_LAUNCH_CHECK();
+        for (int64_t r0 = 0; r0 < rows; r0 += kMostBlocks * kWaves) {
+            hipLaunchKernelGGL((logp_grad_kernel<T, false, false>), dim3(wave_blocks(rows - r0)), dim3(kT), 0, stream,
+                               x, ld, r0, rows, classes, classes, c1, inv_t, g, up, saved, entropy, out, ldo);
+            GRWS_LAUNCH_CHECK();
+        }
         return GRWS_OK;
     }
-    // (at most 2^18 stretches of a row, so 2^13 rows or more of 2^31 threads)
-    const int64_t n = ((int64_t)classes + kGradStretch - 1) / kGradStretch;
+    // (at most 2^15 stretches of a row: a grid's second dimension ends at 2^16)
+    const int64_t pieces = ((int64_t)classes + kGradStretch - 1) / kGradStretch;
+    const int32_t stretch = kGradStretch * (int32_t)((pieces + 32767) / 32768);
+    const int64_t n = ((int64_t)classes + stretch - 1) / stretch;
     const int64_t most = kMostBlocks / n < 1 ? 1 : kMostBlocks / n;
     const bool once = streams(rows * classes * (int64_t)sizeof(T));
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
         const dim3 grid((unsigned)(rows - r0 < most ? rows - r0 : most), (unsigned)n);
 #define GRWS_LOGP_GRAD(ONCE)                                                                                         \
     hipLaunchKernelGGL((logp_grad_kernel<T, true, ONCE>), grid, dim3(kT), 0, stream, x, ld, r0, rows, classes,       \
-                       kGradStretch, c1, inv_t, g, up, saved, entropy, out, ldo)
+                       stretch, c1, inv_t, g, up, saved, entropy, out, ldo)
         if (once) GRWS_LOGP_GRAD(true);
         else GRWS_LOGP_GRAD(false);
 #undef GRWS_LOGP_GRAD

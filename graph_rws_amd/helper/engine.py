@@ -16,8 +16,9 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     dense F32 / F16 / BF16 tensors of one GPU, each listed once."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
-    if not grads or any(g.layout != torch.strided or not g.is_cuda or g.device != grads[0].device
-                        or g.dtype not in _CLIPPED for g in grads) or len({id(g) for g in grads}) != len(grads):
+    if (not grads or len({id(g) for g in grads}) != len(grads)
+            or any(type(g) is not torch.Tensor or g.layout != torch.strided or not g.is_cuda
+                   or g.device != grads[0].device or g.dtype not in _CLIPPED for g in grads)):
         return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
     from ..core import clip_grads
     return clip_grads(grads, max_norm)

@@ -281,6 +281,37 @@ def test_strides_and_alignment(cuda_device, dt, V):
         ref.check_grad(grad, a[:n], b[:n])
 
 
+def test_more_rows_than_a_launch_takes(cuda_device):
+    """A wave a row: 2^25 rows a launch."""
+    n, last = (1 << 25) + 5, 1000
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(1)
+    z = torch.randn(n, 3, generator=g, device=cuda_device, dtype=torch.float16).requires_grad_()
+    index = torch.randint(0, 3, (n,), generator=g, device=cuda_device, dtype=torch.int32)
+    got = log_probs(z, index, top=1)
+    a = torch.ones(n, device=cuda_device)
+    grad, = torch.autograd.grad(got.logp, z, a)
+    tail = z.detach()[-last:].clone().requires_grad_()
+    ref = log_probs(tail, index[-last:], top=1)
+    assert torch.equal(got.logp[-last:], ref.logp) and torch.equal(got.entropy[-last:], ref.entropy)
+    assert torch.equal(got.top_index[-last:], ref.top_index) and torch.equal(got.top_logp[-last:], ref.top_logp)
+    assert torch.equal(grad[-last:], torch.autograd.grad(ref.logp, tail, a[-last:])[0])
+
+
+def test_not_finite_alternatives(cuda_device):
+    """NaN first, as a sort has it; +inf before what is finite."""
+    for V in (300, 20000):
+        z, index, _, _ = _inputs(cuda_device, 3, V, torch.bfloat16, 1, V)
+        z[0, [7, 200, 250]] = math.nan
+        z[1, [9, 100]] = math.inf
+        z[2, ::2] = math.nan
+        order = torch.argsort(z.float(), dim=1, descending=True, stable=True)
+        for top in (2, 8, 20, 200):
+            got = log_probs(z, index, top=top)
+            assert torch.equal(got.top_index[:2].long(), order[:2, :top])
+            assert bool(got.top_index[2].remainder(2).eq(0).all()) or top > V // 2
+
+
 def test_no_rows(cuda_device):
     z = torch.zeros(0, 30, device=cuda_device, requires_grad=True)
     got = log_probs(z, torch.zeros(0, dtype=torch.int64, device=cuda_device), top=4)
