@@ -34,6 +34,14 @@
 // and, for 16,384 rows of width 256, 11% of a call at 172 classes and 25% at
 // 1,024; at 2,048 it would be 40%, which is where it stops.
 //
+// Log probabilities of given classes and entropies (GIVEN) are the same products:
+//   logp_i,j = (z_i,cj - m) / T - ln s       H_i = ln s - ln2 t / s  (logp.h)
+//   dz_iv = (sum_j a_ij [v = c_ij] - p_iv (A_i + b_i (ln p_iv + H_i))) / T
+// The forward's epilogue sums 2^u u beside 2^u, the gradient's multiplies p by
+// the bracket, a fused multiply-add of u.  Alternatives need the logits
+// themselves: those of a block of rows are stored, and only strips whose maximum
+// reaches a bound are read again.
+//
 // F32 operands: x = a + b + c with three bf16 (the top, middle and low 8 of
 // 24 significant bits, truncated, so the split is exact and never
 // overflows), and the product is the sum of the six plane products
@@ -1870,7 +1878,9 @@ __global__ __launch_bounds__(512) void head_given_join_kernel(Targets t, Strips 
 // `top` largest logits: only strips that reach it are read, and of those what
 // does.  The bound is the `top`-th largest of the threads' largest maxima, or
 // nothing where `top` is more than half of the threads (then it rises as the
-// logits go by).
+// logits go by).  1 row of 1,000 strips: 7.0 us (a pool of all strips 10.8);
+// 4,099 rows of 391: 38 us beside 600 for the product that stores their logits
+// (464 without the stores, 647 with stores that pass through the caches).
 constexpr int kListed = 2048;  // strips that are looked at, at a time
 
 template <int MAXK>

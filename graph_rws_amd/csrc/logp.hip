@@ -1,20 +1,21 @@
 // Log probabilities of given classes, entropy and top alternatives of rows of
 // logits in memory, and their gradient (gfx950).
 //
-//   y_v = z_v log2(e) / T     m the largest z, u_v = (z_v - m) log2(e) / T
-//   s = sum 2^u, t = sum 2^u u       log2 p_v = u_v - log2 s
-//   logp_j = ln2 log2 p_cj           H = ln2 (log2 s - t / s)
+//   m the largest z, u_v = (z_v - m) log2(e) / T, s = sum 2^u, t = sum 2^u u
+//   ln p_v = (z_v - m) / T - ln s        logp_j = ln p_cj
+//   H = ln s - ln2 t / s
 //   dz_v = (sum_j a_j [v = c_j] - p_v (A + b (ln p_v + H))) / T
 // with a_j the upstream gradient of logp_j, b that of H, A the sum of a_j.
-// t <= 0 and s >= 1, so H adds two terms of one sign and nothing cancels.  The
-// largest logit is taken off before the factor: masks of the type's lowest
-// value leave zero and do not overflow.
+// t <= 0 and s >= 1, so H adds two terms of one sign and nothing cancels.
 //
 // Forward: one pass.  Every thread keeps its own (m, s, t) and moves them to a
-// new m when a step of 32 logits has a larger one (rare after the first
-// steps); the work-group joins them at the end, in a fixed order.  Top logits
-// come from the same registers (top_pool.h).  Few rows are cut into stretches
-// and joined, short ones take a wave each.
+// new m when some of its logits are larger (rare after the first steps); the
+// work-group joins them at the end, in a fixed order.  Few rows are cut into
+// stretches and joined, short ones take a wave each.  Bound by HBM: 8,192 x
+// 50,048 bf16 124 us, 6.6 TB/s (a bare read 7.1); an element takes 9 of the
+// vector unit's slots, 4 of them for the exponential, 90 us in all.
+// Backward: the logits are read again and the gradient written, 8,192 x 50,048
+// bf16 320 us, 5.1 TB/s (a copy 5.0).
 #include "logp.h"
 #include "top_pool.h"
 
@@ -174,7 +175,7 @@ struct Running {
 // logit of each of its runs of steps, at least `top` threads' largest
 // reach a first bound, and only runs that reach it are looked at again.  So the
 // pass over the row has no barrier and no candidates (8,192 x 50,021 bf16 with
-// 16 alternatives: 470 us with a pool that every step offers to).
+// 16 alternatives: 151 us, 470 with a pool that every step offers to).
 template <typename T>
 struct Runs {
     typedef std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> Order;
@@ -466,10 +467,12 @@ __device__ __forceinline__ void store_vec(void* p, const V& v) {
     }
 }
 
-// Elements at a time of a row's stretch; ROWS rows a work-group (a wave each)
-// or one.  Given classes are put in place after the rest: each wave's stores
-// have left before its own threads (ONE: the work-group's, behind a barrier)
-// write the same places again.
+// 16 bytes a thread at a time of a stretch of one row (ONE), or of four rows, a
+// wave each (1,024 rows of 172: 5 us).  Given classes are put in place after the
+// rest: the wave's stores (ONE: the work-group's, behind a barrier) have left
+// before the same places are written again.  (Rows that begin inside 16 bytes
+// are read and written as they lie: beginning at a whole 16 took 362 us against
+// 351 for 4,099 x 100,003 bf16.)
 template <typename T, bool ONE, bool ONCE>
 __global__ __launch_bounds__(kT) void logp_grad_kernel(const T* __restrict__ logits, int64_t ld, int64_t r0,
                                                        int64_t rows, int32_t classes, int32_t stretch, float c1,

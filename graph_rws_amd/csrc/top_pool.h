@@ -27,7 +27,7 @@ constexpr int kSmallK = 128;
 // 225 us for 64 of 8,192 x 50,021 bf16.
 template <int MAXK>
 struct Sizes {
-    static constexpr int CAP = MAXK <= kSmallK ? 1024 : 3072;
+    static constexpr int CAP = MAXK <= kSmallK ? 1024 : 3 * 1024;
     static constexpr int OFFER = MAXK <= kSmallK ? 2 : 8;
     static constexpr int PER = CAP / kT;
     static_assert(MAXK + kT * OFFER <= CAP, "an offer has to fit");

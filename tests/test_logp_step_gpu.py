@@ -1,0 +1,113 @@
+"""The end of a training step by rewards, as it is used: log probabilities of
+sampled classes and entropies of a graph model's rows, their gradients, the
+gradients' global norm and clipping, the update; against torch's ops on kept
+logits, and captured and replayed.
+
+The fused step's f32 sums differ from torch's by their order and the split
+f32 products: gradients agree to 1e-4 of their largest magnitude, losses to
+1e-5 (the bounds of the fused losses' step tests)."""
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from graph_rws_amd import synth
+from graph_rws_amd.data import BCSRGraph
+from graph_rws_amd.helper import clip_grad_norm_
+from graph_rws_amd.layers import LinearHead, linear_log_probs, log_probs
+from graph_rws_amd.models import GCN_BCSR
+
+pytestmark = pytest.mark.gpu
+
+
+def _problem(dev, nodes=1500, width=40, hidden=48, classes=777):
+    torch.manual_seed(7)
+    g = synth.chung_lu(nodes, 6 * nodes, 2.3, seed=4)
+    graph = BCSRGraph.from_csr(g.row_ptr, g.col_idx, g.values, nodes, nodes, tile_cols=16, device=dev)
+    features = torch.randn(nodes, width, device=dev)
+    idx = (torch.rand(nodes, device=dev) < 0.6).nonzero()[:, 0]
+    model = GCN_BCSR(width, hidden, hidden, 2, dropout=0.0, use_checkpoint=False).to(dev)
+    head = LinearHead(hidden, classes).to(dev)
+    return graph, features, idx, model, head
+
+
+def _reinforce(logp, entropy, reward):
+    return -(reward * logp).mean() - 0.01 * entropy.mean()
+
+
+def test_step_of_rewards_matches_torch_ops(cuda_device):
+    graph, features, idx, model, head = _problem(cuda_device)
+    twin, twin_head = copy.deepcopy(model), copy.deepcopy(head)
+    graphs = model._ensure_graph_list(graph)
+    with torch.no_grad():  # the answers, from the alternatives
+        seen = head.log_probs(model(graphs, features), torch.zeros_like(idx), rows=idx, top=8)
+        pick = torch.multinomial(seen.top_logp.exp(), 1)
+        answers = seen.top_index.gather(1, pick).long()[:, 0]
+        kept = log_probs(head(model(graphs, features)[idx]), answers, top=8)
+    assert float((kept.top_logp - seen.top_logp).abs().max()) < 1e-4
+    again = head.log_probs(model(graphs, features), answers, rows=idx)
+    assert float((again.logp - seen.top_logp.gather(1, pick)[:, 0]).abs().max()) < 1e-5
+    reward = torch.randn(idx.numel(), device=cuda_device)
+    params = [*model.parameters(), *head.parameters()]
+    loss = _reinforce(again.logp, again.entropy, reward)
+    loss.backward()
+    norm = clip_grad_norm_(params, 0.05)
+    twins = [*twin.parameters(), *twin_head.parameters()]
+    logp = torch.log_softmax(twin_head(twin(twin._ensure_graph_list(graph), features)[idx]), 1)
+    want = _reinforce(logp.gather(1, answers[:, None])[:, 0], -(logp.exp() * logp).sum(1), reward)
+    want.backward()
+    twin_norm = torch.nn.utils.clip_grad_norm_(twins, 0.05)
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * max(1.0, abs(float(want.detach())))
+    assert abs(float(norm) - float(twin_norm)) <= 1e-4 * float(twin_norm) and float(norm) > 0.05
+    for p, q in zip(params, twins):
+        assert float((p.grad - q.grad).abs().max()) <= 1e-4 * float(q.grad.abs().max()) + 1e-9
+    before = [p.detach().clone() for p in params]
+    torch.optim.SGD(params, lr=0.5).step()
+    assert all(torch.allclose(p.detach(), b - 0.5 * p.grad) for p, b in zip(params, before))
+
+
+def test_captured_steps(cuda_device):
+    """Two captured steps of one head's copies, replayed in turn with eager
+    ones between; every replay leaves the eager step's weights, bit for bit."""
+    dev = cuda_device
+    torch.manual_seed(3)
+    rows, width, classes = 300, 64, 2000
+    start = LinearHead(width, classes).to(dev)
+    x, index = torch.randn(rows, width, device=dev), torch.randint(0, classes, (rows,), device=dev)
+    reward = torch.randn(rows, device=dev)
+
+    def step(head):
+        got = linear_log_probs(x, head.weight, index, head.bias, temperature=1.1)
+        loss = _reinforce(got.logp, got.entropy, reward)
+        grads = torch.autograd.grad(loss, [head.weight, head.bias])
+        from graph_rws_amd.core import clip_grads
+        norm = clip_grads(grads, 0.01)
+        with torch.no_grad():
+            for p, g in zip((head.weight, head.bias), grads):
+                p.sub_(g, alpha=0.1)
+        return loss.detach(), norm
+
+    warm = copy.deepcopy(start)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        step(warm)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    heads = [copy.deepcopy(start), copy.deepcopy(start)]
+    graphs = []
+    for h in heads:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(h)
+        graphs.append((g, out))
+    eager = copy.deepcopy(start)
+    for turn in range(4):
+        x.copy_(torch.randn(rows, width, device=dev))
+        index.copy_(torch.randint(0, classes, (rows,), device=dev))
+        want = step(eager)
+        for h, (g, out) in zip(heads, graphs):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+            assert torch.equal(h.weight, eager.weight) and torch.equal(h.bias, eager.bias)
