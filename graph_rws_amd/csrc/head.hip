@@ -2000,7 +2000,7 @@ __global__ __launch_bounds__(256) void head_given_rows_kernel(Targets t, RowStat
         const bool live = st.x != INFINITY;
         auto entry = [&](int j, int64_t* cls) {
             *cls = live && dlogp && j < k ? given_at(t, i, j) : -1;
-            if (*cls >= t.classes) *cls = -1;
+            if (*cls < 0 || *cls >= t.classes) *cls = -1;  // (places are compared in 32 bits)
             return *cls >= 0 ? dlogp[i * k + j] : 0.f;
         };
         float sum = 0.f, mag = 0.f;
@@ -2298,7 +2298,8 @@ int check_head(const grws_head* h, bool given = false) {
                        h->ld_weight <= (1 << 21),
                    "head: leading dimensions must be the width at least and 2^21 at most");
     GRWS_CHECK_ARG(h->k >= 0 && h->k <= 1024, "head: at most 1024 teacher entries a row");
-    GRWS_CHECK_ARG(h->temperature > 0.f && h->temperature < INFINITY && kLog2e / h->temperature < INFINITY,
+    GRWS_CHECK_ARG(h->temperature > 0.f && h->temperature < INFINITY &&
+                       (!given || kLog2e / h->temperature < INFINITY),
                    "head: the temperature must be positive");
     if (h->n > 0) {
         GRWS_CHECK_ARG(h->hidden && h->weight, "head: null pointer");

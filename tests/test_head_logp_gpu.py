@@ -229,6 +229,7 @@ def test_bad_rows_and_classes(cuda_device):
             rows[1], rows[2], rows[3] = -1, 2 * n, 2 ** 40
             index[0] = torch.tensor([V, 1, -1])
             index[5] = torch.tensor([2 ** 30, -2 ** 40, 2])
+            index[4] = torch.tensor([-2 ** 40, 0, 2 ** 40])  # in 32 bits: three times class 0
             h[0] = math.nan  # a row that is not asked for
             rows[rows == 0] = 2 * n - 1 if not bool((rows == 2 * n - 1).any()) else rows[4]
             live = torch.ones(n, dtype=torch.bool, device=cuda_device)
