@@ -315,8 +315,9 @@ extern "C" int grws_clip_grads(const void* const* grads, const int32_t* dtypes, 
     if (!cv.ok) return set_error(GRWS_E_CAPACITY, "clip: workspace too small (%zu < %zu)", workspace_bytes, cv.used);
     int parts = 0;
     GRWS_TRY(for_launches(grads, dtypes, sizes, outs, out_dtypes, count, [&](const Tensors& a, unsigned blocks) -> int {
-        if (bytes > kCached) hipLaunchKernelGGL(clip_squares_kernel<true>, dim3(blocks), dim3(kT), 0, stream, a, part + parts);
-        else hipLaunchKernelGGL(clip_squares_kernel<false>, dim3(blocks), dim3(kT), 0, stream, a, part + parts);
+        double* to = part + parts;
+        if (bytes > kCached) hipLaunchKernelGGL(clip_squares_kernel<true>, dim3(blocks), dim3(kT), 0, stream, a, to);
+        else hipLaunchKernelGGL(clip_squares_kernel<false>, dim3(blocks), dim3(kT), 0, stream, a, to);
         GRWS_LAUNCH_CHECK();
         parts += (int)blocks;
         return GRWS_OK;

@@ -47,6 +47,15 @@ __device__ __forceinline__ void add(Stats& a, float z, float m, float c1) {
     a.t = fmaf(e, reach(u), a.t);
 }
 
+// Roundings leave no log probability above zero and no entropy below it (a NaN
+// stays).
+__device__ __forceinline__ float at_most_zero(float x) { return x > 0.f ? 0.f : x; }
+
+__device__ __forceinline__ float entropy_of(const Stats& a) {
+    const float h = kLn2 * (log2f(a.s) - a.t / a.s);
+    return h < 0.f ? 0.f : h;
+}
+
 // The exponentials are 2^(z c - ref), ref the rounded m c, of a largest logit m.
 // c is c1, but a half where m c1 overflows (m a mask of the type's lowest
 // value): floats of that size lie so far apart that any c leaves zero of a z

@@ -36,7 +36,7 @@ struct Given {
 struct Outputs {
     float* logp;      // [rows k]
     float* entropy;   // [rows]
-    float2* saved;    // [rows]: m, log2 s; or NULL
+    float2* saved;    // [rows]: m, s; or NULL
     float* top_logp;  // [rows top]
     int32_t* top_index;
 };
@@ -50,7 +50,7 @@ struct Scale {
 // type's lowest value stays finite).
 struct Row {
     float m, l2, inv_t;  // largest logit, log2 s
-    __device__ __forceinline__ float logp(float z) const { return fmaf(z - m, inv_t, -kLn2 * l2); }
+    __device__ __forceinline__ float logp(float z) const { return at_most_zero(fmaf(z - m, inv_t, -kLn2 * l2)); }
 };
 
 __device__ __forceinline__ Row row_of(const Stats& a, const Scale& sc) {
@@ -85,8 +85,8 @@ __device__ __forceinline__ void put_row(const Stats& a, const Scale& sc, const T
         o.logp[r * g.k + j] = v;
     }
     if (sub != 0) return;
-    o.entropy[r] = kLn2 * (q.l2 - a.t / a.s);
-    if (o.saved) o.saved[r] = make_float2(q.m, q.l2);
+    o.entropy[r] = q.l2 != q.l2 ? q.l2 : entropy_of(a);
+    if (o.saved) o.saved[r] = make_float2(q.m, a.s);
 }
 
 // The pool's alternatives; a key holds its logit.
@@ -223,8 +223,8 @@ __device__ __forceinline__ void offer_runs(Pool<MAXK>& p, Runs<T>& runs, int32_t
             x[e] = 0;
             if (at < count) {
                 const int32_t k = (int32_t)(at / run), i = (int32_t)(at - (int64_t)k * run);  // logit i of the run
-                const int64_t cls = first + (int64_t)(chosen[k] / kT) * steps * kChunk + (int64_t)(i / kVec) * kT * kVec +
-                                    chosen[k] % kT * kVec + i % kVec;
+                const int64_t step = (int64_t)(chosen[k] / kT) * steps * kChunk + (int64_t)(i / kVec) * kT * kVec;
+                const int64_t cls = first + step + chosen[k] % kT * kVec + i % kVec;
                 if (cls < end) x[e] = ((uint64_t)order_of<T>(row[cls]) << class_bits) | (low - (uint32_t)cls);
             }
         }
@@ -447,11 +447,11 @@ __device__ __forceinline__ float given_sum(const Given& g, const Upstream& up, i
 // dz of a logit that is not given: -p (A + b (ln p + H)) / T.  A row of
 // nothing but -inf has no p: zeros, so that it can be left out of a loss.
 struct Slope {
-    float m, l2, c1, k, b2, inv_t;  // k = (A + b H), b2 = b ln2
+    float m, c1, f, k, b2;  // f = -1 / (s T), k = A + b (H - ln s), b2 = b ln2
     __device__ __forceinline__ float of(float z) const {
         if (m == -INFINITY) return 0.f;  // uniform
-        const float u = fmaf(z - m, c1, -l2);
-        return -__builtin_amdgcn_exp2f(u) * fmaf(b2, reach(u), k) * inv_t;
+        const float u = (z - m) * c1;
+        return __builtin_amdgcn_exp2f(u) * f * fmaf(b2, reach(u), k);
     }
 };
 
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(kT) void logp_grad_kernel(const T* __restrict__ log
     const float2 s = saved[r];
     const float b = up.dentropy ? up.dentropy[r] : 0.f;
     const float A = given_sum(g, up, r, classes, threadIdx.x & 63);
-    const Slope f{s.x, s.y, c1, up.dentropy ? fmaf(b, entropy[r], A) : A, b * kLn2, inv_t};
+    const Slope f{s.x, c1, -inv_t / s.y, up.dentropy ? fmaf(b, entropy[r] - kLn2 * log2f(s.y), A) : A, b * kLn2};
     constexpr int E = 16 / sizeof(T);  // a lane's 16 bytes lie next to its neighbour's
     struct Vec {
         T x[E];

@@ -294,6 +294,29 @@ def test_upstream_not_finite_stays_in_its_row(cuda_device):
         ref.check_grads(fine, *clean)
 
 
+@pytest.mark.parametrize("n", [64, 200])
+def test_given_entries_take_the_product_s_probabilities(cuda_device, n):
+    """The logits' gradient of a log probability sums to nothing over the
+    classes, whatever the logits' own rounding, if the probability taken off at
+    a given class is the one that the others have.  A column of ones in weight
+    makes that sum a column of d_hidden.  Its terms have 5 roundings of 2^-23 of
+    a row's sum |a| or fewer (exponential, factor, bracket, product, sum), of
+    either sign: their mean square over the rows is below 5 of them."""
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(8)
+    D, V = 16384, 58
+    w = torch.randn(V, D, generator=g, device=cuda_device) / math.sqrt(D)
+    best = torch.randint(0, V, (n,), generator=g, device=cuda_device)
+    h = torch.randn(n, D, generator=g, device=cuda_device) + 12.0 * w[best]
+    w[:, 0] = 1.0
+    index = torch.stack([best, (best + 3) % V, (best + 3) % V], 1)
+    a = torch.randn(n, 3, generator=g, device=cuda_device)
+    h.requires_grad_()
+    dh, = torch.autograd.grad(linear_log_probs(h, w, index).logp, h, a)
+    off = dh[:, 0].double() / a.double().abs().sum(1)
+    assert float(off.square().mean().sqrt()) < 5 * 2.0 ** -23
+
+
 def test_one_upstream_alone_and_scales(cuda_device):
     for dt in DTYPES:
         h, w, b, rows, index, up = _inputs(cuda_device, 150, 64, 2000, dt, 2, 10, bias=True)
