@@ -2211,5 +2211,6 @@ def clip_grads(grads, max_norm: float, out=None, scale: Optional[torch.Tensor] =
                 raise ValueError("clip_grads: out must be contiguous or have its gradient's strides")
         flat = [g if o.stride() == g.stride() and _one_run(g) else g.contiguous() for o, g in zip(out, grads)]
         norm = _clip_call("clip_grads", flat, out, max_norm, scale)
-    torch.autograd.graph.increment_version(grads if out is None else out)
+    # (tensors made in inference mode have no version)
+    torch.autograd.graph.increment_version([t for t in (grads if out is None else out) if not t.is_inference()])
     return norm

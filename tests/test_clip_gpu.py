@@ -169,6 +169,17 @@ def test_same_bits_and_versions(cuda_device):
         grad_norm([torch.zeros(3, device=cuda_device, dtype=torch.float64)])
 
 
+def test_inference_mode(cuda_device):
+    with torch.inference_mode():
+        grads = _make(cuda_device, [1000, 7], [torch.float32, torch.bfloat16], 9)
+        keep = [g.clone() for g in grads]
+        out = [torch.empty(g.shape, device=cuda_device) for g in grads]
+        _check_norm(clip_grads(grads, 1.0, out=out), _norm(keep), 1007)
+        _check_clipped(out, keep, 1.0)
+        clip_grads(grads, 1.0)
+        _check_clipped(grads, keep, 1.0)
+
+
 def test_other_stream_and_graph(cuda_device):
     """A call on a stream of its own, and two captured ones replayed in turn
     with eager calls between."""

@@ -67,6 +67,33 @@ def test_step_of_rewards_matches_torch_ops(cuda_device):
     assert all(torch.allclose(p.detach(), b - 0.5 * p.grad) for p, b in zip(params, before))
 
 
+def test_inference_mode_and_upstream_layouts(cuda_device):
+    """Scoring in inference mode; upstream gradients that are expanded or lie
+    in columns."""
+    dev = cuda_device
+    torch.manual_seed(4)
+    head = LinearHead(64, 900).to(dev)
+    x, index = torch.randn(50, 64, device=dev), torch.randint(0, 900, (50, 3), device=dev)
+    plain = head.log_probs(x, index, top=4)
+    with torch.inference_mode():
+        seen = head.log_probs(x, index, top=4)
+        kept = log_probs(head(x), index, top=4)
+    assert all(torch.equal(a, b) for a, b in zip(plain, seen))
+    assert float((kept.logp - seen.logp).abs().max()) < 1e-4
+    up = torch.randn(3, 50, device=dev)
+    wide = x[:1].expand(50, 64).requires_grad_()  # one row for all
+    for f in (lambda t: linear_log_probs(t, head.weight, index, head.bias), lambda t: log_probs(head(t), index)):
+        got = f(wide)
+        a = torch.autograd.grad(got.logp, wide, up.t(), retain_graph=True)[0]
+        b = torch.autograd.grad(got.logp, wide, up.t().contiguous(), retain_graph=True)[0]
+        assert torch.equal(a, b)
+        c = torch.autograd.grad([got.logp.sum(), got.entropy.sum()], wide)[0]
+        assert c.shape == (50, 64) and bool(c.isfinite().all())
+        single = x[:1].clone().requires_grad_()
+        total = torch.autograd.grad(f(single.expand(50, 64)).logp, single, up.t())[0]
+        assert float((total - a.sum(0)).abs().max()) <= 2.0 ** -18 * float(a.abs().sum(0).max())
+
+
 def test_captured_steps(cuda_device):
     """Two captured steps of one head's copies, replayed in turn with eager
     ones between; every replay leaves the eager step's weights, bit for bit."""
