@@ -52,7 +52,8 @@ class _LogProbs(Function):
         need = ctx.needs_input_grad[0]
         logp, entropy, saved, top_logp, top_index = _ops.log_probs_fwd(x, index, temperature, top, need)
         if need:
-            ctx.save_for_backward(x, index, saved, entropy)
+            # the argument and not a copy of it, which has no history of its own
+            ctx.save_for_backward(logits, index, saved, entropy)
             ctx.temperature = temperature
         if top:
             ctx.mark_non_differentiable(top_logp, top_index)
@@ -62,10 +63,11 @@ class _LogProbs(Function):
     def backward(ctx, dlogp, dentropy, _dtop, _dindex):
         if dlogp is None and dentropy is None:
             return None, None, None, None
-        x, index, saved, entropy = ctx.saved_tensors
-        grad = _ops.log_probs_bwd(x, index, ctx.temperature, saved, entropy, dlogp, dentropy)
+        logits, index, saved, entropy = ctx.saved_tensors
+        grad = _ops.log_probs_bwd(_ops._unit_columns(logits.detach()), index, ctx.temperature, saved, entropy, dlogp,
+                                  dentropy)
         if torch.is_grad_enabled():  # create_graph=True
-            owners = [x] + [d for d in (dlogp, dentropy) if d is not None]
+            owners = [logits] + [d for d in (dlogp, dentropy) if d is not None]
             grad, = _Once.apply(len(owners), *owners, grad)
         return grad, None, None, None
 

@@ -355,3 +355,15 @@ def test_same_bits_streams_and_graphs(cuda_device):
             eager = step(new.requires_grad_())
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(out, eager))
+
+
+def test_second_derivative_is_refused_whatever_the_strides(cuda_device):
+    """Also beside a term of the loss that has one, and of logits that are
+    copied for the kernels."""
+    index = torch.tensor([0, 2, 4, 1], device=cuda_device)
+    for shape, view in (((4, 5), lambda t: t), ((5, 4), lambda t: t.t()), ((4, 10), lambda t: t[:, ::2]),
+                        ((1, 5), lambda t: t.expand(4, 5))):
+        leaf = torch.randn(shape, device=cuda_device).requires_grad_()
+        g, = torch.autograd.grad(log_probs(view(leaf), index).logp.sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (leaf.square().sum() + g.square().sum()).backward()

@@ -130,3 +130,36 @@ def test_linear_python_refusals():
     h, w, i = torch.zeros(3, 5), torch.zeros(7, 5), torch.zeros(3, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="CUDA"):
         linear_log_probs(h, w, i)
+
+
+def test_second_derivative_is_refused_whatever_the_strides(monkeypatch):
+    """Logits whose columns are not next to each other, or whose rows are one,
+    are copied for the kernels: a second derivative through them is an error as
+    it is through others, beside a term of the loss that has a gradient."""
+    from graph_rws_amd.core import ops
+    from graph_rws_amd.layers import logp as module
+
+    def fwd(x, index, temperature, top, save):
+        assert x.stride(1) == 1 and index.is_contiguous()
+        lp = torch.log_softmax(x / temperature, 1)
+        return lp.gather(1, index[:, None])[:, 0], -(lp.exp() * lp).sum(1), lp[:, :2].contiguous(), None, None
+
+    def bwd(x, index, temperature, saved, entropy, dlogp, dentropy):
+        assert x.stride(1) == 1
+        g = -torch.softmax(x / temperature, 1) * dlogp[:, None]
+        return g.scatter_add(1, index[:, None], dlogp[:, None]) / temperature
+
+    monkeypatch.setattr(ops, "check_log_probs", lambda *a: None)
+    monkeypatch.setattr(ops, "log_probs_fwd", fwd)
+    monkeypatch.setattr(ops, "log_probs_bwd", bwd)
+    index = torch.tensor([0, 2, 4, 1])
+    for shape, view in (((4, 5), lambda t: t), ((5, 4), lambda t: t.t()), ((4, 10), lambda t: t[:, ::2]),
+                        ((1, 5), lambda t: t.expand(4, 5)), ((8,), lambda t: t.as_strided((4, 5), (1, 1)))):
+        leaf = torch.randn(shape, requires_grad=True)
+        first, = torch.autograd.grad(module.log_probs(view(leaf), index).logp.sum(), leaf)
+        twin = leaf.detach().clone().requires_grad_()
+        want, = torch.autograd.grad(torch.log_softmax(view(twin), 1).gather(1, index[:, None]).sum(), twin)
+        assert torch.allclose(first, want, atol=1e-6)
+        g, = torch.autograd.grad(module.log_probs(view(leaf), index).logp.sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (leaf.square().sum() + g.square().sum()).backward()
