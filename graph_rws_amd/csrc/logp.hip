@@ -445,11 +445,12 @@ __device__ __forceinline__ float given_sum(const Given& g, const Upstream& up, i
 }
 
 // dz of a logit that is not given: -p (A + b (ln p + H)) / T.  A row of
-// nothing but -inf has no p: zeros, so that it can be left out of a loss.
+// nothing but -inf (s of 0) has no p: zeros, so that it can be left out of a
+// loss.  NaN beside them, which m does not show, is in s and f: NaN everywhere.
 struct Slope {
     float m, c1, f, k, b2;  // f = -1 / (s T), k = A + b (H - ln s), b2 = b ln2
     __device__ __forceinline__ float of(float z) const {
-        if (m == -INFINITY) return 0.f;  // uniform
+        if (m == -INFINITY) return f == f ? 0.f : f;  // uniform
         const float u = (z - m) * c1;
         return __builtin_amdgcn_exp2f(u) * f * fmaf(b2, reach(u), k);
     }

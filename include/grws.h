@@ -932,7 +932,8 @@ int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, int64_t rows,
 /* no probability; a row of nothing but -inf, or with NaN or +inf, is NaN.  */
 /* Backward of dlogp [rows x k] and dentropy [rows] (NULL: zeros): grad     */
 /* [rows x ldg] in dtype, every element written; a class given twice gets   */
-/* both; zeros in a row of nothing but -inf.  Same inputs, same bits.       */
+/* both; zeros in a row of nothing but -inf, NaN in one with NaN or +inf.   */
+/* Same inputs, same bits.                                                  */
 /* ------------------------------------------------------------------------ */
 size_t grws_log_probs_workspace_bytes(int64_t rows, int64_t classes, int32_t top);
 int grws_log_probs_fwd(const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t classes,

@@ -367,3 +367,27 @@ def test_second_derivative_is_refused_whatever_the_strides(cuda_device):
         g, = torch.autograd.grad(log_probs(view(leaf), index).logp.sum(), leaf, create_graph=True)
         with pytest.raises(RuntimeError, match="second derivative"):
             (leaf.square().sum() + g.square().sum()).backward()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("V", [40, 700, 5000, 140001])
+def test_rows_without_a_number(cuda_device, dt, V):
+    """Rows of NaN alone, or of NaN and -inf, have NaN for a gradient in every
+    place, where one of nothing but -inf has zeros."""
+    for n in (6, 1030) if V < 10000 else (6,):
+        z, index, a, b = _inputs(cuda_device, n, V, dt, 2, V + n)
+        z[1] = math.nan
+        z[2], z[2, V // 2] = -math.inf, math.nan
+        z[3] = -math.inf
+        z[4, V - 1] = math.nan
+        z.requires_grad_()
+        got = log_probs(z, index, top=3)
+        assert bool(got.logp[1:5].isnan().all()) and bool(got.entropy[1:5].isnan().all())
+        for up in ((a, b), (a, None), (None, b)):
+            given = [(o, u) for o, u in zip((got.logp, got.entropy), up) if u is not None]
+            grad, = torch.autograd.grad([o for o, _ in given], [z], [u for _, u in given], retain_graph=True)
+            assert bool(grad[[1, 2, 4]].isnan().all())
+            assert bool((grad[3] == 0).all())
+            rest = [0, *range(5, n)]
+            ref = _Ref(z.detach()[rest], index[rest])
+            ref.check_grad(grad[rest], *(u[rest] if u is not None else None for u in up))
