@@ -1805,11 +1805,13 @@ struct GivenOut {
 
 // A row's statistics to lse, factor and entropy, by one thread.  Entropies of
 // rows without a place in hidden, of nothing but -inf (neither counts in the
-// gradient) or with a NaN or +inf are NaN.
+// gradient) or with a NaN or +inf (whose gradient is NaN) are NaN.
 __device__ __forceinline__ void put_given_row(const Stats& a, float c1, bool live, const GivenOut& o, int64_t i) {
     const float nan = __int_as_float(0x7fc00000);
     float l = INFINITY, f = a.s == a.s ? 0.f : a.s, h = nan;
-    if (live && a.m != -INFINITY) {
+    if (live && a.s != a.s) {
+        l = nan;  // (m does not show a NaN: beside nothing but -inf it is -inf)
+    } else if (live && a.m != -INFINITY) {
         // (against the largest logit and not the log-sum: the exponents that
         // count are small, so that their rounding is)
         l = a.m * c1;

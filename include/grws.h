@@ -889,14 +889,14 @@ int grws_head_bwd(const grws_head* head, const float* lse, const float* target_l
 /* (teacher_logits NULL); any temperature; a negative class asks for nothing */
 /* (log probability 0), one past the last is an error (NaN).  A row whose id */
 /* is out of range, or of nothing but -inf, is NaN and reaches no gradient;  */
-/* one with a NaN or +inf is NaN.  Outputs: logp f32 [n * max(k, 1)],        */
-/* entropy f32 [n] (natural logarithms), saved f32 [2 x n] (what the         */
-/* backward takes); top > 0 (at most min(classes, 1024)): top_logp f32 and   */
-/* top_index int32 [n x top] of the largest logits, largest first, of equal  */
-/* ones the lowest class first (the logits of a block of rows, 1 GiB or 256  */
-/* rows of them, are then in the workspace).  Backward of dlogp and dentropy */
-/* (shaped alike; NULL: zeros): gradients as of grws_head_bwd.  No sync;     */
-/* same inputs, same bits.                                                   */
+/* one with a NaN or +inf is NaN, and so are the gradients that it reaches.  */
+/* Outputs: logp f32 [n * max(k, 1)], entropy f32 [n] (natural logarithms),  */
+/* saved f32 [2 x n] (what the backward takes); top > 0 (at most             */
+/* min(classes, 1024)): top_logp f32 and top_index int32 [n x top] of the    */
+/* largest logits, largest first, of equal ones the lowest class first (the  */
+/* logits of a block of rows, 1 GiB or 256 rows of them, are then in the     */
+/* workspace).  Backward of dlogp and dentropy (shaped alike; NULL: zeros):  */
+/* gradients as of grws_head_bwd.  No sync; same inputs, same bits.          */
 /* ------------------------------------------------------------------------ */
 size_t grws_head_log_probs_fwd_workspace_bytes(const grws_head* head, int32_t top);
 int grws_head_log_probs_fwd(const grws_head* head, int32_t top, float* logp, float* entropy, float* saved,

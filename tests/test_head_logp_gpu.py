@@ -478,3 +478,33 @@ def test_linear_head_autocast_streams_and_graphs(cuda_device):
             eager = step(new.requires_grad_(), w)
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(out, eager))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("k", [1, 3])
+@pytest.mark.parametrize("n,V", [(6, 300), (200, 1500), (1300, 1100)])
+def test_rows_without_a_number(cuda_device, dt, k, n, V):
+    """A hidden row that is not a number makes NaN of its own gradient, of the
+    weight's and of the bias's, as F.linear and log_softmax do; the other rows'
+    are as they are without it."""
+    h, w, b, rows, index, up = _inputs(cuda_device, n, 72, V, dt, k, n, bias=True)
+    _, clean = _run(h, w, b, rows, index, up)
+    h[2] = math.nan
+    h[4, 5] = math.nan
+    rest = torch.ones(n, dtype=torch.bool, device=cuda_device)
+    rest[[2, 4]] = False
+    for top in (0, 3):
+        got, grads = _run(h, w, b, rows, index, up, top=top)
+        assert bool(got.logp[~rest].isnan().all()) and bool(got.entropy[~rest].isnan().all())
+        assert not bool(got.logp[rest].isnan().any()) and not bool(got.entropy[rest].isnan().any())
+        assert bool(grads[0][~rest].isnan().all())
+        assert bool(grads[1].isnan().all()) and bool(grads[2].isnan().all())
+        assert bool(grads[0][rest].isfinite().all())
+        # (the factor in front is the largest row's, which may have been one of the two)
+        far = (grads[0][rest].double() - clean[0][rest].double()).norm() / clean[0][rest].double().norm()
+        assert float(far) < 2 * U[dt] + 2.0 ** -16
+    # a row that has nothing but classes of -inf stays out of the gradients
+    b[:] = -math.inf
+    h.nan_to_num_()
+    _, grads = _run(h, w, b, rows, index, up)
+    assert all(bool((g == 0).all()) for g in grads)
