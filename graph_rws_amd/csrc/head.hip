@@ -60,6 +60,8 @@
 #include "logp.h"
 #include "top_pool.h"
 
+#include <cfloat>
+
 namespace grws {
 namespace {
 
@@ -2009,12 +2011,14 @@ __global__ __launch_bounds__(256) void head_given_rows_kernel(Targets t, RowStat
             return *cls >= 0 ? dlogp[i * k + j] : 0.f;
         };
         float sum = 0.f, mag = 0.f;
+        bool finite = true;  // of this lane's
         for (int jb = 0; jb < k; jb += 64) {
             const int j = jb + lane;
             int64_t cls;
             const float x = entry(j, &cls);
             sum += x;
             mag += fabsf(x);
+            finite = finite && fabsf(x) < INFINITY;
             if (!place) continue;
             float both = x;
             bool first = cls >= 0;
@@ -2043,7 +2047,9 @@ __global__ __launch_bounds__(256) void head_given_rows_kernel(Targets t, RowStat
         }
         const float b = live && dentropy ? dentropy[i] : 0.f, h = live && dentropy ? entropy[i] : 0.f;
         mag += fabsf(b) * (h + 1.f);
-        if (mag < INFINITY) best = fmaxf(best, mag);
+        // (of finite ones the bound is at most the largest float; a NaN or an
+        // infinity is its row's own)
+        if (!__any(!finite) && fabsf(b) < INFINITY && h < INFINITY) best = fmaxf(best, fminf(mag, FLT_MAX));
         if (lane == 0)
             out[i] = live ? GivenRow{dentropy ? fmaf(b, fmaf(kLn2, log2f(st.y), h), sum) : sum, b * kLn2, sum, 0.f}
                           : GivenRow{0.f, 0.f, 0.f, 0.f};

@@ -508,3 +508,23 @@ def test_rows_without_a_number(cuda_device, dt, k, n, V):
     h.nan_to_num_()
     _, grads = _run(h, w, b, rows, index, up)
     assert all(bool((g == 0).all()) for g in grads)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [5, 300])
+def test_upstream_near_the_largest_float(cuda_device, dt, n):
+    """Finite upstream gradients whose row's bound, sum |a| + |b| (H + 1), goes
+    past f32: gradients are those of 2^-20 times it, 2^20 times."""
+    h, w, b, rows, index, up = _inputs(cuda_device, n, 32, 700, dt, 3, 31, bias=True)
+    for t in (h, w, b):  # products with them stay below the largest float
+        t.mul_(2.0 ** -8)
+    a = torch.tensor([1.5 * 2.0 ** 127, -1.5 * 2.0 ** 127, 2.0 ** 100], device=cuda_device).expand(n, 3)
+    e = up[1].sign() * 2.0 ** 126
+    zero = torch.zeros_like
+    for big in ((a, zero(e)), (zero(a), e)):
+        # (another row's bound is in front: the sums are rounded elsewhere)
+        _, x = _run(h, w, b, rows, index, big)
+        _, y = _run(h, w, b, rows, index, tuple(t * 2.0 ** -20 for t in big))
+        for p, q in zip(x[:2], y[:2]):
+            q = q.double() * 2.0 ** 20
+            assert float((p.double() - q).norm() / q.norm()) < 2 * U[dt] + 708 * 2.0 ** -23
