@@ -153,10 +153,22 @@ __global__ __launch_bounds__(kT) void clip_norm_kernel(const double* __restrict_
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
+// keep = f tail.  Beside gradients near the largest float keep may lie below the
+// smallest normal one, where f32 has few bits or none: then f is 2^126 of it
+// (the product stays finite) and tail takes that off.
+struct Factor {
+    float f, tail;
+};
+
+__device__ __forceinline__ Factor factor_of(double keep) {
+    const bool low = fabs(keep) < 0x1p-126;
+    return Factor{(float)(low ? keep * 0x1p126 : keep), low ? 0x1p-126f : 1.f};
+}
+
 // (A lane stores 16 bytes next to its neighbour's, so it reads 8 of 16-bit
 // gradients that go to f32.)
 template <bool ONCE, typename T, typename O>
-__device__ __forceinline__ void scale_chunk(const void* src, void* dst, int64_t from, int64_t size, float f) {
+__device__ __forceinline__ void scale_chunk(const void* src, void* dst, int64_t from, int64_t size, Factor f) {
     constexpr int N = 16 / sizeof(O), LOADS = kChunk / (kT * N);
     const T* x = static_cast<const T*>(src);
     O* o = static_cast<O*>(dst);
@@ -168,7 +180,7 @@ __device__ __forceinline__ void scale_chunk(const void* src, void* dst, int64_t 
         const int64_t at = from + ((int64_t)l * kT + threadIdx.x) * N;
         Vec<O, N> w;
 #pragma unroll
-        for (int e = 0; e < N; ++e) w.x[e] = from_float<O>(to_float(v[l].x[e]) * f);
+        for (int e = 0; e < N; ++e) w.x[e] = from_float<O>(to_float(v[l].x[e]) * f.f * f.tail);
         if (at + N <= size) {
             u32x4_t x4;
             __builtin_memcpy(&x4, &w, sizeof(w));
@@ -194,8 +206,9 @@ __global__ __launch_bounds__(kT) void clip_scale_kernel(Tensors a, const double*
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     double keep = (double)max_norm / (n + 1e-6);
     if (keep > 1.0) keep = 1.0;  // (a NaN stays)
-    const float f = (float)(scale ? keep * (double)*scale : keep);
-    if (in_place && f == 1.f) return;  // uniform
+    if (scale) keep *= (double)*scale;
+    const Factor f = factor_of(keep);
+    if (in_place && f.f == 1.f && f.tail == 1.f) return;  // uniform
     for_chunks(a, [&](int t, int64_t from) {
         const void* x = a.src[t];
         void* o = a.dst[t];

@@ -237,3 +237,18 @@ def test_parameters(cuda_device):
     clip_grad_norm_([a[0], a[0]], 1.0)
     torch.nn.utils.clip_grad_norm_([b[0], b[0]], 1.0)
     assert torch.equal(a[0].grad, b[0].grad)
+
+
+@pytest.mark.parametrize("max_norm", [2.0 ** -7, 2.0 ** -17, 2.0 ** -66, 2.0 ** -113])
+def test_factors_below_the_smallest_float(cuda_device, max_norm):
+    """max_norm / norm is a number that f32 holds with few bits or not at all,
+    the clipped gradients are not.  (The bounds of the file's head.)"""
+    for dt in (torch.float32, torch.bfloat16):
+        g = _make(cuda_device, [4099, 12], [dt] * 2, 3, level=1e36)
+        keep = [t.clone() for t in g]
+        out = [torch.empty(t.shape, device=cuda_device) for t in g]
+        _check_norm(clip_grads(g, max_norm, out=out), _norm(keep), 4111)
+        _check_clipped(out, keep, max_norm)
+        clip_grads(g, max_norm)
+        _check_clipped(g, keep, max_norm)
+        assert not bool((g[0] == 0).all())
