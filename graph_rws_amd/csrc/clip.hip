@@ -202,8 +202,9 @@ __global__ __launch_bounds__(kT) void clip_scale_kernel(Tensors a, const double*
                                                         float max_norm, const float* scale, int32_t in_place,
                                                         float* __restrict__ norm) {
     __shared__ double red[kT / kWave];
-    const double n = norm_of(part, parts, scale, red);
+    double n = norm_of(part, parts, scale, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    if ((float)n == INFINITY) n = INFINITY;  // what f32 does not hold clips as it is returned
     double keep = (double)max_norm / (n + 1e-6);
     if (keep > 1.0) keep = 1.0;  // (a NaN stays)
     if (scale) keep *= (double)*scale;

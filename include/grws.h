@@ -955,9 +955,9 @@ int grws_log_probs_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t ro
 /* outs[i] = grads[i] scale min(1, max_norm / (norm + 1e-6)) in             */
 /* out_dtypes[i]: the gradient's dtype or f32 (NULL: the gradient's);       */
 /* outs[i] may be grads[i] in the same dtype, tensors do not overlap        */
-/* otherwise.  outs NULL: the norm alone.  A norm that is not finite makes  */
-/* zeros and NaN of the gradients, as the formula does.  Same inputs, same  */
-/* bits.                                                                    */
+/* otherwise.  outs NULL: the norm alone.  A norm that is not finite, or    */
+/* past f32 (infinite then), makes zeros and NaN of the gradients, as the   */
+/* formula does.  Same inputs, same bits.                                   */
 /* ------------------------------------------------------------------------ */
 size_t grws_clip_workspace_bytes(int32_t count);
 int grws_clip_grads(const void* const* grads, const int32_t* dtypes, const int64_t* sizes, void* const* outs,

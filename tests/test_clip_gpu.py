@@ -239,6 +239,29 @@ def test_parameters(cuda_device):
     assert torch.equal(a[0].grad, b[0].grad)
 
 
+def test_norm_beyond_f32(cuda_device):
+    """A norm that f32 does not hold is infinite, and clips to zeros, as
+    torch's does."""
+    for dt, level in ((torch.float32, 1e38), (torch.bfloat16, 2.0 ** 126)):
+        g = [torch.full((4099,), level, device=cuda_device, dtype=dt), torch.ones(5, device=cuda_device, dtype=dt)]
+        assert float(grad_norm(g)) == math.inf
+        out = [torch.full(t.shape, 7.0, device=cuda_device) for t in g]
+        assert float(clip_grads(g, 1.0, out=out)) == math.inf
+        assert all(bool((o == 0).all()) for o in out)
+        p = [torch.nn.Parameter(torch.zeros_like(t)) for t in g]
+        for q, t in zip(p, g):
+            q.grad = t.clone()
+        torch.nn.utils.clip_grad_norm_(p, 1.0)
+        assert float(clip_grads(g, 1.0)) == math.inf
+        assert all(torch.equal(t, q.grad) for t, q in zip(g, p))
+        # a scale that brings the norm back
+        g = [torch.full((4099,), level, device=cuda_device, dtype=dt)]
+        scale = torch.tensor(2.0 ** -30, device=cuda_device)
+        ref = _norm(g, 2.0 ** -30)
+        _check_norm(clip_grads(g, 1.0, out=out[:1], scale=scale), ref, 4099)
+        _check_clipped(out[:1], g, 1.0, 2.0 ** -30)
+
+
 @pytest.mark.parametrize("max_norm", [2.0 ** -7, 2.0 ** -17, 2.0 ** -66, 2.0 ** -113])
 def test_factors_below_the_smallest_float(cuda_device, max_norm):
     """max_norm / norm is a number that f32 holds with few bits or not at all,
