@@ -13,15 +13,30 @@ import torch.nn.functional as F
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_(parameters, max_norm) of the 2-norm in
     two launches (core.clip_grads); torch's own where the gradients are not
-    dense F32 / F16 / BF16 tensors of one GPU, each listed once."""
+    dense F32 / F16 / BF16 tensors of one GPU that share no memory."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
-    if (not grads or len({id(g) for g in grads}) != len(grads)
-            or any(type(g) is not torch.Tensor or g.layout != torch.strided or not g.is_cuda
-                   or g.device != grads[0].device or g.dtype not in _CLIPPED for g in grads)):
+    if (not grads or any(type(g) is not torch.Tensor or g.layout != torch.strided or not g.is_cuda
+                         or g.device != grads[0].device or g.dtype not in _CLIPPED for g in grads)
+            or _share_memory(grads)):
         return torch.nn.utils.clip_grad_norm_(parameters, max_norm)
     from ..core import clip_grads
     return clip_grads(grads, max_norm)
+
+
+def _share_memory(grads) -> bool:
+    """Whether the addresses between some tensors' first and last elements
+    overlap, or a tensor's own elements do."""
+    spans = []
+    for g in grads:
+        size = g.nbytes
+        if not g.is_contiguous():  # (which no tensor without elements is)
+            size = (1 + sum((n - 1) * s for n, s in zip(g.shape, g.stride()))) * g.element_size()
+            if size < g.nbytes:
+                return True
+        spans.append((g.data_ptr(), size))
+    spans.sort()
+    return any(a + size > b for (a, size), (b, _) in zip(spans, spans[1:]))
 
 
 _CLIPPED = (torch.float32, torch.float16, torch.bfloat16)

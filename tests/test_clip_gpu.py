@@ -275,3 +275,34 @@ def test_factors_below_the_smallest_float(cuda_device, max_norm):
         clip_grads(g, max_norm)
         _check_clipped(g, keep, max_norm)
         assert not bool((g[0] == 0).all())
+
+
+def test_parameters_whose_gradients_share_memory(cuda_device):
+    """Views of one buffer that overlap go to torch, as a gradient that is
+    listed twice does; ones that lie apart do not.  (Torch scales what is
+    shared more than once and in no order, so nothing is clipped here.)"""
+    from graph_rws_amd.helper import engine
+    buf = torch.randn(64, 48, device=cuda_device)
+
+    def params(*grads):
+        p = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
+        for q, g in zip(p, grads):
+            q.grad = g
+        return p
+
+    for views in ((buf, buf.view(-1)), (buf[:40], buf[30:]), (buf[:, :30], buf[:, 20:]), (buf.view(-1)[5:9], buf.t())):
+        p = params(*views)
+        keep = buf.clone()
+        norm = clip_grad_norm_(p, 1e6)
+        ref = math.sqrt(sum(float((v.double() ** 2).sum()) for v in views))
+        assert abs(float(norm) - ref) <= 2.0 ** -18 * ref
+        assert torch.equal(buf, keep)
+    clipped = []
+    real = engine.torch.nn.utils.clip_grad_norm_
+    try:
+        engine.torch.nn.utils.clip_grad_norm_ = lambda *a, **k: clipped.append(1)
+        clip_grad_norm_(params(buf[:32], buf[32:]), 1.0)
+        clip_grad_norm_(params(buf[::2], buf[:0], torch.ones(3, device=cuda_device)), 1.0)
+    finally:
+        engine.torch.nn.utils.clip_grad_norm_ = real
+    assert not clipped

@@ -85,3 +85,21 @@ def test_parameters_off_the_gpu_go_to_torch():
     assert abs(float(norm) - 26.0 ** 0.5) < 1e-5
     assert abs(float(p[0].grad[0, 0]) - 2.0 / 26.0 ** 0.5) < 1e-5
     assert abs(float(clip_grad_norm_(p[0], 10.0)) - (24.0 / 26.0) ** 0.5) < 1e-5
+
+
+def test_gradients_that_share_memory():
+    """What helper.clip_grad_norm_ leaves to torch: views that overlap, one
+    that overlaps itself, and what only might."""
+    from graph_rws_amd.helper.engine import _share_memory
+    buf = torch.zeros(64, 48)
+    other = torch.zeros(5)
+    for grads in ([buf, buf], [buf, buf.view(-1)], [buf[:40], other, buf[30:]], [buf[:, :30], buf[:, 20:]],
+                  [buf.view(-1)[5:9], buf.t()], [other.expand(3, 5)], [other[:1].expand(7)],
+                  [buf.as_strided((4, 8), (4, 1))], [buf, other, buf[63, 47:]]):
+        assert _share_memory(grads)
+        assert _share_memory(grads[::-1])
+    for grads in ([], [buf], [buf.t()], [buf[:32], buf[32:]], [buf[32:], other, buf[:32]], [buf[::2], other],
+                  [buf[:, ::3]], [other, torch.zeros(0), torch.zeros(())], [torch.zeros(2, 3, 4, 5).permute(3, 0, 2, 1)],
+                  [buf.view(-1)[:7].bfloat16(), buf]):
+        assert not _share_memory(grads)
+        assert not _share_memory(grads[::-1])
