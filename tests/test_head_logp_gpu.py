@@ -528,3 +528,77 @@ def test_upstream_near_the_largest_float(cuda_device, dt, n):
         for p, q in zip(x[:2], y[:2]):
             q = q.double() * 2.0 ** 20
             assert float((p.double() - q).norm() / q.norm()) < 2 * U[dt] + 708 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_lists_in_blocks_and_pieces(cuda_device, dt):
+    """Lists of given classes (repeats, negative and far ones), a bias and rows
+    of a node table, with rows in several blocks and classes in several pieces,
+    against 64 bits.  Bounds, of the sums' magnitudes M (|terms| added up): a
+    probability and its bracket are off by 2^-13 of the row's sum |a| + |b|
+    (|ln p| + H) or less (a logit by 24 steps of 2^-23 of 60 or less, 2^-14; T,
+    sums and exponentials below 2^-15), G's planes by 2^-16, a sum of N terms by
+    N 2^-23, the bias's units of 2^-40 by less, and the result is rounded once."""
+    import ctypes
+    dev = cuda_device
+    n, D, V, k, T = 140000, 8, 9001, 4, 1.25
+    nodes = n + 1234
+    h, w, b, rows, index, up = _inputs(dev, n, D, V, dt, k, 21, nodes=nodes, bias=True)
+    g = torch.Generator(device=dev)
+    g.manual_seed(22)
+    index[:, 2] = index[:, 0]
+    index[torch.rand(n, k, generator=g, device=dev) < 0.2] = -1
+    index[::1000, 3] = V + 5
+    plan = (ctypes.c_int64 * 10)()
+    view = ops.given_call(h, w, index[:, :1], b, rows, 1.0).view
+    assert L.load().grws_head_plan(ctypes.byref(view), 1, plan) == L.GRWS_OK
+    assert plan[0] > 1 and plan[2] > 1, list(plan)
+    got, grads = _run(h, w, b, rows, index, up, T)
+    kept = linear_log_probs(h, w, index, bias=b, rows=rows, temperature=T, top=5)  # blocks of kept logits
+    wd, bd = w.double(), b.double()
+    dw, mw = torch.zeros(2, V, D, dtype=torch.float64, device=dev)
+    db, mb = torch.zeros(2, V, dtype=torch.float64, device=dev)
+    u, tiny = torch.finfo(dt).eps / 2, TINY[dt]
+
+    def close(x, ref, mag, terms, what):
+        tol = (2.0 ** -13 + 2.0 ** -16 + terms * 2.0 ** -23) * mag
+        tol = tol + u * (ref.abs() + tol) + tiny
+        worst = ((x.double() - ref).abs() / tol).max()
+        assert float(worst) <= 1.0, f"{what}: {float(worst)} of the bound"
+
+    seen = torch.zeros(nodes, dtype=torch.bool, device=dev)
+    for i in range(0, n, 20000):
+        s = slice(i, i + 20000)
+        x = h.double()[rows[s]]
+        z = x @ wd.t() + bd
+        lp = torch.log_softmax(z / T, 1)
+        p = lp.exp()
+        H = torch.special.entr(p).sum(1)
+        given = (index[s] >= 0) & (index[s] < V)
+        at = index[s].clamp(0, V - 1)
+        ref = lp.gather(1, at).masked_fill(index[s] < 0, 0.0).masked_fill(index[s] >= V, math.nan)
+        for out in (got, kept):
+            off = (out.logp[s].double() - ref).abs()
+            assert bool((out.logp[s].isnan() == ref.isnan()).all()) and float(off.nan_to_num(0.0).max()) < 2.0 ** -13
+            assert float((out.entropy[s].double() - H).abs().max()) < 2.0 ** -13 * (1 + float(H.max()))
+        best = torch.topk(lp, 5, dim=1).values
+        assert float((kept.top_logp[s].double() - best).abs().max()) < 2.0 ** -13
+        assert float((lp.gather(1, kept.top_index[s].long()) - best).abs().max()) < 2.0 ** -13
+        a = torch.where(given, up[0][s].double(), 0.0)
+        e = up[1][s].double()
+        grad = -p * (a.sum(1)[:, None] + e[:, None] * (lp + H[:, None]))
+        grad = grad.scatter_add_(1, at, a) / T
+        mag = p * (a.abs().sum(1)[:, None] + e.abs()[:, None] * (lp.abs() + H[:, None]))
+        mag = mag.scatter_add_(1, at, a.abs()) / T
+        close(grads[0][rows[s]], grad @ wd, mag @ wd.abs(), V + 8, "d_hidden")
+        seen[rows[s]] = True
+        dw += grad.t() @ x
+        mw += mag.t() @ x.abs()
+        db += grad.sum(0)
+        mb += mag.sum(0)
+    assert bool((grads[0][~seen] == 0).all())
+    close(grads[1], dw, mw, n + 8, "d_weight")
+    close(grads[2], db, mb, n + 8, "d_bias")
+    # far tighter than a sum's worst case, of the whole: G's rounding and the result's
+    for x, ref in ((grads[1], dw), (grads[2], db)):
+        assert float((x.double() - ref).norm() / ref.norm()) < u + 2.0 ** -10
