@@ -1259,7 +1259,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                     const float u = fmaf(acc[i][j][e], c1, -ref), x = __builtin_amdgcn_exp2f(u);
                     s += x;
                     if constexpr (GIVEN) t = fmaf(x, reach(u), t);
-                    tie |= acc[i][j][e] == y && 16 * i + 4 * g + e < l;
+                    else tie |= acc[i][j][e] == y && 16 * i + 4 * g + e < l;
                 }
             s += __shfl_xor(s, 16, kWave);
             s += __shfl_xor(s, 32, kWave);
