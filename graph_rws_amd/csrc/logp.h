@@ -56,6 +56,14 @@ __device__ __forceinline__ float entropy_of(const Stats& a) {
     return h < 0.f ? 0.f : h;
 }
 
+// The exponentials are 2^(z c1 - ref), ref the rounded m c1 of a largest logit
+// m, and what that rounding took is put back.  Where m c1 is 2^30 or more (masks
+// of -1e30, temperatures next to zero) the rounding alone can be 2^6 and soon
+// is more than an exponent: there they are 2^((z - m) c1).
+__device__ __forceinline__ bool is_far(float m, float c1) {
+    return fabsf(m * c1) >= 1073741824.f && fabsf(m) != INFINITY;
+}
+
 // The exponentials are 2^(z c - ref), ref the rounded m c, of a largest logit m.
 // c is c1, but a half where m c1 overflows (m a mask of the type's lowest
 // value): floats of that size lie so far apart that any c leaves zero of a z

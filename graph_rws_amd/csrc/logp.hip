@@ -100,12 +100,18 @@ __device__ __forceinline__ void put_top(Pool<MAXK>& p, const Row& q, int64_t r, 
     });
 }
 
-// What a thread has added: s and t against ref, the rounded m c (see base2),
-// and what that rounding took.
+// What a thread has added: s and t against ref, the rounded m c1, and what that
+// rounding took; or against m c1 itself, where that is far from zero: ref is
+// +inf then, so that the first pass over the logits leaves a t that is not a
+// number, and the second has the differences.
 struct Running {
     Stats a = no_stats();
-    float c = 1.f, ref = 0.f, past = 0.f;
+    float ref = 0.f;
 
+    // what ref's rounding took
+    __device__ __forceinline__ float past(float c1) const {
+        return fabsf(a.m) == INFINITY || fabsf(ref) == INFINITY ? 0.f : fmaf(-a.m, c1, ref);
+    }
     // Adds N logits; the largest of them.
     template <int N>
     __device__ __forceinline__ float add(const float (&z)[N], float c1) {
@@ -113,17 +119,15 @@ struct Running {
 #pragma unroll
         for (int i = 1; i < N; ++i) m = fmaxf(m, z[i]);
         if (m > a.m) {
-            const float to = base2(m, c1), r = m * to, p = fabsf(r) == INFINITY ? 0.f : fmaf(-m, to, r);
-            move(a, (a.m - m) * c1 + (past - p));
+            const float d = (a.m - m) * c1 + past(c1);
             a.m = m;
-            c = to;
-            ref = r;
-            past = p;
+            ref = is_far(m, c1) ? INFINITY : m * c1;
+            move(a, d - past(c1));
         }
         const float s = a.s, t = a.t;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float u = fmaf(z[i], c, -ref), e = __builtin_amdgcn_exp2f(u);
+            const float u = fmaf(z[i], c1, -ref), e = __builtin_amdgcn_exp2f(u);
             a.s += e;
             a.t = fmaf(e, u, a.t);
         }
@@ -132,7 +136,8 @@ struct Running {
             a.t = t;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float u = fmaf(z[i], c, -ref), e = __builtin_amdgcn_exp2f(u);
+                const float u = ref == INFINITY ? (z[i] - a.m) * c1 : fmaf(z[i], c1, -ref);
+                const float e = __builtin_amdgcn_exp2f(u);
                 a.s += e;
                 a.t = fmaf(e, reach(u), a.t);
             }
@@ -164,9 +169,9 @@ struct Running {
         }
         return m;
     }
-    // against m c itself
-    __device__ __forceinline__ Stats stats() {
-        move(a, past);
+    // against m c1 itself
+    __device__ __forceinline__ Stats stats(float c1) {
+        move(a, past(c1));
         return a;
     }
 };
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(kT) void logp_rows_kernel(const T* __restrict__ log
             offer_chunk<MAXK>(p, v, row, c, begin, end, class_bits, top, bound, least);
         }
     }
-    Stats a = join_wave(sum.stats(), sc.c1);
+    Stats a = join_wave(sum.stats(sc.c1), sc.c1);
     if ((threadIdx.x & 63) == 0) {
         sm[threadIdx.x >> 6] = a.m;
         ss[threadIdx.x >> 6] = a.s;

@@ -391,3 +391,34 @@ def test_rows_without_a_number(cuda_device, dt, V):
             rest = [0, *range(5, n)]
             ref = _Ref(z.detach()[rest], index[rest])
             ref.check_grad(grad[rest], *(u[rest] if u is not None else None for u in up))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("V", [700, 5000, 140001])
+def test_far_from_zero(cuda_device, dt, V):
+    """Logits whose size over T is past 2^24, where a product with log2(e) / T
+    has no fraction left: rows of nothing but masks of -1e30 (or what the type
+    holds), large offsets, temperatures next to greedy ones."""
+    most = float(torch.finfo(dt).max)
+    z, index, a, b = _inputs(cuda_device, 9, V, dt, 2, V + 5)
+    z[0] = max(-1e30, -most)
+    z[1] = max(-1e10, -most)
+    z[2] = -1e9 if most > 1e9 else -6e4
+    z[2, ::3] = z[2, 1] / 2  # a mask that is a mask of another
+    z[3] = min(1e30, most)
+    z[4] = (z[4].float() * 1e4).clamp(-most, most).to(dt)
+    z[5] = (z[5].float() * 1e-3 * most).to(dt)
+    z[6] = min(1e30, most / 2)
+    z[6, V - 2] *= -1
+    for temperature in (1.0, 2.0 ** -20, 1e-8, 1e-12, 1e-20, 1e-37):
+        ref = _Ref(z, index, float(torch.tensor(temperature)))
+        x = z.detach().clone().requires_grad_()
+        got = log_probs(x, index, temperature=temperature, top=3)
+        low = ref.logp < -float(torch.finfo(torch.float32).max)
+        assert not bool(got.logp.isnan().any()) and not bool(got.entropy.isnan().any())
+        ref.check(got, index.shape)
+        assert bool((got.logp[low] == -math.inf).all())
+        order = torch.argsort(z.double(), dim=1, descending=True, stable=True)[:, :3]
+        assert torch.equal(got.top_index.long(), order)
+        grad, = torch.autograd.grad(got.logp, [x], [a * temperature])
+        ref.check_grad(grad, a * temperature, None)
