@@ -371,7 +371,14 @@ __device__ __forceinline__ void begin_logits(float4_t (&acc)[TP][TQ], int64_t vf
 }
 
 // The maxima stay logits: two of them can be one float when multiplied by c1,
-// and a hit is a matter of which is larger (base2 in logp.h).
+// and a hit is a matter of which is larger.  The losses' exponentials of a row are
+// 2^(z c - ref), ref the rounded m c, of a largest logit m.  c is c1, but a
+// half where m c1 overflows (m a mask of the type's lowest value): floats of
+// that size lie so far apart that any c leaves zero of a z other than m, and
+// with a power of two m c is exact and leaves one of m.
+__device__ __forceinline__ float base2(float m, float c1) {
+    return fabsf(m * c1) == INFINITY && fabsf(m) != INFINITY ? 0.5f : c1;
+}
 // what makes a strip's sum one against m c1 itself
 __device__ __forceinline__ float past_rounding(float m, float c1) {
     const float ref = m * c1;
@@ -379,8 +386,8 @@ __device__ __forceinline__ float past_rounding(float m, float c1) {
 }
 
 // Log probabilities and entropies: (m, s, t) of each row's strips, s and t
-// against the rounded m c1, and the logits themselves where alternatives are
-// looked for.
+// against the rounded m c1 (far from zero against m c1 itself, see is_far), and
+// the logits themselves where alternatives are looked for.
 struct Strips {
     float4* part;
     int64_t row, strip;  // entries from a row, a strip, to the next
@@ -392,7 +399,7 @@ struct Strips {
 __device__ __forceinline__ Stats exact_strip(const float4& v, float c1) {
     Stats a{v.x, v.y, v.z};
     const float ref = a.m * c1;
-    if (fabsf(ref) != INFINITY) move(a, -fmaf(a.m, c1, -ref));
+    if (fabsf(ref) != INFINITY && !is_far(a.m, c1)) move(a, -fmaf(a.m, c1, -ref));
     return a;
 }
 
@@ -440,7 +447,8 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
             for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
         m = fmaxf(m, __shfl_xor(m, 16, kWave));
         m = fmaxf(m, __shfl_xor(m, 32, kWave));
-        const float c1 = base2(m, a.c1), ref = m == -INFINITY ? 0.f : m * c1;  // nothing but -inf: a sum of zeros
+        const float c1 = GIVEN ? a.c1 : base2(m, a.c1);
+        const float ref = m == -INFINITY ? 0.f : m * c1;  // nothing but -inf: a sum of zeros
         float s = 0.f, t = 0.f;
 #pragma unroll
         for (int i = 0; i < TP; ++i)
@@ -450,6 +458,22 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_stats_kernel(StatsArgs a) {
                 s += x;
                 if constexpr (GIVEN) t = fmaf(x, reach(u), t);
             }
+        if constexpr (GIVEN) {
+            const bool far = is_far(m, c1);
+            if (__any(far)) {
+                float s2 = 0.f, t2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < TP; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = (acc[i][j][e] - m) * c1, x = __builtin_amdgcn_exp2f(u);
+                        s2 += x;
+                        t2 = fmaf(x, reach(u), t2);
+                    }
+                s = far ? s2 : s;
+                t = far ? t2 : t;
+            }
+        }
         s += __shfl_xor(s, 16, kWave);
         s += __shfl_xor(s, 32, kWave);
         if constexpr (GIVEN) {
@@ -514,6 +538,19 @@ struct RowStats {
 // is of the largest one's size: a c of 2^-149 makes one of it.)
 __device__ __forceinline__ float2 base_of(float lse, float c1) {
     return lse == -INFINITY ? make_float2(__uint_as_float(1), 0.f) : make_float2(c1, lse);
+}
+
+// Of log probabilities RowStats has the largest logit m in lse's place, and
+// factor is what makes p = 2^u factor of u = z c1 - ref, ref the rounded m c1,
+// or of u = (z - m) c1 where that is far from zero (is_far).
+struct Ref {
+    float less, ref;  // u = (z - less) c1 - ref
+    bool far;
+};
+
+__device__ __forceinline__ Ref ref_of(float m, float c1) {
+    const bool far = is_far(m, c1);
+    return Ref{far ? m : 0.f, far ? 0.f : m * c1, far};
 }
 
 // The gradient of log probabilities of given classes c_j and of an entropy,
@@ -632,7 +669,9 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
         // of a row that does not count, whose lse is +inf, all are 2^-inf
         // (its hidden row is zeros, so a logit is its bias)
         const float2 st = row_stats[row - (int64_t)tq * BQ];
-        const float lse = st.x, c1 = base_of(lse, a.c1).x, ref = base_of(lse, a.c1).y;
+        const float lse = st.x;
+        const float c1 = GIVEN ? a.c1 : base_of(lse, a.c1).x;
+        const float ref = GIVEN ? ref_of(lse, a.c1).ref : base_of(lse, a.c1).y;
         GivenRow given;
         if constexpr (GIVEN) given = row_given[row - (int64_t)tq * BQ];
         const float s = !GIVEN && a.row_scale && row < a.n ? a.row_scale[row] * a.gscale : a.gscale;
@@ -643,6 +682,15 @@ __global__ __launch_bounds__(WP * WQ * 64) void head_grad_kernel(GradArgs a) {
             for (int i = 0; i < TP; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][j][e] = stray ? -INFINITY : acc[i][j][e];
+        }
+        if constexpr (GIVEN) {
+            const Ref from = ref_of(lse, a.c1);
+            if (__any(from.far)) {
+#pragma unroll
+                for (int i = 0; i < TP; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= from.less;
+            }
         }
 #pragma unroll
         for (int i = 0; i < TP; ++i)
@@ -1249,14 +1297,16 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
             m = fmaxf(m, __shfl_xor(m, 16, kWave));
             m = fmaxf(m, __shfl_xor(m, 32, kWave));
             y = __shfl(y, (((l >> 2) & 3) << 4) | r, kWave);
-            const float c1 = base2(m, a.c1), ref = m == -INFINITY ? 0.f : m * c1;
+            const float c1 = GIVEN ? a.c1 : base2(m, a.c1), ref = m == -INFINITY ? 0.f : m * c1;
+            const bool far = GIVEN && is_far(m, c1);
             float s = 0.f, t = 0.f;
             int tie = 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float u = fmaf(acc[i][j][e], c1, -ref), x = __builtin_amdgcn_exp2f(u);
+                    const float u = far ? (acc[i][j][e] - m) * c1 : fmaf(acc[i][j][e], c1, -ref);
+                    const float x = __builtin_amdgcn_exp2f(u);
                     s += x;
                     if constexpr (GIVEN) t = fmaf(x, reach(u), t);
                     else tie |= acc[i][j][e] == y && 16 * i + 4 * g + e < l;
@@ -1288,7 +1338,9 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
             }
         } else {
             const float2 st = live[j] ? a.stats.of(row) : make_float2(INFINITY, 0.f);
-            const float c1 = base_of(st.x, a.c1).x, ref = base_of(st.x, a.c1).y;
+            const float c1 = GIVEN ? a.c1 : base_of(st.x, a.c1).x;
+            const float ref = GIVEN ? ref_of(st.x, a.c1).ref : base_of(st.x, a.c1).y;
+            const float less = GIVEN ? ref_of(st.x, a.c1).less : 0.f;
             const float sc = !GIVEN && a.row_scale && live[j] ? a.row_scale[row] * a.gscale : a.gscale;
             const float f = GIVEN ? -st.y * sc : st.y * sc;
             GivenRow given{0.f, 0.f, 0.f, 0.f};
@@ -1299,7 +1351,7 @@ __global__ __launch_bounds__(256) void head_few_kernel(FewArgs a) {
                 uint16_t x[4][PLANES > 0 ? PLANES : 1];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float u = fmaf(acc[i][j][e], c1, -ref);
+                    const float u = fmaf(GIVEN ? acc[i][j][e] - less : acc[i][j][e], c1, -ref);
                     float p = __builtin_amdgcn_exp2f(u);
                     if constexpr (GIVEN) p *= fmaf(given.bend, reach(u), given.slope);
                     p = live[j] ? p * f : 0.f;
@@ -1796,32 +1848,30 @@ __global__ __launch_bounds__(256) void head_hidden_out_kernel(const float* __res
 // ---------------------------------------------------------------------------
 // log probabilities of given classes and entropies
 // ---------------------------------------------------------------------------
-// What a call returns and keeps of each row: see RowStats, but lse is the
-// rounded m c1 here, and factor what makes p = 2^(z c1 - lse) factor of it.
+// What a call returns and keeps of each row: see RowStats and Ref.
 struct GivenOut {
     float* logp;     // [n k]
     float* entropy;  // [n]
-    float* lse;      // [n]
+    float* most;     // [n]: m; +inf for a row that does not count
     float* factor;   // [n]
 };
 
-// A row's statistics to lse, factor and entropy, by one thread.  Entropies of
+// A row's statistics to m, factor and entropy, by one thread.  Entropies of
 // rows without a place in hidden, of nothing but -inf (neither counts in the
 // gradient) or with a NaN or +inf (whose gradient is NaN) are NaN.
 __device__ __forceinline__ void put_given_row(const Stats& a, float c1, bool live, const GivenOut& o, int64_t i) {
     const float nan = __int_as_float(0x7fc00000);
-    float l = INFINITY, f = a.s == a.s ? 0.f : a.s, h = nan;
+    float m = INFINITY, f = a.s == a.s ? 0.f : a.s, h = nan;
     if (live && a.s != a.s) {
-        l = nan;  // (m does not show a NaN: beside nothing but -inf it is -inf)
+        m = nan;  // (m does not show a NaN: beside nothing but -inf it is -inf)
     } else if (live && a.m != -INFINITY) {
         // (against the largest logit and not the log-sum: the exponents that
         // count are small, so that their rounding is)
-        l = a.m * c1;
-        f = l == -INFINITY ? (a.s > 0.f ? 1.f / a.s : nan) : __builtin_amdgcn_exp2f(-fmaf(a.m, c1, -l)) / a.s;
-        if (l == INFINITY) l = nan;
+        m = a.m;
+        f = is_far(m, c1) ? 1.f / a.s : __builtin_amdgcn_exp2f(-fmaf(m, c1, -m * c1)) / a.s;
         h = entropy_of(a);
     }
-    o.lse[i] = l;
+    o.most[i] = m;
     o.factor[i] = f;
     o.entropy[i] = h;
 }

@@ -64,14 +64,6 @@ __device__ __forceinline__ bool is_far(float m, float c1) {
     return fabsf(m * c1) >= 1073741824.f && fabsf(m) != INFINITY;
 }
 
-// The exponentials are 2^(z c - ref), ref the rounded m c, of a largest logit m.
-// c is c1, but a half where m c1 overflows (m a mask of the type's lowest
-// value): floats of that size lie so far apart that any c leaves zero of a z
-// other than m, and with a power of two m c is exact and leaves one of m.
-__device__ __forceinline__ float base2(float m, float c1) {
-    return fabsf(m * c1) == INFINITY && fabsf(m) != INFINITY ? 0.5f : c1;
-}
-
 // The wave's, in every lane: the largest m first, then sums against it.
 __device__ __forceinline__ Stats join_wave(Stats a, float c1) {
     float m = a.m;

@@ -602,3 +602,60 @@ def test_lists_in_blocks_and_pieces(cuda_device, dt):
     # far tighter than a sum's worst case, of the whole: G's rounding and the result's
     for x, ref in ((grads[1], dw), (grads[2], db)):
         assert float((x.double() - ref).norm() / ref.norm()) < u + 2.0 ** -10
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,V", [(5, 300), (200, 1500), (1300, 1100)])
+@pytest.mark.parametrize("k", [1, 3])
+def test_far_from_zero(cuda_device, dt, n, V, k):
+    """Whole numbers, whose logits are exact, at temperatures next to greedy
+    ones, and under biases that lie far from zero: logits of 2^24 T and more."""
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(n + k)
+    D = 72
+    h = torch.randint(-2, 3, (n, D), generator=g, device=cuda_device).to(dt)
+    w = torch.randint(-2, 3, (V, D), generator=g, device=cuda_device).to(dt)
+    index = torch.randint(0, V, (n, k), generator=g, device=cuda_device)
+    up = torch.randn(n, k, generator=g, device=cuda_device), torch.randn(n, generator=g, device=cuda_device)
+    z = h.double() @ w.double().t()
+    index[:, 0] = z.argmax(1)
+    zero = torch.zeros(V, device=cuda_device, dtype=dt)
+    far = (zero - 1e30 if dt != torch.float16 else zero - 65504) * 1.0
+    half = zero.clone()
+    half[::2] = far[0]
+    for b, temperature in ((zero, 2.0 ** -20), (zero, 1e-8), (zero, 1e-12), (zero, 1e-30), (zero, 1e-37),
+                           (far, 1.0), (far, 1e-8), (half, 1e-9)):
+        T = float(torch.tensor(temperature))
+        y = (h.float() @ w.float().t() + b.float()).double() / T  # (a logit is rounded to f32 once)
+        lp = torch.log_softmax(y, 1)
+        p = lp.exp()
+        H = torch.special.entr(p).sum(1)
+        want = lp.gather(1, index)
+        a, e = up[0] * T, up[1] * T  # gradients of the size of weights
+        for top in (0, 3):
+            got, grads = _run(h, w, b, None, index, (a, e), temperature, top=top)
+            off = (got.logp.detach().double() - want).abs()
+            # 2^-22 of what lies between, and of a sum's logarithm the sum's steps
+            c = (V / 1024 + 64) * 2.0 ** -23 + 2.0 ** -20
+            same = got.logp.double() == want.clamp(min=-math.inf).where(want > -3.4e38, torch.tensor(-math.inf, dtype=torch.float64, device=cuda_device))
+            assert bool((same | (off <= 2.0 ** -21 * want.abs() + c)).all())
+            assert float((got.entropy.double() - H).abs().max()) <= c * (1 + float(H.max()))
+            if top:
+                best = torch.topk(lp, 3, dim=1).values
+                assert bool(((got.top_logp.double() - best).abs() <= 2.0 ** -21 * best.abs() + c)
+                            .logical_or(best < -3.4e38).all())
+            given = a.double()
+            ent = torch.where(p > 0, lp, 0.0) + H[:, None]
+            gr = -p * (given.sum(1)[:, None] + e.double()[:, None] * ent)
+            mag = p * (given.abs().sum(1)[:, None] + e.double().abs()[:, None] * (ent.abs() + H[:, None]))
+            gr = gr.scatter_add_(1, index, given) / T
+            mag = mag.scatter_add_(1, index, given.abs()) / T
+            u = torch.finfo(dt).eps / 2
+            for x, r, m, steps in ((grads[0], gr @ w.double(), mag @ w.double().abs(), V),
+                                   (grads[1], gr.t() @ h.double(), mag.t() @ h.double().abs(), n)):
+                tol = m * (u + 2.0 ** -13 + (steps + 8) * 2.0 ** -23)
+                if dt == torch.float16:
+                    tol = tol + float((a.abs().sum(1) + e.abs() * (H.float() + 1)).max()) / T * 2.0 ** -30
+                tol = tol + u * (r.abs() + tol) + TINY[dt]
+                worst = ((x.double() - r).abs() / tol).max()
+                assert float(worst) <= 1.0, (temperature, float(worst))
