@@ -306,3 +306,18 @@ def test_parameters_whose_gradients_share_memory(cuda_device):
     finally:
         engine.torch.nn.utils.clip_grad_norm_ = real
     assert not clipped
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """A tensor of 2^32 gradients and more, with another behind it."""
+    n = (1 << 32) + 4099
+    big = torch.full((n,), 0.5, device=cuda_device, dtype=torch.bfloat16)
+    small = torch.full((77,), 3.0, device=cuda_device)
+    big[-1] = 64.0
+    ref = math.sqrt((n - 1) * 0.25 + 64.0 ** 2 + 77 * 9.0)
+    norm = clip_grads([big, small], 1024.0)
+    assert abs(float(norm) - ref) <= ref * 2.0 ** -23
+    f = 1024.0 / (ref + 1e-6)
+    for got, g in ((big[:3], 0.5), (big[1 << 31:(1 << 31) + 3], 0.5), (big[-3:-1], 0.5), (big[-1:], 64.0), (small, 3.0)):
+        want = g * f
+        assert float((got.double() - want).abs().max()) <= want * (2.0 ** -8 + 2.0 ** -22)

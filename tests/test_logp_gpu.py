@@ -422,3 +422,24 @@ def test_far_from_zero(cuda_device, dt, V):
         assert torch.equal(got.top_index.long(), order)
         grad, = torch.autograd.grad(got.logp, [x], [a * temperature])
         ref.check_grad(grad, a * temperature, None)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^32 logits: the last rows as in a call of their own."""
+    n, V, k, last = 70001, 65537, 2, 300
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(2)
+    z = torch.empty(n, V, device=cuda_device, dtype=torch.float16)
+    z.normal_(generator=g)
+    index = torch.randint(0, V, (n, k), generator=g, device=cuda_device)
+    a = torch.randn(n, k, generator=g, device=cuda_device)
+    z.requires_grad_()
+    got = log_probs(z, index, top=3)
+    grad, = torch.autograd.grad([got.logp, got.entropy], [z], [a, a[:, 0]])
+    tail = z.detach()[-last:].clone().requires_grad_()
+    ref = log_probs(tail, index[-last:], top=3)
+    for p, q in zip(got[:2] + got[2:], ref[:2] + ref[2:]):
+        assert torch.allclose(p[-last:].float(), q.float(), rtol=2.0 ** -20, atol=2.0 ** -20)
+    assert torch.equal(got.top_index[-last:], ref.top_index)
+    want, = torch.autograd.grad([ref.logp, ref.entropy], [tail], [a[-last:], a[-last:, 0]])
+    assert float((grad[-last:].float() - want.float()).abs().max()) <= 2.0 ** -10 * float(want.abs().max())
