@@ -2188,7 +2188,8 @@ def clip_grads(grads, max_norm: float, out=None, scale: Optional[torch.Tensor] =
     (what an optimizer with float32 copies of 16-bit parameters reads).  A
     norm that is not finite, or past float32, makes zeros and NaN of the
     gradients, as torch.nn.utils.clip_grad_norm_ does.  Tensors that share
-    memory are an error; no host sync."""
+    memory are an error (among views with gaps it is not looked for: what
+    they share counts in the norm for each); no host sync."""
     grads = _clip_list("clip_grads", grads)
     if not float(max_norm) >= 0.0:
         raise ValueError(f"clip_grads: max_norm must not be negative (got {max_norm})")

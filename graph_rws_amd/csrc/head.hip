@@ -2187,7 +2187,7 @@ constexpr int64_t kJoinBlocks = 128;
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 // Rows are taken in blocks where the scratch would otherwise grow with rows x
 // classes: the strips' statistics of a forward block stay within kPartBytes
-// (8 bytes a row and strip), and a backward block leaves G room for
+// (8 bytes a row and strip, 16 of log probabilities), and a backward block leaves G room for
 // kLeastPiece classes a piece.  At most kBlockRows rows, so that no launch
 // has 2^32 threads.
 constexpr int64_t kPartBytes = (int64_t)512 << 20;
@@ -2198,9 +2198,12 @@ constexpr int64_t kFewClasses = 1024;  // up to here G has a second plane
 // few rows, or hidden rows of few columns (nearly parallel rows of W), do not
 // average: one plane of G left 16-bit gradients 1.6 to 3.2 times as far from 64
 // bits as their own rounding at 3 to 300 rows, and 1.6 to 1.9 times at widths of
-// 16 and 32, where it is 1.4 to 1.5 otherwise.  Two planes cost 10 to 40% of the
-// backward there (3 rows x 12,000 x 512: 53 us against 48, 16 x 131,072 x 2,048:
-// 729 against 543), and 60 to 70% of many wide rows, which keep one.
+// 16 and 32, where it is 1.4 to 1.5 otherwise: one rounding more of the result's
+// size, as that of 16-bit logits' gradients would be.  Two planes cost 10 to 40% of
+// the backward there (3 rows x 12,000 x 512: 53 us against 48, 16 x 131,072 x 2,048:
+// 729 against 543), and 60 to 70% of many wide rows, which keep one.  At the border
+// 1,024 rows of two planes are 1.00 times their own rounding off, 1,025 of one 1.42:
+// 122 us against 94 for 12,000 x 512, 655 against 520 for 32,000 x 2,048.
 constexpr int64_t kFewGiven = 1024, kNarrow = 64;
 // Rows up to which head_few_kernel makes the logits.  Forward calls on 32,000 x
 // 2,048, replayed in a graph, against the products (on packed W, where it has
