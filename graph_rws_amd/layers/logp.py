@@ -78,10 +78,11 @@ def log_probs(logits: torch.Tensor, index: torch.Tensor, temperature: float = 1.
     index int32 or int64 [n] or [n, k] (k <= 1024): the classes whose log
     probabilities are returned, in its shape; a negative one asks for nothing
     (log probability 0, no gradient), one past the last class is an error
-    (NaN, no gradient).  A class of logit -inf has log probability -inf and
-    adds nothing to the entropy; a row of nothing but -inf is NaN, its
-    gradient zeros; a row with NaN or +inf is NaN, and so is its gradient.
-    top <= min(classes, 1024).  No host sync; no second derivative."""
+    (NaN, no gradient).  A class of logit -inf, or further below the row's
+    largest one than float32 holds, has log probability -inf and adds nothing
+    to the entropy; a row of nothing but -inf is NaN, its gradient zeros; a
+    row with NaN or +inf is NaN, and so is its gradient.  top <= min(classes,
+    1024).  No host sync; no second derivative."""
     _ops.check_log_probs(logits, index, temperature, top)
     return LogProbs(*_LogProbs.apply(logits, index, float(temperature), int(top)))
 

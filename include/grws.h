@@ -928,8 +928,9 @@ int grws_top_logits(const void* logits, int32_t dtype, int64_t ld, int64_t rows,
 /* entropy f32 [rows] (natural logarithms), saved f32 [rows x 2] (what the  */
 /* backward takes; may be NULL).  top > 0 (at most min(classes, 1024)):     */
 /* top_logp f32 and top_index int32 [rows x top], largest first, of equal   */
-/* logits the lowest class first, NaN as the largest.  A class of -inf has  */
-/* no probability; a row of nothing but -inf, or with NaN or +inf, is NaN.  */
+/* logits the lowest class first, NaN as the largest.  A class of -inf, or  */
+/* further below the row's largest logit than f32 holds, has no probability; */
+/* a row of nothing but -inf, or with NaN or +inf, is NaN.                  */
 /* Backward of dlogp [rows x k] and dentropy [rows] (NULL: zeros): grad     */
 /* [rows x ldg] in dtype, every element written; a class given twice gets   */
 /* both; zeros in a row of nothing but -inf, NaN in one with NaN or +inf.   */
