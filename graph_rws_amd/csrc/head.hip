@@ -2123,6 +2123,7 @@ __global__ __launch_bounds__(256) void head_given_scale_kernel(const float* __re
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (m * factor > FLT_MAX) m = FLT_MAX / factor;  // a gradient past f32 stays in its row
     auto share = [&](float x) { return m > 0.f ? x / m : x * 0.f; };
     const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
     if (first == 0) *alpha = m * factor;

@@ -659,3 +659,20 @@ def test_far_from_zero(cuda_device, dt, n, V, k):
                 tol = tol + u * (r.abs() + tol) + TINY[dt]
                 worst = ((x.double() - r).abs() / tol).max()
                 assert float(worst) <= 1.0, (temperature, float(worst))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [6, 300])
+def test_a_gradient_past_f32_stays_in_its_row(cuda_device, dt, n):
+    """A row whose upstream over T is more than f32 holds; the others' hidden
+    gradients are as without it (rounded beside another factor)."""
+    T = 2.0 ** -100
+    h, w, b, rows, index, up = _inputs(cuda_device, n, 40, 500, dt, 1, 41)
+    a, e = up[0].sign().clone(), torch.zeros_like(up[1])
+    _, clean = _run(h, w, b, rows, index, (a, e), T)
+    a[3] = 2.0 ** 40
+    _, grads = _run(h, w, b, rows, index, (a, e), T)
+    rest = torch.arange(n, device=cuda_device) != 3
+    x, y = grads[0][rest].double(), clean[0][rest].double()
+    assert bool(y.isfinite().all()) and float((x - y).norm() / y.norm()) < 2 * U[dt] + 508 * 2.0 ** -23
+    assert not bool(grads[0][3].isfinite().all())
